@@ -416,6 +416,84 @@ int sf_lm_head_argmax_rows(const void *w, const void *x, int x_dtype, float *log
                            int B, int32_t *tokens_out, void *workspace, size_t workspace_bytes,
                            void *stream);
 
+/* ---- rotary positions given row by row (the reference's RoPE is rotate-half over
+ * the whole head at one offset, siliconfer/model/layers.py:58-66) -------------------
+ * The first 2 rot_pairs dims of a head turn pair by pair, pair i of a row at position p
+ * by the angle p inv_freq[i] (64 bits): y1 = x1 c - x2 s, y2 = x2 c + x1 s with
+ * c, s = scale cos, scale sin of it; pairs are (i, i + rot_pairs), or (2i, 2i + 1) where
+ * `interleaved`; the other dims are copied. `scale` carries a long-context scaling's
+ * factor (1 for none). q [B][T][H][D] -> q_out and, where KVH > 0, k [B][T][KVH][D] ->
+ * k_out, all of `dtype`; an output may be its input. strides: NULL for contiguous
+ * tensors, else 12 element strides (batch, row, head of q, q_out, k, k_out; a head's
+ * dims are contiguous). positions: int32, or int64 where pos_i64; [B][T], or [T] for
+ * every sequence where !pos_per_seq. Any even part of the head up to 1024 dims. */
+int sf_rotary(const void *q, void *q_out, const void *k, void *k_out, int dtype, const void *positions,
+              int pos_i64, int pos_per_seq, const double *inv_freq, int rot_pairs, float scale,
+              int interleaved, int B, int T, int H, int KVH, int D, const long long *strides,
+              void *stream);
+/* The same rotation of the q and k heads of fused projection rows qkv
+ * [B][T][(H + 2 KVH) D] (in_dtype), then the int8 quantize-append of k and v (the rule of
+ * sf_kv_quant_append) into slots n_b + t of a cache [B][KVH][T_cap][D], n_b =
+ * lengths[b] (device), or `start` where lengths is NULL: a cache that drops tokens holds
+ * a token in a slot other than its position. Rotated q goes to q_out [B][T][H][D].
+ * slot_positions [B][KVH][T_cap] (or NULL) gets the positions, scores (or NULL) zeros, at
+ * the same slots. A token whose slot would lie past T_cap is not stored. D <= 256 and a
+ * multiple of 8. */
+int sf_rotary_kv_append(const void *qkv, int in_dtype, const void *positions, int pos_i64,
+                        int pos_per_seq, const double *inv_freq, int rot_pairs, float scale,
+                        int interleaved, void *q_out, int q_dtype, int8_t *k_codes, void *k_scales,
+                        int8_t *v_codes, void *v_scales, int scale_dtype, int32_t *slot_positions,
+                        float *scores, const int32_t *lengths, int start, int B, int T, int H, int KVH,
+                        int D, int T_cap, void *stream);
+
+/* ---- a cache that keeps what is attended to (no counterpart in the reference) ------
+ * Decode attention that scores the cache it reads. Row t of q [B][Tq][H][D] sees the
+ * first n_b - Tq + t + 1 of sequence b's n_b slots, n_b = lengths[b] + T (device lengths),
+ * or T where lengths is NULL, cut to [0, T_max]; a row that sees none gives zeros. With
+ * w = softmax(scale q K^T): out [B][Tq][H][D] = w V, and scores [B][KVH][T_cap] (fp32)
+ * += w summed over the rows and the kv head's query heads, slots past n_b untouched.
+ * Tq <= 32. n_splits <= 0 picks a count. T_max (<= T_cap) bounds n_b and sizes the
+ * workspace: sf_attn_scored_workspace_bytes(...) bytes, 256-byte aligned, no initial
+ * contents needed; calls that share one must not overlap. */
+size_t sf_attn_scored_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits);
+int sf_attn_decode_scored_i8kv(const void *q, int q_dtype, const int8_t *k_codes, const void *k_scales,
+                               const int8_t *v_codes, const void *v_scales, int scale_dtype, float *scores,
+                               void *out, int out_dtype, void *workspace, size_t workspace_bytes, int B,
+                               int Tq, int H, int KVH, const int32_t *lengths, int T, int T_max, int T_cap,
+                               int D, float scale, int n_splits, void *stream);
+/* Of the n_b = lengths[b] (or T where lengths is NULL) slots of each (sequence, kv head)
+ * keep `budget`: first those of the newest `recent` tokens (positions >= seen[b] - recent;
+ * seen_host where seen is NULL) in order, then the largest scores; a NaN score counts as
+ * -inf, equal ones go to the lower slot. The kept slots behind the budget move, in order, into the
+ * holes below it: codes, scales, scores and positions, in place; what lies at and past
+ * lengths_out[b] = min(n_b, budget) is left as it was. lengths_out must not be `lengths`.
+ * Sequences within the budget are untouched. workspace: 16-byte aligned,
+ * sf_kv_evict_workspace_bytes(B, KVH, budget, T_cap, or T where lengths is NULL) bytes. */
+size_t sf_kv_evict_workspace_bytes(int B, int KVH, int budget, int T_max);
+int sf_kv_evict(int8_t *k_codes, void *k_scales, int8_t *v_codes, void *v_scales, int scale_dtype,
+                float *scores, int32_t *positions, const int32_t *lengths, int T, const int32_t *seen,
+                int seen_host, int budget, int recent, int32_t *lengths_out, void *workspace,
+                size_t workspace_bytes, int B, int KVH, int T_cap, int D, void *stream);
+
+/* ---- a token a row from given random numbers ---------------------------------------
+ * The reference's sampling rules (siliconfer/engine/generate.py:24-67: temperature, top-k,
+ * top-p) and min-p, drawn from u [B] in [0, 1). A row's tokens are taken in descending
+ * order of their logits (equal ones by ascending index; NaN counts as -inf) and weigh
+ * exp((x - max) / temperature); top_k > 0 keeps the first k and the ties of the k-th,
+ * top_p < 1 those before which at most top_p of the remaining weight lies, min_p > 0 those
+ * that weigh at least min_p of the largest. The token is the first whose running weight
+ * exceeds u times the weight kept; temperature <= 0 takes the largest logit. A row
+ * without a logit above -inf gives -1. logprobs (or NULL): the log of the token's share
+ * of the weight kept. logits [B][V] of `dtype`, rows row_stride elements apart; each of
+ * the settings for all rows, or a row's own from a device array [B] where that is not
+ * NULL. workspace: sf_sample_workspace_bytes(B, V) bytes, 256-byte aligned (may be 0 ->
+ * NULL ok), no initial contents needed; calls that share one must not overlap. */
+size_t sf_sample_workspace_bytes(int B, int V);
+int sf_sample(const void *logits, int dtype, long long row_stride, int B, int V, const float *u,
+              float temperature, int top_k, float top_p, float min_p, const float *temperatures,
+              const int32_t *top_ks, const float *top_ps, const float *min_ps, int32_t *tokens,
+              float *logprobs, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- a chain of dependent decode GEMVs in one persistent launch (no
  * counterpart in the reference, which runs each Q4Linear of a layer as its own
  * call, /root/reference/siliconfer/model/layers.py:93-95, 133, 139-144) -------

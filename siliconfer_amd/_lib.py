@@ -11,6 +11,7 @@ present.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -104,6 +105,21 @@ _SIGS = {
     "sf_lm_head_rows_workspace_bytes": (_c_sz, [_c_i, _c_i]),
     "sf_lm_head_argmax_rows": (_c_i, [_c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_i, _c_p, _c_p, _c_sz,
                                       _c_p]),
+    "sf_rotary": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_p, _c_i, _c_f, _c_i, _c_i,
+                         _c_i, _c_i, _c_i, _c_i, _c_p, _c_p]),
+    "sf_rotary_kv_append": (_c_i, [_c_p, _c_i, _c_p, _c_i, _c_i, _c_p, _c_i, _c_f, _c_i, _c_p, _c_i, _c_p,
+                                   _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i,
+                                   _c_i, _c_i, _c_p]),
+    "sf_attn_scored_workspace_bytes": (_c_sz, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "sf_attn_decode_scored_i8kv": (_c_i, [_c_p, _c_i, _c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_i, _c_p,
+                                          _c_sz, _c_i, _c_i, _c_i, _c_i, _c_p, _c_i, _c_i, _c_i, _c_i,
+                                          _c_f, _c_i, _c_p]),
+    "sf_kv_evict_workspace_bytes": (_c_sz, [_c_i, _c_i, _c_i, _c_i]),
+    "sf_kv_evict": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_i,
+                           _c_p, _c_p, _c_sz, _c_i, _c_i, _c_i, _c_i, _c_p]),
+    "sf_sample_workspace_bytes": (_c_sz, [_c_i, _c_i]),
+    "sf_sample": (_c_i, [_c_p, _c_i, ctypes.c_longlong, _c_i, _c_i, _c_p, _c_f, _c_i, _c_f, _c_f, _c_p,
+                         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p]),
     "sf_q4_chain_workspace_bytes": (_c_sz, [_c_p, _c_i]),
     "sf_q4_chain": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_p, _c_sz, _c_i, _c_i,
                            _c_p]),
@@ -189,6 +205,62 @@ def stream(t: torch.Tensor | None = None) -> int:
     # most of the 13.1 us of host time that one small Q4Linear call took (8.4 now)
     return torch._C._cuda_getCurrentRawStream(t.get_device() if t is not None
                                               else torch.cuda.current_device())
+
+
+def on_device(t: torch.Tensor):
+    """A context in which t's device is the current one (launches go there)."""
+    return _NOTHING if torch.cuda.current_device() == t.get_device() else torch.cuda.device(t.device)
+
+
+_NOTHING = contextlib.nullcontext()
+_scratch: dict = {}
+
+
+def scratch(device: torch.device, stream_handle: int, nbytes: int) -> torch.Tensor:
+    """Workspace of one call: kept a (device, stream) and grown on demand, whose
+    calls run one after the other; while a graph is recorded a tensor of the graph's
+    own, so that no two graphs share one."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    key = (device, stream_handle)
+    ws = _scratch.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _scratch[key] = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
+    return ws
+
+
+def lengths_arg(lengths, B: int, device: torch.device, name: str = "lengths") -> tuple[int | None, int]:
+    """(device pointer or None, host value) of lengths given as int32 [B] or one int."""
+    if not isinstance(lengths, torch.Tensor):
+        n = int(lengths)
+        if not 0 <= n < 1 << 31:
+            raise SFError(f"{name} {n} outside 0 .. 2^31 - 1")
+        return None, n
+    if (lengths.dtype is not torch.int32 or lengths.shape != (B,) or lengths.device != device
+            or not lengths.is_contiguous()):
+        raise SFError(f"{name} must be an int, or a contiguous int32 tensor [{B}] on the cache's device")
+    return lengths.data_ptr(), 0
+
+
+def check_cache(device: torch.device, k_codes, k_scales, v_codes, v_scales, positions=None,
+                scores=None) -> None:
+    """The buffers of an int8 cache: codes [B, KVH, T_cap, D], the others [B, KVH, T_cap]."""
+    rows = k_codes.shape[:3]
+    if k_codes.dtype is not torch.int8 or v_codes.dtype is not torch.int8:
+        raise SFError("KV codes must be int8")
+    if k_scales.dtype != v_scales.dtype or k_scales.dtype not in (torch.float16, torch.float32):
+        raise SFError("k/v scales must both be float16 or both float32")
+    for t, n, dtype in ((k_codes, "k_codes", None), (v_codes, "v_codes", None), (k_scales, "k_scales", None),
+                        (v_scales, "v_scales", None), (positions, "slot positions", torch.int32),
+                        (scores, "scores", torch.float32)):
+        if t is None:
+            continue
+        if t.device != device or not t.is_contiguous():
+            raise SFError(f"{n} must be contiguous on {device}")
+        if t.shape[:3] != rows or (t.dim() != 3 and n[2:] != "codes"):
+            raise SFError(f"{n} must be {list(rows)} (got {list(t.shape)})")
+        if dtype is not None and t.dtype is not dtype:
+            raise SFError(f"{n} must be {dtype}")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -29,6 +29,7 @@
 
 #include <mutex>
 
+#include "attn_common.h"
 #include "sf_common.h"
 #include "split_merge.h"
 
@@ -408,20 +409,6 @@ k_attn_decode(const void *__restrict__ q, const int8_t *__restrict__ kc,
 // the output).
 constexpr int kMfmaMaxSplits = 128;
 
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-
-// 8 int8 codes (two dwords, byte order kept) -> 8 exact fp16 values: the
-// offset-binary byte b + 128 in the low mantissa byte of fp16 1024, minus 1152.
-__device__ __forceinline__ half8_t i8x8_to_h8(uint32_t lo, uint32_t hi) {
-  const uint32_t a = lo ^ 0x80808080u, b = hi ^ 0x80808080u;
-  const half2_t off = {(f16)-1152.f, (f16)-1152.f};
-  const half2_t p0 = sf_bitcast<half2_t>(__builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) + off;
-  const half2_t p1 = sf_bitcast<half2_t>(__builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) + off;
-  const half2_t p2 = sf_bitcast<half2_t>(__builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) + off;
-  const half2_t p3 = sf_bitcast<half2_t>(__builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) + off;
-  return half8_t{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
-}
-
 template <int D, int NW>
 constexpr int attn_mfma_smem_floats() {
   // V tiles [NW][32][D + 8] bytes, then wave states m, l [NW][16] and O [NW][16][D]
@@ -440,19 +427,6 @@ constexpr int attn_mfma_smem_floats() {
 // path) has arrived; rows are clamped into the cache and tokens at or past the
 // length are masked. Tiles start on 32-token boundaries, so when T_cap % 4 ==
 // 0 (vscale) a lane's 8 scales are two aligned 4-token loads.
-// max / sum of a value and its partners 16 and 32 lanes away (see sf_swap16_pair)
-__device__ __forceinline__ float max_x16_x32(float v) {
-  float2_t p = sf_swap16_pair(v);
-  v = fmaxf(p.x, p.y);
-  p = sf_swap32_pair(v);
-  return fmaxf(p.x, p.y);
-}
-__device__ __forceinline__ float sum_x16_x32(float v) {
-  float2_t p = sf_swap16_pair(v);
-  v = p.x + p.y;
-  p = sf_swap32_pair(v);
-  return p.x + p.y;
-}
 // The weights P * V scale as fp16 halves: times 2^10, and less for a query row
 // whose largest weight pm (or V scale vm, in fp32) would overflow.
 constexpr float kVMul = 1024.f, kPvMax = 32768.f;

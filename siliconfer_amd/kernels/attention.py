@@ -111,3 +111,55 @@ def fused_quantized_attention_decode(q, k_codes, k_scales, v_codes, v_scales,
     q = q.contiguous()
     return attention_decode(q, k_codes.contiguous(), k_scales.contiguous(), v_codes.contiguous(),
                             v_scales.contiguous(), n_splits=n_tiles)
+
+
+def attention_decode_scored(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
+                            v_codes: torch.Tensor, v_scales: torch.Tensor, scores: torch.Tensor, *,
+                            lengths, add: int = 0, max_length: int | None = None,
+                            n_splits: int | None = None, scale: float | None = None,
+                            out: torch.Tensor | None = None,
+                            out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """Attention of q [B, H, D], or of the Tq newest rows q [B, Tq, H, D] (Tq <= 32),
+    over the first lengths[b] + add slots of an int8 cache (codes [B, KVH, T_cap, D],
+    scales [B, KVH, T_cap]), and the softmax weights, summed over the rows and each kv
+    head's query heads, added to scores (fp32 [B, KVH, T_cap]). Row t of Tq sees the
+    slots up to its own, lengths[b] + add - Tq + t; a row that sees none gives zeros.
+    `lengths`: int32 [B] on the device, or one int. Device lengths are cut to
+    `max_length` (the capacity where it is not given), which sizes the workspace."""
+    three = q.dim() == 3
+    if not three and q.dim() != 4:
+        raise SFError("q must be [B, n_heads, head_dim] or [B, rows, n_heads, head_dim]")
+    _lib.require_device(q, "q")
+    B, H, D = q.shape[0], q.shape[-2], q.shape[-1]
+    Tq = 1 if three else q.shape[1]
+    if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+        raise SFError("k_codes / v_codes must both be [B, n_kv_heads, T, head_dim]")
+    KVH, T_cap = k_codes.shape[1], k_codes.shape[2]
+    if k_codes.shape[0] != B or k_codes.shape[3] != D:
+        raise SFError("cache shape does not match q")
+    if D > _MAX_HEAD_DIM:
+        raise ValueError(f"head_dim={D} exceeds kernel's compile-time max {_MAX_HEAD_DIM}")
+    _lib.check_cache(q.device, k_codes, k_scales, v_codes, v_scales, None, scores)
+    dev_len, T = _lib.lengths_arg(lengths, B, q.device)
+    T += add
+    T_max = T_cap if max_length is None else max_length
+    if dev_len is None:
+        if T > T_max:
+            raise SFError(f"{T} slots of a cache of {T_max}")
+        T_max = T
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+    elif out.shape != q.shape or out.device != q.device or not out.is_contiguous():
+        raise SFError("out must be contiguous, of q's shape and on its device")
+    lib = _lib.load()
+    n = n_splits or 0
+    with _lib.on_device(q):
+        st = _lib.stream(q)
+        ws = _lib.scratch(q.device, st, lib.sf_attn_scored_workspace_bytes(B, Tq, H, KVH, T_max, D, n))
+        rc = lib.sf_attn_decode_scored_i8kv(
+            q.data_ptr(), _lib.dt(q), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
+            v_scales.data_ptr(), _lib.dt(k_scales), scores.data_ptr(), out.data_ptr(), _lib.dt(out), ws.data_ptr(),
+            ws.numel(), B, Tq, H, KVH, dev_len, T, T_max, T_cap, D, D ** -0.5 if scale is None else scale, n, st)
+    if rc:
+        _lib.check(rc, "sf_attn_decode_scored_i8kv")
+    return out

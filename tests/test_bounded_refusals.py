@@ -1,0 +1,163 @@
+"""Refusals of the bounded cache's operators and of sampling, without a GPU: the C entry
+points check shapes, types, pointers and workspaces before any launch, the Python ones
+devices and shapes."""
+
+import pytest
+import torch
+
+from siliconfer_amd import _lib
+from siliconfer_amd._lib import SFError
+from siliconfer_amd.kernels.attention import attention_decode_scored
+from siliconfer_amd.kernels.eviction import evict
+from siliconfer_amd.kernels.rotary import rotary, rotary_kv_append
+from siliconfer_amd.kernels.sampling import sample
+
+P = 4096  # a pointer that is never followed: every call below is refused before its launch
+F32, F16, BF16 = _lib.SF_F32, _lib.SF_F16, _lib.SF_BF16
+
+
+def refused(rc, code, text):
+    assert rc == code and text in _lib.last_error(), (rc, _lib.last_error())
+
+
+def rot(**kw):
+    a = dict(q=P, q_out=P, k=P, k_out=P, dtype=F32, positions=P, pos_i64=0, pos_per_seq=1, inv_freq=P, pairs=32,
+             scale=1.0, interleaved=0, B=1, T=1, H=14, KVH=2, D=64, strides=None, stream=None)
+    a.update(kw)
+    return _lib.load().sf_rotary(*a.values())
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(q=None), -1, "null pointer"), (dict(k_out=None), -1, "null pointer"), (dict(positions=None), -1, "null"),
+    (dict(inv_freq=None), -1, "null"), (dict(dtype=3), -1, "bad dtype"), (dict(pairs=0), -1, "rotated pairs"),
+    (dict(pairs=33), -1, "33 rotated pairs in a head of 64"), (dict(pairs=513, D=2048), -2, "at most 512"),
+    (dict(B=-1), -1, "invalid rotary shape"), (dict(H=0), -1, "invalid rotary shape"),
+    (dict(B=1 << 16, T=1 << 16), -1, "exceed the grid"),
+])
+def test_rotary_c(kw, code, text):
+    refused(rot(**kw), code, text)
+
+
+def test_nothing_to_do_is_no_error():
+    assert rot(T=0) == 0 and rot(B=0, q=None) == 0
+    assert append(T=0) == 0
+    assert samp(B=0, logits=None) == 0
+
+
+def append(**kw):
+    a = dict(qkv=P, in_dtype=F32, positions=P, pos_i64=0, pos_per_seq=1, inv_freq=P, pairs=32, scale=1.0,
+             interleaved=0, q_out=P, q_dtype=F32, k_codes=P, k_scales=P, v_codes=P, v_scales=P, scale_dtype=F16,
+             slots=None, scores=None, lengths=None, start=0, B=1, T=1, H=14, KVH=2, D=64, T_cap=128, stream=None)
+    a.update(kw)
+    return _lib.load().sf_rotary_kv_append(*a.values())
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(start=128), -1, "KV cache overflow: 128 + 1 > capacity 128"), (dict(start=-1), -1, "overflow"),
+    (dict(start=2 ** 31 - 1, T=2), -1, "overflow"),
+    (dict(H=13), -1, "not a multiple"), (dict(KVH=0), -1, "not a multiple"), (dict(D=66), -2, "D % 8 == 0"),
+    (dict(D=264), -2, "D <= 256"), (dict(scale_dtype=BF16), -1, "bad scale dtype"), (dict(q_dtype=9), -1, "bad input"),
+    (dict(v_scales=None), -1, "null"), (dict(B=1 << 20, T=1 << 10, lengths=P), -1, "exceed the grid"),
+])
+def test_append_c(kw, code, text):
+    refused(append(**kw), code, text)
+
+
+def scored(**kw):
+    a = dict(q=P, q_dtype=F32, k_codes=P, k_scales=P, v_codes=P, v_scales=P, scale_dtype=F16, scores=P, out=P,
+             out_dtype=F32, ws=P, ws_bytes=1 << 40, B=1, Tq=1, H=14, KVH=2, lengths=None, T=100, T_max=100, T_cap=128,
+             D=64, scale=0.125, n_splits=0, stream=None)
+    a.update(kw)
+    return _lib.load().sf_attn_decode_scored_i8kv(*a.values())
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(T=101), -1, "invalid attention shape"), (dict(T=-1), -1, "invalid attention shape"),
+    (dict(T_max=129), -1, "invalid attention shape"), (dict(lengths=P, T_max=-1), -1, "invalid attention shape"),
+    (dict(B=0), -1, "invalid attention shape"), (dict(Tq=0), -1, "invalid attention shape"),
+    (dict(H=15), -1, "not a multiple"), (dict(D=264), -1, "exceeds kernel's compile-time max 256"),
+    (dict(D=60), -2, "multiple of 8"), (dict(Tq=33), -2, "at most 32"), (dict(H=258), -2, "at most 128"),
+    (dict(scale_dtype=BF16), -1, "bad scale dtype"), (dict(q_dtype=-1), -1, "bad q/out dtype"),
+    (dict(scores=None), -1, "null"), (dict(k_codes=P + 4), -1, "8-byte aligned"), (dict(q=P + 8), -1, "16-byte"),
+    (dict(ws=None), -1, "workspace"), (dict(ws=P + 16), -1, "256-byte aligned"), (dict(ws_bytes=100), -1, "too small"),
+    (dict(B=70000), -1, "exceed the grid"),
+])
+def test_scored_c(kw, code, text):
+    refused(scored(**kw), code, text)
+
+
+def ev(**kw):
+    a = dict(k_codes=P, k_scales=P, v_codes=P, v_scales=P, scale_dtype=F16, scores=P, positions=P, lengths=None, T=100,
+             seen=None, seen_host=200, budget=50, recent=10, out=P, ws=P, ws_bytes=1 << 40, B=1, KVH=2, T_cap=128,
+             D=64, stream=None)
+    a.update(kw)
+    return _lib.load().sf_kv_evict(*a.values())
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(T=129), -1, "129 slots of a capacity of 128"), (dict(T=-1), -1, "slots of a capacity"),
+    (dict(budget=0, recent=0), -1, "budget > 0"), (dict(recent=51), -1, "recent <= budget"),
+    (dict(recent=-1), -1, "0 <= recent"), (dict(D=12), -2, "D % 8 == 0"), (dict(T_cap=1 << 21), -2, "at most 2097151"),
+    (dict(KVH=70000), -1, "exceed the grid"), (dict(positions=None), -1, "null"), (dict(out=None), -1, "null"),
+    (dict(v_codes=P + 1), -1, "8-byte aligned"), (dict(ws=None), -1, "16-byte aligned"),
+    (dict(ws_bytes=8), -1, "too small"), (dict(lengths=P, out=P), -1, "lengths_out must not be lengths"),
+])
+def test_evict_c(kw, code, text):
+    refused(ev(**kw), code, text)
+
+
+def samp(**kw):
+    a = dict(logits=P, dtype=F32, stride=1000, B=2, V=1000, u=P, t=1.0, k=0, p=1.0, m=0.0, ts=None, ks=None, ps=None,
+             ms=None, tokens=P, lp=None, ws=P, ws_bytes=1 << 40, stream=None)
+    a.update(kw)
+    return _lib.load().sf_sample(*a.values())
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(V=0), -1, "invalid sampling shape"), (dict(B=-1), -1, "invalid sampling shape"),
+    (dict(V=(1 << 24) + 1), -2, "at most 16777216"), (dict(dtype=3), -1, "bad dtype"), (dict(stride=-1), -1, "row stride"),
+    (dict(t=float("nan")), -1, "temperature"), (dict(k=-1), -1, "top_k >= 0"), (dict(p=0.0), -1, "top_p > 0"),
+    (dict(p=float("nan")), -1, "top_p > 0"), (dict(m=1.5), -1, "min_p <= 1"), (dict(m=-0.1), -1, "0 <= min_p"),
+    (dict(u=None), -1, "null"), (dict(tokens=None), -1, "null"),
+])
+def test_sample_c(kw, code, text):
+    refused(samp(**kw), code, text)
+
+
+def test_workspace_sizes():
+    lib = _lib.load()
+    assert lib.sf_attn_scored_workspace_bytes(1, 1, 14, 3, 100, 64, 0) == 0  # 14 heads over 3
+    one = lib.sf_attn_scored_workspace_bytes(1, 1, 14, 2, 1000, 64, 4)
+    assert one >= 14 * (4 * 64 + 4 * 2 + 1000) * 4
+    assert lib.sf_attn_scored_workspace_bytes(64, 32, 128, 8, 131072, 128, 0) > 2 ** 32
+    assert lib.sf_kv_evict_workspace_bytes(2, 4, 100, 300) >= 2 * 4 * (4 + 100 * 8)
+    assert lib.sf_kv_evict_workspace_bytes(2, 4, 300, 100) > 0
+
+
+def test_python_layers_refuse_host_tensors_and_shapes():
+    q, f, pos = torch.zeros(1, 1, 2, 64), torch.zeros(32, dtype=torch.float64), torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(SFError, match="device tensor"):
+        rotary(q, None, pos, f)
+    kc, ks = torch.zeros(1, 1, 8, 64, dtype=torch.int8), torch.zeros(1, 1, 8)
+    with pytest.raises(SFError, match="device tensor"):
+        rotary_kv_append(torch.zeros(1, 1, 256), pos, f, kc, ks, kc, ks, n_heads=2, lengths=0)
+    with pytest.raises(SFError, match="device tensor"):
+        attention_decode_scored(torch.zeros(1, 2, 64), kc, ks, kc, ks, ks, lengths=3)
+    with pytest.raises(SFError, match="device tensor"):
+        evict(kc, ks, kc, ks, ks, ks.int(), 8, 8, 4)
+    with pytest.raises(SFError, match="device tensor"):
+        sample(torch.zeros(2, 10), torch.zeros(2))
+
+
+def test_cache_checks():
+    c, s, i = torch.zeros(1, 2, 8, 64, dtype=torch.int8), torch.zeros(1, 2, 8), torch.zeros(1, 2, 8, dtype=torch.int32)
+    cpu = torch.device("cpu")
+    _lib.check_cache(cpu, c, s, c, s, i, s)
+    for bad in ((c.short(), s, c, s, i, s), (c, s.half(), c, s, i, s), (c, s.bfloat16(), c, s.bfloat16(), i, s),
+                (c, s, c, s, i.long(), s), (c, s, c, s, i, s.double()), (c, s[:, :, :7], c, s, i, s),
+                (c, s.unsqueeze(-1), c, s, i, s), (c.transpose(2, 3), s, c, s, i, s)):
+        with pytest.raises(SFError):
+            _lib.check_cache(cpu, *bad)
+    for bad in (-1, 2 ** 31, torch.zeros(2), torch.zeros(3, dtype=torch.int32)):
+        with pytest.raises(SFError):
+            _lib.lengths_arg(bad, 2, cpu)
