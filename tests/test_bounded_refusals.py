@@ -118,7 +118,8 @@ def samp(**kw):
     (dict(V=(1 << 24) + 1), -2, "at most 16777216"), (dict(dtype=3), -1, "bad dtype"), (dict(stride=-1), -1, "row stride"),
     (dict(t=float("nan")), -1, "temperature"), (dict(k=-1), -1, "top_k >= 0"), (dict(p=0.0), -1, "top_p > 0"),
     (dict(p=float("nan")), -1, "top_p > 0"), (dict(m=1.5), -1, "min_p <= 1"), (dict(m=-0.1), -1, "0 <= min_p"),
-    (dict(u=None), -1, "null"), (dict(tokens=None), -1, "null"),
+    (dict(u=None), -1, "null"), (dict(tokens=None), -1, "null"), (dict(ws=None), -1, "256-byte aligned"),
+    (dict(ws_bytes=100), -1, "too small"), (dict(B=1 << 30, V=1 << 20), -1, "exceed the grid"),
 ])
 def test_sample_c(kw, code, text):
     refused(samp(**kw), code, text)
@@ -132,6 +133,7 @@ def test_workspace_sizes():
     assert lib.sf_attn_scored_workspace_bytes(64, 32, 128, 8, 131072, 128, 0) > 2 ** 32
     assert lib.sf_kv_evict_workspace_bytes(2, 4, 100, 300) >= 2 * 4 * (4 + 100 * 8)
     assert lib.sf_kv_evict_workspace_bytes(2, 4, 300, 100) > 0
+    assert lib.sf_sample_workspace_bytes(3, 0) == 0 and lib.sf_sample_workspace_bytes(3, 100) > 0
 
 
 def test_python_layers_refuse_host_tensors_and_shapes():
