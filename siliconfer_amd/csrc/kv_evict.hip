@@ -10,11 +10,16 @@
 // and destinations are apart, every copy is independent of the others, and the
 // least is moved.
 //
-// k_evict_select: one workgroup a (sequence, kv head). The threshold t is the
-// largest key that `budget` slots reach, found two bits at a time from the top
-// (three counts a step, packed in one 64-bit sum: no atomics). Then t's ties by
-// ascending slot and the (hole, donor) list by ballots over the waves' segments.
-// k_evict_move copies the list's pairs: codes, scales, scores, positions.
+// k_evict_select: one workgroup a (sequence, kv head), the keys in its registers. The
+// threshold t is the largest key that `budget` slots reach: radix selection, 11 + 11 + 10
+// bits, each a histogram of counts in LDS (integer atomics: their order changes nothing)
+// and a scan of it from the top; the newest tokens' slots are counted by ballots and left
+// out of it. Then the (hole, donor) list by ballots over the waves' segments. Few moves
+// are made by the same workgroup, many by a second launch over every CU.
+// Bound by the latency of its dozen barriers and of one read of scores and positions:
+// 9.0 us for 2 heads of 1088 slots, moves among them, 14.2 + 7.5 for 32 heads of up to 8191
+// cut to 2048 (a search of the threshold bit pair by bit pair with counts over the
+// workgroup, keys in registers: 13.4 + 4.0 and 88 + 6.6; keys read again each time: 25 and 71).
 #include "sf_common.h"
 
 namespace {
@@ -33,19 +38,6 @@ __device__ __forceinline__ uint32_t evict_key(float score, int position, long lo
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum over the workgroup; every thread gets it. `red` holds one value a wave.
-__device__ __forceinline__ unsigned long long block_sum(unsigned long long v, unsigned long long *red) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  __syncthreads();  // the previous sum has been read
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  unsigned long long s = 0;
-#pragma unroll
-  for (int w = 0; w < kSelWaves; ++w) s += red[w];
-  return s;
-}
-
 // The sum of v over the waves before this one, and over all of them.
 __device__ __forceinline__ int waves_before(int v, int *cnt, int *total) {
   __syncthreads();
@@ -61,111 +53,216 @@ __device__ __forceinline__ int waves_before(int v, int *cnt, int *total) {
   return before;
 }
 
-__global__ void __launch_bounds__(kSelThreads)
-k_evict_select(const float *__restrict__ scores, const int *__restrict__ positions,
-               const int *__restrict__ lengths, int T, const int *__restrict__ seen, int seen_host, int budget,
-               int recent, int *__restrict__ lengths_out, int *__restrict__ counts, int2 *__restrict__ pairs,
-               int max_moves, int KVH, int T_cap) {
-  __shared__ unsigned long long red[kSelWaves];
-  __shared__ int cnt[kSelWaves];
-  const int h = blockIdx.x, b = blockIdx.y, bh = b * KVH + h;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = max(0, min(lengths ? lengths[b] : T, T_cap));
-  if (h == 0 && threadIdx.x == 0) lengths_out[b] = min(n, budget);
-  if (n <= budget) {
-    if (threadIdx.x == 0) counts[bh] = 0;
-    return;
+struct EvictArgs {
+  int8_t *kc, *vc;
+  void *ks, *vs;
+  float *scores;
+  int *positions;
+  const int *lengths, *seen;
+  int *lengths_out, *counts;
+  int2 *pairs;
+  int T, seen_host, budget, recent, max_moves, KVH, T_cap, D;
+  int wide, scale_bytes;  // 16-byte pieces of codes, else 8; 2 or 4
+  int moves;              // the selecting workgroup moves its pairs itself
+};
+
+// Copies a head's n pairs, items first, first + step, ...: the codes in pieces of VB bytes
+// (a pair's K, then its V), then the pairs' scales, scores and positions.
+template <int VB>
+__device__ void move_pairs(const EvictArgs &a, int bh, int n, const int2 *list, uint32_t first, uint32_t step) {
+  const uint32_t half = a.D / VB, per = 2 * half, items = (uint32_t)n * per;  // (2^20 pairs of 64 at most)
+  const size_t row0 = (size_t)bh * a.T_cap;
+#pragma unroll 4
+  for (uint32_t e = first; e < items; e += step) {
+    const uint32_t m = e / per, i = e - m * per;
+    const int2 mv = list[m];
+    int8_t *c = i < half ? a.kc : a.vc;
+    const size_t at = (size_t)(i < half ? i : i - half) * VB, to = (row0 + mv.x) * a.D + at, from = (row0 + mv.y) * a.D + at;
+    if constexpr (VB == 16) *(u32x4 *)(c + to) = *(const u32x4 *)(c + from);
+    else *(u32x2 *)(c + to) = *(const u32x2 *)(c + from);
   }
-  const long long first_recent = (long long)(seen ? seen[b] : seen_host) - recent;
-  const float *sc = scores + (size_t)bh * T_cap;
-  const int *ps = positions + (size_t)bh * T_cap;
-  auto key = [&](int i) { return evict_key(sc[i], ps[i], first_recent); };
-  uint32_t t = 0;
-  for (int shift = 30; shift >= 0; shift -= 2) {
-    const uint32_t c1 = t | (1u << shift), c2 = t | (2u << shift), c3 = t | (3u << shift);
-    unsigned long long c = 0;  // three counts of 21 bits
-    for (int i = threadIdx.x; i < n; i += kSelThreads) {
-      const uint32_t k = key(i);
-      c += (k >= c1 ? 1ull : 0ull) | (k >= c2 ? 1ull << 21 : 0ull) | (k >= c3 ? 1ull << 42 : 0ull);
+  for (uint32_t m = first; m < (uint32_t)n; m += step) {
+    const size_t to = row0 + list[m].x, from = row0 + list[m].y;
+    if (a.scale_bytes == 2) {
+      const uint16_t k = ((const uint16_t *)a.ks)[from], v = ((const uint16_t *)a.vs)[from];
+      ((uint16_t *)a.ks)[to] = k;
+      ((uint16_t *)a.vs)[to] = v;
+    } else {
+      const uint32_t k = ((const uint32_t *)a.ks)[from], v = ((const uint32_t *)a.vs)[from];
+      ((uint32_t *)a.ks)[to] = k;
+      ((uint32_t *)a.vs)[to] = v;
     }
-    c = block_sum(c, red);
-    const int n1 = (int)(c & 0x1fffff), n2 = (int)(c >> 21 & 0x1fffff), n3 = (int)(c >> 42);
-    t = n3 >= budget ? c3 : n2 >= budget ? c2 : n1 >= budget ? c1 : t;
-  }
-  // ties of t that stay: the first `stay` of them by slot
-  const int per = ((n + kSelWaves - 1) / kSelWaves + 63) & ~63;  // a wave's slots
-  const int lo = min(wave * per, n), hi = min(lo + per, n);
-  int above = 0, ties = 0;
-  for (int i0 = lo; i0 < hi; i0 += 64) {
-    const uint32_t k = i0 + lane < hi ? key(i0 + lane) : 0;
-    const bool in = i0 + lane < hi;
-    above += __popcll(__ballot(in && k > t));
-    ties += __popcll(__ballot(in && k == t));
-  }
-  int n_above, n_ties;
-  waves_before(above, cnt, &n_above);
-  const int tie0 = waves_before(ties, cnt, &n_ties), stay = budget - n_above;
-  int first[2], total[2];
-  for (int pass = 0; pass < 2; ++pass) {  // count the wave's holes and donors, then list them
-    int seen_ties = tie0, holes = 0, donors = 0;
-    for (int i0 = lo; i0 < hi; i0 += 64) {
-      const int i = i0 + lane;
-      const bool in = i < hi;
-      const uint32_t k = in ? key(i) : 0;
-      const unsigned long long below = (1ull << lane) - 1, tie = __ballot(in && k == t);
-      const bool kept = in && (k > t || (k == t && seen_ties + __popcll(tie & below) < stay));
-      const unsigned long long hole = __ballot(in && !kept && i < budget), donor = __ballot(kept && i >= budget);
-      if (pass) {
-        const int at = first[0] + holes + __popcll(hole & below), from = first[1] + donors + __popcll(donor & below);
-        int2 *list = pairs + (size_t)bh * max_moves;
-        if (hole >> lane & 1) list[at].x = i;
-        if (donor >> lane & 1) list[from].y = i;
-      }
-      seen_ties += __popcll(tie);
-      holes += __popcll(hole);
-      donors += __popcll(donor);
-    }
-    if (!pass) {
-      first[0] = waves_before(holes, cnt, &total[0]);
-      first[1] = waves_before(donors, cnt, &total[1]);
-      if (threadIdx.x == 0) counts[bh] = total[0];
-    }
+    const float f = a.scores[from];
+    const int p = a.positions[from];
+    a.scores[to] = f;
+    a.positions[to] = p;
   }
 }
 
-// VB bytes a thread (16 or 8): D / VB threads move one pair's K codes, as many its V
-// codes, and one thread its scales, score and position.
-template <int VB, int SB>
-__global__ void __launch_bounds__(kMoveThreads)
-k_evict_move(int8_t *__restrict__ kc, void *__restrict__ ks, int8_t *__restrict__ vc, void *__restrict__ vs,
-             float *__restrict__ scores, int *__restrict__ positions, const int *__restrict__ counts,
-             const int2 *__restrict__ pairs, int max_moves, int KVH, int T_cap, int D) {
-  const int bh = blockIdx.z * KVH + blockIdx.y;
-  const int n = counts[bh], per = 2 * (D / VB) + 1;
-  const int2 *list = pairs + (size_t)bh * max_moves;
-  const size_t row0 = (size_t)bh * T_cap;
-  const long long items = (long long)n * per;
-  for (long long e = (long long)blockIdx.x * kMoveThreads + threadIdx.x; e < items;
-       e += (long long)gridDim.x * kMoveThreads) {
-    const int m = (int)(e / per), i = (int)(e - (long long)m * per);
-    const size_t to = row0 + list[m].x, from = row0 + list[m].y;
-    if (i < per - 1) {
-      int8_t *c = i < D / VB ? kc : vc;
-      const size_t at = (size_t)(i < D / VB ? i : i - D / VB) * VB;
-      if constexpr (VB == 16) *(u32x4 *)(c + to * D + at) = *(const u32x4 *)(c + from * D + at);
-      else *(u32x2 *)(c + to * D + at) = *(const u32x2 *)(c + from * D + at);
-    } else {
-      if constexpr (SB == 2) {
-        ((uint16_t *)ks)[to] = ((const uint16_t *)ks)[from];
-        ((uint16_t *)vs)[to] = ((const uint16_t *)vs)[from];
+// KEYS: keys held in LDS (0: read again from memory on every pass; held in registers, 32 a
+// thread, the unrolled passes outgrew the instruction cache: 24 us where LDS takes 14.2).
+// Wave w has the slots from w 64 steps on, step r's lane l slot w 64 steps + 64 r + l,
+// so that an ascending order over slots is one over (wave, r, lane).
+template <int KEYS>
+__global__ void __launch_bounds__(kSelThreads)
+k_evict_select(EvictArgs a) {
+  constexpr int kDigits = 2048;
+  __shared__ uint32_t keys[KEYS ? KEYS : 1];
+  __shared__ int hist[kDigits];
+  __shared__ int cnt[kSelWaves];
+  __shared__ int found[3];
+  const int h = blockIdx.x, b = blockIdx.y, bh = b * a.KVH + h, budget = a.budget;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = max(0, min(a.lengths ? a.lengths[b] : a.T, a.T_cap));
+  if (h == 0 && threadIdx.x == 0) a.lengths_out[b] = min(n, budget);
+  if (n <= budget) {
+    if (threadIdx.x == 0) a.counts[bh] = 0;
+    return;
+  }
+  const long long first_recent = (long long)(a.seen ? a.seen[b] : a.seen_host) - a.recent;
+  const float *sc = a.scores + (size_t)bh * a.T_cap;
+  const int *ps = a.positions + (size_t)bh * a.T_cap;
+  const int steps = (n + kSelThreads - 1) / kSelThreads;
+  const int lo = min(wave * 64 * steps, n), hi = min(lo + 64 * steps, n);
+  constexpr int U = 4;  // steps whose loads fly together
+  // each(f): f(the step's first slot, in range?, key) over the wave's slots in order
+  auto each = [&](auto f) {
+    for (int i0 = lo; i0 < hi; i0 += 64 * U) {
+      uint32_t k[U];
+      if constexpr (KEYS != 0) {  // (a wave reads only what it wrote itself)
+#pragma unroll
+        for (int u = 0; u < U; ++u) k[u] = keys[min(i0 + 64 * u + lane, n - 1)];
       } else {
-        ((uint32_t *)ks)[to] = ((const uint32_t *)ks)[from];
-        ((uint32_t *)vs)[to] = ((const uint32_t *)vs)[from];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = min(i0 + 64 * u + lane, n - 1);
+          k[u] = evict_key(sc[i], ps[i], first_recent);
+        }
       }
-      scores[to] = scores[from];
-      positions[to] = positions[from];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + 64 * u < hi) f(i0 + 64 * u, i0 + 64 * u + lane < hi, k[u]);
+    }
+  };
+  // the newest tokens counted, the others' highest digits into the histogram
+  hist[threadIdx.x] = 0;
+  hist[threadIdx.x + kSelThreads] = 0;
+  __syncthreads();
+  int newest = 0, n_newest;
+  for (int i0 = lo; i0 < hi; i0 += 64 * U) {
+    float f[U];
+    int p[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + 64 * u + lane, n - 1);
+      f[u] = sc[i];
+      p[u] = ps[i];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 64 * u + lane;
+      const uint32_t k = evict_key(f[u], p[u], first_recent);
+      if (KEYS != 0 && i < hi) keys[KEYS ? i : 0] = k;
+      newest += __popcll(__ballot(i < hi && k == kProtected));
+      if (i < hi && k != kProtected) atomicAdd(&hist[k >> 21], 1);
     }
   }
+  waves_before(newest, cnt, &n_newest);  // (a barrier: the histogram is whole)
+  // t: the key of the last slot that stays; `stay` of its ties do
+  uint32_t t = kProtected;
+  int stay = budget, n_ties = n_newest;
+  if (n_newest < budget) {
+    uint32_t prefix = 0, mask = 0;
+    stay = budget - n_newest;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t digits = pass == 2 ? 1023u : 2047u;
+      if (pass) {
+        hist[threadIdx.x] = 0;
+        hist[threadIdx.x + kSelThreads] = 0;
+        __syncthreads();
+        each([&](int, bool in, uint32_t k) {
+          if (in && k != kProtected && (k & mask) == prefix) atomicAdd(&hist[k >> shift & digits], 1);
+        });
+        __syncthreads();
+      }
+      // thread i: digits 2047 - 2 i and 2046 - 2 i
+      const int2 own = ((const int2 *)hist)[kSelThreads - 1 - threadIdx.x];
+      int run = own.x + own.y;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int v = __shfl_up(run, off, 64);
+        if (lane >= off) run += v;
+      }
+      int all;
+      run += waves_before(__shfl(run, 63, 64), cnt, &all);
+      const int before = run - own.x - own.y;
+      if (before < stay && stay <= run) {
+        const bool high = stay <= before + own.y;
+        found[0] = 2047 - 2 * (int)threadIdx.x - !high;
+        found[1] = high ? before : before + own.y;
+        found[2] = high ? own.y : own.x;
+      }
+      __syncthreads();
+      prefix |= (uint32_t)found[0] << shift;
+      mask |= digits << shift;
+      stay -= found[1];
+      n_ties = found[2];
+    }
+    t = prefix;
+  }
+  const unsigned long long below = (1ull << lane) - 1;
+  int tie0 = 0;
+  const bool all_ties = n_ties == stay;  // (distinct scores: no ranks to find)
+  if (!all_ties) {
+    int ties = 0, total;
+    each([&](int, bool in, uint32_t k) { ties += __popcll(__ballot(in && k == t)); });
+    tie0 = waves_before(ties, cnt, &total);
+  }
+  // the wave's holes and donors, counted, then listed
+  int seen_ties = tie0, holes = 0, donors = 0;
+  auto sort_out = [&](int i0, bool in, uint32_t k, unsigned long long *hole, unsigned long long *donor) {
+    bool stays = in && k >= t;
+    if (!all_ties) {
+      const unsigned long long tie = __ballot(in && k == t);
+      stays = in && (k > t || (k == t && seen_ties + __popcll(tie & below) < stay));
+      seen_ties += __popcll(tie);
+    }
+    *hole = __ballot(in && !stays && i0 + lane < budget);
+    *donor = __ballot(stays && i0 + lane >= budget);
+  };
+  each([&](int i0, bool in, uint32_t k) {
+    unsigned long long hole, donor;
+    sort_out(i0, in, k, &hole, &donor);
+    holes += __popcll(hole);
+    donors += __popcll(donor);
+  });
+  int n_holes, n_donors;
+  int at = waves_before(holes, cnt, &n_holes), from = waves_before(donors, cnt, &n_donors);
+  if (threadIdx.x == 0) a.counts[bh] = n_holes;
+  seen_ties = tie0;
+  int2 *list = a.pairs + (size_t)bh * a.max_moves;
+  each([&](int i0, bool in, uint32_t k) {
+    unsigned long long hole, donor;
+    sort_out(i0, in, k, &hole, &donor);
+    if (hole >> lane & 1) list[at + __popcll(hole & below)].x = i0 + lane;
+    if (donor >> lane & 1) list[from + __popcll(donor & below)].y = i0 + lane;
+    at += __popcll(hole);
+    from += __popcll(donor);
+  });
+  if (a.moves) {
+    __syncthreads();
+    if (a.wide) move_pairs<16>(a, bh, n_holes, list, threadIdx.x, kSelThreads);
+    else move_pairs<8>(a, bh, n_holes, list, threadIdx.x, kSelThreads);
+  }
+}
+
+__global__ void __launch_bounds__(kMoveThreads) k_evict_move(EvictArgs a) {
+  const int bh = blockIdx.z * a.KVH + blockIdx.y;
+  const int2 *list = a.pairs + (size_t)bh * a.max_moves;
+  const long long first = (long long)blockIdx.x * kMoveThreads + threadIdx.x, step = (long long)gridDim.x * kMoveThreads;
+  if (a.wide) move_pairs<16>(a, bh, a.counts[bh], list, first, step);
+  else move_pairs<8>(a, bh, a.counts[bh], list, first, step);
 }
 
 }  // namespace
@@ -208,24 +305,20 @@ extern "C" int sf_kv_evict(int8_t *k_codes, void *k_scales, int8_t *v_codes, voi
   int *counts = (int *)workspace;
   int2 *pairs = (int2 *)((char *)workspace + sf_align256((size_t)B * KVH * sizeof(int)));
   hipStream_t st = (hipStream_t)stream;
-  k_evict_select<<<dim3(KVH, B), kSelThreads, 0, st>>>(scores, positions, lengths, T, seen, seen_host, budget,
-                                                      recent, lengths_out, counts, pairs, most, KVH, T_cap);
-  if (most) {
-    const bool wide = D % 16 == 0 && (((uintptr_t)k_codes | (uintptr_t)v_codes) & 15) == 0;
-    const long long items = (long long)most * (2 * (D / (wide ? 16 : 8)) + 1);
-    const long long blocks = (items + kMoveThreads - 1) / kMoveThreads;
-    const dim3 grid((unsigned)(blocks < 64 ? blocks : 64), KVH, B);
-#define SF_MOVE(VB, SB)                                                                                     \
-  k_evict_move<VB, SB><<<grid, kMoveThreads, 0, st>>>(k_codes, k_scales, v_codes, v_scales, scores, positions, \
-                                                      counts, pairs, most, KVH, T_cap, D)
-    if (wide) {
-      if (scale_dtype == SF_F16) SF_MOVE(16, 2);
-      else SF_MOVE(16, 4);
-    } else {
-      if (scale_dtype == SF_F16) SF_MOVE(8, 2);
-      else SF_MOVE(8, 4);
-    }
-#undef SF_MOVE
+  const int wide = D % 16 == 0 && (((uintptr_t)k_codes | (uintptr_t)v_codes) & 15) == 0;
+  // up to 64 KB a head: moved by the selecting workgroup (measured {RULE})
+  const int moves = (long long)most * (2 * D + 12) <= 64 << 10;
+  const EvictArgs a = {k_codes, v_codes, k_scales, v_scales, scores, positions, lengths, seen, lengths_out, counts,
+                       pairs, T, seen_host, budget, recent, most, KVH, T_cap, D, wide,
+                       scale_dtype == SF_F16 ? 2 : 4, moves};
+  const dim3 heads(KVH, B);
+  if (T_max <= 2048) k_evict_select<2048><<<heads, kSelThreads, 0, st>>>(a);
+  else if (T_max <= 12288) k_evict_select<12288><<<heads, kSelThreads, 0, st>>>(a);
+  else if (T_max <= 32768) k_evict_select<32768><<<heads, kSelThreads, 0, st>>>(a);
+  else k_evict_select<0><<<heads, kSelThreads, 0, st>>>(a);
+  if (most && !moves) {
+    const long long blocks = ((long long)most * (2 * (D / (wide ? 16 : 8)) + 1) + kMoveThreads - 1) / kMoveThreads;
+    k_evict_move<<<dim3((unsigned)(blocks < 64 ? blocks : 64), KVH, B), kMoveThreads, 0, st>>>(a);
   }
   return sf_check_launch("sf_kv_evict");
 }
