@@ -73,7 +73,6 @@ constexpr int kRotTable = 1024;  // cos / sin pairs of a workgroup's rows
 // How a workgroup's work is cut: `rows` rows of `items` items, `per` a head.
 struct RotaryCut {
   int rows, items, per, n_rows;
-  int stream;                   // past the caches: outputs that the L2s could not hold
   uint32_t inv_items, inv_per;  // ceil(2^32 / .), exact below 2^16 items; 0 stands for a division by 1
 };
 __device__ __forceinline__ int div_by(int e, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)e, inv) : e; }
@@ -118,13 +117,14 @@ struct Vec {
 // turn with them), loaded before the workgroup computes its cos / sin table. Else an item
 // is one pair, or one dim past the rotated part. Bound by the memory stream; rows of a
 // workgroup share nothing, several are taken together only to fill its threads.
-// 8191 rows of 32 / 8 heads of 128, bf16 (168 MB): single dims and the library's sincos 88 us,
-// this 29.8 (5.6 TB/s; a plain 1 GiB copy reaches 5.1).
+// 8191 rows of 32 / 8 heads of 128, bf16 (168 MB), us a call in a row of them: single dims and
+// the library's sincos 90, this 34.7 (a 1 GiB copy's rate would take 33). Two, four items a thread
+// take 38.2, 40.1, and stores past the caches end the kernel sooner, but not the call.
 template <int DT, bool VEC, bool INTER>
 __global__ void __launch_bounds__(kRotThreads)
 k_rotary(RotaryRows q, RotaryRows k, RotaryPos pos, const double *__restrict__ inv_freq, int P, float scale, int T,
          int D, RotaryCut cut) {
-  constexpr int E = Vec<DT>::E, kItems = 4;  // a thread's items per round
+  constexpr int E = Vec<DT>::E, kItems = 1;  // a thread's items per round
   __shared__ float2_t cs[kRotTable];
   const int row0 = blockIdx.x * cut.rows, rows = min(cut.rows, cut.n_rows - row0);
   const int n = rows * cut.items, turned = VEC ? (INTER ? 2 * P / E : P / E) : P;
@@ -141,10 +141,6 @@ k_rotary(RotaryRows q, RotaryRows k, RotaryPos pos, const double *__restrict__ i
     const int h = hh < q.heads ? hh : hh - q.heads;
     return Item{x.in, x.out, (size_t)(b * x.ib + t * x.it + h * x.ih), (size_t)(b * x.ob + t * x.ot + h * x.oh),
                 eh - hh * cut.per, r * P};
-  };
-  auto put = [&](char *o, u32x4 w) {
-    if (cut.stream) __builtin_nontemporal_store(w, (u32x4 *)o);
-    else *(u32x4 *)o = w;
   };
   bool have_cs = false;
   for (int e0 = threadIdx.x; e0 - (int)threadIdx.x < n; e0 += kItems * kRotThreads) {
@@ -196,11 +192,11 @@ k_rotary(RotaryRows q, RotaryRows k, RotaryPos pos, const double *__restrict__ i
               a.v[j] = y.x;
               c.v[j] = y.y;
             }
-            put(o + P * sz, c.pack());
+            *(u32x4 *)(o + P * sz) = c.pack();
           }
           lo[u] = a.pack();
         }
-        put(o, lo[u]);
+        *(u32x4 *)o = lo[u];
       } else {
         const Item x = item(e);
         if (x.i < P) {
@@ -328,11 +324,8 @@ extern "C" int sf_rotary(const void *q, void *q_out, const void *k, void *k_out,
   SF_REQUIRE((long long)(H + KVH) * cut.per < 65536, SF_EUNSUPPORTED, "%d heads of %d dims a row: too wide", H + KVH, D);
   cut.items = (H + KVH) * cut.per;
   cut.n_rows = B * T;
-  // 168 MB in and out: 37.2 us with ordinary stores, 29.8 past the caches; what the
-  // eight 4 MB L2s can hold stays there for the next launch
-  cut.stream = (long long)cut.n_rows * (H + KVH) * D * (16 / E) > 32ll << 20;
-  // rows a workgroup: four items a thread, while that leaves two workgroups a CU
-  int rows = 4 * kRotThreads / cut.items;
+  // rows a workgroup: one item a thread, while that leaves two workgroups a CU
+  int rows = kRotThreads / cut.items;
   if (rows > cut.n_rows / 512) rows = cut.n_rows / 512;
   if (rows > kRotTable / rot_pairs) rows = kRotTable / rot_pairs;
   if (rows > 65535 / cut.items) rows = 65535 / cut.items;
