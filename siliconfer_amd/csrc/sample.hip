@@ -11,24 +11,25 @@
 // with no logit above -inf gives token -1 (log probability -inf); a logit of +inf
 // weighs 1 and every finite one beside it 0.
 //
-// Bins: the logits' axis is cut at the multiples of T kDelta, the same places for
-// every part of a row whatever its maximum. A weight is held relative to its bin's
-// upper edge, e = exp(-kDelta (j + 1 - x / (T kDelta))), as the integer e 2^36
-// rounded: sums within a bin are exact in any order, so the counting atomics change
-// no result, and a token's share is off by at most 2^-37 of itself. Bins are joined
-// in 64-bit floats in a fixed order. Tokens 40 nats and more below the maximum (256
-// bins) weigh nothing.
+// Bins: the logits' axis is cut at the multiples of T kDelta, the same places for every
+// part of a row whatever its maximum. A weight is held relative to its bin's middle, as
+// the integer 2^36 e^y, y within kDelta / 2: sums within a bin are exact in any order, so
+// the counting atomics change no result, and a token's share is off by some 3e-10 of
+// itself. Bins are joined in 64-bit floats in a fixed order. Tokens 32 nats and more below
+// the maximum (256 bins, 1e-14 of its weight) weigh nothing.
 //
 // k_sample_bins: a workgroup a chunk of 8192 logits, held in registers: the chunk's
 // maximum, then its 256 bins' counts and weights in one 64-bit LDS atomic an element
 // (count << 50 | weight), and the list of its best elements, whole bins up to
 // kListCap of them.
-// k_sample_pick: a workgroup a row joins the chunks' bins. Each filter's end and the
-// draw lie in one bin that the bins' prefix sums name; its elements come from the
-// chunks' lists where these hold the whole bin, from the row again where not, and are
-// ordered by counting. A bin of more than kBinCap elements (dense ties, temperatures
-// that squeeze the row into few bins) is searched by radix selection over the order
-// bits instead: eight bits a pass over the row.
+// k_sample_pick: a workgroup a row joins the chunks' bins. Where the bins up to the end of
+// what the filters leave (or, without any, up to the draw) hold at most kHeadCap elements,
+// these are gathered from the chunks' lists (from the row again where a list ends before
+// them) and one wave orders them by counting and applies every rule to the ordered
+// weights. Otherwise each filter's end and the draw are looked up one after the other in
+// the one bin that the bins' prefix sums name; a bin of more than kBinCap elements (dense
+// ties, temperatures that squeeze the row into few bins) is searched by radix selection
+// over the order bits instead, eight bits a pass over the row.
 #include <math.h>
 
 #include "sf_common.h"
@@ -38,12 +39,15 @@ namespace {
 typedef unsigned long long u64;
 constexpr int kSampThreads = 1024;
 constexpr int kSampWaves = kSampThreads / 64;
+constexpr int kBinThreads = 1024;   // of the first kernel
+constexpr int kBinWaves = kBinThreads / 64;
 constexpr int kPerThread = 8;
-constexpr int kChunk = kSampThreads * kPerThread;
+constexpr int kChunk = kBinThreads * kPerThread;
 constexpr int kBins = 256;
-constexpr double kDelta = 0.15625;  // nats a bin
+constexpr double kDelta = 0.125;    // nats a bin
 constexpr int kListCap = 128;       // elements of a chunk's list
 constexpr int kBinCap = 1024;       // elements of a bin ordered by counting
+constexpr int kHeadCap = 512;       // elements of the head: eight a lane of one wave
 constexpr int kCountShift = 50;     // 8192 weights of up to 2^36 take 49 bits and a little
 constexpr u64 kWeightMask = (1ull << kCountShift) - 1;
 
@@ -71,37 +75,46 @@ struct RowParams {
 // infinite temperature from turning infinite logits into NaN.
 __device__ __forceinline__ double bins_per_logit(float T) { return fmax(1.0 / ((double)T * kDelta), 1e-300); }
 
+// x per and its part past the whole number `top` (exact) in 32 fractional bits: the sum
+// with 1.5 2^20 holds the whole part in its high word and the rest in its low word. Each
+// operation rounded on its own: shifting by whole numbers commutes with the rounding, so
+// every chunk and the row agree on a logit's bin.
+__device__ __forceinline__ u64 place_of(float x, double per, double top) {
+#pragma clang fp contract(off)
+  return (u64)__double_as_longlong(fmax((double)x * per - top, -4096.0) + 1572864.0);
+}
+__device__ __forceinline__ int whole_of(u64 place) { return (int)(place >> 32 & 0xfffff) - 0x80000; }
+// The bin number of a row's (chunk's) maximum: its own place relative to it is in [0, 1).
+__device__ __forceinline__ double top_bin(float m, double per) {
+#pragma clang fp contract(off)
+  const double f = floor((double)m * per);
+  return f + (double)whole_of(place_of(m, per, f));
+}
+
 struct Binned {
   int bin;  // below the bin of `top`; kBins and more: no weight
   u64 w;
 };
-// Where x lies below the bin number `top` (a floor in 64 bits), and its weight. exp(-kDelta
-// r) by its series about r = 1/2 to the seventh power: kDelta / 2 to the eighth over 8! is
-// 3e-14. Explicit fmas, so that every kernel gets the same bits.
-__device__ __forceinline__ Binned bin_of(float x, double per, double top) {
-  const double t = (double)x * per, j = floor(t), below = j == top ? 0.0 : top - j;
-  Binned r;
-  r.bin = below < (double)kBins ? (int)below : kBins;  // (NaN: no weight)
-  const double z = -kDelta * (j == t && isinf(t) ? -0.5 : (j - t) + 0.5);
-  double p = 1.0 / 5040;
-  p = fma(p, z, 1.0 / 720);
-  p = fma(p, z, 1.0 / 120);
-  p = fma(p, z, 1.0 / 24);
-  p = fma(p, z, 1.0 / 6);
-  p = fma(p, z, 0.5);
-  p = fma(p, z, 1.0);
-  p = fma(p, z, 1.0);
-  // exp(-kDelta / 2) 2^36 p as an integer: the low bits of its sum with 2^52
-  const double unit = 0.92484881321620482 * 68719476736.0;
-  r.w = (u64)__double_as_longlong(fma(p, unit, 4503599627370496.0)) & ((1ull << 52) - 1);
-  return r;
+// Where x lies below the bin number `top`, and its weight (plus `add`). With s / 2^32 the
+// place's distance from the bin's middle, y = kDelta s / 2^32 and 2^36 e^y = 2^36 + 2 s +
+// 2^36 (y^2 / 2 + ... + y^5 / 120), the bracket in fp32: its rounding (0.002 2^-23) and the
+// next term (y^6 / 720) are 3e-10 at most.
+__device__ __forceinline__ Binned bin_of(float x, double per, double top, u64 add = 0) {
+  static_assert(kDelta == 0.125, "2^36 kDelta s / 2^32 = 2 s");
+  const u64 v = place_of(x, per, top);
+  const int s = (int)((uint32_t)v ^ 0x80000000u);
+  const float y = (float)s * (float)(kDelta * 0x1p-32);
+  const float tail = y * y * fmaf(y, fmaf(y, fmaf(y, 0x1p36f / 120, 0x1p36f / 24), 0x1p36f / 6), 0x1p35f);
+  return Binned{-whole_of(v), (u64)((long long)s * 2 + (long long)((1ull << 36) + add)) + (uint32_t)tail};
 }
+// A row with infinite logits draws among them alone: they count as 0, all others as -inf.
+__device__ __forceinline__ float flat_value(float x) { return x == INFINITY ? 0.f : -INFINITY; }
 
 // What a chunk leaves in the workspace.
 struct ChunkOut {
-  double top;       // its maximum's bin number
+  double top;       // its maximum's bin number (inf: infinite logits)
   u64 best;         // its maximum: key << 32 | ~index
-  int list_n, pad;
+  int list_n, list_bins;  // the list's elements, the bins it has whole
   u64 bins[kBins];  // count << kCountShift | weight
   u64 list[kListCap];
 };
@@ -116,11 +129,11 @@ __device__ __forceinline__ u64 wave_max(u64 v) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kSampThreads)
+__global__ void __launch_bounds__(kBinThreads)
 k_sample_bins(const void *__restrict__ logits, long long row_stride, int V, int chunks, RowParams rp,
               ChunkOut *__restrict__ outs) {
   __shared__ u64 bins[kBins];
-  __shared__ u64 red[kSampWaves];
+  __shared__ float red[kBinWaves];
   __shared__ int list_bins, list_n;
   const int b = blockIdx.x / chunks, c = blockIdx.x - b * chunks;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -130,41 +143,57 @@ k_sample_bins(const void *__restrict__ logits, long long row_stride, int V, int 
   float x[kPerThread];
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
-    const int i = i0 + k * kSampThreads;
+    const int i = i0 + k * kBinThreads;
     x[k] = i < V ? sf_load_as_f32<DT>(logits, row + i) : -INFINITY;
   }
-  u64 best = 0;
+  const float T = rp.t(b);
+  float m = x[0];
 #pragma unroll
-  for (int k = 0; k < kPerThread; ++k) {
-    const u64 e = (u64)order_key(x[k]) << 32 | (uint32_t)~(i0 + k * kSampThreads);
-    best = e > best ? e : best;
-  }
-  best = wave_max(best);
-  if (lane == 0) red[wave] = best;
+  for (int k = 1; k < kPerThread; ++k) m = fmaxf(m, x[k]);  // (drops NaN; of NaN alone it is undone below)
+  m = sf_wave_max(m != m ? -INFINITY : m);
+  if (lane == 0) red[wave] = m;
   if (threadIdx.x < kBins) bins[threadIdx.x] = 0;
   if (threadIdx.x == 0) list_n = 0;
   __syncthreads();
-  best = red[0];
+  m = red[lane & (kBinWaves - 1)];
+  m = sf_wave_max(m);
+  if (!(T > 0.f)) {  // the largest logit's lowest index is all that counts
+    u64 best = 0;
 #pragma unroll
-  for (int w = 1; w < kSampWaves; ++w) best = red[w] > best ? red[w] : best;
-  const float T = rp.t(b), m = key_value((uint32_t)(best >> 32));
-  const bool none = (uint32_t)(best >> 32) == kNoKey || !(T > 0.f);  // nothing here to weigh
-  const double per = bins_per_logit(T), top = floor((double)m * per);
-  if (threadIdx.x == 0) {
-    o->top = top;
-    o->best = best;
+    for (int k = 0; k < kPerThread; ++k)
+      if (x[k] == m) {
+        const u64 e = (u64)order_key(m) << 32 | (uint32_t)~(i0 + k * kBinThreads);
+        best = e > best ? e : best;
+      }
+    best = wave_max(best);
+    if (lane == 0) bins[wave] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < kBinWaves; ++w) best = bins[w] > best ? bins[w] : best;
+      o->best = best ? best : (u64)kNoKey << 32;
+    }
+    return;
   }
-  if (none) {
+  if (threadIdx.x == 0) o->best = (u64)order_key(m) << 32;
+  const bool flat = m == INFINITY;
+  if (flat) {
+    m = 0.f;
+#pragma unroll
+    for (int k = 0; k < kPerThread; ++k) x[k] = flat_value(x[k]);
+  }
+  const double per = bins_per_logit(T), top = m > -INFINITY ? top_bin(m, per) : -INFINITY;
+  if (threadIdx.x == 0) o->top = flat ? INFINITY : top;
+  if (!(m > -INFINITY)) {  // nothing here to weigh
     if (threadIdx.x < kBins) o->bins[threadIdx.x] = 0;
-    if (threadIdx.x == 0) o->list_n = 0;
+    if (threadIdx.x == 0) o->list_n = 0, o->list_bins = kBins;
     return;
   }
   int bin[kPerThread];
 #pragma unroll
   for (int k = 0; k < kPerThread; ++k) {
-    const Binned e = bin_of(x[k], per, top);
-    bin[k] = x[k] > -INFINITY ? e.bin : kBins;
-    if (bin[k] < kBins) atomicAdd(&bins[bin[k]], 1ull << kCountShift | e.w);
+    const Binned e = bin_of(x[k], per, top, 1ull << kCountShift);
+    bin[k] = e.bin;  // (-inf and NaN lie past the bins)
+    if ((unsigned)bin[k] < (unsigned)kBins) atomicAdd(&bins[bin[k]], e.w);
   }
   __syncthreads();
   if (threadIdx.x < kBins) o->bins[threadIdx.x] = bins[threadIdx.x];
@@ -194,15 +223,15 @@ k_sample_bins(const void *__restrict__ logits, long long row_stride, int V, int 
   for (int k = 0; k < kPerThread; ++k)
     if (bin[k] < list_bins) {
       const int at = atomicAdd(&list_n, 1);
-      o->list[at] = (u64)order_key(x[k]) << 32 | (uint32_t)~(i0 + k * kSampThreads);
+      o->list[at] = (u64)order_key(x[k]) << 32 | (uint32_t)~(i0 + k * kBinThreads);
     }
   __syncthreads();
-  if (threadIdx.x == 0) o->list_n = list_n;
+  if (threadIdx.x == 0) o->list_n = list_n, o->list_bins = list_bins;
 }
 
-struct Found {   // a place in a bin's order: the r-th token (from 0) with this logit
+struct Found {   // a place in a bin's order: the r-th (from 0) of `ties` tokens with this logit
   uint32_t key;
-  u64 r;
+  u64 r, ties;   // (ties: of a search by count)
   u64 upto;      // weight of the bin's tokens up to and with it
   int index;     // its index, where the search knows it, else -1
 };
@@ -212,7 +241,8 @@ struct PickSmem {
   int n[kBins];       // and count
   double before[kBins + 1], fac[kBins];  // weight before the bin, exp(-kDelta i) 2^-36
   int n_before[kBins + 1];
-  u64 raw[kBinCap], el[kBinCap], run[kBinCap];
+  __attribute__((aligned(16))) u64 raw[kBinCap + 16];
+  u64 el[kBinCap], run[kBinCap];
   u64 hist[256];
   u64 red[kSampWaves];
   u64 tmp[4];
@@ -236,58 +266,89 @@ struct Row {
   const void *logits;
   size_t row;
   int V, chunks;
-  double per, top;
+  double per, top, chunk_top;  // (the top that chunks are compared with)
+  bool flat;
   const ChunkOut *outs;
   PickSmem &sm;
   int held;  // the bin whose elements lie in sm.el, in order (-1: none)
 
-  __device__ __forceinline__ float at(int i) const { return sf_load_as_f32<DT>(logits, row + i); }
-  __device__ __forceinline__ u64 weight(uint32_t key) const { return bin_of(key_value(key), per, top).w; }
-  __device__ __forceinline__ bool in(float x, int bin) const {
-    return x > -INFINITY && bin_of(x, per, top).bin == bin;
+  __device__ __forceinline__ float at(int i) const {
+    const float x = sf_load_as_f32<DT>(logits, row + i);
+    return flat ? flat_value(x) : x;
   }
-
-  // The elements of a bin of at most kBinCap into sm.el in order, running weights into sm.run.
-  __device__ void hold(int bin) {
-    if (held == bin) return;
-    held = bin;
-    const int n = sm.n[bin];
+  // f(index, logit) over the row's logits, the loads of eight in flight together
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int i0 = threadIdx.x; i0 - (int)threadIdx.x < V; i0 += 8 * kSampThreads) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = at(min(i0 + k * kSampThreads, V - 1));
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i0 + k * kSampThreads < V) f(i0 + k * kSampThreads, x[k]);
+    }
+  }
+  // The row's elements that `is` takes by their bin into sm.raw (count: sm.n_raw), up to
+  // bin `last`: from the chunks' lists where these have every bin up to it.
+  template <class Is>
+  __device__ __forceinline__ void gather(int last, Is is) {
     __syncthreads();
     if (threadIdx.x == 0) sm.n_raw = sm.uncovered = 0;
     __syncthreads();
-    // a chunk's list has the bin where its elements up to it fit the list
     for (int c = threadIdx.x >> 6; c < chunks; c += kSampWaves) {
       const ChunkOut &o = outs[c];
-      const double shift = o.top == top ? 0.0 : top - o.top;
+      const double shift = o.top == chunk_top ? 0.0 : chunk_top - o.top;
       const int ln = o.list_n, lane = threadIdx.x & 63;
-      int here = 0, listed = 0;  // the chunk's elements in the bin, and of them in its list
-      if (shift <= (double)bin) here = (int)(o.bins[bin - (int)shift] >> kCountShift);
-      for (int i = lane; i - lane < ln; i += 64) {
-        const u64 e = i < ln ? o.list[i] : 0;
-        const bool is = i < ln && in(key_value((uint32_t)(e >> 32)), bin);
-        if (is) sm.raw[atomicAdd(&sm.n_raw, 1)] = e;
-        listed += __popcll(__ballot(is));
-      }
-      if (lane == 0 && listed < here) sm.uncovered = 1;
+      const u64 e0 = lane < ln ? o.list[lane] : 0, e1 = lane + 64 < ln ? o.list[lane + 64] : 0;
+      if (!(shift <= (double)last)) continue;  // it has nothing there
+      if (last - (int)shift >= o.list_bins) sm.uncovered = 1;
+      if (lane < ln && is(bin_of(key_value((uint32_t)(e0 >> 32)), per, top).bin)) sm.raw[atomicAdd(&sm.n_raw, 1)] = e0;
+      if (lane + 64 < ln && is(bin_of(key_value((uint32_t)(e1 >> 32)), per, top).bin)) sm.raw[atomicAdd(&sm.n_raw, 1)] = e1;
     }
     __syncthreads();
     if (sm.uncovered) {
       __syncthreads();
       if (threadIdx.x == 0) sm.n_raw = 0;
       __syncthreads();
-      for (int i = threadIdx.x; i < V; i += kSampThreads) {
-        const float x = at(i);
-        if (in(x, bin)) sm.raw[atomicAdd(&sm.n_raw, 1)] = (u64)order_key(x) << 32 | (uint32_t)~i;
-      }
+      each([&](int i, float x) {
+        if (is(bin_of(x, per, top).bin)) sm.raw[atomicAdd(&sm.n_raw, 1)] = (u64)order_key(x) << 32 | (uint32_t)~i;
+      });
       __syncthreads();
     }
+  }
+
+  __device__ __forceinline__ u64 weight(uint32_t key) const { return bin_of(key_value(key), per, top).w; }
+  __device__ __forceinline__ bool in(float x, int bin) const {
+    return bin_of(x, per, top).bin == bin;
+  }
+
+  // sm.raw's n elements into sm.el in descending order, by counting the larger ones: sixteen
+  // at a time, so that their LDS reads fly together.
+  __device__ __forceinline__ void order(int n) {
+    if (threadIdx.x < 16) sm.raw[n + threadIdx.x] = 0;
+    __syncthreads();
     if ((int)threadIdx.x < n) {
       const u64 e = sm.raw[threadIdx.x];
       int rank = 0;
-      for (int i = 0; i < n; ++i) rank += sm.raw[i] > e;
+      for (int i0 = 0; i0 < n; i0 += 16) {
+        ulonglong2 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = ((const ulonglong2 *)sm.raw)[i0 / 2 + j];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rank += (v[j].x > e) + (v[j].y > e);
+      }
       sm.el[rank] = e;
     }
     __syncthreads();
+  }
+
+  // The elements of a bin of at most kBinCap into sm.el in order, running weights into sm.run.
+  __device__ __forceinline__ void hold(int bin) {
+    if (held == bin) return;
+    held = bin;
+    const int n = sm.n[bin];
+    gather(bin, [&](int at) { return at == bin; });
+    order(n);
     // running weights: a wave's scan, then the waves before it
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 run = (int)threadIdx.x < n ? weight((uint32_t)(sm.el[threadIdx.x] >> 32)) : 0;
@@ -304,7 +365,7 @@ struct Row {
   }
 
   // The bin's first token whose running count, or weight, exceeds x (the last where none does).
-  __device__ Found find(int bin, double x, bool by_count) {
+  __device__ __forceinline__ Found find(int bin, double x, bool by_count) {
     const int n = sm.n[bin];
     if (n <= kBinCap) {
       hold(bin);
@@ -313,8 +374,9 @@ struct Row {
       const int passed = (int)block_sum(t < n && !over, sm);
       const int j = min(passed, n - 1);
       const uint32_t key = (uint32_t)(sm.el[j] >> 32);
-      const u64 r = block_sum(t < j && (uint32_t)(sm.el[t] >> 32) == key, sm);
-      return Found{key, r, sm.run[j], (int)~(uint32_t)sm.el[j]};
+      const bool tie = t < n && (uint32_t)(sm.el[t] >> 32) == key;
+      const u64 c = block_sum((u64)tie << 32 | (tie && t < j), sm);
+      return Found{key, c & 0xffffffffu, c >> 32, sm.run[j], (int)~(uint32_t)sm.el[j]};
     }
     // radix selection over the order bits of the bin's elements
     const u64 all = by_count ? (u64)n : sm.w[bin];
@@ -325,14 +387,13 @@ struct Row {
       __syncthreads();
       if (threadIdx.x < 256) sm.hist[threadIdx.x] = 0;
       __syncthreads();
-      for (int i = threadIdx.x; i < V; i += kSampThreads) {
-        const float v = at(i);
+      each([&](int, float v) {
         const uint32_t k = order_key(v);
-        if ((k & mask) == prefix && v > -INFINITY) {
+        if ((k & mask) == prefix) {
           const Binned e = bin_of(v, per, top);
           if (e.bin == bin) atomicAdd(&sm.hist[k >> shift & 255], by_count ? 1ull : e.w);
         }
-      }
+      });
       __syncthreads();
       if (threadIdx.x < 64) {  // lane l: digits 255 - 4 l down to 252 - 4 l
         u64 own = 0, d[4];
@@ -366,58 +427,42 @@ struct Row {
       above = sm.tmp[1];
     }
     const u64 w = weight(prefix), r = by_count ? target - above : (target - above) / w;
-    u64 upto = above + (r + 1) * w;
+    u64 upto = above + (r + 1) * w, ties = 0;
     if (by_count) {  // the weight above it has not been summed yet
       u64 s = 0;
-      for (int i = threadIdx.x; i < V; i += kSampThreads) {
-        const float v = at(i);
-        if (order_key(v) > prefix && in(v, bin)) s += bin_of(v, per, top).w;
-      }
+      each([&](int, float v) {
+        const uint32_t k = order_key(v);
+        if (k > prefix && in(v, bin)) s += bin_of(v, per, top).w;
+        ties += k == prefix;
+      });
       upto = block_sum(s, sm) + (r + 1) * w;
+      ties = block_sum(ties, sm);
     }
-    return Found{prefix, r, upto, -1};
+    return Found{prefix, r, ties, upto, -1};
   }
 
-  // Tokens of the bin with this logit.
-  __device__ u64 ties(int bin, uint32_t key) {
-    u64 c = 0;
-    if (sm.n[bin] <= kBinCap) {
-      hold(bin);
-      c = (int)threadIdx.x < sm.n[bin] && (uint32_t)(sm.el[threadIdx.x] >> 32) == key;
-    } else {
-      for (int i = threadIdx.x; i < V; i += kSampThreads) c += order_key(at(i)) == key;
-    }
-    return block_sum(c, sm);
-  }
-
-  // Count and weight of the bin's tokens that weigh at least `least` of the largest.
-  __device__ void heavy(int bin, double M, double inv_t, uint32_t kmax, double least, u64 *count, u64 *sum) {
+  // Weight of the bin's tokens that weigh at least `least` of the largest.
+  __device__ __forceinline__ u64 heavy(int bin, double M, double inv_t, uint32_t kmax, double least) {
     auto is = [&](uint32_t k) {
       return k == kmax || exp(((double)key_value(k) - M) * inv_t) >= least;
     };
-    u64 c = 0, s = 0;
+    u64 s = 0;
     if (sm.n[bin] <= kBinCap) {
       hold(bin);
       if ((int)threadIdx.x < sm.n[bin]) {
         const uint32_t k = (uint32_t)(sm.el[threadIdx.x] >> 32);
-        c = is(k);
-        s = c ? weight(k) : 0;
+        s = is(k) ? weight(k) : 0;
       }
     } else {
-      for (int i = threadIdx.x; i < V; i += kSampThreads) {
-        const float v = at(i);
-        if (in(v, bin) && is(order_key(v))) {
-          ++c;
-          s += bin_of(v, per, top).w;
-        }
-      }
+      each([&](int, float v) {
+        if (in(v, bin) && is(order_key(v))) s += bin_of(v, per, top).w;
+      });
     }
-    *count = block_sum(c, sm);
-    *sum = block_sum(s, sm);
+    return block_sum(s, sm);
   }
 
   // The index of the r-th token with this logit.
-  __device__ int index_of(uint32_t key, u64 r) {
+  __device__ __forceinline__ int index_of(uint32_t key, u64 r) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int per_wave = ((V + kSampWaves - 1) / kSampWaves + 63) & ~63;
     const int lo = min(wave * per_wave, V), hi = min(lo + per_wave, V);
@@ -438,11 +483,24 @@ struct Row {
     return (int)sm.tmp[2];
   }
 
+  // The first bin at which `is` holds (it holds from there on), kBins where none: every
+  // wave finds it by itself.
+  template <class Is>
+  __device__ __forceinline__ int first_bin(Is is) const {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < kBins / 64; ++j) n += __popcll(__ballot(!is(lane + 64 * j)));
+    return n;
+  }
   // The first bin up to `last` whose weight, with that of the bins before it, exceeds x.
-  __device__ int bin_past(double x, int last) {
-    const int t = threadIdx.x;
-    const int j = (int)block_sum(t <= last && t < kBins && !(sm.before[t + 1] > x), sm);
-    return min(j, last);
+  __device__ __forceinline__ int bin_past(double x, int last) const {
+    return min(first_bin([&](int t) { return sm.before[t + 1] > x; }), last);
+  }
+  // ln of a token's share of `total`.
+  __device__ __forceinline__ float logprob(uint32_t key, uint32_t kmax, double M, double inv_t, double total) const {
+    return (float)((key == kmax ? 0.0 : ((double)key_value(key) - M) * inv_t) -
+                   log(total / ((double)weight(kmax) * sm.fac[0])));
   }
 };
 
@@ -457,7 +515,7 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
   u64 best = 0;
   for (int c = lane; c < chunks; c += 64) best = o[c].best > best ? o[c].best : best;
   best = wave_max(best);
-  const uint32_t kmax = (uint32_t)(best >> 32);
+  uint32_t kmax = (uint32_t)(best >> 32);
   const float T = rp.t(b);
   const bool empty = kmax == kNoKey;
   if (empty || !(T > 0.f)) {
@@ -467,14 +525,17 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
     }
     return;
   }
+  const bool flat = key_value(kmax) == INFINITY;
+  if (flat) kmax = order_key(0.f);
   const double M = (double)key_value(kmax), inv_t = fmax(1.0 / (double)T, 1e-300), per = bins_per_logit(T);
-  Row<DT> row = {logits, (size_t)b * row_stride, V, chunks, per, floor(M * per), o, sm, -1};
+  Row<DT> row = {logits, (size_t)b * row_stride, V, chunks, per, top_bin((float)M, per), 0, flat, o, sm, -1};
+  row.chunk_top = flat ? INFINITY : row.top;
   // the row's bins: four threads a bin, each every fourth chunk
   {
     const int bin = threadIdx.x & (kBins - 1), part = threadIdx.x / kBins;
     u64 n = 0, w = 0;
     for (int c = part; c < chunks; c += kSampThreads / kBins) {
-      const double shift = o[c].top == row.top ? 0.0 : row.top - o[c].top;
+      const double shift = o[c].top == row.chunk_top ? 0.0 : row.chunk_top - o[c].top;
       if (shift <= (double)bin) {
         const u64 v = o[c].bins[bin - (int)shift];
         n += v >> kCountShift;
@@ -492,7 +553,7 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
       }
       sm.n[bin] = (int)n;
       sm.w[bin] = w;
-      sm.fac[bin] = exp(-kDelta * bin) * (1.0 / 68719476736.0);
+      sm.fac[bin] = exp(-kDelta * bin) * 0x1p-36;
     }
   }
   __syncthreads();
@@ -528,64 +589,143 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
     }
   }
   __syncthreads();
+  const int k = rp.top_ks ? rp.top_ks[b] : rp.top_k;
+  const float tp = rp.top_ps ? rp.top_ps[b] : rp.top_p, mp = rp.min_ps ? rp.min_ps[b] : rp.min_p;
+  const double uu = fmin(fmax((double)u[b], 0.0), 1.0), least = fmin((double)mp, 1.0);
+  const bool by_k = k > 0 && k < sm.n_before[kBins], by_p = tp < 1.f, by_m = mp > 0.f;
+  int m_bin = kBins;  // the bin of the least weight that min-p leaves
+  if (by_m) {
+    const double below = row.top - floor(M * per + log(least) * (1.0 / kDelta));
+    m_bin = below < (double)kBins ? max(0, (int)below) : kBins;
+  }
+  // The head: the bins up to the end of what the filters leave. top-p's share is of what
+  // top-k left, so where both are set the head reaches to the k-th token.
+  const int k_bin = by_k ? row.first_bin([&](int t) { return sm.n_before[t + 1] >= k; }) : kBins - 1;
+  int head = k_bin;
+  if (!by_k) {
+    const double x = by_p ? fmax((double)tp, 0.0) * sm.before[kBins] : by_m ? sm.before[kBins] : uu * sm.before[kBins];
+    head = min(row.bin_past(x, kBins - 1), m_bin);
+  }
+  if (sm.n_before[head + 1] <= kHeadCap) {
+    row.gather(head, [&](int at) { return at <= head; });
+    const int n = sm.n_raw;
+    row.order(n);
+    if (threadIdx.x >= 64) return;
+    // lane l: the places P l .. P l + P - 1 of the order
+    constexpr int P = kHeadCap / 64;
+    uint32_t key[P];
+    double w[P], upto[P], sum = 0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const int i = P * lane + j;
+      key[j] = i < n ? (uint32_t)(sm.el[i] >> 32) : 0;
+      const Binned e = bin_of(key_value(key[j]), per, row.top);
+      w[j] = i < n ? (double)e.w * sm.fac[min(e.bin, kBins - 1)] : 0.0;
+      sum += w[j];
+    }
+    double run = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const double v = __shfl_up(run, off, 64);
+      if (lane >= off) run += v;
+    }
+    double before = __shfl_up(run, 1, 64);
+    if (lane == 0) before = 0;
+#pragma unroll
+    for (int j = 0; j < P; ++j) upto[j] = j == P - 1 ? run : (j ? upto[j - 1] : before) + w[j];
+    // how many places, from the first on, a condition holds at; a value at a place
+    auto count = [&](auto is) {
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < P; ++j) c += __popcll(__ballot(P * lane + j < n && is(j)));
+      return c;
+    };
+    auto upto_at = [&](int i) {
+      double v = 0;
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        if (i % P == j) v = upto[j];
+      return __shfl(v, i / P, 64);
+    };
+    int kept = n;
+    double total = sm.before[kBins];
+    if (by_k) {
+      const uint32_t kth = (uint32_t)(sm.el[k - 1] >> 32);
+      kept = count([&](int j) { return key[j] >= kth; });
+      total = upto_at(kept - 1);
+    }
+    if (by_p) {
+      const double bound = fmax((double)tp, 0.0) * total;
+      kept = min(kept, count([&](int j) { return (j ? upto[j - 1] : before) <= bound; }));
+    }
+    if (by_m)
+      kept = min(kept, count([&](int j) { return key[j] == kmax || exp(((double)key_value(key[j]) - M) * inv_t) >= least; }));
+    kept = max(kept, 1);
+    if (by_k || by_p || by_m) total = upto_at(kept - 1);
+    const double target = uu * total;
+    const int at = min(count([&](int j) { return upto[j] <= target; }), kept - 1);
+    if (lane == 0) {
+      const u64 e = sm.el[at];
+      tokens[b] = (int)~(uint32_t)e;
+      if (logprobs) logprobs[b] = row.logprob((uint32_t)(e >> 32), kmax, M, inv_t, total);
+    }
+    return;
+  }
   // What stays: the bins before `last`, and of that bin the tokens before and with the
   // (r + 1)-th that has the logit `key`: `upto` of weight. At first everything.
   int last = kBins - 1;
   uint32_t key = 0;
   u64 r = ~0ull >> 1, upto = sm.w[kBins - 1];
   auto weight_kept = [&]() { return sm.before[last] + (double)upto * sm.fac[last]; };
-  const int k = rp.top_ks ? rp.top_ks[b] : rp.top_k;
-  if (k > 0 && k < sm.n_before[kBins]) {
-    const int t = threadIdx.x;
-    last = (int)block_sum(t < kBins && sm.n_before[t + 1] < k, sm);
-    const Found f = row.find(last, (double)(k - 1 - sm.n_before[last]), true);
-    const u64 n = row.ties(last, f.key);
-    key = f.key;
-    upto = f.upto + (n - 1 - f.r) * row.weight(key);
-    r = n - 1;
-  }
-  const float tp = rp.top_ps ? rp.top_ps[b] : rp.top_p;
-  if (tp < 1.f) {
-    const double bound = fmax((double)tp, 0.0) * weight_kept();
-    const int bin = row.bin_past(bound, last);
-    const Found f = row.find(bin, (bound - sm.before[bin]) / sm.fac[bin], false);
-    if (bin < last || f.key > key || (f.key == key && f.r < r)) {
+  double total = 0;
+  Found f;
+#pragma unroll 1  // (one copy of the search: the code of four costs more than the jumps)
+  for (int stage = 0; stage < 4; ++stage) {
+    int bin = k_bin;
+    double x = 0;
+    if (stage == 0) {  // top-k
+      if (!by_k) continue;
+      x = (double)(k - 1 - sm.n_before[bin]);
+    } else if (stage == 1) {  // top-p
+      if (!by_p) continue;
+      const double bound = fmax((double)tp, 0.0) * weight_kept();
+      bin = row.bin_past(bound, last);
+      x = (bound - sm.before[bin]) / sm.fac[bin];
+    } else if (stage == 2) {  // min-p: those that weigh enough, all before any other
+      if (!by_m || m_bin > last) continue;
+      const u64 w = row.heavy(m_bin, M, inv_t, kmax, least);
+      if (m_bin < last || w < upto) {
+        last = m_bin;
+        upto = w;
+      }
+      continue;
+    } else {  // the draw
+      total = weight_kept();
+      const double target = uu * total;
+      bin = row.bin_past(target, last);
+      // (rounding, or a last bin of which nothing stays: the last token that does)
+      while (bin > 0 && (bin == last ? upto == 0 : sm.w[bin] == 0)) --bin;
+      x = (target - sm.before[bin]) / sm.fac[bin];
+      const double most = (double)(bin == last ? upto : sm.w[bin]);
+      if (!(x < most)) x = most - 1.0;
+    }
+    f = row.find(bin, x, stage == 0);
+    if (stage == 0) {  // the ties of the k-th stay too
+      last = bin;
+      key = f.key;
+      upto = f.upto + (f.ties - 1 - f.r) * row.weight(key);
+      r = f.ties - 1;
+    } else if (stage == 1 && (bin < last || f.key > key || (f.key == key && f.r < r))) {
       last = bin;
       key = f.key;
       r = f.r;
       upto = f.upto;
     }
   }
-  const float mp = rp.min_ps ? rp.min_ps[b] : rp.min_p;
-  if (mp > 0.f) {
-    const double least = fmin((double)mp, 1.0), below = row.top - floor(M * per + log(least) * (1.0 / kDelta));
-    const int bin = below < (double)kBins ? max(0, (int)below) : kBins;  // (an infinite M: bin 0 by the next line)
-    const int at = isinf(M) ? 0 : bin;
-    if (at <= last) {
-      u64 n, w;
-      row.heavy(at, M, inv_t, kmax, least, &n, &w);
-      if (at < last || w < upto) {
-        last = at;
-        upto = w;
-        key = 0;  // which of them: those that weigh enough, all before any other
-        r = ~0ull >> 1;
-      }
-    }
-  }
-  const double total = weight_kept(), target = fmin(fmax((double)u[b], 0.0), 1.0) * total;
-  int bin = row.bin_past(target, last);
-  // (rounding, or a last bin of which nothing stays: the last token that does)
-  while (bin > 0 && (bin == last ? upto == 0 : sm.w[bin] == 0)) --bin;
-  double x = (target - sm.before[bin]) / sm.fac[bin];
-  const double most = (double)(bin == last ? upto : sm.w[bin]);
-  if (!(x < most)) x = most - 1.0;
-  const Found f = row.find(bin, x, false);
   const int token = f.index >= 0 ? f.index : row.index_of(f.key, f.r);
   if (threadIdx.x == 0) {
     tokens[b] = token;
-    if (logprobs)
-      logprobs[b] = (float)((f.key == kmax ? 0.0 : ((double)key_value(f.key) - M) * inv_t) -
-                            log(total / ((double)row.weight(kmax) * sm.fac[0])));
+    if (logprobs) logprobs[b] = row.logprob(f.key, kmax, M, inv_t, total);
   }
 }
 
@@ -621,7 +761,7 @@ extern "C" int sf_sample(const void *logits, int dtype, long long row_stride, in
   hipStream_t st = (hipStream_t)stream;
 #define SF_SAMP(DT)                                                                                                \
   do {                                                                                                             \
-    k_sample_bins<DT><<<(unsigned)(B * chunks), kSampThreads, 0, st>>>(logits, row_stride, V, (int)chunks, rp, outs); \
+    k_sample_bins<DT><<<(unsigned)(B * chunks), kBinThreads, 0, st>>>(logits, row_stride, V, (int)chunks, rp, outs); \
     k_sample_pick<DT><<<B, kSampThreads, 0, st>>>(logits, row_stride, V, (int)chunks, u, rp, outs, tokens, logprobs); \
   } while (0)
   if (dtype == SF_F32) SF_SAMP(SF_F32);
