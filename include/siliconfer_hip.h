@@ -486,13 +486,16 @@ int sf_kv_evict(int8_t *k_codes, void *k_scales, int8_t *v_codes, void *v_scales
  * without a logit above -inf gives -1. logprobs (or NULL): the log of the token's share
  * of the weight kept. logits [B][V] of `dtype`, rows row_stride elements apart; each of
  * the settings for all rows, or a row's own from a device array [B] where that is not
- * NULL. workspace: sf_sample_workspace_bytes(B, V) bytes, 256-byte aligned (may be 0 ->
- * NULL ok), no initial contents needed; calls that share one must not overlap. */
+ * NULL. For steps replayed from a HIP graph, `at` (or NULL) is a device index: row b takes
+ * the number u[*at + at_add + b] of u_n (kept inside them) and its token also goes to
+ * hist[*at + at_add + b], hist (or NULL) as long as u. workspace:
+ * sf_sample_workspace_bytes(B, V) bytes, 256-byte aligned, no initial contents needed; calls that share one must not overlap. */
 size_t sf_sample_workspace_bytes(int B, int V);
 int sf_sample(const void *logits, int dtype, long long row_stride, int B, int V, const float *u,
               float temperature, int top_k, float top_p, float min_p, const float *temperatures,
               const int32_t *top_ks, const float *top_ps, const float *min_ps, int32_t *tokens,
-              float *logprobs, void *workspace, size_t workspace_bytes, void *stream);
+              float *logprobs, const int32_t *at, int at_add, int u_n, int32_t *hist, void *workspace,
+              size_t workspace_bytes, void *stream);
 
 /* ---- a chain of dependent decode GEMVs in one persistent launch (no
  * counterpart in the reference, which runs each Q4Linear of a layer as its own

@@ -119,7 +119,7 @@ _SIGS = {
                            _c_p, _c_p, _c_sz, _c_i, _c_i, _c_i, _c_i, _c_p]),
     "sf_sample_workspace_bytes": (_c_sz, [_c_i, _c_i]),
     "sf_sample": (_c_i, [_c_p, _c_i, ctypes.c_longlong, _c_i, _c_i, _c_p, _c_f, _c_i, _c_f, _c_f, _c_p,
-                         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_sz, _c_p]),
+                         _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_i, _c_p, _c_p, _c_sz, _c_p]),
     "sf_q4_chain_workspace_bytes": (_c_sz, [_c_p, _c_i]),
     "sf_q4_chain": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_p, _c_sz, _c_i, _c_i,
                            _c_p]),

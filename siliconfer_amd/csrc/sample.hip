@@ -68,7 +68,14 @@ struct RowParams {
   int top_k;
   const float *temperatures, *top_ps, *min_ps;
   const int *top_ks;
+  const int32_t *at;  // or null: row b's number is u[*at + at_add + b] of u_n, its token also hist[..]
+  int32_t *hist;
+  int at_add, u_n, B;
   __device__ __forceinline__ float t(int b) const { return temperatures ? temperatures[b] : temperature; }
+  // where row b's number lies (kept inside u)
+  __device__ __forceinline__ int place(int b) const {
+    return at ? (int)max(0ll, min((long long)*at + at_add, (long long)u_n - B)) + b : b;
+  }
 };
 
 // 1 / (T kDelta): a logit's place on the bins' axis is x times it. The floor keeps an
@@ -521,6 +528,7 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
   if (empty || !(T > 0.f)) {
     if (threadIdx.x == 0) {
       tokens[b] = empty ? -1 : (int)~(uint32_t)best;
+      if (rp.hist) rp.hist[rp.place(b)] = empty ? -1 : (int)~(uint32_t)best;
       if (logprobs) logprobs[b] = empty ? -INFINITY : 0.f;
     }
     return;
@@ -591,7 +599,8 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
   __syncthreads();
   const int k = rp.top_ks ? rp.top_ks[b] : rp.top_k;
   const float tp = rp.top_ps ? rp.top_ps[b] : rp.top_p, mp = rp.min_ps ? rp.min_ps[b] : rp.min_p;
-  const double uu = fmin(fmax((double)u[b], 0.0), 1.0), least = fmin((double)mp, 1.0);
+  const int place = rp.place(b);
+  const double uu = fmin(fmax((double)u[place], 0.0), 1.0), least = fmin((double)mp, 1.0);
   const bool by_k = k > 0 && k < sm.n_before[kBins], by_p = tp < 1.f, by_m = mp > 0.f;
   int m_bin = kBins;  // the bin of the least weight that min-p leaves
   if (by_m) {
@@ -667,6 +676,7 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
     if (lane == 0) {
       const u64 e = sm.el[at];
       tokens[b] = (int)~(uint32_t)e;
+      if (rp.hist) rp.hist[place] = (int)~(uint32_t)e;
       if (logprobs) logprobs[b] = row.logprob((uint32_t)(e >> 32), kmax, M, inv_t, total);
     }
     return;
@@ -725,6 +735,7 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
   const int token = f.index >= 0 ? f.index : row.index_of(f.key, f.r);
   if (threadIdx.x == 0) {
     tokens[b] = token;
+    if (rp.hist) rp.hist[place] = token;
     if (logprobs) logprobs[b] = row.logprob(f.key, kmax, M, inv_t, total);
   }
 }
@@ -741,7 +752,7 @@ extern "C" size_t sf_sample_workspace_bytes(int B, int V) {
 extern "C" int sf_sample(const void *logits, int dtype, long long row_stride, int B, int V, const float *u,
                          float temperature, int top_k, float top_p, float min_p, const float *temperatures,
                          const int32_t *top_ks, const float *top_ps, const float *min_ps, int32_t *tokens,
-                         float *logprobs, void *workspace, size_t workspace_bytes, void *stream) {
+                         float *logprobs, const int32_t *at, int at_add, int u_n, int32_t *hist, void *workspace, size_t workspace_bytes, void *stream) {
   SF_REQUIRE(B >= 0 && V > 0, SF_EINVAL, "invalid sampling shape B=%d V=%d", B, V);
   SF_REQUIRE(V <= (1 << 24), SF_EUNSUPPORTED, "V=%d: at most 16777216 tokens", V);
   SF_REQUIRE(dtype >= SF_F32 && dtype <= SF_BF16, SF_EINVAL, "bad dtype %d", dtype);
@@ -751,12 +762,13 @@ extern "C" int sf_sample(const void *logits, int dtype, long long row_stride, in
              temperature);
   if (B == 0) return SF_OK;
   SF_REQUIRE(logits && u && tokens, SF_EINVAL, "null pointer argument");
+  SF_REQUIRE(at ? u_n >= B : !hist, SF_EINVAL, at ? "%d numbers for %d rows" : "hist without at", u_n, B);
   const long long chunks = sample_chunks(V);
   SF_REQUIRE(B * chunks <= 0x7fffffffLL, SF_EINVAL, "B=%d rows of %d exceed the grid", B, V);
   SF_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0, SF_EINVAL, "workspace must be 256-byte aligned");
   const size_t need = sf_sample_workspace_bytes(B, V);
   SF_REQUIRE(workspace_bytes >= need, SF_EINVAL, "sampling workspace too small: %zu < %zu", workspace_bytes, need);
-  const RowParams rp = {temperature, top_p, min_p, top_k, temperatures, top_ps, min_ps, top_ks};
+  const RowParams rp = {temperature, top_p, min_p, top_k, temperatures, top_ps, min_ps, top_ks, at, hist, at_add, u_n, B};
   ChunkOut *outs = (ChunkOut *)workspace;
   hipStream_t st = (hipStream_t)stream;
 #define SF_SAMP(DT)                                                                                                \

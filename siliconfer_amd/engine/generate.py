@@ -17,8 +17,12 @@ How it runs on MI355X:
   * sampling (temperature > 0 or a repetition penalty): eager decode steps
     that keep the fp32 logits; the next token is drawn on the device with
     torch (the reference's rules: penalty on previously generated ids,
-    temperature, top-k, top-p nucleus, generate.py:24-67) and written back as
-    the step's token.
+    temperature, top-k, top-p nucleus, generate.py:24-67, and min-p) and written
+    back as the step's token;
+  * sampling with `uniforms`, one number in [0, 1) a token: the draw is part of
+    the captured step (`sf_sample`, the same rules without the penalty), so
+    tokens stay on the device as in the greedy path, and the same numbers give
+    the same tokens.
 
 KV cache: this decoder keeps the int8 cache (the reference's
 `quantize_kv_cache=True` path, kv_cache.py:49-126) and has no full-precision one.
@@ -30,6 +34,7 @@ default is the fp16 one (generate.py:124, 135).
 
 from __future__ import annotations
 
+import math
 import time
 from collections.abc import Callable
 from dataclasses import dataclass
@@ -61,6 +66,7 @@ class SamplingParams:
     top_k: int = 0
     repetition_penalty: float = 1.0
     max_tokens: int = 128
+    min_p: float = 0.0  # tokens below min_p of the largest probability are dropped (0: none)
 
 
 def _is_greedy(p: SamplingParams) -> bool:
@@ -89,6 +95,9 @@ def sample_token(logits: torch.Tensor, params: SamplingParams,
         drop = (torch.cumsum(probs, dim=-1) - probs) > params.top_p
         srt = torch.where(drop, torch.full_like(srt, float("-inf")), srt)
         row = torch.empty_like(row).scatter_(0, order, srt)
+    if params.min_p > 0:
+        floor = row.max() + math.log(params.min_p)
+        row = torch.where(row < floor, torch.full_like(row, float("-inf")), row)
     probs = torch.softmax(row, dim=-1)
     return int(torch.multinomial(probs, 1, generator=generator).item())
 
@@ -124,13 +133,22 @@ def generate(model: LlamaModel, prompt_ids, params: SamplingParams | None = None
              eos_token_id: int | None = None, stream: bool = False,
              on_token: Callable[[int], None] | None = None,
              quantize_kv_cache: bool | None = None,
-             generator: torch.Generator | None = None) -> GenerationResult:
+             generator: torch.Generator | None = None,
+             uniforms=None) -> GenerationResult:
     """Prefill the prompt, then decode up to `params.max_tokens - 1` more
     tokens, stopping after `eos_token_id`. `on_token` gets every token as it
     is produced (else `stream` prints it); `decode_tok_s` counts the tokens
-    after the first over the time after prefill, as the reference does."""
+    after the first over the time after prefill, as the reference does.
+    `uniforms` (at least max_tokens numbers in [0, 1): a tensor, an array or a
+    list) draws token i from uniforms[i] on the device; `generator` is then unused."""
     check_kv_cache_flag(quantize_kv_cache)
     params = params or SamplingParams()
+    if uniforms is not None:
+        if params.repetition_penalty != 1.0:
+            raise SFError("uniforms: the draw on the device has no repetition penalty")
+        uniforms = torch.as_tensor(uniforms, dtype=torch.float32).reshape(-1)
+        if uniforms.numel() < params.max_tokens:
+            raise SFError(f"{uniforms.numel()} uniforms for {params.max_tokens} tokens")
     ids = _prompt_array(prompt_ids)
     if ids.size + params.max_tokens > model.max_seq + 1:
         raise SFError("prompt + max_tokens exceeds the cache capacity")
@@ -144,17 +162,23 @@ def generate(model: LlamaModel, prompt_ids, params: SamplingParams | None = None
         elif stream:
             print(tok, end=" ", flush=True)
 
-    greedy = _is_greedy(params)
+    drawn = uniforms is not None  # on the device, from the caller's numbers
+    greedy = _is_greedy(params) and not drawn
     if greedy and model.graph is None:
         model.capture()
     model.reset()
+    if drawn:
+        model.set_sampling(params.temperature, params.top_k, params.top_p, params.min_p,
+                           uniforms[:params.max_tokens], start=int(ids.size) - 1)
     torch.cuda.synchronize(model.device)
     t0 = time.perf_counter()
     first = model.prefill(ids, want_logits=not greedy)
     if not greedy:
         torch.cuda.synchronize(model.device)
     t1 = time.perf_counter()  # the prefill clock stops before the first draw (generate.py:139-141)
-    if not greedy:
+    if drawn:
+        first = model.draw()
+    elif not greedy:
         first = sample_token(model.logits, params, out, generator)
         model.token.fill_(first)
     emit(first)
@@ -162,10 +186,10 @@ def generate(model: LlamaModel, prompt_ids, params: SamplingParams | None = None
     budget = params.max_tokens - 1
     done = eos_token_id is not None and first == eos_token_id
     while budget > 0 and not done:
-        if greedy:
+        if greedy or drawn:
             n = min(budget, CHUNK) if (emit_each or eos_token_id is not None) else budget
             start = model.pos
-            model.replay(n)
+            (model.replay_sampled if drawn else model.replay)(n)
             toks = model.hist[start:start + n].cpu().tolist()
             for j, tok in enumerate(toks):
                 emit(tok)

@@ -63,7 +63,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     B, T, H, D = q.shape
     KVH = 0
     if out_q is None:
-        out_q = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+        out_q = torch.empty_like(q, memory_format=torch.contiguous_format)
     plain = q.is_contiguous() and out_q.is_contiguous()
     if out_q.shape != q.shape or out_q.dtype != q.dtype or out_q.device != q.device:
         raise SFError("out_q must have q's shape, dtype and device")
@@ -73,7 +73,7 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
         if k.shape[0] != B or k.shape[1] != T or k.shape[3] != D or k.dtype != q.dtype or k.device != q.device:
             raise SFError("k must match q in batch, rows, head_dim, dtype and device")
         if out_k is None:
-            out_k = torch.empty((B, T, KVH, D), dtype=k.dtype, device=k.device)
+            out_k = torch.empty_like(k, memory_format=torch.contiguous_format)
         elif out_k.shape != k.shape or out_k.dtype != k.dtype or out_k.device != k.device:
             raise SFError("out_k must have k's shape, dtype and device")
         plain = plain and k.is_contiguous() and out_k.is_contiguous()

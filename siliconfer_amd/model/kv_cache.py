@@ -164,3 +164,82 @@ def make_quantized_cache(n_layers: int, capacity: int = 4096,
                          scale_dtype: torch.dtype = torch.float16) -> list[QuantizedKVCache]:
     """One fresh QuantizedKVCache per transformer layer."""
     return [QuantizedKVCache(capacity, scale_dtype) for _ in range(n_layers)]
+
+
+class BoundedKVCache(QuantizedKVCache):
+    """An int8 cache that keeps at most `budget` tokens a kv head: it counts the
+    attention weight that every slot receives (`scores`) and, once it holds more than
+    budget + slack, drops the slots with the least of it; those of the newest `recent`
+    tokens (a quarter of the budget by default) stay. Each kv head keeps tokens of its
+    own, in any order, with their `positions`; `length()` counts slots, `seen` the
+    tokens that went through. Keys are cached turned to their positions."""
+
+    def __init__(self, budget: int, recent: int | None = None, slack: int = 64,
+                 scale_dtype: torch.dtype = torch.float16) -> None:
+        recent = budget // 4 if recent is None else recent
+        if not (budget > 0 and 0 <= recent <= budget and slack >= 0):
+            raise SFError(f"need budget > 0, 0 <= recent <= budget, slack >= 0 (got {budget}, {recent}, {slack})")
+        super().__init__(budget + slack + 1, scale_dtype)
+        self.budget, self.recent, self.slack = int(budget), int(recent), int(slack)
+        self.seen = 0
+        self.scores = self.positions = None
+
+    def _ensure(self, k: torch.Tensor, need: int) -> None:
+        before = self._qk
+        super()._ensure(k, need)
+        if self._qk is before:
+            return
+        shape = self._qk.shape[:3]
+        scores = torch.zeros(shape, dtype=torch.float32, device=self._qk.device)
+        positions = torch.zeros(shape, dtype=torch.int32, device=self._qk.device)
+        if self.scores is not None and self._len:
+            scores[:, :, :self._len].copy_(self.scores[:, :, :self._len])
+            positions[:, :, :self._len].copy_(self.positions[:, :, :self._len])
+        self.scores, self.positions = scores, positions
+
+    def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Append keys that are turned already, and values, [B, KVH, T, D]."""
+        n, T = self._len, k.shape[2]
+        super().append(k, v)
+        self.scores[:, :, n:n + T] = 0
+        self.positions[:, :, n:n + T] = torch.arange(self.seen, self.seen + T, dtype=torch.int32, device=k.device)
+        self.seen += T
+
+    def append_rotary(self, qkv: torch.Tensor, n_heads: int, n_kv_heads: int, rotary,
+                      out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Append the next tokens' fused q|k|v rows [B, T, (H + 2 KVH) D], keys turned to
+        their positions; returns the turned q [B, T, H, D]."""
+        from ..kernels.rotary import rotary_kv_append
+        B, T, W = qkv.shape
+        D = W // (n_heads + 2 * n_kv_heads)
+        self.reserve(B, n_kv_heads, D, self._len + T, qkv.device)
+        positions = torch.arange(self.seen, self.seen + T, dtype=torch.int32, device=qkv.device)
+        q = rotary_kv_append(qkv, positions, rotary.on(qkv.device), *self.buffers(), n_heads=n_heads,
+                             lengths=self._len, interleaved=rotary.interleaved, scale=rotary.scale,
+                             slot_positions=self.positions, scores=self.scores, out_dtype=out_dtype)
+        self._len += T
+        self.seen += T
+        return q
+
+    def attend(self, q: torch.Tensor, scale: float | None = None) -> torch.Tensor:
+        """Attention of the newest rows q [B, T, H, D] (T <= 32) over the cache, their
+        weights added to the scores; fp32."""
+        from ..kernels.attention import attention_decode_scored
+        return attention_decode_scored(q, *self.buffers(), self.scores, lengths=self._len, scale=scale)
+
+    def evict(self) -> None:
+        """Cut the cache to its budget where it holds more than budget + slack."""
+        from ..kernels.eviction import evict
+        if self._len > self.budget + self.slack:
+            evict(*self.buffers(), self.scores, self.positions, self._len, self.seen, self.budget, self.recent)
+            self._len = self.budget
+
+    def set_length(self, n: int) -> None:
+        raise SFError("a bounded cache's slots are set by append and evict")
+
+    def trim(self, n: int) -> None:
+        """Keep the first n positions: refused once tokens were dropped."""
+        if self.seen != self._len and n < self.seen:
+            raise SFError("a bounded cache that dropped tokens cannot be trimmed")
+        super().trim(n)
+        self.seen = min(self.seen, max(0, int(n)))

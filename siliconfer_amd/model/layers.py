@@ -31,9 +31,11 @@ import torch
 
 from .. import _lib
 from .._lib import SFError
+from ..kernels.rotary import rotary, rotary_kv_append
 from .config import ModelConfig, rope_freqs as _rope_freqs_np
-from .kv_cache import QuantizedKVCache, dequantize_kv
+from .kv_cache import BoundedKVCache, QuantizedKVCache, dequantize_kv
 from .q4_linear import Q4Linear, project_group
+from .rope import Rotary
 
 
 def _on_device(x: torch.Tensor) -> None:
@@ -128,10 +130,18 @@ def _sdpa_causal(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offset: int,
 
 class Attention(torch.nn.Module):
     """Grouped-query attention (layers.py:69-129). `__call__(x, cache)` with x
-    [B, T, hidden] returns (o_proj(attention) [B, T, hidden] fp32, cache)."""
+    [B, T, hidden] returns (o_proj(attention) [B, T, hidden] fp32, cache).
 
-    def __init__(self, config: ModelConfig, rope_freqs: torch.Tensor, device=None) -> None:
+    `rotary` replaces the rotate-half RoPE of `rope_freqs` (interleaved pairs, part of
+    the head, scaled frequencies). A `BoundedKVCache`, at any batch, scores its slots
+    and drops the least attended ones; of a prompt, the last OBSERVED rows score."""
+
+    OBSERVED = 16
+
+    def __init__(self, config: ModelConfig, rope_freqs: torch.Tensor, device=None,
+                 rotary: Rotary | None = None) -> None:
         super().__init__()
+        self.rotary = rotary
         self.num_heads = config.num_attention_heads
         self.num_kv_heads = config.num_key_value_heads
         self.head_dim = config.head_dim
@@ -159,17 +169,22 @@ class Attention(torch.nn.Module):
         _on_device(x)  # every route runs on the GPU; none on the host
         B, T, _ = x.shape
         H, KVH, D = self.num_heads, self.num_kv_heads, self.head_dim
+        bounded = isinstance(cache, BoundedKVCache)
         int8_batch1 = isinstance(cache, QuantizedKVCache) and B == 1
         qkv = None
-        if int8_batch1:
+        if int8_batch1 or bounded:
             qkv = project_group(_lib.SF_GROUP_CONCAT, (self.q_proj, self.k_proj, self.v_proj), x)
         if qkv is None:
             q = _project(self.q_proj, x)
             k = _project(self.k_proj, x)
             v = _project(self.v_proj, x)
-        if int8_batch1:
+        if int8_batch1 or bounded:
             if qkv is None:
-                qkv = torch.cat([q.reshape(T, -1), k.reshape(T, -1), v.reshape(T, -1)], dim=1).contiguous()
+                qkv = torch.cat([t.reshape(B * T, -1) for t in (q, k, v)], dim=1).contiguous()
+        if bounded:
+            out = self._bounded(qkv.view(B, T, -1), cache)
+            return _project(self.o_proj, out.reshape(B, T, H * D)), cache
+        if int8_batch1:
             out = self._int8_batch1(qkv, cache, T, x.device)
             return _project(self.o_proj, out.reshape(1, T, H * D)), cache
         q = q.reshape(B, T, H, D).transpose(1, 2)
@@ -181,8 +196,11 @@ class Attention(torch.nn.Module):
             offset = cache[0].shape[2]
         else:
             offset = 0
-        q = apply_rope(q, offset, self.rope_freqs)
-        k = apply_rope(k, offset, self.rope_freqs)
+        if self.rotary is not None:
+            q, k = self._turn(q, k, offset)
+        else:
+            q = apply_rope(q, offset, self.rope_freqs)
+            k = apply_rope(k, offset, self.rope_freqs)
         if isinstance(cache, QuantizedKVCache):
             cache.append(k, v)
             kc, vc = dequantize_kv(cache.q_k, cache.s_k, torch.float32), dequantize_kv(cache.q_v, cache.s_v,
@@ -198,6 +216,38 @@ class Attention(torch.nn.Module):
         a = _sdpa_causal(q, kc, vc, offset, self.scale)
         return _project(self.o_proj, a.transpose(1, 2).reshape(B, T, H * D)), new_cache
 
+    def _turn(self, q: torch.Tensor, k: torch.Tensor, offset: int):
+        """q, k [B, heads, T, D] turned by `rotary` at positions offset .. in their layout."""
+        r = self.rotary
+        pos = torch.arange(offset, offset + q.shape[2], dtype=torch.int32, device=q.device)
+        q, k = rotary(q.transpose(1, 2), k.transpose(1, 2), pos, r.on(q.device), interleaved=r.interleaved,
+                      scale=r.scale)
+        return q.transpose(1, 2), k.transpose(1, 2)
+
+    def _bounded(self, qkv: torch.Tensor, cache: BoundedKVCache) -> torch.Tensor:
+        """[B, T, H, D] fp32 from q|k|v rows [B, T, (H + 2 KVH) D]: the rows appended, attention
+        over the whole cache, then what exceeds its bound dropped."""
+        B, T, _ = qkv.shape
+        H, KVH, D = self.num_heads, self.num_kv_heads, self.head_dim
+        if self.rotary is None:  # rotate-half over the whole head, of the given frequencies
+            self.rotary_half = getattr(self, "rotary_half", None) or Rotary(
+                self.rope_freqs.detach().double().cpu().numpy())
+        q = cache.append_rotary(qkv, H, KVH, self.rotary or self.rotary_half)
+        if T <= self.OBSERVED:
+            out = cache.attend(q, self.scale)
+        else:
+            out = torch.empty((B, T, H, D), dtype=torch.float32, device=qkv.device)
+            kq, ks, vq, vs = cache.buffers()
+            lib, st, n = _lib.load(), _lib.stream(qkv), cache.length()
+            for b in range(B):  # (the prompt attention reads one sequence's cache)
+                _lib.check(lib.sf_attn_prefill_i8kv(
+                    q[b].data_ptr(), _lib.SF_F32, kq[b].data_ptr(), ks[b].data_ptr(), vq[b].data_ptr(),
+                    vs[b].data_ptr(), _lib.dt(ks), out[b].data_ptr(), _lib.SF_F32, T, H, KVH, n - T, kq.shape[2], D,
+                    float(self.scale), st), "sf_attn_prefill_i8kv")
+            out[:, -self.OBSERVED:] = cache.attend(q[:, -self.OBSERVED:].contiguous(), self.scale)
+        cache.evict()
+        return out
+
     def _int8_batch1(self, qkv, cache: QuantizedKVCache, T: int, device) -> torch.Tensor:
         """From q|k|v rows [T, (H + 2 KVH) D]: RoPE + int8 append in one launch, then decode or causal prefill
         attention over the cache in place; returns [T, H, D] fp32."""
@@ -207,13 +257,19 @@ class Attention(torch.nn.Module):
         cache.reserve(1, KVH, D, offset + T, device)
         kq, ks, vq, vs = cache.buffers()
         T_cap = kq.shape[2]
-        cos_t, sin_t = self._tables(offset + T, device)
-        q_rot = torch.empty((T, H, D), dtype=torch.float32, device=device)
         st = _lib.stream(qkv)
-        _lib.check(lib.sf_rope_kv_append(qkv.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0],
-                                         q_rot.data_ptr(), _lib.SF_F32, kq.data_ptr(), ks.data_ptr(),
-                                         vq.data_ptr(), vs.data_ptr(), _lib.dt(ks), T, H, KVH, D, T_cap,
-                                         None, offset, st), "sf_rope_kv_append")
+        if self.rotary is not None:
+            r = self.rotary
+            pos = torch.arange(offset, offset + T, dtype=torch.int32, device=device)
+            q_rot = rotary_kv_append(qkv.view(1, T, -1), pos, r.on(device), kq, ks, vq, vs, n_heads=H, lengths=offset,
+                                     interleaved=r.interleaved, scale=r.scale).view(T, H, D)
+        else:
+            cos_t, sin_t = self._tables(offset + T, device)
+            q_rot = torch.empty((T, H, D), dtype=torch.float32, device=device)
+            _lib.check(lib.sf_rope_kv_append(qkv.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0],
+                                             q_rot.data_ptr(), _lib.SF_F32, kq.data_ptr(), ks.data_ptr(),
+                                             vq.data_ptr(), vs.data_ptr(), _lib.dt(ks), T, H, KVH, D, T_cap,
+                                             None, offset, st), "sf_rope_kv_append")
         cache.set_length(offset + T)
         if T == 1:
             from ..kernels.attention import attention_decode
@@ -255,9 +311,10 @@ class MLP(torch.nn.Module):
 class TransformerBlock(torch.nn.Module):
     """x + attn(norm(x)), then + mlp(norm(x)) (layers.py:147-163)."""
 
-    def __init__(self, config: ModelConfig, rope_freqs: torch.Tensor, device=None) -> None:
+    def __init__(self, config: ModelConfig, rope_freqs: torch.Tensor, device=None,
+                 rotary: Rotary | None = None) -> None:
         super().__init__()
-        self.self_attn = Attention(config, rope_freqs, device)
+        self.self_attn = Attention(config, rope_freqs, device, rotary)
         self.mlp = MLP(config, device)
         self.input_layernorm = RMSNorm(config.hidden_size, config.rms_norm_eps, device)
         self.post_attention_layernorm = RMSNorm(config.hidden_size, config.rms_norm_eps, device)
@@ -270,13 +327,13 @@ class TransformerBlock(torch.nn.Module):
 
     @classmethod
     def from_weights(cls, config: ModelConfig, weights: dict, layer: int, rope_freqs: torch.Tensor,
-                     group_size: int = 128, device=None) -> "TransformerBlock":
+                     group_size: int = 128, device=None, rotary: Rotary | None = None) -> "TransformerBlock":
         """Layer `layer` of a checkpoint dict in the HuggingFace naming: packed
         projections (`<p>.q4_packed`, `.q4_scales`, `.q4_zeros`, as
         `pack_and_replace_linears` leaves them) become Q4Linear, dense ones
         (`<p>.weight`) torch Linear, biases and norm weights fp32."""
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-        blk = cls(config, rope_freqs, dev)
+        blk = cls(config, rope_freqs, dev, rotary)
         pre = f"model.layers.{layer}"
         for parent, mod in (("self_attn", blk.self_attn), ("mlp", blk.mlp)):
             for name in (("q_proj", "k_proj", "v_proj", "o_proj") if parent == "self_attn"

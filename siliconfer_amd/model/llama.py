@@ -32,6 +32,7 @@ import torch
 from .. import _lib
 from .._lib import SFError
 from ..kernels.q4 import Q4Weight, matmul_group
+from ..kernels.sampling import sample
 from .config import ModelConfig, rope_tables
 
 _DT = {torch.float32: _lib.SF_F32, torch.float16: _lib.SF_F16, torch.bfloat16: _lib.SF_BF16}
@@ -170,6 +171,7 @@ class LlamaModel:
             _DT[act_dtype]))
         self.pos = 0
         self.graph = None
+        self._sampled_graph = self._u = None
         self._verify_graphs = {}
         self._rows_plans = {}
         self._gemm_plans = {}
@@ -727,6 +729,59 @@ class LlamaModel:
             raise SFError("decode would exceed the cache capacity")
         for _ in range(n):
             self.graph.replay()
+        self.pos += n
+
+    # ------------------------------------------------- sampling on the device
+    def set_sampling(self, temperature: float, top_k: int, top_p: float, min_p: float, uniforms,
+                     start: int) -> None:
+        """Settings and numbers of the tokens that `draw` and `replay_sampled`
+        draw: the token behind position p takes uniforms[p - start]. They stay in
+        device memory, so one recorded step serves every setting."""
+        if top_k < 0 or not top_p > 0 or not 0 <= min_p <= 1 or temperature != temperature:
+            raise SFError(f"need top_k >= 0, top_p > 0, 0 <= min_p <= 1 (got {top_k}, {top_p}, {min_p}; "
+                          f"temperature {temperature})")
+        u = torch.as_tensor(uniforms, dtype=torch.float32).reshape(-1).to(self.device)
+        if start < 0 or start + u.numel() > self.max_seq + 1:
+            raise SFError(f"{u.numel()} numbers from position {start} exceed the cache capacity {self.max_seq}")
+        if self._u is None:  # fixed buffers: the recorded step keeps their addresses
+            self._u = torch.zeros((self.max_seq + 1,), dtype=torch.float32, device=self.device)
+            self._settings = torch.zeros((3,), dtype=torch.float32, device=self.device)
+            self._top_k = torch.zeros((1,), dtype=torch.int32, device=self.device)
+        self._u[start:start + u.numel()].copy_(u)
+        self._settings.copy_(torch.tensor([temperature, top_p, min_p]))
+        self._top_k.fill_(int(top_k))
+
+    def _draw(self) -> None:
+        """The token behind the last position from `self.logits`, to `self.token`
+        and `self.hist` (the position counter is one past it)."""
+        s = self._settings
+        sample(self.logits.view(1, -1), self._u, temperature=s[0:1], top_k=self._top_k, top_p=s[1:2],
+               min_p=s[2:3], out=self.token, at=self.pos_dev, at_add=-1, hist=self.hist)
+
+    def draw(self) -> int:
+        """Draw the token behind the prompt from its last row's logits."""
+        if self._u is None:
+            raise SFError("set_sampling() first")
+        self._draw()
+        return int(self.token.item())
+
+    def replay_sampled(self, n: int = 1) -> None:
+        """n decode steps that draw their tokens (recorded on first use): the
+        greedy step with its logits kept, then the draw in the token's place."""
+        if self._u is None:
+            raise SFError("set_sampling() first")
+        if self.pos + n > self.max_seq:
+            raise SFError("decode would exceed the cache capacity")
+        if self._sampled_graph is None:
+            torch.cuda.synchronize(self.device)
+            s, g = torch.cuda.Stream(self.device), torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                self.decode_step(logits=True)
+                self._draw()
+            torch.cuda.synchronize(self.device)
+            self._sampled_graph = g
+        for _ in range(n):
+            self._sampled_graph.replay()
         self.pos += n
 
     # -------------------------------------------------------------- generate

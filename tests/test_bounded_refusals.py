@@ -108,7 +108,7 @@ def test_evict_c(kw, code, text):
 
 def samp(**kw):
     a = dict(logits=P, dtype=F32, stride=1000, B=2, V=1000, u=P, t=1.0, k=0, p=1.0, m=0.0, ts=None, ks=None, ps=None,
-             ms=None, tokens=P, lp=None, ws=P, ws_bytes=1 << 40, stream=None)
+             ms=None, tokens=P, lp=None, at=None, add=0, un=2, hist=None, ws=P, ws_bytes=1 << 40, stream=None)
     a.update(kw)
     return _lib.load().sf_sample(*a.values())
 
@@ -119,6 +119,7 @@ def samp(**kw):
     (dict(t=float("nan")), -1, "temperature"), (dict(k=-1), -1, "top_k >= 0"), (dict(p=0.0), -1, "top_p > 0"),
     (dict(p=float("nan")), -1, "top_p > 0"), (dict(m=1.5), -1, "min_p <= 1"), (dict(m=-0.1), -1, "0 <= min_p"),
     (dict(u=None), -1, "null"), (dict(tokens=None), -1, "null"), (dict(ws=None), -1, "256-byte aligned"),
+    (dict(at=P, un=1), -1, "1 numbers for 2 rows"), (dict(hist=P), -1, "hist without at"),
     (dict(ws_bytes=100), -1, "too small"), (dict(B=1 << 30, V=1 << 20), -1, "exceed the grid"),
 ])
 def test_sample_c(kw, code, text):

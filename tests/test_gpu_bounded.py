@@ -1,0 +1,191 @@
+"""The bounded cache's operators together, as the framework runs them: tokens turned
+and appended, attention that scores the slots, eviction, and drawn tokens, step by step
+against the 64-bit oracle; the Attention module over a bounded cache; generation from
+given numbers."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import bounded
+from siliconfer_amd._lib import SFError
+from siliconfer_amd.engine.generate import SamplingParams, generate, sample_token
+from siliconfer_amd.kernels.rotary import rotary
+from siliconfer_amd.model import BoundedKVCache, QuantizedKVCache, Rotary, rotary_frequencies
+from siliconfer_amd.model.config import ModelConfig
+from siliconfer_amd.model.layers import Attention, compute_rope_freqs
+from siliconfer_amd.model.llama import LlamaModel
+
+pytestmark = pytest.mark.gpu
+H, KVH, D = 6, 2, 64
+
+
+def buffers(c):
+    return [t.cpu().numpy().copy() for t in (*c.buffers(), c.scores, c.positions)]
+
+
+@pytest.mark.parametrize("B,steps", [(1, [20] + [1] * 30), (3, [5, 1, 1, 16, 1, 9] + [1] * 12)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_steps_against_the_oracle(dev, B, steps, interleaved):
+    r = Rotary(*rotary_frequencies(48, 1e4, {"type": "yarn", "factor": 4.0}, trained=64), interleaved)
+    cache = BoundedKVCache(budget=16, recent=4, slack=3)
+    g = torch.Generator().manual_seed(B)
+    seen = length = 0
+    for T in steps:
+        qkv = torch.randn(B, T, (H + 2 * KVH) * D, generator=g).to(dev)
+        q = cache.append_rotary(qkv, H, KVH, r)
+        length, seen = length + T, seen + T
+        assert cache.length() == length and cache.seen == seen
+        x = qkv.view(B, T, H + 2 * KVH, D)
+        pos = torch.arange(seen - T, seen, device=dev)
+        want_q, _ = rotary(x[:, :, :H], None, pos, r.on(dev), interleaved=interleaved, scale=r.scale)
+        assert torch.equal(q, want_q)
+        kc, ks, vc, vs, sc, ps = buffers(cache)
+        assert (sc[:, :, length - T:length] == 0).all()
+        assert np.array_equal(ps[:, :, length - T:length], np.broadcast_to(pos.cpu().numpy(), (B, KVH, T)))
+        out = cache.attend(q)
+        ref, add, ob, ab = bounded.attention_scored(q.cpu().numpy(), kc, ks, vc, vs, [length] * B)
+        assert (abs(out.cpu().numpy() - ref) <= ob + 2.0 ** -24 * abs(ref)).all()
+        before = buffers(cache)
+        want = sc.astype(np.float64) + add
+        assert (abs(before[4] - want) <= ab + 2.0 ** -24 * abs(want)).all()
+        cache.evict()
+        if length > 16 + 3:
+            expect, n = bounded.evict(before, before[4], before[5], [length] * B, [seen] * B, 16, 4)
+            length = int(n[0])
+            assert length == 16
+            after = buffers(cache)
+            # as bytes: slots never written hold anything, NaN too
+            assert all(np.array_equal(a.view(np.uint8), e.view(np.uint8)) for a, e in zip(after, expect))
+            assert set(range(seen - 4, seen)) <= set(after[5][0, 0, :16].tolist())
+        assert cache.length() == length <= 19
+
+
+def test_the_cache_s_own_rules(dev):
+    cache = BoundedKVCache(budget=8, slack=2)
+    k = torch.randn(1, 2, 12, 64, generator=torch.Generator().manual_seed(0)).to(dev)
+    cache.append(k[:, :, :5], k[:, :, :5])
+    cache.trim(3)
+    assert cache.length() == cache.seen == 3
+    cache.append(k, k)
+    assert cache.length() == cache.seen == 15 and cache.positions[0, 0, :15].tolist() == list(range(15))
+    cache.evict()
+    assert cache.length() == 8 and cache.seen == 15
+    with pytest.raises(SFError, match="cannot be trimmed"):
+        cache.trim(4)
+    with pytest.raises(SFError):
+        cache.set_length(2)
+    for bad in ((0,), (8, 9), (8, 2, -1)):
+        with pytest.raises(SFError):
+            BoundedKVCache(*bad)
+
+
+def layer(dev, rot):
+    c = ModelConfig(hidden_size=128, num_attention_heads=4, num_key_value_heads=2, head_dim=64, rope_theta=1e4)
+    torch.manual_seed(3)
+    return Attention(c, compute_rope_freqs(c, dev), dev, rot)
+
+
+@pytest.mark.parametrize("rot", [None, Rotary(*rotary_frequencies(32, 1e4), interleaved=True)], ids=["half", "part"])
+def test_attention_within_the_bound_equals_the_unbounded_cache(dev, rot):
+    """A bound that is never reached: prompts (scored by their last rows), chunks and
+    single tokens give what the plain int8 cache gives, which for `rot` holds the same
+    codes (2e-5: fp32 sums in another order) and for rotate-half codes of fp32 angles
+    (the 2e-3 bar of the attention tests)."""
+    attn = layer(dev, rot)
+    g = torch.Generator().manual_seed(4)
+    plain, bound = QuantizedKVCache(64), BoundedKVCache(budget=200)
+    for T in (40, 7, 1, 1, 33, 1):
+        x = torch.randn(1, T, 128, generator=g).to(dev)
+        with torch.no_grad():
+            a, _ = attn(x, plain)
+            b, c = attn(x, bound)
+        assert c is bound and b.shape == a.shape
+        err = ((a - b).norm() / a.norm()).item()
+        assert err <= (2e-5 if rot else 2e-3), (T, err)
+    assert bound.length() == plain.length() == 83
+    # every observed row adds 1 a query head: 4 heads over 2 kv heads, of the prompts' rows the last 16
+    assert torch.allclose(bound.scores[0, :, :83].sum(-1).cpu(), torch.full((2,), 2.0 * (16 + 7 + 1 + 1 + 16 + 1)), rtol=1e-5)
+
+
+def test_batched_attention_over_a_bounded_cache(dev):
+    """A batch equals its sequences one by one, past evictions (2e-5 as above)."""
+    attn = layer(dev, None)
+    g = torch.Generator().manual_seed(5)
+    both, each = BoundedKVCache(24, 6, 4), [BoundedKVCache(24, 6, 4) for _ in range(2)]
+    for T in [30] + [1] * 12 + [18, 1, 1]:
+        x = torch.randn(2, T, 128, generator=g).to(dev)
+        with torch.no_grad():
+            a, _ = attn(x, both)
+            b = torch.cat([attn(x[i:i + 1], each[i])[0] for i in range(2)])
+        assert ((a - b).norm() / b.norm()).item() <= 2e-5, T
+    assert both.length() == each[0].length() <= 28
+    for i in range(2):
+        n = both.length()
+        assert torch.equal(both.positions[i, :, :n], each[i].positions[0, :, :n])
+
+
+def test_rotary_over_every_cache_form(dev):
+    """The same layer without a cache, over full-precision tensors and over int8 codes."""
+    rot = Rotary(*rotary_frequencies(32, 1e4), interleaved=True)
+    attn = layer(dev, rot)
+    x = torch.randn(1, 9, 128, generator=torch.Generator().manual_seed(6)).to(dev)
+    with torch.no_grad():
+        full, _ = attn(x)
+        head, kv = attn(x[:, :5])
+        tail, _ = attn(x[:, 5:], kv)
+        int8, _ = attn(x, QuantizedKVCache(16))
+    assert ((torch.cat([head, tail], 1) - full).norm() / full.norm()).item() <= 2e-5
+    assert ((int8 - full).norm() / full.norm()).item() <= 2e-2  # 8-bit codes
+
+
+@pytest.fixture(scope="module")
+def model():
+    c = ModelConfig(hidden_size=128, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2,
+                    num_key_value_heads=1, head_dim=64, vocab_size=1000, rope_theta=1e4, tie_word_embeddings=True)
+    return LlamaModel.random_init(c, seed=7, group_size=64, max_seq=96, std=0.15)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(temperature=0.7, top_k=40, top_p=0.9), dict(min_p=0.05), dict(temperature=0.0)])
+def test_generate_from_given_numbers(dev, model, kw):
+    """Every token is the oracle's draw from the step's logits; replays, callbacks and the
+    end of sequence behave as in the greedy path."""
+    u = np.random.default_rng(8).random(40).astype(np.float32)
+    params = SamplingParams(max_tokens=40, **kw)
+    prompt = [5, 17, 300, 4, 9]
+    got = generate(model, prompt, params, uniforms=u)
+    p = dict(temperature=params.temperature, top_k=params.top_k, top_p=float(np.float32(params.top_p)),
+             min_p=float(np.float32(params.min_p)))
+    p["temperature"] = float(np.float32(p["temperature"]))
+    model.reset()
+    model.prefill(prompt, want_logits=True)
+    for i, tok in enumerate(got.token_ids):
+        want, _, near = bounded.sample(model.logits.cpu().numpy(), float(u[i]), **p)
+        assert tok == want or tok in near, (i, tok, want)
+        model.token.fill_(tok)
+        model.decode_step(logits=True)
+        model.pos += 1
+    seen = []
+    again = generate(model, prompt, params, uniforms=torch.from_numpy(u), on_token=seen.append)
+    assert again.token_ids == got.token_ids == seen
+    eos = got.token_ids[20]
+    cut = generate(model, prompt, params, uniforms=u.tolist(), eos_token_id=eos)
+    assert cut.token_ids == got.token_ids[:got.token_ids.index(eos) + 1]
+    if params.temperature == 0:
+        assert got.token_ids == generate(model, prompt, params).token_ids
+
+
+def test_generate_refusals(dev, model):
+    with pytest.raises(SFError, match="3 uniforms for 4 tokens"):
+        generate(model, [1], SamplingParams(max_tokens=4), uniforms=[0.1, 0.2, 0.3])
+    with pytest.raises(SFError, match="repetition penalty"):
+        generate(model, [1], SamplingParams(max_tokens=1, repetition_penalty=1.2), uniforms=[0.1])
+    with pytest.raises(SFError, match="min_p <= 1"):
+        generate(model, [1], SamplingParams(max_tokens=1, min_p=1.5), uniforms=[0.1])
+
+
+def test_sample_token_min_p(dev):
+    x = torch.log(torch.tensor([0.5, 0.3, 0.15, 0.05], device=dev))
+    g = torch.Generator(device=dev).manual_seed(0)
+    drawn = {sample_token(x, SamplingParams(min_p=0.4), generator=g) for _ in range(200)}
+    assert drawn == {0, 1}
