@@ -245,22 +245,32 @@ def lengths_arg(lengths, B: int, device: torch.device, name: str = "lengths") ->
 def check_cache(device: torch.device, k_codes, k_scales, v_codes, v_scales, positions=None,
                 scores=None) -> None:
     """The buffers of an int8 cache: codes [B, KVH, T_cap, D], the others [B, KVH, T_cap]."""
-    rows = k_codes.shape[:3]
     if k_codes.dtype is not torch.int8 or v_codes.dtype is not torch.int8:
         raise SFError("KV codes must be int8")
-    if k_scales.dtype != v_scales.dtype or k_scales.dtype not in (torch.float16, torch.float32):
+    if k_scales.dtype is not v_scales.dtype or k_scales.dtype not in (torch.float16, torch.float32):
         raise SFError("k/v scales must both be float16 or both float32")
-    for t, n, dtype in ((k_codes, "k_codes", None), (v_codes, "v_codes", None), (k_scales, "k_scales", None),
-                        (v_scales, "v_scales", None), (positions, "slot positions", torch.int32),
-                        (scores, "scores", torch.float32)):
-        if t is None:
-            continue
-        if t.device != device or not t.is_contiguous():
-            raise SFError(f"{n} must be contiguous on {device}")
-        if t.shape[:3] != rows or (t.dim() != 3 and n[2:] != "codes"):
-            raise SFError(f"{n} must be {list(rows)} (got {list(t.shape)})")
-        if dtype is not None and t.dtype is not dtype:
-            raise SFError(f"{n} must be {dtype}")
+    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
+        raise SFError("k_codes / v_codes must both be [B, n_kv_heads, T, head_dim]")
+    rows = k_codes.shape[:3]
+    _check_buffer(k_codes, "k_codes", None, device)
+    _check_buffer(v_codes, "v_codes", None, device)
+    _check_buffer(k_scales, "k_scales", rows, device)
+    _check_buffer(v_scales, "v_scales", rows, device)
+    if positions is not None:
+        _check_buffer(positions, "slot positions", rows, device)
+        if positions.dtype is not torch.int32:
+            raise SFError("slot positions must be int32")
+    if scores is not None:
+        _check_buffer(scores, "scores", rows, device)
+        if scores.dtype is not torch.float32:
+            raise SFError("scores must be float32")
+
+
+def _check_buffer(t: torch.Tensor, name: str, rows, device: torch.device) -> None:
+    if not t.is_contiguous() or t.device != device:
+        raise SFError(f"{name} must be contiguous on {device}")
+    if rows is not None and t.shape != rows:
+        raise SFError(f"{name} must be {list(rows)} (got {list(t.shape)})")
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -14,6 +14,7 @@ count for MI355X (`default_splits`) rather than
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -113,6 +114,12 @@ def fused_quantized_attention_decode(q, k_codes, k_scales, v_codes, v_scales,
                             v_scales.contiguous(), n_splits=n_tiles)
 
 
+@functools.lru_cache(maxsize=256)
+def _scored_bytes(B: int, Tq: int, H: int, KVH: int, T_max: int, D: int, n: int) -> int:
+    """sf_attn_scored_workspace_bytes of a shape."""
+    return int(_lib.load().sf_attn_scored_workspace_bytes(B, Tq, H, KVH, T_max, D, n))
+
+
 def attention_decode_scored(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
                             v_codes: torch.Tensor, v_scales: torch.Tensor, scores: torch.Tensor, *,
                             lengths, add: int = 0, max_length: int | None = None,
@@ -132,10 +139,10 @@ def attention_decode_scored(q: torch.Tensor, k_codes: torch.Tensor, k_scales: to
     _lib.require_device(q, "q")
     B, H, D = q.shape[0], q.shape[-2], q.shape[-1]
     Tq = 1 if three else q.shape[1]
-    if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+    if k_codes.dim() != 4:
         raise SFError("k_codes / v_codes must both be [B, n_kv_heads, T, head_dim]")
-    KVH, T_cap = k_codes.shape[1], k_codes.shape[2]
-    if k_codes.shape[0] != B or k_codes.shape[3] != D:
+    Bc, KVH, T_cap, Dc = k_codes.shape
+    if Bc != B or Dc != D:
         raise SFError("cache shape does not match q")
     if D > _MAX_HEAD_DIM:
         raise ValueError(f"head_dim={D} exceeds kernel's compile-time max {_MAX_HEAD_DIM}")
@@ -148,14 +155,14 @@ def attention_decode_scored(q: torch.Tensor, k_codes: torch.Tensor, k_scales: to
             raise SFError(f"{T} slots of a cache of {T_max}")
         T_max = T
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+        out = torch.empty_like(q, dtype=out_dtype)
     elif out.shape != q.shape or out.device != q.device or not out.is_contiguous():
         raise SFError("out must be contiguous, of q's shape and on its device")
     lib = _lib.load()
     n = n_splits or 0
     with _lib.on_device(q):
         st = _lib.stream(q)
-        ws = _lib.scratch(q.device, st, lib.sf_attn_scored_workspace_bytes(B, Tq, H, KVH, T_max, D, n))
+        ws = _lib.scratch(q.device, st, _scored_bytes(B, Tq, H, KVH, T_max, D, n))
         rc = lib.sf_attn_decode_scored_i8kv(
             q.data_ptr(), _lib.dt(q), k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(),
             v_scales.data_ptr(), _lib.dt(k_scales), scores.data_ptr(), out.data_ptr(), _lib.dt(out), ws.data_ptr(),

@@ -26,7 +26,7 @@ def evict(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, 
     had so far): int32 [B] on the device, or one int for all. Slots at and past the
     new length are left as they were."""
     _lib.require_device(k_codes, "k_codes")
-    if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+    if k_codes.dim() != 4:
         raise SFError("k_codes / v_codes must both be [B, n_kv_heads, T, head_dim]")
     B, KVH, T_cap, D = k_codes.shape
     _lib.check_cache(k_codes.device, k_codes, k_scales, v_codes, v_scales, positions, scores)

@@ -111,7 +111,7 @@ def rotary_kv_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch
     [B] on the device, or one int for every sequence; they are not changed. Device
     lengths are not checked against the capacity: a token past it is not stored."""
     _lib.require_device(qkv, "qkv")
-    if qkv.dim() != 3 or k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+    if qkv.dim() != 3 or k_codes.dim() != 4:
         raise SFError("qkv must be [B, T, width], k_codes / v_codes both [B, n_kv_heads, T, head_dim]")
     B, T, W = qkv.shape
     KVH, T_cap, D = k_codes.shape[1:]
