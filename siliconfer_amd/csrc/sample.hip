@@ -141,6 +141,7 @@ k_sample_bins(const void *__restrict__ logits, long long row_stride, int V, int 
               ChunkOut *__restrict__ outs) {
   __shared__ u64 bins[kBins];
   __shared__ float red[kBinWaves];
+  __shared__ uint2 list[kListCap];
   __shared__ int list_bins, list_n;
   const int b = blockIdx.x / chunks, c = blockIdx.x - b * chunks;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -226,13 +227,19 @@ k_sample_bins(const void *__restrict__ logits, long long row_stride, int V, int 
     if (lane == 0) list_bins = full == 64 ? kBins : 4 * full + fit;
   }
   __syncthreads();
+  // the list: a thread's hits take consecutive places of it in LDS, then it goes out whole
+  int hits = 0;
 #pragma unroll
-  for (int k = 0; k < kPerThread; ++k)
-    if (bin[k] < list_bins) {
-      const int at = atomicAdd(&list_n, 1);
-      o->list[at] = (u64)order_key(x[k]) << 32 | (uint32_t)~(i0 + k * kBinThreads);
-    }
+  for (int k = 0; k < kPerThread; ++k) hits += bin[k] < list_bins;
+  if (hits) {
+    int at = atomicAdd(&list_n, hits);
+#pragma unroll
+    for (int k = 0; k < kPerThread; ++k)
+      if (bin[k] < list_bins) list[at++] = make_uint2(i0 + k * kBinThreads, sf_bitcast<uint32_t>(x[k]));
+  }
   __syncthreads();
+  if ((int)threadIdx.x < list_n)
+    o->list[threadIdx.x] = (u64)order_key(sf_bitcast<float>(list[threadIdx.x].y)) << 32 | (uint32_t)~list[threadIdx.x].x;
   if (threadIdx.x == 0) o->list_n = list_n, o->list_bins = list_bins;
 }
 
@@ -519,9 +526,20 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
   __shared__ PickSmem sm;
   const int b = blockIdx.x, lane = threadIdx.x & 63;
   const ChunkOut *o = outs + (size_t)b * chunks;
+  // the chunks' bins and lists are on their way before the maximum says where they belong
+  constexpr int kAhead = 8, kParts = kSampThreads / kBins;  // (32 chunks: 262144 tokens)
+  const int my_bin = threadIdx.x & (kBins - 1), part = threadIdx.x / kBins;
+  u64 v[kAhead];
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    const int c = part + j * kParts;
+    v[j] = c < chunks ? o[c].bins[my_bin] : 0;
+  }
   u64 best = 0;
   for (int c = lane; c < chunks; c += 64) best = o[c].best > best ? o[c].best : best;
+  if (threadIdx.x < kBins) sm.w[threadIdx.x] = 0, sm.n[threadIdx.x] = 0;
   best = wave_max(best);
+  __syncthreads();
   uint32_t kmax = (uint32_t)(best >> 32);
   const float T = rp.t(b);
   const bool empty = kmax == kNoKey;
@@ -538,32 +556,18 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
   const double M = (double)key_value(kmax), inv_t = fmax(1.0 / (double)T, 1e-300), per = bins_per_logit(T);
   Row<DT> row = {logits, (size_t)b * row_stride, V, chunks, per, top_bin((float)M, per), 0, flat, o, sm, -1};
   row.chunk_top = flat ? INFINITY : row.top;
-  // the row's bins: four threads a bin, each every fourth chunk
-  {
-    const int bin = threadIdx.x & (kBins - 1), part = threadIdx.x / kBins;
-    u64 n = 0, w = 0;
-    for (int c = part; c < chunks; c += kSampThreads / kBins) {
-      const double shift = o[c].top == row.chunk_top ? 0.0 : row.chunk_top - o[c].top;
-      if (shift <= (double)bin) {
-        const u64 v = o[c].bins[bin - (int)shift];
-        n += v >> kCountShift;
-        w += v & kWeightMask;
-      }
-    }
-    sm.raw[threadIdx.x] = n;
-    sm.el[threadIdx.x] = w;
-    __syncthreads();
-    if (threadIdx.x < kBins) {
+  // the row's bins (whole numbers: the order of the additions changes nothing)
+  for (int c = part, j = 0; c < chunks; c += kParts, ++j) {
+    const double shift = o[c].top == row.chunk_top ? 0.0 : row.chunk_top - o[c].top;
+    u64 e = j < kAhead ? 0 : o[c].bins[my_bin];
 #pragma unroll
-      for (int j = 1; j < kSampThreads / kBins; ++j) {
-        n += sm.raw[threadIdx.x + j * kBins];
-        w += sm.el[threadIdx.x + j * kBins];
-      }
-      sm.n[bin] = (int)n;
-      sm.w[bin] = w;
-      sm.fac[bin] = exp(-kDelta * bin) * 0x1p-36;
+    for (int i = 0; i < kAhead; ++i) e = i == j ? v[i] : e;
+    if (e && shift < (double)(kBins - my_bin)) {
+      atomicAdd(&sm.w[my_bin + (int)shift], e & kWeightMask);
+      atomicAdd(&sm.n[my_bin + (int)shift], (int)(e >> kCountShift));
     }
   }
+  if (threadIdx.x < kBins) sm.fac[threadIdx.x] = exp(-kDelta * (int)threadIdx.x) * 0x1p-36;
   __syncthreads();
   if (threadIdx.x < 64) {  // prefix sums, lane l: bins 4 l .. 4 l + 3
     double v[4], sum = 0;
