@@ -209,7 +209,7 @@ def stream(t: torch.Tensor | None = None) -> int:
 
 def on_device(t: torch.Tensor):
     """A context in which t's device is the current one (launches go there)."""
-    return _NOTHING if torch.cuda.current_device() == t.get_device() else torch.cuda.device(t.device)
+    return _NOTHING if torch._C._cuda_getDevice() == t.get_device() else torch.cuda.device(t.device)
 
 
 _NOTHING = contextlib.nullcontext()
@@ -220,7 +220,7 @@ def scratch(device: torch.device, stream_handle: int, nbytes: int) -> torch.Tens
     """Workspace of one call: kept a (device, stream) and grown on demand, whose
     calls run one after the other; while a graph is recorded a tensor of the graph's
     own, so that no two graphs share one."""
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
     key = (device, stream_handle)
     ws = _scratch.get(key)
@@ -244,7 +244,26 @@ def lengths_arg(lengths, B: int, device: torch.device, name: str = "lengths") ->
 
 def check_cache(device: torch.device, k_codes, k_scales, v_codes, v_scales, positions=None,
                 scores=None) -> None:
-    """The buffers of an int8 cache: codes [B, KVH, T_cap, D], the others [B, KVH, T_cap]."""
+    """The buffers of an int8 cache: codes [B, KVH, T_cap, D], the others [B, KVH, T_cap],
+    all contiguous on `device`."""
+    at, rows, i8, dt = device.index, k_codes.shape[:-1], torch.int8, k_scales.dtype
+    if not (k_codes.get_device() == v_codes.get_device() == k_scales.get_device() == v_scales.get_device() == at
+            and k_codes.dtype is i8 and v_codes.dtype is i8 and v_scales.dtype is dt
+            and (dt is torch.float16 or dt is torch.float32) and v_codes.shape == k_codes.shape
+            and k_scales.shape == rows and v_scales.shape == rows and k_codes.is_contiguous()
+            and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()):
+        _explain_cache(device, k_codes, k_scales, v_codes, v_scales)
+    if positions is not None:
+        _check_buffer(positions, "slot positions", rows, device)
+        if positions.dtype is not torch.int32:
+            raise SFError("slot positions must be int32")
+    if scores is not None:
+        _check_buffer(scores, "scores", rows, device)
+        if scores.dtype is not torch.float32:
+            raise SFError("scores must be float32")
+
+
+def _explain_cache(device: torch.device, k_codes, k_scales, v_codes, v_scales) -> None:
     if k_codes.dtype is not torch.int8 or v_codes.dtype is not torch.int8:
         raise SFError("KV codes must be int8")
     if k_scales.dtype is not v_scales.dtype or k_scales.dtype not in (torch.float16, torch.float32):
@@ -256,14 +275,6 @@ def check_cache(device: torch.device, k_codes, k_scales, v_codes, v_scales, posi
     _check_buffer(v_codes, "v_codes", None, device)
     _check_buffer(k_scales, "k_scales", rows, device)
     _check_buffer(v_scales, "v_scales", rows, device)
-    if positions is not None:
-        _check_buffer(positions, "slot positions", rows, device)
-        if positions.dtype is not torch.int32:
-            raise SFError("slot positions must be int32")
-    if scores is not None:
-        _check_buffer(scores, "scores", rows, device)
-        if scores.dtype is not torch.float32:
-            raise SFError("scores must be float32")
 
 
 def _check_buffer(t: torch.Tensor, name: str, rows, device: torch.device) -> None:

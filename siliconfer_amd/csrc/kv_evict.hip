@@ -168,7 +168,7 @@ k_evict_select(EvictArgs a) {
     }
   }
   waves_before(newest, cnt, &n_newest);  // (a barrier: the histogram is whole)
-  // t: the key of the last slot that stays; `stay` of its ties do
+  // t: the key from which on slots stay; of the n_ties with (at least) its digits `stay` do
   uint32_t t = kProtected;
   int stay = budget, n_ties = n_newest;
   if (n_newest < budget) {
@@ -208,6 +208,7 @@ k_evict_select(EvictArgs a) {
       mask |= digits << shift;
       stay -= found[1];
       n_ties = found[2];
+      if (n_ties == stay) break;  // every key from this digit on stays: no lower digits to find
     }
     t = prefix;
   }

@@ -25,19 +25,19 @@ _STRIDES = ctypes.c_longlong * 12
 _INT = (torch.int32, torch.int64)
 
 
-def _positions(positions: torch.Tensor, B: int, T: int, x: torch.Tensor) -> tuple[int, int]:
+def _positions(positions: torch.Tensor, B: int, T: int, x: torch.Tensor) -> tuple[bool, bool]:
     """(int64?, one row of positions a sequence?) of positions [B, T] or [T]."""
-    if positions.dtype not in _INT or not positions.is_contiguous() or positions.device != x.device:
+    dt, shape = positions.dtype, positions.shape
+    if dt not in _INT or not positions.is_contiguous() or positions.get_device() != x.get_device():
         raise SFError("positions must be contiguous int32 or int64 on the rows' device")
-    shape = tuple(positions.shape)
     if shape != (B, T) and shape != (T,):
         raise SFError(f"positions must be [{B}, {T}] or [{T}] (got {list(shape)})")
-    return positions.dtype is torch.int64, len(shape) == 2
+    return dt is torch.int64, len(shape) == 2
 
 
 def _pairs(inv_freq: torch.Tensor, D: int, x: torch.Tensor) -> int:
     if (inv_freq.dtype is not torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous()
-            or inv_freq.device != x.device):
+            or inv_freq.get_device() != x.get_device()):
         raise SFError("inv_freq must be a contiguous 1-D float64 tensor on the rows' device")
     n = inv_freq.shape[0]
     if not 0 < 2 * n <= D:
