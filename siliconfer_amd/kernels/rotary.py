@@ -83,6 +83,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     pairs = _pairs(inv_freq, D, q)
     strides = None
     if not plain:
+        for o in (out_q, out_k):
+            if o is not None and any(st == 0 and n > 1 for st, n in zip(o.stride(), o.shape)):
+                raise SFError("an output's rows must not share memory")
         _rows(out_q, "out_q")
         s = list(q.stride()[:3]) + list(out_q.stride()[:3])
         if k is not None:

@@ -11,6 +11,7 @@ from oracle import bounded
 from siliconfer_amd._lib import SFError
 from siliconfer_amd.engine.generate import SamplingParams, generate, sample_token
 from siliconfer_amd.kernels.rotary import rotary
+from siliconfer_amd.kernels.sampling import sample
 from siliconfer_amd.model import BoundedKVCache, QuantizedKVCache, Rotary, rotary_frequencies
 from siliconfer_amd.model.config import ModelConfig
 from siliconfer_amd.model.layers import Attention, compute_rope_freqs
@@ -137,6 +138,63 @@ def test_rotary_over_every_cache_form(dev):
         int8, _ = attn(x, QuantizedKVCache(16))
     assert ((torch.cat([head, tail], 1) - full).norm() / full.norm()).item() <= 2e-5
     assert ((int8 - full).norm() / full.norm()).item() <= 2e-2  # 8-bit codes
+
+
+def test_side_streams_keep_to_their_own_workspaces(dev):
+    """The same calls, interleaved over two streams, give what one stream gives."""
+    g = torch.Generator().manual_seed(9)
+    r = Rotary(*rotary_frequencies(64, 1e4))
+    qkv = [torch.randn(2, 600 if i == 0 else 1, (H + 2 * KVH) * D, generator=g).to(dev) for i in range(6)]
+    logits = torch.randn(4, 40000, generator=g).to(dev)
+    u = torch.rand(4, generator=g).to(dev)
+
+    def work():
+        cache, out = BoundedKVCache(300, 30, 0), []
+        for x in qkv:
+            q = cache.append_rotary(x, H, KVH, r)
+            out.append(cache.attend(q[:, -8:].contiguous()))
+            cache.evict()
+            n = cache.length()
+            out += [cache.scores[:, :, :n].clone(), cache.positions[:, :, :n].clone(), sample(logits, u, top_p=0.9)]
+        return out
+
+    want = work()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+    torch.cuda.synchronize()
+    for one in got:
+        assert all(torch.equal(a, b) for a, b in zip(one, want))
+
+
+def test_rotary_refuses_outputs_that_share_memory(dev):
+    q = torch.zeros(1, 3, 2, 64, device=dev)
+    f = Rotary(*rotary_frequencies(64)).on(dev)
+    pos = torch.arange(3, device=dev)
+    with pytest.raises(SFError, match="share memory"):
+        rotary(q, None, pos, f, out_q=q[:, :1].expand(1, 3, 2, 64))
+    with pytest.raises(SFError, match="head's dims"):
+        rotary(q.transpose(2, 3), None, pos, f[:1])
+    for bad in (pos.float(), pos[:2], pos.view(3, 1)):
+        with pytest.raises(SFError, match="positions"):
+            rotary(q, None, bad, f)
+    for bad in (f.float(), f.view(2, 16), torch.cat([f, f])):
+        with pytest.raises(SFError):
+            rotary(q, None, pos, bad)
+
+
+def test_sample_refusals(dev):
+    x, u = torch.zeros(2, 10, device=dev), torch.zeros(2, device=dev)
+    i = torch.zeros(1, dtype=torch.int32, device=dev)
+    for args, kw in (((x.t(), u), {}), ((x[0], u), {}), ((x, u.double()), {}), ((x, u[:1]), {}), ((x.double(), u), {}),
+                     ((x, u), dict(top_k=u)), ((x, u), dict(temperature=u[:1])), ((x, u), dict(hist=i)),
+                     ((x, u[:1]), dict(at=i)), ((x, u), dict(at=i, hist=u)), ((x, u), dict(out=u)),
+                     ((x, u), dict(top_p=0.0)), ((x, u), dict(min_p=2.0)), ((x, u), dict(temperature=float("nan")))):
+        with pytest.raises(SFError):
+            sample(*args, **kw)
 
 
 @pytest.fixture(scope="module")
