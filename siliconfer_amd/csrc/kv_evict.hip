@@ -17,7 +17,7 @@
 // out of it. Then the (hole, donor) list by ballots over the waves' segments. Few moves
 // are made by the same workgroup, many by a second launch over every CU.
 // Bound by the latency of its dozen barriers and of one read of scores and positions:
-// 9.0 us for 2 heads of 1088 slots, moves among them, 14.2 + 7.5 for 32 heads of up to 8191
+// 7.8 us for 2 heads of 1088 slots, moves among them, 13.3 + 7.4 for 32 heads of up to 8191
 // cut to 2048 (a search of the threshold bit pair by bit pair with counts over the
 // workgroup, keys in registers: 13.4 + 4.0 and 88 + 6.6; keys read again each time: 25 and 71).
 #include "sf_common.h"
@@ -307,7 +307,8 @@ extern "C" int sf_kv_evict(int8_t *k_codes, void *k_scales, int8_t *v_codes, voi
   int2 *pairs = (int2 *)((char *)workspace + sf_align256((size_t)B * KVH * sizeof(int)));
   hipStream_t st = (hipStream_t)stream;
   const int wide = D % 16 == 0 && (((uintptr_t)k_codes | (uintptr_t)v_codes) & 15) == 0;
-  // up to 64 KB a head: moved by the selecting workgroup (measured {RULE})
+  // up to 64 KB a head: moved by the selecting workgroup, a launch (2 us and its wait) less;
+  // 2 heads of 64 slots of 64 dims 13.4 + 4.0 us in two launches, 1.5 of the one's 7.8 here
   const int moves = (long long)most * (2 * D + 12) <= 64 << 10;
   const EvictArgs a = {k_codes, v_codes, k_scales, v_scales, scores, positions, lengths, seen, lengths_out, counts,
                        pairs, T, seen_host, budget, recent, most, KVH, T_cap, D, wide,

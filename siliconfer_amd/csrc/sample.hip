@@ -30,6 +30,12 @@
 // the one bin that the bins' prefix sums name; a bin of more than kBinCap elements (dense
 // ties, temperatures that squeeze the row into few bins) is searched by radix selection
 // over the order bits instead, eight bits a pass over the row.
+// Measured (us, first + second launch; a workgroup a row with radix passes over it in
+// brackets): 1 x 151936 fp32, top-k 50 and top-p, 6.1 + 9.5 (865); 64 x 151936 bf16, a
+// row's own settings, 19.0 + 13.6 (993), of them 3.8 for the bytes at a copy's rate. The
+// first launch is bound by VALU issue (47 instructions an element, half of the time) and
+// the five barriers of its workgroups, two a CU at a time; the second by the latency of
+// some twenty dependent steps of one workgroup a row.
 #include <math.h>
 
 #include "sf_common.h"
@@ -149,10 +155,16 @@ k_sample_bins(const void *__restrict__ logits, long long row_stride, int V, int 
   ChunkOut *o = outs + blockIdx.x;
   const int i0 = c * kChunk + threadIdx.x;
   float x[kPerThread];
+  if ((c + 1) * kChunk <= V) {
+    const size_t first = row + i0;
 #pragma unroll
-  for (int k = 0; k < kPerThread; ++k) {
-    const int i = i0 + k * kBinThreads;
-    x[k] = i < V ? sf_load_as_f32<DT>(logits, row + i) : -INFINITY;
+    for (int k = 0; k < kPerThread; ++k) x[k] = sf_load_as_f32<DT>(logits, first + k * kBinThreads);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPerThread; ++k) {
+      const int i = i0 + k * kBinThreads;
+      x[k] = i < V ? sf_load_as_f32<DT>(logits, row + i) : -INFINITY;
+    }
   }
   const float T = rp.t(b);
   float m = x[0];
@@ -255,12 +267,12 @@ struct PickSmem {
   int n[kBins];       // and count
   double before[kBins + 1], fac[kBins];  // weight before the bin, exp(-kDelta i) 2^-36
   int n_before[kBins + 1];
-  __attribute__((aligned(16))) u64 raw[kBinCap + 16];
-  u64 el[kBinCap], run[kBinCap];
+  u64 raw[kBinCap], el[kBinCap], run[kBinCap];
   u64 hist[256];
   u64 red[kSampWaves];
   u64 tmp[4];
-  int n_raw, uncovered;
+  int cursor[kBins];
+  int uncovered;
 };
 
 __device__ __forceinline__ u64 block_sum(u64 v, PickSmem &sm) {
@@ -302,13 +314,19 @@ struct Row {
         if (i0 + k * kSampThreads < V) f(i0 + k * kSampThreads, x[k]);
     }
   }
-  // The row's elements that `is` takes by their bin into sm.raw (count: sm.n_raw), up to
-  // bin `last`: from the chunks' lists where these have every bin up to it.
-  template <class Is>
-  __device__ __forceinline__ void gather(int last, Is is) {
-    __syncthreads();
-    if (threadIdx.x == 0) sm.n_raw = sm.uncovered = 0;
-    __syncthreads();
+  // The row's elements of the bins first .. last into sm.raw, bin after bin: from the chunks'
+  // lists where these have every bin up to `last`. Room has been made by the bins' counts.
+  __device__ __forceinline__ void gather(int first, int last) {
+    auto put = [&](int bin, u64 e) {
+      if (first <= bin && bin <= last) sm.raw[sm.n_before[bin] - sm.n_before[first] + atomicAdd(&sm.cursor[bin], 1)] = e;
+    };
+    auto clear = [&]() {
+      __syncthreads();
+      if (threadIdx.x < kBins) sm.cursor[threadIdx.x] = 0;
+      if (threadIdx.x == 0) sm.uncovered = 0;
+      __syncthreads();
+    };
+    clear();
     for (int c = threadIdx.x >> 6; c < chunks; c += kSampWaves) {
       const ChunkOut &o = outs[c];
       const double shift = o.top == chunk_top ? 0.0 : chunk_top - o.top;
@@ -316,17 +334,13 @@ struct Row {
       const u64 e0 = lane < ln ? o.list[lane] : 0, e1 = lane + 64 < ln ? o.list[lane + 64] : 0;
       if (!(shift <= (double)last)) continue;  // it has nothing there
       if (last - (int)shift >= o.list_bins) sm.uncovered = 1;
-      if (lane < ln && is(bin_of(key_value((uint32_t)(e0 >> 32)), per, top).bin)) sm.raw[atomicAdd(&sm.n_raw, 1)] = e0;
-      if (lane + 64 < ln && is(bin_of(key_value((uint32_t)(e1 >> 32)), per, top).bin)) sm.raw[atomicAdd(&sm.n_raw, 1)] = e1;
+      if (lane < ln) put(bin_of(key_value((uint32_t)(e0 >> 32)), per, top).bin, e0);
+      if (lane + 64 < ln) put(bin_of(key_value((uint32_t)(e1 >> 32)), per, top).bin, e1);
     }
     __syncthreads();
     if (sm.uncovered) {
-      __syncthreads();
-      if (threadIdx.x == 0) sm.n_raw = 0;
-      __syncthreads();
-      each([&](int i, float x) {
-        if (is(bin_of(x, per, top).bin)) sm.raw[atomicAdd(&sm.n_raw, 1)] = (u64)order_key(x) << 32 | (uint32_t)~i;
-      });
+      clear();
+      each([&](int i, float x) { put(bin_of(x, per, top).bin, (u64)order_key(x) << 32 | (uint32_t)~i); });
       __syncthreads();
     }
   }
@@ -336,20 +350,20 @@ struct Row {
     return bin_of(x, per, top).bin == bin;
   }
 
-  // sm.raw's n elements into sm.el in descending order, by counting the larger ones: sixteen
-  // at a time, so that their LDS reads fly together.
-  __device__ __forceinline__ void order(int n) {
-    if (threadIdx.x < 16) sm.raw[n + threadIdx.x] = 0;
-    __syncthreads();
+  // Those elements (n of them) into sm.el in descending order: each counts the larger ones
+  // of its bin, eight at a time so that their LDS reads fly together.
+  __device__ __forceinline__ void order(int first, int n) {
     if ((int)threadIdx.x < n) {
       const u64 e = sm.raw[threadIdx.x];
-      int rank = 0;
-      for (int i0 = 0; i0 < n; i0 += 16) {
-        ulonglong2 v[8];
+      const int bin = bin_of(key_value((uint32_t)(e >> 32)), per, top).bin;
+      const int lo = sm.n_before[bin] - sm.n_before[first], hi = sm.n_before[bin + 1] - sm.n_before[first];
+      int rank = lo;
+      for (int i0 = lo; i0 < hi; i0 += 8) {
+        u64 v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = ((const ulonglong2 *)sm.raw)[i0 / 2 + j];
+        for (int j = 0; j < 8; ++j) v[j] = sm.raw[min(i0 + j, hi - 1)];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) rank += (v[j].x > e) + (v[j].y > e);
+        for (int j = 0; j < 8; ++j) rank += i0 + j < hi && v[j] > e;
       }
       sm.el[rank] = e;
     }
@@ -361,8 +375,8 @@ struct Row {
     if (held == bin) return;
     held = bin;
     const int n = sm.n[bin];
-    gather(bin, [&](int at) { return at == bin; });
-    order(n);
+    gather(bin, bin);
+    order(bin, n);
     // running weights: a wave's scan, then the waves before it
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 run = (int)threadIdx.x < n ? weight((uint32_t)(sm.el[threadIdx.x] >> 32)) : 0;
@@ -620,9 +634,9 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
     head = min(row.bin_past(x, kBins - 1), m_bin);
   }
   if (sm.n_before[head + 1] <= kHeadCap) {
-    row.gather(head, [&](int at) { return at <= head; });
-    const int n = sm.n_raw;
-    row.order(n);
+    const int n = sm.n_before[head + 1];
+    row.gather(0, head);
+    row.order(0, n);
     if (threadIdx.x >= 64) return;
     // lane l: the places P l .. P l + P - 1 of the order
     constexpr int P = kHeadCap / 64;
