@@ -307,9 +307,10 @@ extern "C" int sf_kv_evict(int8_t *k_codes, void *k_scales, int8_t *v_codes, voi
   int2 *pairs = (int2 *)((char *)workspace + sf_align256((size_t)B * KVH * sizeof(int)));
   hipStream_t st = (hipStream_t)stream;
   const int wide = D % 16 == 0 && (((uintptr_t)k_codes | (uintptr_t)v_codes) & 15) == 0;
-  // up to 64 KB a head: moved by the selecting workgroup, a launch (2 us and its wait) less;
-  // 2 heads of 64 slots of 64 dims 13.4 + 4.0 us in two launches, 1.5 of the one's 7.8 here
-  const int moves = (long long)most * (2 * D + 12) <= 64 << 10;
+  // Moved by the selecting workgroup up to 96 KB a head (us in one launch / two, moves of
+  // every head to choose: 2 heads of 8 KB 7.6 / 9.3, 32 of 67 KB 9.8 / 10.4, 32 of 134 KB
+  // 12.5 / 12.7, 8 of 134 KB 12.0 / 11.5, 32 of 268 KB 15.3 / 15.0, 32 of 1.6 MB 30.7 / 21.2).
+  const int moves = (long long)most * (2 * D + 12) <= 96 << 10;
   const EvictArgs a = {k_codes, v_codes, k_scales, v_scales, scores, positions, lengths, seen, lengths_out, counts,
                        pairs, T, seen_host, budget, recent, most, KVH, T_cap, D, wide,
                        scale_dtype == SF_F16 ? 2 : 4, moves};

@@ -340,7 +340,11 @@ struct Row {
     __syncthreads();
     if (sm.uncovered) {
       clear();
-      each([&](int i, float x) { put(bin_of(x, per, top).bin, (u64)order_key(x) << 32 | (uint32_t)~i); });
+      // (the bins' range of logits, one bin wider each way, first; then exactly)
+      const float from = (float)((top - last - 2) / per), to = (float)((top - first + 2) / per);
+      each([&](int i, float x) {
+        if (x >= from && x <= to) put(bin_of(x, per, top).bin, (u64)order_key(x) << 32 | (uint32_t)~i);
+      });
       __syncthreads();
     }
   }
