@@ -27,13 +27,15 @@
 // these are gathered from the chunks' lists (from the row again where a list ends before
 // them) and one wave orders them by counting and applies every rule to the ordered
 // weights. Otherwise each filter's end and the draw are looked up one after the other in
-// the one bin that the bins' prefix sums name; a bin of more than kBinCap elements (dense
-// ties, temperatures that squeeze the row into few bins) is searched by radix selection
-// over the order bits instead, eight bits a pass over the row.
+// the one bin that the bins' prefix sums name; a bin of more than kBinCap elements (a large
+// vocabulary's bulk, dense ties) is cut into 256 ranges of keys, a pass over the row, until
+// the one that the search falls into can be ordered, as a rule after one pass.
 // Measured (us, first + second launch; a workgroup a row with radix passes over it in
 // brackets): 1 x 151936 fp32, top-k 50 and top-p, 6.1 + 9.5 (865); 64 x 151936 bf16, a
-// row's own settings, 19.0 + 13.6 (993), of them 3.8 for the bytes at a copy's rate. The
-// first launch is bound by VALU issue (47 instructions an element, half of the time) and
+// row's own settings, 19.0 + 13.6 (993), of them 3.8 for the bytes at a copy's rate; at
+// temperature alone a draw past the head re-reads its row: 8 x 32000 6.1 + 17.6 (two rows
+// in three within the head), of normal logits, none within it, 37 a call, 8 x 151936 112
+// (the one workgroup's VALU: some 45 a pass). The first launch is bound by VALU issue (47 instructions an element, half of the time) and
 // the five barriers of its workgroups, two a CU at a time; the second by the latency of
 // some twenty dependent steps of one workgroup a row.
 #include <math.h>
@@ -52,7 +54,7 @@ constexpr int kChunk = kBinThreads * kPerThread;
 constexpr int kBins = 256;
 constexpr double kDelta = 0.125;    // nats a bin
 constexpr int kListCap = 128;       // elements of a chunk's list
-constexpr int kBinCap = 1024;       // elements of a bin ordered by counting
+constexpr int kBinCap = 1024;       // elements of a bin, or of a range of keys, ordered at once
 constexpr int kHeadCap = 512;       // elements of the head: eight a lane of one wave
 constexpr int kCountShift = 50;     // 8192 weights of up to 2^36 take 49 bits and a little
 constexpr u64 kWeightMask = (1ull << kCountShift) - 1;
@@ -360,28 +362,79 @@ struct Row {
     if ((int)threadIdx.x < n) {
       const u64 e = sm.raw[threadIdx.x];
       const int bin = bin_of(key_value((uint32_t)(e >> 32)), per, top).bin;
-      const int lo = sm.n_before[bin] - sm.n_before[first], hi = sm.n_before[bin + 1] - sm.n_before[first];
-      int rank = lo;
-      for (int i0 = lo; i0 < hi; i0 += 8) {
-        u64 v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = sm.raw[min(i0 + j, hi - 1)];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) rank += i0 + j < hi && v[j] > e;
-      }
-      sm.el[rank] = e;
+      order_one(e, sm.raw, sm.n_before[bin] - sm.n_before[first], sm.n_before[bin + 1] - sm.n_before[first]);
     }
     __syncthreads();
+  }
+  // One element of from[lo .. hi) to its place.
+  __device__ __forceinline__ void order_one(u64 e, const u64 *from, int lo, int hi) {
+    int rank = lo;
+    for (int i0 = lo; i0 < hi; i0 += 8) {
+      u64 v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = from[min(i0 + j, hi - 1)];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rank += i0 + j < hi && v[j] > e;
+    }
+    sm.el[rank] = e;
+  }
+
+  // sm.raw's n elements, of the keys base .. base + 2^bits - 1, into sm.el in order, and their
+  // running weights into sm.run: by 256 ranges of keys, then by counting within a range (all
+  // of 1000 against each other: 27 us).
+  __device__ __forceinline__ void order_keys(uint32_t base, int bits, int n) {
+    const int lane = threadIdx.x, shift = max(bits - 8, 0);
+    const bool own = (int)threadIdx.x < n;
+    const u64 e = own ? sm.raw[threadIdx.x] : 0;
+    const int part = own ? 255 - (int)(((uint32_t)(e >> 32) - base) >> shift) : 0;
+    __syncthreads();
+    if (threadIdx.x < 256) sm.cursor[threadIdx.x] = 0;
+    __syncthreads();
+    const int slot = own ? atomicAdd(&sm.cursor[part], 1) : 0;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      int c[4], run = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) run += c[j] = sm.cursor[4 * lane + j];
+      const int sum = run;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(run, off, 64);
+        if (lane >= off) run += o;
+      }
+      run -= sum;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sm.hist[4 * lane + j] = run;
+        run += c[j];
+      }
+    }
+    __syncthreads();
+    const int lo = (int)sm.hist[part], hi = lo + sm.cursor[part];
+    if (own) sm.run[lo + slot] = e;
+    __syncthreads();
+    if (own) order_one(e, sm.run, lo, hi);
+    __syncthreads();
+    scan(n);
+  }
+  // The range of keys of a bin, two bins wider each way.
+  __device__ __forceinline__ void keys_of(int bin, uint32_t &base, int &bits) const {
+    base = order_key((float)((top - bin - 2) / per));
+    bits = 32 - __clz((int)((order_key((float)((top - bin + 2) / per)) - base) | 1));
   }
 
   // The elements of a bin of at most kBinCap into sm.el in order, running weights into sm.run.
   __device__ __forceinline__ void hold(int bin) {
     if (held == bin) return;
     held = bin;
-    const int n = sm.n[bin];
+    uint32_t base;
+    int bits;
+    keys_of(bin, base, bits);
     gather(bin, bin);
-    order(bin, n);
-    // running weights: a wave's scan, then the waves before it
+    order_keys(base, bits, sm.n[bin]);
+  }
+  // a wave's scan, then the waves before it
+  __device__ __forceinline__ void scan(int n) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 run = (int)threadIdx.x < n ? weight((uint32_t)(sm.el[threadIdx.x] >> 32)) : 0;
 #pragma unroll
@@ -398,79 +451,98 @@ struct Row {
 
   // The bin's first token whose running count, or weight, exceeds x (the last where none does).
   __device__ __forceinline__ Found find(int bin, double x, bool by_count) {
-    const int n = sm.n[bin];
+    int n = sm.n[bin];
+    const u64 all = by_count ? (u64)n : sm.w[bin];
+    u64 target = x >= (double)all ? all - 1 : x > 0 ? (u64)x : 0;
+    u64 above_w = 0;
     if (n <= kBinCap) {
       hold(bin);
-      const int t = threadIdx.x;
-      const bool over = t < n && (by_count ? (double)(t + 1) : (double)sm.run[t]) > x;
-      const int passed = (int)block_sum(t < n && !over, sm);
-      const int j = min(passed, n - 1);
-      const uint32_t key = (uint32_t)(sm.el[j] >> 32);
-      const bool tie = t < n && (uint32_t)(sm.el[t] >> 32) == key;
-      const u64 c = block_sum((u64)tie << 32 | (tie && t < j), sm);
-      return Found{key, c & 0xffffffffu, c >> 32, sm.run[j], (int)~(uint32_t)sm.el[j]};
-    }
-    // radix selection over the order bits of the bin's elements
-    const u64 all = by_count ? (u64)n : sm.w[bin];
-    const u64 target = x >= (double)all ? all - 1 : x > 0 ? (u64)x : 0;
-    uint32_t prefix = 0, mask = 0;
-    u64 above = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (threadIdx.x < 256) sm.hist[threadIdx.x] = 0;
-      __syncthreads();
-      each([&](int, float v) {
-        const uint32_t k = order_key(v);
-        if ((k & mask) == prefix) {
-          const Binned e = bin_of(v, per, top);
-          if (e.bin == bin) atomicAdd(&sm.hist[k >> shift & 255], by_count ? 1ull : e.w);
-        }
-      });
-      __syncthreads();
-      if (threadIdx.x < 64) {  // lane l: digits 255 - 4 l down to 252 - 4 l
-        u64 own = 0, d[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) own += d[j] = sm.hist[255 - 4 * (int)threadIdx.x - j];
-        u64 run = own;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          const u64 o = __shfl_up(run, off, 64);
-          if ((int)threadIdx.x >= off) run += o;
-        }
-        u64 before = above + run - own;
-        if (before <= target && target < above + run) {
-          int digit = -1;
-          u64 start = 0;
+    } else {
+      // The range of keys that the target falls into, 256 parts of it a pass over the row
+      // (highest first: their counts and weights), until a part's elements can be ordered
+      // or it is a single key.
+      held = -1;
+      uint32_t base;  // keys base .. base + 2^bits - 1
+      int bits;
+      keys_of(bin, base, bits);
+#pragma unroll 1
+      do {
+        const int shift = max(bits - 8, 0);
+        __syncthreads();
+        if (threadIdx.x < 256) sm.hist[threadIdx.x] = 0, sm.cursor[threadIdx.x] = 0;
+        __syncthreads();
+        each([&](int, float v) {
+          const uint32_t k = order_key(v) - base;
+          if ((u64)k >> bits == 0) {
+            const Binned e = bin_of(v, per, top);
+            if (e.bin == bin) {
+              atomicAdd(&sm.hist[255 - (k >> shift)], e.w);
+              atomicAdd(&sm.cursor[255 - (k >> shift)], 1);
+            }
+          }
+        });
+        __syncthreads();
+        if (threadIdx.x < 64) {  // lane l: parts 4 l .. 4 l + 3
+          const int lane = threadIdx.x;
+          u64 w = 0, c = 0;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if (digit < 0 && target < before + d[j]) {
-              digit = 255 - 4 * threadIdx.x - j;
-              start = before;
-            }
-            before += d[j];
+            w += sm.hist[4 * lane + j];
+            c += sm.cursor[4 * lane + j];
           }
-          sm.tmp[0] = digit;
-          sm.tmp[1] = start;
+          u64 w_run = w, c_run = c;
+#pragma unroll
+          for (int off = 1; off < 64; off <<= 1) {
+            const u64 ow = __shfl_up(w_run, off, 64), oc = __shfl_up(c_run, off, 64);
+            if (lane >= off) {
+              w_run += ow;
+              c_run += oc;
+            }
+          }
+          w_run -= w;
+          c_run -= c;
+          for (int j = 4 * lane; j < 4 * lane + 4; ++j) {
+            const u64 wj = sm.hist[j], cj = sm.cursor[j];
+            const u64 before = by_count ? c_run : w_run;
+            if (before <= target && target < before + (by_count ? cj : wj)) {
+              sm.tmp[0] = j;
+              sm.tmp[1] = w_run;
+              sm.tmp[2] = c_run;
+            }
+            w_run += wj;
+            c_run += cj;
+          }
         }
+        __syncthreads();
+        const int part = (int)sm.tmp[0];
+        base += (uint32_t)(255 - part) << shift;
+        bits = shift;
+        above_w += sm.tmp[1];
+        target -= by_count ? sm.tmp[2] : sm.tmp[1];
+        n = sm.cursor[part];
+      } while (n > kBinCap && bits > 0);
+      if (n > kBinCap) {  // ties alone
+        const u64 w = weight(base), r = by_count ? target : target / w;
+        return Found{base, r, (u64)n, above_w + (r + 1) * w, -1};
       }
       __syncthreads();
-      prefix |= (uint32_t)sm.tmp[0] << shift;
-      mask |= 255u << shift;
-      above = sm.tmp[1];
-    }
-    const u64 w = weight(prefix), r = by_count ? target - above : (target - above) / w;
-    u64 upto = above + (r + 1) * w, ties = 0;
-    if (by_count) {  // the weight above it has not been summed yet
-      u64 s = 0;
-      each([&](int, float v) {
+      if (threadIdx.x == 0) sm.cursor[0] = 0;
+      __syncthreads();
+      each([&](int i, float v) {
         const uint32_t k = order_key(v);
-        if (k > prefix && in(v, bin)) s += bin_of(v, per, top).w;
-        ties += k == prefix;
+        if ((u64)(k - base) >> bits == 0 && in(v, bin)) sm.raw[atomicAdd(&sm.cursor[0], 1)] = (u64)k << 32 | (uint32_t)~i;
       });
-      upto = block_sum(s, sm) + (r + 1) * w;
-      ties = block_sum(ties, sm);
+      __syncthreads();
+      order_keys(base, bits, n);
     }
-    return Found{prefix, r, ties, upto, -1};
+    const int t = threadIdx.x;
+    const bool over = t < n && (by_count ? (u64)(t + 1) : sm.run[t]) > target;
+    const int passed = (int)block_sum(t < n && !over, sm);
+    const int j = min(passed, n - 1);
+    const uint32_t key = (uint32_t)(sm.el[j] >> 32);
+    const bool tie = t < n && (uint32_t)(sm.el[t] >> 32) == key;
+    const u64 c = block_sum((u64)tie << 32 | (tie && t < j), sm);
+    return Found{key, c & 0xffffffffu, c >> 32, above_w + sm.run[j], (int)~(uint32_t)sm.el[j]};
   }
 
   // Weight of the bin's tokens that weigh at least `least` of the largest.

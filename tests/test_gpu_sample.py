@@ -149,3 +149,18 @@ def test_graph_replays(dev):
         want = sample(x, u, top_p=0.9)
         torch.cuda.synchronize()
         assert torch.equal(tok, want)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=9001), dict(top_p=0.6), dict(min_p=0.95), dict(temperature=8.0),
+                                dict(temperature=30.0, top_k=12345, top_p=0.7, min_p=0.9)], ids=str)
+def test_crowded_bins(dev, kw):
+    """Thousands of tokens within an eighth of a nat: spread over many keys, around zero
+    (where the keys' ranges are widest), around a power of two, a few values with many
+    ties each among single ones, and large values that the temperature brings together."""
+    rng = np.random.default_rng(5)
+    V = 40000
+    x = np.stack([rng.normal(0, 1, V), rng.uniform(-0.06, 0.06, V), 4 + rng.uniform(-0.05, 0.05, V),
+                  np.where(rng.random(V) < 0.5, 1 + rng.integers(0, 5, V) * 2.0 ** -9, rng.normal(1, 0.02, V)),
+                  rng.normal(0, 1e-40, V), -1000 + rng.normal(0, 0.3, V)]).astype(np.float32)
+    for u in (0.0, 0.37, 0.5, 0.93, 1 - 2 ** -24):
+        check(dev, torch.from_numpy(x), np.full(6, u), **kw)
