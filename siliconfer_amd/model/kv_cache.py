@@ -238,8 +238,9 @@ class BoundedKVCache(QuantizedKVCache):
         raise SFError("a bounded cache's slots are set by append and evict")
 
     def trim(self, n: int) -> None:
-        """Keep the first n positions: refused once tokens were dropped."""
-        if self.seen != self._len and n < self.seen:
+        """Keep the first n positions; once tokens were dropped all or none of them.
+        The scores keep what the rows behind them added."""
+        if self.seen != self._len and 0 < n < self.seen:
             raise SFError("a bounded cache that dropped tokens cannot be trimmed")
         super().trim(n)
         self.seen = min(self.seen, max(0, int(n)))

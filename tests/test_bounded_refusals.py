@@ -11,6 +11,7 @@ from siliconfer_amd.kernels.attention import attention_decode_scored
 from siliconfer_amd.kernels.eviction import evict
 from siliconfer_amd.kernels.rotary import rotary, rotary_kv_append
 from siliconfer_amd.kernels.sampling import sample
+from siliconfer_amd.model import BoundedKVCache
 
 P = 4096  # a pointer that is never followed: every call below is refused before its launch
 F32, F16, BF16 = _lib.SF_F32, _lib.SF_F16, _lib.SF_BF16
@@ -164,3 +165,17 @@ def test_cache_checks():
     for bad in (-1, 2 ** 31, torch.zeros(2), torch.zeros(3, dtype=torch.int32)):
         with pytest.raises(SFError):
             _lib.lengths_arg(bad, 2, cpu)
+
+
+def test_a_bounded_cache_starts_again():
+    """trim(0) begins a new sequence in the same buffers, tokens dropped or not."""
+    cache = BoundedKVCache(4, slack=2)
+    for length, seen in ((4, 9), (5, 5), (0, 0)):
+        cache._len, cache.seen = length, seen
+        cache.trim(0)
+        assert cache.length() == 0 and cache.seen == 0
+    cache._len, cache.seen = 4, 9
+    with pytest.raises(SFError, match="cannot be trimmed"):
+        cache.trim(3)
+    cache.trim(9)
+    assert cache.length() == 4 and cache.seen == 9
