@@ -12,6 +12,9 @@ path. It is the checker the HIP kernels are compared against:
 * `oracle.attention`  — int8 KV quantization and textbook softmax attention plus
   the split-T flash combine (reference `siliconfer/model/kv_cache.py`,
   `siliconfer/kernels/metal/q4_attention.py`).
+* `oracle.bounded`    — 64-bit rotary positions, scored decode attention, eviction by
+  score and drawing tokens from given numbers (the rules of reference
+  `siliconfer/engine/generate.py:24-67` for the draw; the others have no counterpart).
 * `oracle.cpu`        — ctypes bindings to `q4_cpu.c` (C restatement of the
   reference's scalar CPU kernels, used as the timed CPU baseline) and to
   `_ref/libref_q4.so` (the reference's own `q4_gemv.cpp`/`q4_gemm.cpp`

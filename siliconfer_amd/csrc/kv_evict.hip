@@ -10,7 +10,7 @@
 // and destinations are apart, every copy is independent of the others, and the
 // least is moved.
 //
-// k_evict_select: one workgroup a (sequence, kv head), the keys in its registers. The
+// k_evict_select: one workgroup a (sequence, kv head), up to 12288 keys in LDS. The
 // threshold t is the largest key that `budget` slots reach: radix selection, 11 + 11 + 10
 // bits, each a histogram of counts in LDS (integer atomics: their order changes nothing)
 // and a scan of it from the top; the newest tokens' slots are counted by ballots and left
