@@ -18,7 +18,7 @@
 // itself. Bins are joined in 64-bit floats in a fixed order. Tokens 32 nats and more below
 // the maximum (256 bins, 1e-14 of its weight) weigh nothing.
 //
-// k_sample_bins: a workgroup a chunk of 8192 logits, held in registers: the chunk's
+// k_sample_bins: a workgroup a chunk of 10240 logits, held in registers: the chunk's
 // maximum, then its 256 bins' counts and weights in one 64-bit LDS atomic an element
 // (count << 50 | weight), and the list of its best elements, whole bins up to
 // kListCap of them.
@@ -31,13 +31,14 @@
 // vocabulary's bulk, dense ties) is cut into 256 ranges of keys, a pass over the row, until
 // the one that the search falls into can be ordered, as a rule after one pass.
 // Measured (us, first + second launch; a workgroup a row with radix passes over it in
-// brackets): 1 x 151936 fp32, top-k 50 and top-p, 6.1 + 9.5 (865); 64 x 151936 bf16, a
-// row's own settings, 19.0 + 13.6 (993), of them 3.8 for the bytes at a copy's rate; at
-// temperature alone a draw past the head re-reads its row: 8 x 32000 6.1 + 17.6 (two rows
-// in three within the head), of normal logits, none within it, 37 a call, 8 x 151936 112
-// (the one workgroup's VALU: some 45 a pass). The first launch is bound by VALU issue (47 instructions an element, half of the time) and
-// the five barriers of its workgroups, two a CU at a time; the second by the latency of
-// some twenty dependent steps of one workgroup a row.
+// brackets): 1 x 151936 fp32, top-k 50 and top-p, 6.6 + 8.8 (865); 64 x 151936 bf16, a
+// row's own settings, 17.8 + 13.0 (993), of them 3.8 for the bytes at a copy's rate; at
+// temperature alone a draw past the head re-reads its row: 8 x 32000 6.5 + 17.4 (6.8 with
+// all draws within the head), of normal logits, none within it, 37 a call, 8 x 151936 112
+// (the one workgroup's VALU: some 45 a pass). The first launch is bound by VALU issue (42
+// instructions an element, two thirds of the time) and the five barriers of its
+// workgroups, two a CU at a time; the second by the latency of some twenty dependent steps
+// of one workgroup a row.
 #include <math.h>
 
 #include "sf_common.h"
@@ -49,14 +50,14 @@ constexpr int kSampThreads = 1024;
 constexpr int kSampWaves = kSampThreads / 64;
 constexpr int kBinThreads = 1024;   // of the first kernel
 constexpr int kBinWaves = kBinThreads / 64;
-constexpr int kPerThread = 8;
+constexpr int kPerThread = 10;      // (64 rows of 151936: 29.8 us a call, with 8 31.2, with 12 29.8)
 constexpr int kChunk = kBinThreads * kPerThread;
 constexpr int kBins = 256;
 constexpr double kDelta = 0.125;    // nats a bin
 constexpr int kListCap = 128;       // elements of a chunk's list
 constexpr int kBinCap = 1024;       // elements of a bin, or of a range of keys, ordered at once
 constexpr int kHeadCap = 512;       // elements of the head: eight a lane of one wave
-constexpr int kCountShift = 50;     // 8192 weights of up to 2^36 take 49 bits and a little
+constexpr int kCountShift = 50;     // 10240 weights of up to 1.07 2^36 take 49.5 bits
 constexpr u64 kWeightMask = (1ull << kCountShift) - 1;
 
 // Order-preserving bits of a logit (never 0); -inf and NaN share the lowest.
