@@ -489,7 +489,8 @@ int sf_kv_evict(int8_t *k_codes, void *k_scales, int8_t *v_codes, void *v_scales
  * NULL. For steps replayed from a HIP graph, `at` (or NULL) is a device index: row b takes
  * the number u[*at + at_add + b] of u_n (kept inside them) and its token also goes to
  * hist[*at + at_add + b], hist (or NULL) as long as u. workspace:
- * sf_sample_workspace_bytes(B, V) bytes, 256-byte aligned, no initial contents needed; calls that share one must not overlap. */
+ * sf_sample_workspace_bytes(B, V) bytes, 256-byte aligned, no initial contents needed;
+ * calls that share one must not overlap. */
 size_t sf_sample_workspace_bytes(int B, int V);
 int sf_sample(const void *logits, int dtype, long long row_stride, int B, int V, const float *u,
               float temperature, int top_k, float top_p, float min_p, const float *temperatures,

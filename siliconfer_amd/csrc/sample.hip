@@ -59,6 +59,7 @@ constexpr int kBinCap = 1024;       // elements of a bin, or of a range of keys,
 constexpr int kHeadCap = 512;       // elements of the head: eight a lane of one wave
 constexpr int kCountShift = 50;     // 10240 weights of up to 1.07 2^36 take 49.5 bits
 constexpr u64 kWeightMask = (1ull << kCountShift) - 1;
+static_assert(kChunk * 1.07 < (1ull << (kCountShift - 36)) && kChunk < (1 << (64 - kCountShift)), "a bin's weight and count");
 
 // Order-preserving bits of a logit (never 0); -inf and NaN share the lowest.
 __device__ __forceinline__ uint32_t order_key(float x) {
