@@ -18,11 +18,32 @@ import numpy as np
 
 @dataclass
 class RoPEScalingConfig:
+    """A checkpoint's rope_scaling entry. `original_max_position_embeddings` reads 8192 (the
+    reference's default) where the entry has none; `original_given` keeps that apart, since
+    scalings other than llama3 then go by the model's max_position_embeddings. `extra`:
+    the entry's other fields."""
+
     type: str = ""
     factor: float = 1.0
     low_freq_factor: float = 1.0
     high_freq_factor: float = 4.0
-    original_max_position_embeddings: int = 8192
+    original_max_position_embeddings: int | None = None
+    extra: dict[str, Any] = field(default_factory=dict)
+    original_given: bool | None = field(default=None, repr=False)
+
+    def __post_init__(self) -> None:
+        if self.original_given is None:
+            self.original_given = self.original_max_position_embeddings is not None
+        if self.original_max_position_embeddings is None:
+            self.original_max_position_embeddings = 8192
+
+    def entry(self) -> dict[str, Any]:
+        """The entry as a checkpoint has it."""
+        raw = dict(self.extra, type=self.type, factor=self.factor, low_freq_factor=self.low_freq_factor,
+                   high_freq_factor=self.high_freq_factor)
+        if self.original_given or self.original_max_position_embeddings != 8192:
+            raw["original_max_position_embeddings"] = self.original_max_position_embeddings
+        return raw
 
 
 @dataclass
@@ -72,8 +93,10 @@ class ModelConfig:
                 factor=raw_rope.get("factor", 1.0),
                 low_freq_factor=raw_rope.get("low_freq_factor", 1.0),
                 high_freq_factor=raw_rope.get("high_freq_factor", 4.0),
-                original_max_position_embeddings=raw_rope.get(
-                    "original_max_position_embeddings", 8192),
+                original_max_position_embeddings=raw_rope.get("original_max_position_embeddings"),
+                extra={k: v for k, v in raw_rope.items() if k not in (
+                    "type", "rope_type", "factor", "low_freq_factor", "high_freq_factor",
+                    "original_max_position_embeddings")},
             )
         return cls(
             architectures=raw.get("architectures", []),
@@ -106,11 +129,7 @@ class ModelConfig:
             "hidden_act", "torch_dtype", "bos_token_id", "eos_token_id", "attention_bias",
             "model_type")}
         if self.rope_scaling is not None:
-            r = self.rope_scaling
-            raw["rope_scaling"] = {"type": r.type, "factor": r.factor,
-                                   "low_freq_factor": r.low_freq_factor,
-                                   "high_freq_factor": r.high_freq_factor,
-                                   "original_max_position_embeddings": r.original_max_position_embeddings}
+            raw["rope_scaling"] = self.rope_scaling.entry()
         return raw
 
     @classmethod

@@ -9,7 +9,9 @@ Scaling types, by the names and fields of a HuggingFace `rope_scaling` entry:
            length, from the length that is asked for on
   llama3   slow pairs divided by `factor`, fast ones kept, a ramp between
   yarn     the ramp in numbers of turns over the trained length (beta_fast,
-           beta_slow), and cos / sin times 0.1 ln(factor) + 1
+           beta_slow), and cos / sin times 0.1 ln(factor) + 1 (attention_factor in its
+           place where given; mscale, mscale_all_dim and truncate false are refused)
+A field that is null counts as absent.
 """
 
 from __future__ import annotations
@@ -35,7 +37,7 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
         raise SFError(f"need an even rotary_dim and theta > 0 (got {rotary_dim}, {theta})")
     i = np.arange(0, rotary_dim, 2, dtype=np.float64)
     f = float(theta) ** (-i / rotary_dim)
-    sc = dict(scaling or {})
+    sc = {k: v for k, v in (scaling or {}).items() if v is not None}
     kind = sc.get("rope_type", sc.get("type", "")) or "default"
     if kind == "default":
         return f, 1.0
@@ -60,6 +62,9 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: dict | 
         keep = np.clip((turns - lo) / (hi - lo), 0, 1) if hi != lo else (turns >= hi).astype(np.float64)
         return f / factor * (1 - keep) + f * keep, 1.0
     if kind == "yarn":
+        other = [k for k in ("mscale", "mscale_all_dim") if k in sc] + ["truncate"] * (not sc.get("truncate", True))
+        if other:  # they would change the factor, or the ramp's ends
+            raise SFError(f"rope scaling 'yarn' with {', '.join(other)}")
         at = lambda turns: rotary_dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(theta))
         lo = max(math.floor(at(float(sc.get("beta_fast", 32.0)))), 0)
         hi = min(math.ceil(at(float(sc.get("beta_slow", 1.0)))), rotary_dim - 1)
@@ -84,12 +89,13 @@ class Rotary:
     @classmethod
     def from_config(cls, config: ModelConfig, rotary_dim: int | None = None, interleaved: bool = False,
                     scaling: dict | None = None, length: int | None = None) -> "Rotary":
-        """Of a model's head_dim, theta and rope_scaling (or `scaling` in its place)."""
+        """Of a model's head_dim, theta and rope_scaling (or `scaling` in its place). An entry
+        that names no trained length goes by max_position_embeddings, llama3 by 8192 as in
+        `config.rope_freqs`."""
         if scaling is None and config.rope_scaling is not None:
-            s = config.rope_scaling
-            scaling = {"type": s.type, "factor": s.factor, "low_freq_factor": s.low_freq_factor,
-                       "high_freq_factor": s.high_freq_factor,
-                       "original_max_position_embeddings": s.original_max_position_embeddings}
+            scaling = config.rope_scaling.entry()
+            if config.rope_scaling.type == "llama3":
+                scaling["original_max_position_embeddings"] = config.rope_scaling.original_max_position_embeddings
         r = config.head_dim if rotary_dim is None else rotary_dim
         if r > config.head_dim:
             raise SFError(f"rotary_dim {r} exceeds the head's {config.head_dim}")
