@@ -41,6 +41,7 @@
 // of one workgroup a row.
 #include <math.h>
 
+#include "sample_place.h"
 #include "sf_common.h"
 
 namespace {
@@ -52,8 +53,6 @@ constexpr int kBinThreads = 1024;   // of the first kernel
 constexpr int kBinWaves = kBinThreads / 64;
 constexpr int kPerThread = 10;      // (64 rows of 151936: 29.8 us a call, with 8 31.2, with 12 29.8)
 constexpr int kChunk = kBinThreads * kPerThread;
-constexpr int kBins = 256;
-constexpr double kDelta = 0.125;    // nats a bin
 constexpr int kListCap = 128;       // elements of a chunk's list
 constexpr int kBinCap = 1024;       // elements of a bin, or of a range of keys, ordered at once
 constexpr int kHeadCap = 512;       // elements of the head: eight a lane of one wave
@@ -88,42 +87,6 @@ struct RowParams {
   }
 };
 
-// 1 / (T kDelta): a logit's place on the bins' axis is x times it. The floor keeps an
-// infinite temperature from turning infinite logits into NaN.
-__device__ __forceinline__ double bins_per_logit(float T) { return fmax(1.0 / ((double)T * kDelta), 1e-300); }
-
-// x per and its part past the whole number `top` (exact) in 32 fractional bits: the sum
-// with 1.5 2^20 holds the whole part in its high word and the rest in its low word. Each
-// operation rounded on its own: shifting by whole numbers commutes with the rounding, so
-// every chunk and the row agree on a logit's bin.
-__device__ __forceinline__ u64 place_of(float x, double per, double top) {
-#pragma clang fp contract(off)
-  return (u64)__double_as_longlong(fmax((double)x * per - top, -4096.0) + 1572864.0);
-}
-__device__ __forceinline__ int whole_of(u64 place) { return (int)(place >> 32 & 0xfffff) - 0x80000; }
-// The bin number of a row's (chunk's) maximum: its own place relative to it is in [0, 1).
-__device__ __forceinline__ double top_bin(float m, double per) {
-#pragma clang fp contract(off)
-  const double f = floor((double)m * per);
-  return f + (double)whole_of(place_of(m, per, f));
-}
-
-struct Binned {
-  int bin;  // below the bin of `top`; kBins and more: no weight
-  u64 w;
-};
-// Where x lies below the bin number `top`, and its weight (plus `add`). With s / 2^32 the
-// place's distance from the bin's middle, y = kDelta s / 2^32 and 2^36 e^y = 2^36 + 2 s +
-// 2^36 (y^2 / 2 + ... + y^5 / 120), the bracket in fp32: its rounding (0.002 2^-23) and the
-// next term (y^6 / 720) are 3e-10 at most.
-__device__ __forceinline__ Binned bin_of(float x, double per, double top, u64 add = 0) {
-  static_assert(kDelta == 0.125, "2^36 kDelta s / 2^32 = 2 s");
-  const u64 v = place_of(x, per, top);
-  const int s = (int)((uint32_t)v ^ 0x80000000u);
-  const float y = (float)s * (float)(kDelta * 0x1p-32);
-  const float tail = y * y * fmaf(y, fmaf(y, fmaf(y, 0x1p36f / 120, 0x1p36f / 24), 0x1p36f / 6), 0x1p35f);
-  return Binned{-whole_of(v), (u64)((long long)s * 2 + (long long)((1ull << 36) + add)) + (uint32_t)tail};
-}
 // A row with infinite logits draws among them alone: they count as 0, all others as -inf.
 __device__ __forceinline__ float flat_value(float x) { return x == INFINITY ? 0.f : -INFINITY; }
 
@@ -345,7 +308,7 @@ struct Row {
     if (sm.uncovered) {
       clear();
       // (the bins' range of logits, one bin wider each way, first; then exactly)
-      const float from = (float)((top - last - 2) / per), to = (float)((top - first + 2) / per);
+      const float from = (float)logit_at(top, last + 2, per), to = (float)logit_at(top, first - 2, per);
       each([&](int i, float x) {
         if (x >= from && x <= to) put(bin_of(x, per, top).bin, (u64)order_key(x) << 32 | (uint32_t)~i);
       });
@@ -421,8 +384,8 @@ struct Row {
   }
   // The range of keys of a bin, two bins wider each way.
   __device__ __forceinline__ void keys_of(int bin, uint32_t &base, int &bits) const {
-    base = order_key((float)((top - bin - 2) / per));
-    bits = 32 - __clz((int)((order_key((float)((top - bin + 2) / per)) - base) | 1));
+    base = order_key((float)logit_at(top, bin + 2, per));
+    bits = 32 - __clz((int)((order_key((float)logit_at(top, bin - 2, per)) - base) | 1));
   }
 
   // The elements of a bin of at most kBinCap into sm.el in order, running weights into sm.run.
@@ -700,7 +663,7 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
   const bool by_k = k > 0 && k < sm.n_before[kBins], by_p = tp < 1.f, by_m = mp > 0.f;
   int m_bin = kBins;  // the bin of the least weight that min-p leaves
   if (by_m) {
-    const double below = row.top - floor(M * per + log(least) * (1.0 / kDelta));
+    const double below = row.top - floor(axis_of((float)M, per) + log(least) * (1.0 / kDelta));
     m_bin = below < (double)kBins ? max(0, (int)below) : kBins;
   }
   // The head: the bins up to the end of what the filters leave. top-p's share is of what
@@ -792,11 +755,6 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
     if (stage == 0) {  // top-k
       if (!by_k) continue;
       x = (double)(k - 1 - sm.n_before[bin]);
-    } else if (stage == 1) {  // top-p
-      if (!by_p) continue;
-      const double bound = fmax((double)tp, 0.0) * weight_kept();
-      bin = row.bin_past(bound, last);
-      x = (bound - sm.before[bin]) / sm.fac[bin];
     } else if (stage == 2) {  // min-p: those that weigh enough, all before any other
       if (!by_m || m_bin > last) continue;
       const u64 w = row.heavy(m_bin, M, inv_t, kmax, least);
@@ -805,11 +763,13 @@ k_sample_pick(const void *__restrict__ logits, long long row_stride, int V, int 
         upto = w;
       }
       continue;
-    } else {  // the draw
+    } else {  // top-p's end, then the draw
+      if (stage == 1 && !by_p) continue;
       total = weight_kept();
-      const double target = uu * total;
+      const double target = (stage == 1 ? fmax((double)tp, 0.0) : uu) * total;
       bin = row.bin_past(target, last);
-      // (rounding, or a last bin of which nothing stays: the last token that does)
+      // (an empty bin, by the prefix sums' rounding, or a last one of which nothing stays:
+      // the last token before it)
       while (bin > 0 && (bin == last ? upto == 0 : sm.w[bin] == 0)) --bin;
       x = (target - sm.before[bin]) / sm.fac[bin];
       const double most = (double)(bin == last ? upto : sm.w[bin]);

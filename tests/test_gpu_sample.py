@@ -164,3 +164,19 @@ def test_crowded_bins(dev, kw):
                   rng.normal(0, 1e-40, V), -1000 + rng.normal(0, 0.3, V)]).astype(np.float32)
     for u in (0.0, 0.37, 0.5, 0.93, 1 - 2 ** -24):
         check(dev, torch.from_numpy(x), np.full(6, u), **kw)
+
+
+@pytest.mark.parametrize("T", [0.6, 1.0, 1.37])
+@pytest.mark.parametrize("kw", [dict(), dict(top_p=0.999), dict(top_k=50000), dict(min_p=1e-9)], ids=str)
+def test_the_last_token_of_a_crowded_bin(dev, T, kw):
+    """Rows over several chunks whose maxima lie in different bins, thousands of tokens in the last
+    bin (a floor of equal logits, or spread within it), and numbers at and past the end of [0, 1)."""
+    rng = np.random.default_rng(7)
+    V = 60000
+    x = np.concatenate([rng.normal(-9, 0.02, (6, V)), rng.choice([-9.0, -8.97, -9.03], (2, V)), np.full((2, V), -9.0)])
+    for r in range(10):
+        at = rng.choice(V, 40, replace=False)
+        x[r, at] = rng.uniform(-7, 6, 40)
+    x = (x * T).astype(np.float32)
+    for u in (1.0, 2.0, 1 - 2.0 ** -24, 0.9999):
+        check(dev, torch.from_numpy(x), np.full(10, u), temperature=T, **kw)
