@@ -213,19 +213,27 @@ def on_device(t: torch.Tensor):
 
 
 _NOTHING = contextlib.nullcontext()
-_scratch: dict = {}
+
+
+class _Scratch(threading.local):
+    def __init__(self) -> None:
+        self.held: dict = {}
+
+
+_scratch = _Scratch()
 
 
 def scratch(device: torch.device, stream_handle: int, nbytes: int) -> torch.Tensor:
-    """Workspace of one call: kept a (device, stream) and grown on demand, whose
-    calls run one after the other; while a graph is recorded a tensor of the graph's
-    own, so that no two graphs share one."""
+    """Workspace of one call: kept a (host thread, device, stream) and grown on demand. A
+    thread's calls on a stream run one after the other; two threads' launches on it may
+    interleave, since a call gives up the interpreter's lock. While a graph is recorded a
+    tensor of the graph's own, so that no two graphs share one."""
     if torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
-    key = (device, stream_handle)
-    ws = _scratch.get(key)
+    held, key = _scratch.held, (device, stream_handle)
+    ws = held.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _scratch[key] = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
+        ws = held[key] = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
     return ws
 
 

@@ -40,18 +40,10 @@ def default_splits(B: int, n_kv_heads: int, T: int, head_dim: int = 64) -> int:
     return int(_lib.load().sf_attn_default_splits_d(B, n_kv_heads, T, head_dim))
 
 
-_workspaces: dict = {}
-
-
 def workspace(device: torch.device, stream_handle: int, nbytes: int) -> torch.Tensor:
-    """Attention workspace (the split partials), one per (device, stream), grown
-    on demand; nothing in it needs clearing between calls."""
-    key = (device, stream_handle)
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = torch.empty(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
-        _workspaces[key] = ws
-    return ws
+    """Attention workspace (the split partials): `_lib.scratch`; nothing in it needs
+    clearing between calls."""
+    return _lib.scratch(device, stream_handle, nbytes)
 
 
 def attention_decode(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,

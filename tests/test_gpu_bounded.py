@@ -247,3 +247,44 @@ def test_sample_token_min_p(dev):
     g = torch.Generator(device=dev).manual_seed(0)
     drawn = {sample_token(x, SamplingParams(min_p=0.4), generator=g) for _ in range(200)}
     assert drawn == {0, 1}
+
+
+def test_two_host_threads_on_one_stream(dev):
+    """Attention, eviction and sampling called from two threads at once, on the same stream and at
+    different sizes, give what one thread gives."""
+    import threading
+
+    def inputs(i):
+        g = torch.Generator().manual_seed(20 + i)
+        return (torch.randn(1 + i, 900 - 500 * i, (H + 2 * KVH) * D, generator=g).to(dev),
+                torch.randn(3 + 5 * i, 30000 + 60000 * i, generator=g).to(dev), torch.rand(3 + 5 * i, generator=g).to(dev))
+
+    r = Rotary(*rotary_frequencies(64, 1e4))
+    r.on(dev)
+
+    def work(qkv, logits, u):
+        out = []
+        for _ in range(15):
+            cache = BoundedKVCache(200, 20, 0)
+            q = cache.append_rotary(qkv, H, KVH, r)
+            out.append(cache.attend(q[:, -8:].contiguous()))
+            cache.evict()
+            out += [cache.scores[:, :, :200].clone(), cache.positions[:, :, :200].clone(), sample(logits, u, top_p=0.9)]
+        return out
+
+    data = [inputs(i) for i in range(2)]
+    want, got = [work(*d)[:4] for d in data], [None, None]
+
+    def thread(i):
+        got[i] = work(*data[i])
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 60
+        for j, t in enumerate(got[i]):
+            assert torch.equal(t, want[i][j % 4]), (i, j)
