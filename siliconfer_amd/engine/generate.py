@@ -73,11 +73,17 @@ def _is_greedy(p: SamplingParams) -> bool:
     return p.temperature <= 0 and p.repetition_penalty == 1.0
 
 
+def _check_min_p(p: SamplingParams) -> None:
+    if not 0 <= p.min_p <= 1:  # (above 1 no token would be left to draw)
+        raise SFError(f"need 0 <= min_p <= 1 (got {p.min_p})")
+
+
 def sample_token(logits: torch.Tensor, params: SamplingParams,
                  generated_ids: list[int] | None = None,
                  generator: torch.Generator | None = None) -> int:
     """Next token from one row of logits ([V], or [..., V] whose last row is
     used), by the reference's rules (generate.py:24-67)."""
+    _check_min_p(params)
     row = logits.reshape(-1, logits.shape[-1])[-1].float().clone()
     if params.repetition_penalty != 1.0 and generated_ids:
         ids = torch.as_tensor(sorted(set(generated_ids)), device=row.device, dtype=torch.long)
@@ -143,6 +149,7 @@ def generate(model: LlamaModel, prompt_ids, params: SamplingParams | None = None
     list) draws token i from uniforms[i] on the device; `generator` is then unused."""
     check_kv_cache_flag(quantize_kv_cache)
     params = params or SamplingParams()
+    _check_min_p(params)
     if uniforms is not None:
         if params.repetition_penalty != 1.0:
             raise SFError("uniforms: the draw on the device has no repetition penalty")

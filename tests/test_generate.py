@@ -85,3 +85,19 @@ def test_reference_signatures():
     check_kv_cache_flag(True)
     with pytest.raises(RuntimeError, match="int8 KV cache only"):
         check_kv_cache_flag(False)
+
+
+@pytest.mark.parametrize("min_p", [1.5, 1 + 2 ** -20, -0.1, float("nan")])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_min_p_outside_0_to_1_is_refused(min_p, temperature):
+    """Before anything runs: above 1 every token would be dropped and the draw fail on the device."""
+    from siliconfer_amd._lib import SFError
+    from siliconfer_amd.engine.generate import generate
+    params = SamplingParams(temperature=temperature, min_p=min_p)
+    with pytest.raises(SFError, match="min_p <= 1"):
+        sample_token(torch.tensor([0.1, 0.2]), params)
+    for uniforms in (None, [0.5] * 200):
+        with pytest.raises(SFError, match="min_p <= 1"):
+            generate(None, [1, 2], params, uniforms=uniforms)
+    for ok in (0.0, 1.0):
+        assert sample_token(torch.tensor([0.1, 0.7, 0.7]), SamplingParams(min_p=ok, top_k=2)) in (1, 2)
