@@ -172,7 +172,9 @@ class BoundedKVCache(QuantizedKVCache):
     budget + slack, drops the slots with the least of it; those of the newest `recent`
     tokens (a quarter of the budget by default) stay. Each kv head keeps tokens of its
     own, in any order, with their `positions`; `length()` counts slots, `seen` the
-    tokens that went through. Keys are cached turned to their positions."""
+    tokens that went through. Keys are cached turned to their positions. The buffers have
+    budget + slack + 1 slots; for a longer prompt they grow, until `release` or the first
+    append after the cut that fits those again."""
 
     def __init__(self, budget: int, recent: int | None = None, slack: int = 64,
                  scale_dtype: torch.dtype = torch.float16) -> None:
@@ -185,6 +187,8 @@ class BoundedKVCache(QuantizedKVCache):
         self.scores = self.positions = None
 
     def _ensure(self, k: torch.Tensor, need: int) -> None:
+        if need <= self.budget + self.slack + 1:
+            self.release()
         before = self._qk
         super()._ensure(k, need)
         if self._qk is before:
@@ -233,6 +237,19 @@ class BoundedKVCache(QuantizedKVCache):
         if self._len > self.budget + self.slack:
             evict(*self.buffers(), self.scores, self.positions, self._len, self.seen, self.budget, self.recent)
             self._len = self.budget
+
+    def release(self) -> None:
+        """Let buffers that grew for a prompt go back to budget + slack + 1 slots, if what is
+        kept fits them."""
+        base, n = self.budget + self.slack + 1, self._len
+        if self._qk is None or self._qk.shape[2] <= base or n > base:
+            return
+        old = (*self.buffers(), self.scores, self.positions)
+        new = [t.new_zeros((*t.shape[:2], base, *t.shape[3:])) for t in old]
+        for a, b in zip(new, old):
+            a[:, :, :n].copy_(b[:, :, :n])
+        self._qk, self._sk, self._qv, self._sv, self.scores, self.positions = new
+        self.capacity = base
 
     def set_length(self, n: int) -> None:
         raise SFError("a bounded cache's slots are set by append and evict")

@@ -248,6 +248,7 @@ class Attention(torch.nn.Module):
                     float(self.scale), st), "sf_attn_prefill_i8kv")
             out[:, -self.OBSERVED:] = cache.attend(q[:, -self.OBSERVED:].contiguous(), self.scale)
         cache.evict()
+        cache.release()  # (a prompt's buffers, before the next layer allocates its own)
         return out
 
     def _int8_batch1(self, qkv, cache: QuantizedKVCache, T: int, device) -> torch.Tensor:

@@ -179,3 +179,58 @@ def test_a_bounded_cache_starts_again():
         cache.trim(3)
     cache.trim(9)
     assert cache.length() == 4 and cache.seen == 9
+
+
+def test_a_bounded_cache_gives_a_prompt_s_buffers_back(monkeypatch):
+    """Past an eviction the buffers go back to budget + slack + 1 slots with what was kept: by
+    release(), or by the first append that fits. (The eviction itself is stood in for on the host.)"""
+    from siliconfer_amd.kernels import eviction
+
+    def newest(kc, ks, vc, vs, scores, positions, length, seen, budget, recent):
+        for t in (kc, ks, vc, vs, scores, positions):
+            t[:, :, :budget] = t[:, :, length - budget:length].clone()
+
+    monkeypatch.setattr(eviction, "evict", newest)
+    cache = BoundedKVCache(20, 5, slack=3)
+
+    def fill(T):  # what append_rotary does, without its kernel
+        n = cache._len
+        cache.reserve(2, 3, 16, n + T, torch.device("cpu"))
+        for i, t in enumerate((*cache.buffers(), cache.scores, cache.positions)):
+            at = torch.arange(cache.seen, cache.seen + T) + i
+            t[:, :, n:n + T] = at.to(t.dtype).view(1, 1, T, *[1] * (t.dim() - 3))
+        cache._len, cache.seen = n + T, cache.seen + T
+
+    def check(first, n):
+        for i, t in enumerate((*cache.buffers(), cache.scores, cache.positions)):
+            want = (torch.arange(first, first + n) + i).to(t.dtype)
+            assert t.shape[2] == 24 == cache.capacity and t.is_contiguous()
+            assert torch.equal(t[:, :, :n].reshape(2, 3, n, -1)[..., 0], want.expand(2, 3, n))
+
+    fill(7)
+    assert cache.buffers()[0].shape[2] == 24
+    cache.evict()
+    check(0, 7)
+    fill(100)
+    assert cache.buffers()[0].shape[2] >= 107
+    cache.evict()
+    assert cache.length() == 20 and cache.seen == 107
+    cache.release()
+    check(87, 20)
+    fill(100)
+    cache.evict()
+    fill(2)
+    check(187, 22)
+    before = [t.data_ptr() for t in cache.buffers()]
+    for _ in range(7):  # a decode loop stays in its buffers
+        fill(1)
+        cache.evict()
+    assert [t.data_ptr() for t in cache.buffers()] == before and cache.length() == 21
+    cache.trim(0)
+    fill(200)
+    assert cache.buffers()[0].shape[2] >= 200
+    cache.release()  # (does not fit)
+    assert cache.buffers()[0].shape[2] >= 200 and cache.length() == 200
+    cache.trim(22)
+    fill(2)
+    check(0, 24)

@@ -288,3 +288,32 @@ def test_two_host_threads_on_one_stream(dev):
         assert len(got[i]) == 60
         for j, t in enumerate(got[i]):
             assert torch.equal(t, want[i][j % 4]), (i, j)
+
+
+def test_buffers_after_a_long_prompt(dev):
+    """A prompt far past the bound: after its eviction the cache's buffers have their own size again
+    and hold the oracle's choice; the steps behind it run on."""
+    r = Rotary(*rotary_frequencies(64, 1e4))
+    cache, g = BoundedKVCache(24, 6, 4), torch.Generator().manual_seed(11)
+    for T in (500, 1, 1, 300, 1):
+        q = cache.append_rotary(torch.randn(2, T, (H + 2 * KVH) * D, generator=g).to(dev), H, KVH, r)
+        cache.attend(q[:, -8:].contiguous())
+        length, seen, before = cache.length(), cache.seen, buffers(cache)
+        cache.evict()
+        cache.release()
+        if length > 28:
+            expect, _ = bounded.evict(before, before[4], before[5], [length] * 2, [seen] * 2, 24, 6)
+            for got, want in zip(buffers(cache), expect):
+                assert got.shape[2] == 29 and np.array_equal(got[:, :, :24], want[:, :, :24])
+        assert cache.capacity == cache.buffers()[0].shape[2] == 29 and cache.length() <= 28
+
+
+def test_a_layer_s_cache_after_a_long_prompt(dev):
+    """The layer's own path leaves a prompt's buffers at the bound."""
+    attn, cache = layer(dev, None), BoundedKVCache(24, 6, 4)
+    x = torch.randn(2, 400, 128, generator=torch.Generator().manual_seed(12)).to(dev)
+    with torch.no_grad():
+        for T in (400, 1, 100, 1):
+            attn(x[:, :T], cache)
+            assert all(t.shape[2] == 29 for t in (*cache.buffers(), cache.scores, cache.positions))
+    assert cache.length() == 25 and cache.seen == 502
