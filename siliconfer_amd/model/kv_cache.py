@@ -251,6 +251,11 @@ class BoundedKVCache(QuantizedKVCache):
         self._qk, self._sk, self._qv, self._sv, self.scores, self.positions = new
         self.capacity = base
 
+    def nbytes(self) -> int:
+        """Footprint of the valid slots: codes, scales, scores and positions."""
+        rows = 0 if self._qk is None else self._qk.shape[0] * self._qk.shape[1] * self._len
+        return super().nbytes() + 8 * rows
+
     def set_length(self, n: int) -> None:
         raise SFError("a bounded cache's slots are set by append and evict")
 

@@ -234,3 +234,15 @@ def test_a_bounded_cache_gives_a_prompt_s_buffers_back(monkeypatch):
     cache.trim(22)
     fill(2)
     check(0, 24)
+
+
+@pytest.mark.parametrize("scale_dtype,size", [(torch.float16, 2), (torch.float32, 4)])
+def test_a_bounded_cache_s_size(scale_dtype, size):
+    """nbytes counts a slot's codes and scales, and its score and position a kv head."""
+    cache = BoundedKVCache(20, scale_dtype=scale_dtype)
+    assert cache.nbytes() == 0
+    cache.reserve(2, 3, 16, 10, torch.device("cpu"))
+    cache._len = 10
+    assert cache.nbytes() == sum(t[:, :, :10].numel() * t.element_size()
+                                 for t in (*cache.buffers(), cache.scores, cache.positions))
+    assert cache.nbytes() == 2 * 3 * 10 * (2 * (16 + size) + 8)
