@@ -17,7 +17,8 @@ other cache forms — none, or a (k, v) tuple of full-precision tensors — and
 batches above one with an int8 cache take the reference's own route on the
 device: RoPE, concatenation (or the int8 append and the dequantized cache)
 and softmax attention with the causal mask, in fp32 torch operations. With
-`rotary` (a `Rotary`) positions follow its frequencies and pair layout, and a
+`rotary` (a `Rotary`) positions follow its frequencies and pair layout (by
+`kernels.rotary`, differentiable where that route is), and a
 `BoundedKVCache` keeps the tokens that attention weighs most, at any batch.
 
 Activations: projections return fp32 (Q4Linear's contract); RMSNorm returns
