@@ -144,7 +144,7 @@ class Attention(torch.nn.Module):
     def __init__(self, config: ModelConfig, rope_freqs: torch.Tensor, device=None,
                  rotary: Rotary | None = None) -> None:
         super().__init__()
-        self.rotary = rotary
+        self.rotary, self._half = rotary, None
         self.num_heads = config.num_attention_heads
         self.num_kv_heads = config.num_key_value_heads
         self.head_dim = config.head_dim
@@ -156,6 +156,19 @@ class Attention(torch.nn.Module):
         self.v_proj = _dense(H, self.num_kv_heads * D, bias, device)
         self.o_proj = _dense(self.num_heads * D, H, False, device)
         self._cos = self._sin = None
+        self._rotary_of(device)
+
+    def _rotary_of(self, device) -> Rotary:
+        """`rotary`, or rotate-half over the whole head of `rope_freqs` (made when these are
+        given), its frequencies on the device."""
+        r = self.rotary
+        if r is None:
+            if self._half is None or self._half[0] is not self.rope_freqs:
+                self._half = self.rope_freqs, Rotary(self.rope_freqs.detach().double().cpu().numpy())
+            r = self._half[1]
+        if device is not None:
+            r.on(device)
+        return r
 
     def _tables(self, need: int, device) -> tuple[torch.Tensor, torch.Tensor]:
         """fp32 [P, D/2] tables of cos / sin(position * freq), P >= need, built
@@ -232,10 +245,7 @@ class Attention(torch.nn.Module):
         over the whole cache, then what exceeds its bound dropped."""
         B, T, _ = qkv.shape
         H, KVH, D = self.num_heads, self.num_kv_heads, self.head_dim
-        if self.rotary is None:  # rotate-half over the whole head, of the given frequencies
-            self.rotary_half = getattr(self, "rotary_half", None) or Rotary(
-                self.rope_freqs.detach().double().cpu().numpy())
-        q = cache.append_rotary(qkv, H, KVH, self.rotary or self.rotary_half)
+        q = cache.append_rotary(qkv, H, KVH, self._rotary_of(None))
         if T <= self.OBSERVED:
             out = cache.attend(q, self.scale)
         else:

@@ -103,7 +103,15 @@ class Rotary:
                    interleaved)
 
     def on(self, device) -> torch.Tensor:
+        """The frequencies on `device`, copied there when it first asks."""
         f = self._on.get(device)
         if f is None:
-            f = self._on[device] = torch.from_numpy(self.inv_freq).to(device)
+            d = torch.device(device)
+            if d.type == "cuda":
+                d = torch.device("cuda", torch.cuda.current_device() if d.index is None else d.index)
+                if d not in self._on and torch._C._cuda_isCurrentStreamCapturing():
+                    raise SFError("Rotary.on(device): once before a graph is recorded (it copies from the host)")
+            f = self._on.get(d)
+            if f is None:
+                f = self._on[d] = torch.from_numpy(self.inv_freq).to(d)
         return f

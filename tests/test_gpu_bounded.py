@@ -317,3 +317,25 @@ def test_a_layer_s_cache_after_a_long_prompt(dev):
             attn(x[:, :T], cache)
             assert all(t.shape[2] == 29 for t in (*cache.buffers(), cache.scores, cache.positions))
     assert cache.length() == 25 and cache.seen == 502
+
+
+@pytest.mark.parametrize("rot", [None, lambda: Rotary(*rotary_frequencies(32, 1e4))], ids=["half", "given"])
+@pytest.mark.parametrize("where", ["cuda", "cuda:0"])
+def test_a_layer_s_first_call_does_not_wait_for_the_device(dev, rot, where):
+    """The frequencies are on the device from the layer's construction on: no call copies to or from the host."""
+    attn, cache = layer(where, rot and rot()), BoundedKVCache(40, 8, 4)
+    x = torch.randn(2, 30, 128, generator=torch.Generator().manual_seed(13)).to(dev)
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        with torch.no_grad():
+            outs = [attn(x[:, :T], cache)[0] for T in (30, 1, 20, 1)]
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    # other frequencies given to the layer later are taken from then on
+    other = compute_rope_freqs(ModelConfig(head_dim=64, rope_theta=50.0), dev)
+    again, cache = layer(where, rot and rot()), BoundedKVCache(40, 8, 4)
+    with torch.no_grad():
+        assert torch.equal(again(x, cache)[0], outs[0])
+        again.rope_freqs, cache = other, BoundedKVCache(40, 8, 4)
+        assert torch.equal(again(x, cache)[0], outs[0]) == (rot is not None)

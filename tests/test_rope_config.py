@@ -93,3 +93,16 @@ def test_fields_that_would_change_the_result_are_refused(field):
         rotary_frequencies(64, 1e4, entry, trained=4096)
     with pytest.raises(SFError, match=next(iter(field))):
         Rotary.from_config(config(entry))
+
+
+def test_frequencies_are_not_copied_while_a_graph_is_recorded(monkeypatch):
+    """A copy from host memory would end the recording: a first on() there is refused."""
+    import torch
+
+    r = Rotary(*rotary_frequencies(16))
+    cpu = torch.device("cpu")
+    assert r.on("cpu") is r.on(cpu)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: True)
+    assert r.on(cpu).shape == (8,)
+    with pytest.raises(SFError, match="before a graph is recorded"):
+        r.on(torch.device("cuda", 0))
