@@ -544,6 +544,10 @@ extern "C" int sf_attn_decode_scored_i8kv(const void *q, int q_dtype, const int8
   SF_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes) & 7) == 0, SF_EINVAL,
              "KV code buffers must be 8-byte aligned");
   SF_REQUIRE(((uintptr_t)q & 15) == 0, SF_EINVAL, "q must be 16-byte aligned");
+  // 256 slots a workgroup of the second launch where that gives every CU two, else 64
+  const bool many = (long long)B * KVH * ((T_max + 255) / 256) >= 512;
+  const int rows = B * Tq * H, per = many ? 256 : 64, tok_blocks = (T_max + per - 1) / per;
+  SF_REQUIRE((long long)B * KVH * tok_blocks + rows <= 0x7fffffffLL, SF_EINVAL, "B=%d T_max=%d exceed the grid", B, T_max);
   n_splits = scored_splits(B, Tq, H, KVH, T_max, D, n_splits);
   size_t ml_off, s_off;
   const size_t need = scored_parts(B, Tq, H, T_max, D, n_splits, &ml_off, &s_off);
@@ -576,10 +580,6 @@ extern "C" int sf_attn_decode_scored_i8kv(const void *q, int q_dtype, const int8
 #undef SF_SC_S
 #undef SF_SC_D
 #undef SF_SC
-  // 256 slots a workgroup where that gives every CU two, else 64
-  const bool many = (long long)B * KVH * ((T_max + 255) / 256) >= 512;
-  const int rows = B * Tq * H, per = many ? 256 : 64, tok_blocks = (T_max + per - 1) / per;
-  SF_REQUIRE((long long)B * KVH * tok_blocks + rows <= 0x7fffffffLL, SF_EINVAL, "B=%d T_max=%d exceed the grid", B, T_max);
   const FinishArgs f = {acc, ml, sw, scores, out, lengths, out_dtype, T, T_max, T_cap, Tq, H, KVH, D, n_splits, tok_blocks};
   // LDS: the splits' weights and the parts' sums, or two words a row
   const size_t lds_out = (kScMaxSplits + 4 * kScThreads) * sizeof(float), lds_w = 2 * (size_t)R * sizeof(float);

@@ -2,6 +2,9 @@
 points check shapes, types, pointers and workspaces before any launch, the Python ones
 devices and shapes."""
 
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -246,3 +249,34 @@ def test_a_bounded_cache_s_size(scale_dtype, size):
     assert cache.nbytes() == sum(t[:, :, :10].numel() * t.element_size()
                                  for t in (*cache.buffers(), cache.scores, cache.positions))
     assert cache.nbytes() == 2 * 3 * 10 * (2 * (16 + size) + 8)
+
+
+COUNT = r"""
+extern "C" {
+int launches = 0;
+unsigned __hipPushCallConfiguration(...) { ++launches; return 1; }  // (not 0: the launch is left out)
+}
+"""
+ASK = """
+import ctypes, sys
+count = ctypes.CDLL(sys.argv[1], ctypes.RTLD_GLOBAL)  # found before the runtime's own
+lib = ctypes.CDLL(sys.argv[2])
+i, p, z = ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t
+f = lib.sf_attn_decode_scored_i8kv
+f.argtypes = [p, i, p, p, p, p, i, p, p, i, p, z, i, i, i, i, p, i, i, i, i, ctypes.c_float, i, p]
+for T_max in map(int, sys.argv[3:]):
+    print(f(4096, 0, 4096, 4096, 4096, 4096, 1, 4096, 4096, 0, 4096, 1 << 62, 65535, 1, 1, 1, 4096, 0, T_max, T_max, 64,
+            0.125, 1, None), ctypes.c_int.in_dll(count, "launches").value)
+"""
+
+
+def test_scored_attention_checks_both_grids_before_a_launch(tmp_path):
+    """65535 sequences of 2^23 slots, 256 a workgroup of the second launch, are past 2^31 workgroups with
+    its rows: refused with nothing launched (the launch is stood in for by a counter)."""
+    (tmp_path / "count.cpp").write_text(COUNT)
+    so = tmp_path / "count.so"
+    subprocess.run(["g++", "-shared", "-fPIC", str(tmp_path / "count.cpp"), "-o", str(so)], check=True)
+    got = subprocess.run([sys.executable, "-c", ASK, str(so), _lib.LIB_PATH, str(1 << 23), str((1 << 23) + 1), "4096"],
+                         check=True, capture_output=True, text=True, timeout=100).stdout.split()
+    assert got[:4] == ["-1", "0", "-1", "0"], got
+    assert got[5] == "2", got  # (the counter counts: a call within the grid has its two launches)
