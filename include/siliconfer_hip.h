@@ -452,7 +452,7 @@ int sf_rotary_kv_append(const void *qkv, int in_dtype, const void *positions, in
  * or T where lengths is NULL, cut to [0, T_max]; a row that sees none gives zeros. With
  * w = softmax(scale q K^T): out [B][Tq][H][D] = w V, and scores [B][KVH][T_cap] (fp32)
  * += w summed over the rows and the kv head's query heads, slots past n_b untouched.
- * Tq <= 32. n_splits <= 0 picks a count. T_max (<= T_cap) bounds n_b and sizes the
+ * Tq <= 32. n_splits <= 0 picks a count. T_max (<= T_cap, <= 2^31 - 256) bounds n_b and sizes the
  * workspace: sf_attn_scored_workspace_bytes(...) bytes, 256-byte aligned, no initial
  * contents needed; calls that share one must not overlap. */
 size_t sf_attn_scored_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits);

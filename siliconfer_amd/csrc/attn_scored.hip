@@ -42,6 +42,7 @@ constexpr int kScThreads = 256;
 constexpr int kScWaves = kScThreads / 64;
 constexpr int kScMaxSplits = 128;
 constexpr int kScMaxRows = 32;       // query rows a sequence (Tq)
+constexpr int kScMaxSlots = 0x7fffff00;  // a slot number rounded up to a block of 256 stays an int
 
 struct ScoredArgs {
   const void *q;
@@ -513,7 +514,7 @@ int scored_splits(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits)
 }  // namespace
 
 extern "C" size_t sf_attn_scored_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits) {
-  if (B <= 0 || Tq <= 0 || H <= 0 || KVH <= 0 || H % KVH || T_max < 0 || D <= 0) return 0;
+  if (B <= 0 || Tq <= 0 || H <= 0 || KVH <= 0 || H % KVH || T_max < 0 || T_max > kScMaxSlots || D <= 0) return 0;
   size_t ml, s;
   return scored_parts(B, Tq, H, T_max, D, scored_splits(B, Tq, H, KVH, T_max, D, n_splits), &ml, &s);
 }
@@ -532,6 +533,7 @@ extern "C" int sf_attn_decode_scored_i8kv(const void *q, int q_dtype, const int8
   SF_REQUIRE(D <= 256, SF_EINVAL, "head_dim=%d exceeds kernel's compile-time max 256", D);
   SF_REQUIRE(D % 8 == 0, SF_EUNSUPPORTED, "head_dim=%d: need a multiple of 8", D);
   SF_REQUIRE(Tq <= kScMaxRows, SF_EUNSUPPORTED, "%d query rows a sequence: at most %d", Tq, kScMaxRows);
+  SF_REQUIRE(T_max <= kScMaxSlots, SF_EUNSUPPORTED, "T_max=%d: at most %d slots", T_max, kScMaxSlots);
   const int G = H / KVH;
   SF_REQUIRE(G <= 128, SF_EUNSUPPORTED, "%d query heads a kv head: at most 128", G);
   const int R = Tq * G, nrb = (R + 15) / 16;

@@ -280,3 +280,12 @@ def test_scored_attention_checks_both_grids_before_a_launch(tmp_path):
                          check=True, capture_output=True, text=True, timeout=100).stdout.split()
     assert got[:4] == ["-1", "0", "-1", "0"], got
     assert got[5] == "2", got  # (the counter counts: a call within the grid has its two launches)
+
+
+def test_scored_attention_s_longest_cache():
+    """Slots are rounded up to tiles and blocks in 32 bits: lengths within 255 of 2^31 are refused by name."""
+    lib = _lib.load()
+    for T in (0x7fffff01, 0x7fffffe0, 0x7fffffff):
+        refused(scored(ws_bytes=1 << 62, T=T, T_max=T, T_cap=T, D=8), -2, "2147483392 slots")
+        assert lib.sf_attn_scored_workspace_bytes(1, 1, 14, 2, T, 8, 0) == 0
+    assert lib.sf_attn_scored_workspace_bytes(1, 1, 14, 2, 0x7fffff00, 8, 0) > 14 * 4 * 0x7fffff00
