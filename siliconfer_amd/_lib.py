@@ -237,6 +237,13 @@ def scratch(device: torch.device, stream_handle: int, nbytes: int) -> torch.Tens
     return ws
 
 
+def check_ints(name: str, *numbers: int) -> None:
+    """Refuse numbers that a C int cannot hold (ctypes would cut them to their low half)."""
+    for v in numbers:
+        if not -0x80000000 <= v <= 0x7fffffff:
+            raise SFError(f"{name} {v} does not fit 32 bits")
+
+
 def lengths_arg(lengths, B: int, device: torch.device, name: str = "lengths") -> tuple[int | None, int]:
     """(device pointer or None, host value) of lengths given as int32 [B] or one int."""
     if not isinstance(lengths, torch.Tensor):

@@ -125,6 +125,8 @@ def attention_decode_scored(q: torch.Tensor, k_codes: torch.Tensor, k_scales: to
     slots up to its own, lengths[b] + add - Tq + t; a row that sees none gives zeros.
     `lengths`: int32 [B] on the device, or one int. Device lengths are cut to
     `max_length` (the capacity where it is not given), which sizes the workspace."""
+    n = n_splits or 0
+    _lib.check_ints("add / n_splits / max_length", add, n, max_length or 0)
     three = q.dim() == 3
     if not three and q.dim() != 4:
         raise SFError("q must be [B, n_heads, head_dim] or [B, rows, n_heads, head_dim]")
@@ -151,7 +153,6 @@ def attention_decode_scored(q: torch.Tensor, k_codes: torch.Tensor, k_scales: to
     elif out.shape != q.shape or out.device != q.device or not out.is_contiguous():
         raise SFError("out must be contiguous, of q's shape and on its device")
     lib = _lib.load()
-    n = n_splits or 0
     with _lib.on_device(q):
         st = _lib.stream(q)
         ws = _lib.scratch(q.device, st, _scored_bytes(B, Tq, H, KVH, T_max, D, n))

@@ -289,3 +289,18 @@ def test_scored_attention_s_longest_cache():
         refused(scored(ws_bytes=1 << 62, T=T, T_max=T, T_cap=T, D=8), -2, "2147483392 slots")
         assert lib.sf_attn_scored_workspace_bytes(1, 1, 14, 2, T, 8, 0) == 0
     assert lib.sf_attn_scored_workspace_bytes(1, 1, 14, 2, 0x7fffff00, 8, 0) > 14 * 4 * 0x7fffff00
+
+
+@pytest.mark.parametrize("big", [2 ** 32 + 5, 2 ** 31, -(2 ** 32) + 5])
+def test_numbers_past_32_bits_are_refused(big):
+    """They would reach the C entries cut to their low half."""
+    kc, ks = torch.zeros(1, 1, 8, 64, dtype=torch.int8), torch.zeros(1, 1, 8)
+    q, x, u = torch.zeros(1, 2, 64), torch.zeros(2, 10), torch.zeros(2)
+    for call in (lambda: evict(kc, ks, kc, ks, ks, ks.int(), 8, 8, big),
+                 lambda: evict(kc, ks, kc, ks, ks, ks.int(), 8, 8, 4, big),
+                 lambda: sample(x, u, top_k=big), lambda: sample(x, u, at=ks, at_add=big),
+                 lambda: attention_decode_scored(q, kc, ks, kc, ks, ks, lengths=3, add=big),
+                 lambda: attention_decode_scored(q, kc, ks, kc, ks, ks, lengths=3, max_length=big),
+                 lambda: attention_decode_scored(q, kc, ks, kc, ks, ks, lengths=3, n_splits=big)):
+        with pytest.raises(SFError, match="32 bits"):
+            call()
