@@ -22,14 +22,18 @@ from .. import _lib
 from .._lib import SFError
 
 
-def _append(k: torch.Tensor, v: torch.Tensor, qk, sk, qv, sv, t_off: int) -> None:
+def _check_kv(k: torch.Tensor, v: torch.Tensor) -> None:
     for t, n in ((k, "k"), (v, "v")):
         _lib.require_device(t, n)
-    B, KVH, Tn, D = k.shape
-    if v.shape != k.shape:
+    if k.dim() != 4 or v.shape != k.shape:
         raise SFError("k and v must have the same shape")
     if k.dtype not in (torch.float16, torch.bfloat16, torch.float32) or v.dtype != k.dtype:
         raise SFError(f"unsupported KV dtype {k.dtype}")
+
+
+def _append(k: torch.Tensor, v: torch.Tensor, qk, sk, qv, sv, t_off: int) -> None:
+    _check_kv(k, v)
+    B, KVH, Tn, D = k.shape
     T_cap = qk.shape[2]
     rc = _lib.load().sf_kv_quant_append(k.data_ptr(), v.data_ptr(), _lib.dt(k), qk.data_ptr(),
                                         sk.data_ptr(), qv.data_ptr(), sv.data_ptr(), _lib.dt(sk),
@@ -151,6 +155,7 @@ class QuantizedKVCache:
         """Quantize new (k, v) straight into the buffers at the current length."""
         k = k.contiguous()
         v = v.contiguous()
+        _check_kv(k, v)  # (before any buffer is made for them)
         self._ensure(k, self._len + k.shape[2])
         _append(k, v, self._qk, self._sk, self._qv, self._sv, self._len)
         self._len += k.shape[2]
@@ -214,8 +219,12 @@ class BoundedKVCache(QuantizedKVCache):
         """Append the next tokens' fused q|k|v rows [B, T, (H + 2 KVH) D], keys turned to
         their positions; returns the turned q [B, T, H, D]."""
         from ..kernels.rotary import rotary_kv_append
-        B, T, W = qkv.shape
-        D = W // (n_heads + 2 * n_kv_heads)
+        _lib.require_device(qkv, "qkv")  # (all before any buffer is made for the rows)
+        B, T, W = qkv.shape if qkv.dim() == 3 else (0, 0, 0)
+        D = W // (n_heads + 2 * n_kv_heads) if n_heads > 0 and n_kv_heads > 0 and n_heads % n_kv_heads == 0 else 0
+        if D == 0 or D % 8 or D > 256 or W != (n_heads + 2 * n_kv_heads) * D:
+            raise SFError(f"qkv {list(qkv.shape)} does not hold {n_heads} and 2 x {n_kv_heads} heads of a multiple of 8 "
+                          "dims up to 256")
         self.reserve(B, n_kv_heads, D, self._len + T, qkv.device)
         positions = torch.arange(self.seen, self.seen + T, dtype=torch.int32, device=qkv.device)
         q = rotary_kv_append(qkv, positions, rotary.on(qkv.device), *self.buffers(), n_heads=n_heads,

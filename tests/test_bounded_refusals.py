@@ -14,7 +14,7 @@ from siliconfer_amd.kernels.attention import attention_decode_scored
 from siliconfer_amd.kernels.eviction import evict
 from siliconfer_amd.kernels.rotary import rotary, rotary_kv_append
 from siliconfer_amd.kernels.sampling import sample
-from siliconfer_amd.model import BoundedKVCache
+from siliconfer_amd.model import BoundedKVCache, QuantizedKVCache, Rotary, rotary_frequencies
 
 P = 4096  # a pointer that is never followed: every call below is refused before its launch
 F32, F16, BF16 = _lib.SF_F32, _lib.SF_F16, _lib.SF_BF16
@@ -304,3 +304,22 @@ def test_numbers_past_32_bits_are_refused(big):
                  lambda: attention_decode_scored(q, kc, ks, kc, ks, ks, lengths=3, n_splits=big)):
         with pytest.raises(SFError, match="32 bits"):
             call()
+
+
+def test_a_refused_append_leaves_no_buffers_behind():
+    """Buffers made for a call that is then refused would not fit the next, right one."""
+    rot = Rotary(*rotary_frequencies(64))
+    cpu = torch.zeros(1, 3, 6 * 64)
+    for qkv, heads, kv_heads in ((cpu, 4, 1), (torch.zeros(3, 6 * 64), 4, 1), (torch.zeros(1, 3, 385), 4, 1),
+                                 (torch.zeros(1, 3, 7 * 64), 3, 2), (torch.zeros(1, 3, 6 * 60), 4, 1),
+                                 (torch.zeros(1, 3, 6 * 264), 4, 1), (cpu, 4, 0), (cpu, 0, 1)):
+        cache = BoundedKVCache(16)
+        with pytest.raises(SFError):
+            cache.append_rotary(qkv, heads, kv_heads, rot)
+        assert cache.buffers() == (None,) * 4 and cache.length() == cache.seen == 0
+    k = torch.zeros(1, 2, 3, 64)
+    for made in (BoundedKVCache(16), QuantizedKVCache(16)):
+        for a, b in ((k, k), (k, k[:, :1]), (k.double(), k.double())):
+            with pytest.raises(SFError):
+                made.append(a, b)
+            assert made.buffers() == (None,) * 4 and made.length() == 0
