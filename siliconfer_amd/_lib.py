@@ -237,11 +237,12 @@ def scratch(device: torch.device, stream_handle: int, nbytes: int) -> torch.Tens
     return ws
 
 
-def check_ints(name: str, *numbers: int) -> None:
-    """Refuse numbers that a C int cannot hold (ctypes would cut them to their low half)."""
-    for v in numbers:
-        if not -0x80000000 <= v <= 0x7fffffff:
-            raise SFError(f"{name} {v} does not fit 32 bits")
+INT_MIN, INT_MAX = -0x80000000, 0x7fffffff
+
+
+def refuse_int(**numbers):
+    """Raise for numbers of which a C int cannot hold one (ctypes would cut it to its low half)."""
+    raise SFError(", ".join(f"{k} {v}" for k, v in numbers.items()) + ": numbers must fit 32 bits")
 
 
 def lengths_arg(lengths, B: int, device: torch.device, name: str = "lengths") -> tuple[int | None, int]:

@@ -126,7 +126,9 @@ def attention_decode_scored(q: torch.Tensor, k_codes: torch.Tensor, k_scales: to
     `lengths`: int32 [B] on the device, or one int. Device lengths are cut to
     `max_length` (the capacity where it is not given), which sizes the workspace."""
     n = n_splits or 0
-    _lib.check_ints("add / n_splits / max_length", add, n, max_length or 0)
+    if not (_lib.INT_MIN <= add <= _lib.INT_MAX and _lib.INT_MIN <= n <= _lib.INT_MAX
+            and _lib.INT_MIN <= (max_length or 0) <= _lib.INT_MAX):
+        _lib.refuse_int(add=add, n_splits=n, max_length=max_length)
     three = q.dim() == 3
     if not three and q.dim() != 4:
         raise SFError("q must be [B, n_heads, head_dim] or [B, rows, n_heads, head_dim]")

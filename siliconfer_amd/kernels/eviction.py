@@ -25,7 +25,8 @@ def evict(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, 
     int32 [B]: min(length, budget). `lengths` and `seen` (the tokens each sequence has
     had so far): int32 [B] on the device, or one int for all. Slots at and past the
     new length are left as they were."""
-    _lib.check_ints("budget / recent", budget, recent)
+    if not (_lib.INT_MIN <= budget <= _lib.INT_MAX and _lib.INT_MIN <= recent <= _lib.INT_MAX):
+        _lib.refuse_int(budget=budget, recent=recent)
     _lib.require_device(k_codes, "k_codes")
     if k_codes.dim() != 4:
         raise SFError("k_codes / v_codes must both be [B, n_kv_heads, T, head_dim]")

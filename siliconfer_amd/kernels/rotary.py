@@ -60,32 +60,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     """(q turned, k turned) at positions [B, T] or [T], in q's dtype. `out_q` /
     `out_k` may be the inputs themselves; other outputs must not overlap them, and
     inputs that need a gradient take none. Differentiable in q and k."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         if out_q is not None or out_k is not None:
             raise SFError("rotary: inputs that need a gradient take no out_q / out_k")
         return _Turn.apply(q, k, positions, inv_freq, interleaved, scale)
-    return _rotary(q, k, positions, inv_freq, interleaved, scale, out_q, out_k)
-
-
-class _Turn(torch.autograd.Function):
-    """A turn by an angle is orthogonal but for its scale: the gradient is turned back by
-    the same kernel, at the opposite positions."""
-
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, interleaved, scale):
-        ctx.save_for_backward(positions, inv_freq)
-        ctx.how = interleaved, scale
-        return _rotary(q, k, positions, inv_freq, interleaved, scale)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        positions, inv_freq = ctx.saved_tensors
-        gq, gk = (g if g is None or g.stride(3) == 1 else g.contiguous() for g in (gq, gk))
-        return (*_rotary(gq, gk, -positions, inv_freq, *ctx.how), None, None, None, None)
-
-
-def _rotary(q, k, positions, inv_freq, interleaved, scale, out_q=None, out_k=None):
     _rows(q, "q")
     B, T, H, D = q.shape
     KVH = 0
@@ -127,6 +105,24 @@ def _rotary(q, k, positions, inv_freq, interleaved, scale, out_q=None, out_k=Non
     if rc:
         _lib.check(rc, "sf_rotary")
     return out_q, out_k
+
+
+class _Turn(torch.autograd.Function):
+    """A turn by an angle is orthogonal but for its scale: the gradient is turned back by
+    the same kernel, at the opposite positions. (Both run with gradients off.)"""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, interleaved, scale):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = dict(interleaved=interleaved, scale=scale)
+        return rotary(q, k, positions, inv_freq, **ctx.how)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        positions, inv_freq = ctx.saved_tensors
+        gq, gk = (g if g is None or g.stride(3) == 1 else g.contiguous() for g in (gq, gk))
+        return (*rotary(gq, gk, -positions, inv_freq, **ctx.how), None, None, None, None)
 
 
 def rotary_kv_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,

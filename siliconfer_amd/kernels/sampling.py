@@ -36,7 +36,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     above -inf gives -1. For steps replayed from a graph, `at`, int32 [1] on the device,
     counts the steps: u then holds every step's numbers (fp32 [n], n >= B), row b takes
     u[at + at_add + b], and its token also goes to the same place of `hist`, int32 [n]."""
-    _lib.check_ints("top_k / at_add", 0 if isinstance(top_k, torch.Tensor) else top_k, at_add)
+    k = 0 if isinstance(top_k, torch.Tensor) else top_k
+    if not (_lib.INT_MIN <= at_add <= _lib.INT_MAX and _lib.INT_MIN <= k <= _lib.INT_MAX):
+        _lib.refuse_int(top_k=top_k, at_add=at_add)
     if not logits.is_cuda:
         raise SFError(f"logits must be a device tensor (got {logits.device})")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] != 1):
