@@ -14,15 +14,20 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "siliconfer_amd", "csrc")
 
 SHIM = r"""
+#include <xmmintrin.h>
 #include "sample_place.h"
 // of n logits: bins and weights below the bin of the maximum m; returns the bin number of m
-extern "C" double bins(const float *x, long n, float T, float m, int *bin, unsigned long long *w) {
+extern "C" double bins(const float *x, long n, double temperature, float m, int *bin, unsigned long long *w) {
+  const unsigned mode = _mm_getcsr();  // a library that is loaded beside may have turned subnormals off; kernels have them
+  _mm_setcsr(mode & ~0x8040u);
+  const volatile float T = (float)temperature;
   const double per = bins_per_logit(T), top = top_bin(m, per);
   for (long i = 0; i < n; ++i) {
     const Binned b = bin_of(x[i], per, top);
     bin[i] = b.bin;
     w[i] = b.w;
   }
+  _mm_setcsr(mode);
   return top;
 }
 """
@@ -36,7 +41,7 @@ def bins(tmp_path_factory):
                     "-o", str(d / "shim.so")], check=True)
     f = ctypes.CDLL(str(d / "shim.so")).bins
     f.restype = ctypes.c_double
-    f.argtypes = [ctypes.c_void_p, ctypes.c_long, ctypes.c_float, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p]
+    f.argtypes = [ctypes.c_void_p, ctypes.c_long, ctypes.c_double, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p]
 
     def call(x, T, m):
         x = np.ascontiguousarray(x, np.float32)
