@@ -27,7 +27,7 @@
 // Measured (us, split + finishing launch): 1501 slots at 14/2 heads of 64 4.2 + 3.8; four
 // ragged sequences of up to 8191 (50 MB of cache, 10.2 us at a copy's rate) at 32/8 heads
 // of 128 16.3 + 5.5, from 24.8 + 15.3 with loads and math of a tile in turn, two merge
-// launches and a serial loop over the splits. VALU issue is half of the split's time (the
+// launches and a serial loop over the splits. VALU issue is 44% of the split's time (the
 // conversion of codes and the softmax of 16 rows where a kv head has 4), the rest launch,
 // first loads and the merge of its waves.
 #include <math.h>
@@ -505,6 +505,14 @@ size_t scored_parts(int B, int Tq, int H, int T_max, int D, int S, size_t *ml_of
   return *s_off + rows * scored_tp(T_max) * sizeof(float);
 }
 
+// The decode attention's rule, with a block of 16 query rows a kv head. Measured for these kernels
+// (us a call in a replayed graph, both launches, at the rule's count; other counts in
+// parentheses), 14 / 2 heads of 64, fp16: 500 slots 7.1 (16; 4: 7.3, 8: 7.1); 1501 7.2 (47; 12: 7.3, 32:
+// 7.1); 4096 7.2 (64; 32: 7.4, 96: 8.0); 16384 9.9 (128; 48: 9.9, 64: 9.2); 16 fp32 rows over 2000
+// 15.8 (19; 8: 14.8, 16: 14.1, 32: 15.4). 32 / 8 heads of 128, bf16: 2000 9.3 (32; 16: 9.4, 48: 11.4);
+// 8191 14.9 (64; 32: 14.1, 128: 19.5); four ragged sequences of 1000 10.0 (8; 4: 11.4, 16: 11.2), of
+// 8191 23.5 (16; 8: 27.7, 24: 23.2, 32: 24.4); eight of 2001, fp32, 16.3 (8; 4: 17.8, 16: 18.2); sixteen of 4000
+// 35.4 (4; 2: 42.3, 6: 35.1, 8: 35.7). 32 / 32 heads, four of 2000 21.7 (4; 2: 26.1, 8: 23.4).
 int scored_splits(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits) {
   const int blocks = (Tq * (H / KVH) + 15) / 16;
   if (n_splits <= 0) n_splits = sf_attn_default_splits_d(B, KVH * blocks, T_max, D);
@@ -546,7 +554,10 @@ extern "C" int sf_attn_decode_scored_i8kv(const void *q, int q_dtype, const int8
   SF_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes) & 7) == 0, SF_EINVAL,
              "KV code buffers must be 8-byte aligned");
   SF_REQUIRE(((uintptr_t)q & 15) == 0, SF_EINVAL, "q must be 16-byte aligned");
-  // 256 slots a workgroup of the second launch where that gives every CU two, else 64
+  // 256 slots a workgroup of the second launch where that gives every CU two, else 64. us a call
+  // with 256 / 64, shapes as above: 128 workgroups of 256 (one sequence of 16384, 2 kv heads) 9.7 / 9.9,
+  // 12 of them 7.7 / 7.3, 16 rows 18.9 / 15.8; 256 (8191, 8 kv heads) 14.7 / 15.1; 512 16.7 / 18.2;
+  // 1024 23.9 / 26.6 and 22.3 / 25.1.
   const bool many = (long long)B * KVH * ((T_max + 255) / 256) >= 512;
   const int rows = B * Tq * H, per = many ? 256 : 64, tok_blocks = (T_max + per - 1) / per;
   SF_REQUIRE((long long)B * KVH * tok_blocks + rows <= 0x7fffffffLL, SF_EINVAL, "B=%d T_max=%d exceed the grid", B, T_max);

@@ -32,10 +32,10 @@
 // the one that the search falls into can be ordered, as a rule after one pass.
 // Measured (us, first + second launch; a workgroup a row with radix passes over it in
 // brackets): 1 x 151936 fp32, top-k 50 and top-p, 6.6 + 8.8 (865); 64 x 151936 bf16, a
-// row's own settings, 17.8 + 13.0 (993), of them 3.8 for the bytes at a copy's rate; at
-// temperature alone a draw past the head re-reads its row: 8 x 32000 6.5 + 17.4 (6.8 with
-// all draws within the head), of normal logits, none within it, 37 a call, 8 x 151936 112
-// (the one workgroup's VALU: some 45 a pass). The first launch is bound by VALU issue (42
+// row's own settings, 18.4 + 12.9 (993), of them 3.8 for the bytes at a copy's rate; at
+// temperature alone a draw past the head re-reads its row: 8 x 32000 6.5 + 17.6 (6.8 with
+// all draws within the head), of normal logits, none within it, 38 a call, 8 x 151936 114
+// (the one workgroup's VALU: some 45 a pass). The first launch is bound by VALU issue (43
 // instructions an element, two thirds of the time) and the five barriers of its
 // workgroups, two a CU at a time; the second by the latency of some twenty dependent steps
 // of one workgroup a row.
@@ -51,7 +51,11 @@ constexpr int kSampThreads = 1024;
 constexpr int kSampWaves = kSampThreads / 64;
 constexpr int kBinThreads = 1024;   // of the first kernel
 constexpr int kBinWaves = kBinThreads / 64;
-constexpr int kPerThread = 10;      // (64 rows of 151936: 29.8 us a call, with 8 31.2, with 12 29.8)
+// Logits a thread holds. us a call in a replayed graph, fp32, top-k 50 and top-p, with 10 (4; 6; 8;
+// 12): 1 x 32000 14.2 (13.7; 13.8; 14.1; 14.5), 64 x 32000 16.6 (17.1; 17.6; 16.6; 16.7), 64 x 50257
+// 19.6 (22.4; 20.7; 19.1; 20.1), 1 x 151936 15.4 (18.6; 16.7; 16.0; 15.7), 64 x 151936 29.3 (41.1;
+// 34.5; 31.2; 29.6).
+constexpr int kPerThread = 10;
 constexpr int kChunk = kBinThreads * kPerThread;
 constexpr int kListCap = 128;       // elements of a chunk's list
 constexpr int kBinCap = 1024;       // elements of a bin, or of a range of keys, ordered at once

@@ -32,7 +32,7 @@ draws use torch on the device from a generator seeded with `seed` (the
 reference seeds MLX's generator and draws its acceptance uniforms from
 Python's `random`; both are replaced by the one seeded torch generator). As in
 the reference, sampling here uses the temperature only (no top-k / top-p /
-repetition penalty, :53-59).
+min-p / repetition penalty, :53-59).
 
 Differences a caller can see:
   * K + 1 must fit the verify's 8 rows: K > 7 raises; with `dynamic_K`, K
