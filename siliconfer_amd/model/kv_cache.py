@@ -178,8 +178,8 @@ class BoundedKVCache(QuantizedKVCache):
     tokens (a quarter of the budget by default) stay. Each kv head keeps tokens of its
     own, in any order, with their `positions`; `length()` counts slots, `seen` the
     tokens that went through. Keys are cached turned to their positions. The buffers have
-    budget + slack + 1 slots; for a longer prompt they grow, until `release` or the first
-    append after the cut that fits those again."""
+    budget + slack + 1 slots; for a longer prompt (or by `reserve`) they grow, until
+    `release` or the first append after a cut that fits those again."""
 
     def __init__(self, budget: int, recent: int | None = None, slack: int = 64,
                  scale_dtype: torch.dtype = torch.float16) -> None:
@@ -190,9 +190,12 @@ class BoundedKVCache(QuantizedKVCache):
         self.budget, self.recent, self.slack = int(budget), int(recent), int(slack)
         self.seen = 0
         self.scores = self.positions = None
+        self._cut = False  # shortened since the buffers were last asked to hold more than the bound
 
     def _ensure(self, k: torch.Tensor, need: int) -> None:
-        if need <= self.budget + self.slack + 1:
+        if need > self.budget + self.slack + 1:
+            self._cut = False
+        elif self._cut:
             self.release()
         before = self._qk
         super()._ensure(k, need)
@@ -246,6 +249,7 @@ class BoundedKVCache(QuantizedKVCache):
         if self._len > self.budget + self.slack:
             evict(*self.buffers(), self.scores, self.positions, self._len, self.seen, self.budget, self.recent)
             self._len = self.budget
+            self._cut = True
 
     def release(self) -> None:
         """Let buffers that grew for a prompt go back to budget + slack + 1 slots, if what is
@@ -259,6 +263,7 @@ class BoundedKVCache(QuantizedKVCache):
             a[:, :, :n].copy_(b[:, :, :n])
         self._qk, self._sk, self._qv, self._sv, self.scores, self.positions = new
         self.capacity = base
+        self._cut = False
 
     def nbytes(self) -> int:
         """Footprint of the valid slots: codes, scales, scores and positions."""
@@ -275,3 +280,4 @@ class BoundedKVCache(QuantizedKVCache):
             raise SFError("a bounded cache that dropped tokens cannot be trimmed")
         super().trim(n)
         self.seen = min(self.seen, max(0, int(n)))
+        self._cut = True

@@ -258,8 +258,10 @@ class Attention(torch.nn.Module):
                     vs[b].data_ptr(), _lib.dt(ks), out[b].data_ptr(), _lib.SF_F32, T, H, KVH, n - T, kq.shape[2], D,
                     float(self.scale), st), "sf_attn_prefill_i8kv")
             out[:, -self.OBSERVED:] = cache.attend(q[:, -self.OBSERVED:].contiguous(), self.scale)
+        n = cache.length()
         cache.evict()
-        cache.release()  # (a prompt's buffers, before the next layer allocates its own)
+        if cache.length() < n:
+            cache.release()  # (a prompt's buffers, before the next layer allocates its own)
         return out
 
     def _int8_batch1(self, qkv, cache: QuantizedKVCache, T: int, device) -> torch.Tensor:

@@ -323,3 +323,23 @@ def test_a_refused_append_leaves_no_buffers_behind():
             with pytest.raises(SFError):
                 made.append(a, b)
             assert made.buffers() == (None,) * 4 and made.length() == 0
+
+
+def test_a_reservation_in_a_bounded_cache_is_kept(monkeypatch):
+    """reserve() holds through appends and evictions that cut nothing; buffers go back past a cut only."""
+    from siliconfer_amd.kernels import eviction
+    monkeypatch.setattr(eviction, "evict", lambda *a: None)
+    cache, cpu = BoundedKVCache(20, 5, slack=3), torch.device("cpu")
+    cache.reserve(1, 2, 16, 400, cpu)
+    first = [t.data_ptr() for t in (*cache.buffers(), cache.scores, cache.positions)]
+    for n in range(1, 24):
+        cache.reserve(1, 2, 16, n, cpu)  # as an append does
+        cache._len = cache.seen = n
+        cache.evict()
+    assert [t.data_ptr() for t in (*cache.buffers(), cache.scores, cache.positions)] == first
+    cache.reserve(1, 2, 16, 24, cpu)
+    cache._len = cache.seen = 24
+    cache.evict()
+    assert cache.length() == 20
+    cache.reserve(1, 2, 16, 21, cpu)
+    assert cache.buffers()[0].shape[2] == 24
