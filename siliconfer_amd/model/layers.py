@@ -156,7 +156,8 @@ class Attention(torch.nn.Module):
         self.v_proj = _dense(H, self.num_kv_heads * D, bias, device)
         self.o_proj = _dense(self.num_heads * D, H, False, device)
         self._cos = self._sin = None
-        self._rotary_of(device)
+        if rotary is not None or (isinstance(rope_freqs, torch.Tensor) and not rope_freqs.is_meta):
+            self._rotary_of(device)
 
     def _rotary_of(self, device) -> Rotary:
         """`rotary`, or rotate-half over the whole head of `rope_freqs` (made when these are

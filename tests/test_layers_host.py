@@ -49,3 +49,12 @@ def test_checkpoint_arrays_from_numpy_or_torch():
     for src in (h, torch.from_numpy(h)):
         t = _f32(src)
         assert t.dtype == torch.float32 and t.tolist() == [1.5, -2.25]
+
+
+def test_a_layer_is_built_without_its_frequencies_values():
+    """Frequencies that have no values yet (the meta device), or none beside a Rotary, do not stop the construction."""
+    from siliconfer_amd.model import Rotary, rotary_frequencies
+
+    attn = Attention(CFG, compute_rope_freqs(CFG).to("meta"), device="meta")
+    assert attn.q_proj.weight.is_meta
+    assert Attention(CFG, None, "cpu", Rotary(*rotary_frequencies(16))).rope_freqs is None
