@@ -431,6 +431,28 @@ int sf_rotary(const void *q, void *q_out, const void *k, void *k_out, int dtype,
               int pos_i64, int pos_per_seq, const double *inv_freq, int rot_pairs, float scale,
               int interleaved, int B, int T, int H, int KVH, int D, const long long *strides,
               void *stream);
+/* Queries and keys normed a head, then turned as above, in one pass: each head x of D dims
+ * becomes x / sqrt(mean(x^2) + eps) * weight ([D] of weight_dtype, q's heads and k's each
+ * their own) before its pairs turn, in fp32 with one rounding to `dtype`. D <= 256. */
+int sf_qk_norm_rotary(const void *q, void *q_out, const void *k, void *k_out, int dtype,
+                      const void *q_weight, const void *k_weight, int weight_dtype, float eps,
+                      const void *positions, int pos_i64, int pos_per_seq, const double *inv_freq,
+                      int rot_pairs, float scale, int interleaved, int B, int T, int H, int KVH, int D,
+                      const long long *strides, void *stream);
+/* Its gradients: from the rows q, k as they were given and the outputs' gradients q_grad,
+ * k_grad to dq_out, dk_out (all of `dtype`) and dq_weight, dk_weight (fp32 [D], summed over
+ * all rows and heads in a fixed order). strides: NULL, or 18 element strides (batch, row,
+ * head of q, q_grad, dq_out, k, k_grad, dk_out). B, T > 0. The workspace is 16-byte aligned;
+ * nothing in it needs clearing. */
+size_t sf_qk_norm_backward_workspace_bytes(int B, int T, int H, int KVH, int D);
+int sf_qk_norm_rotary_backward(const void *q, const void *q_grad, void *dq_out, const void *k,
+                               const void *k_grad, void *dk_out, int dtype, const void *q_weight,
+                               const void *k_weight, int weight_dtype, float *dq_weight,
+                               float *dk_weight, float eps, const void *positions, int pos_i64,
+                               int pos_per_seq, const double *inv_freq, int rot_pairs, float scale,
+                               int interleaved, int B, int T, int H, int KVH, int D,
+                               const long long *strides, void *workspace, size_t workspace_bytes,
+                               void *stream);
 /* The same rotation of the q and k heads of fused projection rows qkv
  * [B][T][(H + 2 KVH) D] (in_dtype), then the int8 quantize-append of k and v (the rule of
  * sf_kv_quant_append) into slots n_b + t of a cache [B][KVH][T_cap][D], n_b =
@@ -445,6 +467,44 @@ int sf_rotary_kv_append(const void *qkv, int in_dtype, const void *positions, in
                         int8_t *v_codes, void *v_scales, int scale_dtype, int32_t *slot_positions,
                         float *scores, const int32_t *lengths, int start, int B, int T, int H, int KVH,
                         int D, int T_cap, void *stream);
+
+/* ---- a KV cache held in 4 bits (no counterpart in the reference) ----------------------
+ * codes uint8 [B][KVH][T_cap][D / 2], the even dim of two in the low half of a byte; params
+ * fp16 [B][KVH][T_cap][D / group][2], (s, m) a group of dims: a value is m + s code, with
+ * m = min x, s = (max x - min x) / 15 (fp32, then fp16, held within fp16's range) and code =
+ * clip(rint((x - m) / s), 0, 15), ties to even, 0 where s is 0; x in 64 bits. A group with a
+ * value that is not finite gets NaN for both. D a multiple of 16 up to 256; group 32, 64, 128
+ * or D.
+ * Appends k and v [B, T, KVH, D] (strides: 9 element strides, batch, row, head of q, k, v;
+ * whole 8 elements, pointers 16-byte aligned) to slots n_b + t, n_b = lengths[b] (device) or
+ * `start`; a token whose slot would lie past T_cap is not stored. With q_weight / k_weight
+ * ([D] of weight_dtype, or NULL) q's / k's heads are normed as in sf_qk_norm_rotary, and with
+ * rot_pairs > 0 both turn as in sf_rotary. q [B, T, H, D] goes to q_out [B][T][H][D]; H = 0
+ * where there is none. */
+int sf_kv_q4_append(const void *q, const void *k, const void *v, int in_dtype, const long long *strides,
+                    const void *q_weight, const void *k_weight, int weight_dtype, float eps,
+                    const void *positions, int pos_i64, int pos_per_seq, const double *inv_freq,
+                    int rot_pairs, float scale, int interleaved, void *q_out, int q_dtype,
+                    uint8_t *k_codes, void *k_params, uint8_t *v_codes, void *v_params, int group,
+                    const int32_t *lengths, int start, int B, int T, int H, int KVH, int D, int T_cap,
+                    void *stream);
+/* The values of T slots of B x KVH heads to out [B][KVH][T][D]; strides: 6 element strides
+ * (batch, head, slot of codes, in bytes, and of params, in fp16 numbers). */
+int sf_kv_q4_dequant(const uint8_t *codes, const void *params, void *out, int out_dtype, int group,
+                     const long long *strides, int B, int KVH, int T, int D, void *stream);
+/* Attention of the Tq newest rows a sequence, q [B][Tq][H][D], over the first n_b slots of
+ * such a cache: softmax(scale q K^T) V to out [B][Tq][H][D], rounded once to out_dtype. n_b =
+ * lengths[b] + T (device lengths, T may be negative) cut to 0 .. T_max, or T where lengths is
+ * NULL; row t sees the first n_b - Tq + t + 1 slots, a row that sees none gives zeros, and what
+ * a row does not see may hold anything. n_splits <= 0: the kernel's own choice; at most 128
+ * are used. The workspace (sf_attn_q4_workspace_bytes, 256-byte aligned; none for 0 bytes)
+ * needs no clearing. q and the cache's buffers 16-byte aligned. */
+size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits);
+int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, const void *k_params,
+                 const uint8_t *v_codes, const void *v_params, int group, void *out, int out_dtype,
+                 void *workspace, size_t workspace_bytes, int B, int Tq, int H, int KVH,
+                 const int32_t *lengths, int T, int T_max, int T_cap, int D, float scale, int n_splits,
+                 void *stream);
 
 /* ---- a cache that keeps what is attended to (no counterpart in the reference) ------
  * Decode attention that scores the cache it reads. Row t of q [B][Tq][H][D] sees the

@@ -107,6 +107,12 @@ _SIGS = {
                                       _c_p]),
     "sf_rotary": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_p, _c_i, _c_f, _c_i, _c_i,
                          _c_i, _c_i, _c_i, _c_i, _c_p, _c_p]),
+    "sf_qk_norm_rotary": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_i, _c_f, _c_p, _c_i, _c_i, _c_p, _c_i,
+                                 _c_f, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_p, _c_p]),
+    "sf_qk_norm_backward_workspace_bytes": (_c_sz, [_c_i, _c_i, _c_i, _c_i, _c_i]),
+    "sf_qk_norm_rotary_backward": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_i, _c_p, _c_p,
+                                          _c_f, _c_p, _c_i, _c_i, _c_p, _c_i, _c_f, _c_i, _c_i, _c_i, _c_i, _c_i,
+                                          _c_i, _c_p, _c_p, _c_sz, _c_p]),
     "sf_rotary_kv_append": (_c_i, [_c_p, _c_i, _c_p, _c_i, _c_i, _c_p, _c_i, _c_f, _c_i, _c_p, _c_i, _c_p,
                                    _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i,
                                    _c_i, _c_i, _c_p]),
@@ -114,6 +120,13 @@ _SIGS = {
     "sf_attn_decode_scored_i8kv": (_c_i, [_c_p, _c_i, _c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_i, _c_p,
                                           _c_sz, _c_i, _c_i, _c_i, _c_i, _c_p, _c_i, _c_i, _c_i, _c_i,
                                           _c_f, _c_i, _c_p]),
+    "sf_kv_q4_append": (_c_i, [_c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_p, _c_i, _c_f, _c_p, _c_i, _c_i, _c_p, _c_i,
+                               _c_f, _c_i, _c_p, _c_i, _c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_i, _c_i,
+                               _c_i, _c_i, _c_i, _c_p]),
+    "sf_kv_q4_dequant": (_c_i, [_c_p, _c_p, _c_p, _c_i, _c_i, _c_p, _c_i, _c_i, _c_i, _c_i, _c_p]),
+    "sf_attn_q4_workspace_bytes": (_c_sz, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "sf_attn_q4kv": (_c_i, [_c_p, _c_i, _c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_p, _c_sz, _c_i, _c_i, _c_i, _c_i,
+                            _c_p, _c_i, _c_i, _c_i, _c_i, _c_f, _c_i, _c_p]),
     "sf_kv_evict_workspace_bytes": (_c_sz, [_c_i, _c_i, _c_i, _c_i]),
     "sf_kv_evict": (_c_i, [_c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_i,
                            _c_p, _c_p, _c_sz, _c_i, _c_i, _c_i, _c_i, _c_p]),

@@ -33,8 +33,8 @@ HIPCC_FLAGS = [
 # (without this the compiler keeps them in AGPRs and moves them back and forth
 # around the softmax and the accumulator rescaling; measured 1.5% faster).
 _VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-FILE_FLAGS = {f: _VGPR_FORM for f in ("kv_attn.hip", "attn_scored.hip", "q4_gemm_rows_f16.hip", "q4_gemm_rows_bf16.hip",
-                                      "q4_gemm_rows_f32.hip")}
+FILE_FLAGS = {f: _VGPR_FORM for f in ("kv_attn.hip", "attn_scored.hip", "attn_q4.hip", "q4_gemm_rows_f16.hip",
+                                      "q4_gemm_rows_bf16.hip", "q4_gemm_rows_f32.hip")}
 
 
 def _hipcc() -> str:

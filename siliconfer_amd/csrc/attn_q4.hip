@@ -1,0 +1,596 @@
+// attn_q4.hip — attention over a KV cache held in 4 bits (gfx950).
+//
+// For Tq query rows a sequence (row t sees the first n - Tq + t + 1 of its n slots):
+//   out = softmax(scale q K^T) V,  K = s c + m and V alike, (s, m) a group of g dims.
+// A group's part of a score is s (q . c) + m sum(q), of an output sum(p s c) + sum(p m):
+// the codes c go through the matrix units as they are, s and m join in fp32.
+//
+// The codes as MFMA operands: v_mfma_f32_16x16x32_f16 takes fp16's subnormals at their
+// value, so a code in the low bits of a half is c 2^-24, and one four bits higher 16 c 2^-24:
+// w & 0x000f000f and w & 0x00f000f0 of a word of eight codes are two operand registers (codes
+// 0, 4 and 1, 5), the same of w >> 8 the others: five operations for eight codes. The other
+// operand takes the same order and, for the odd pairs, a sixteenth.
+//
+// k_q4_split: one workgroup a (split, kv head and 16 of its rows, sequence); its four waves
+// take 64-slot tiles. S^T = K q^T and O^T = V^T P^T with the query rows on the 16-wide side:
+//   * row m of S^T's block h is slot 4 m + h of the tile, so lane l holds row l % 16 and the 16
+//     neighbouring slots 16 (l / 16) .. of it, value (h, i) slot 4 i + h;
+//   * V^T comes through LDS with ds_read_b64_tr_b4, which hands a lane one dim's codes of 16
+//     slots: both B operands' order;
+//   * q (fp32) and P as fp16 high and low parts, q brought to a largest magnitude of 2^13..2^14
+//     by a power of two a row, P times the V scale likewise by the largest one that the row
+//     has met: what the low part drops is below 2^-22 of the value and 2^-38 of the row's
+//     largest. fp16 and bf16 queries are exact in the high part alone; for a bf16 output P's low
+//     part is left out (2^-12 of a weight beside the 2^-9 of the output's rounding).
+// Maxima, sums, m's part and the partials are fp32.
+#include <math.h>
+
+#include "attn_common.h"
+#include "sf_common.h"
+#include "split_merge.h"
+
+int sf_q4_cache_check(int D, int g);  // kv_q4.hip
+
+namespace {
+
+constexpr int kQaThreads = 256;
+constexpr int kQaWaves = kQaThreads / 64;
+constexpr int kQaMaxSplits = 128;
+constexpr int kQaMaxSlots = 0x7fffff00;
+
+struct Q4Attn {
+  const void *q;
+  const uint8_t *kc, *vc;
+  const uint32_t *kp, *vp;
+  void *out;
+  float *part_acc, *part_ml;
+  const int *lengths;
+  int odt, T, T_max, T_cap, Tq, H, KVH, D, g, n_splits;
+  float qscale;
+};
+
+__device__ __forceinline__ int q4_len(const int *lengths, int T, int T_max, int b) {
+  const long long n = (long long)(lengths ? lengths[b] : 0) + T;
+  return n < 0 ? 0 : n > T_max ? T_max : (int)n;
+}
+
+// The power of two that takes a magnitude v to [2^13, 2^14) (1 for 0, and within the
+// range of fp32's exponents).
+__device__ __forceinline__ float q4_fit14(float v) {
+  const int e = (int)(sf_bitcast<uint32_t>(v) >> 23 & 255);
+  const int f = 127 + 13 + 127 - e;
+  return v == 0.f ? 1.f : sf_bitcast<float>((uint32_t)(f < 1 ? 1 : f > 253 ? 253 : f) << 23);
+}
+
+// Eight codes as fp16 subnormals: codes 0, 4, 1, 5, 2, 6, 3, 7, times 2^-24, the pairs 1, 5 and
+// 3, 7 times 16 more.
+__device__ __forceinline__ half8_t q4_codes(uint32_t w) {
+  const uint32_t x = w >> 8;
+  const u32x4 r = {w & 0x000f000fu, w & 0x00f000f0u, x & 0x000f000fu, x & 0x00f000f0u};
+  return sf_bitcast<half8_t>(r);
+}
+
+// Eight codes less 8, exact: codes 0, 4, 1, 5, 2, 6, 3, 7.
+__device__ __forceinline__ half8_t q4_signed(uint32_t w) {
+  const uint32_t x = w >> 8;
+  const half2_t a = {(f16)-1032.f, (f16)-1032.f}, b = {(f16)-72.f, (f16)-72.f};
+  const half2_t p0 = sf_bitcast<half2_t>((w & 0x000f000fu) | 0x64006400u) + a;
+  const half2_t p1 = sf_bitcast<half2_t>((w & 0x00f000f0u) | 0x54005400u) + b;
+  const half2_t p2 = sf_bitcast<half2_t>((x & 0x000f000fu) | 0x64006400u) + a;
+  const half2_t p3 = sf_bitcast<half2_t>((x & 0x00f000f0u) | 0x54005400u) + b;
+  return half8_t{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+}
+
+__device__ __forceinline__ float q4_lo(uint32_t w) { return (float)sf_bitcast<f16>((uint16_t)(w & 0xffffu)); }
+__device__ __forceinline__ float q4_hi(uint32_t w) { return (float)sf_bitcast<f16>((uint16_t)(w >> 16)); }
+
+// Two fp32 values as a pair of fp16 high parts and, SPLIT, of what they leave.
+template <bool SPLIT>
+__device__ __forceinline__ void q4_halves(float a, float b, uint32_t &hi, uint32_t &lo) {
+  a = sf_opaque(a);
+  b = sf_opaque(b);
+  const f16 x = (f16)a, y = (f16)b;
+  hi = sf_bitcast<uint16_t>(x) | (uint32_t)sf_bitcast<uint16_t>(y) << 16;
+  if constexpr (SPLIT)
+    lo = sf_bitcast<uint16_t>((f16)(a - (float)x)) | (uint32_t)sf_bitcast<uint16_t>((f16)(b - (float)y)) << 16;
+}
+
+// DP: the head's dims rounded up to 64, 128 or 256. NGT groups of 32 KSGT dims fill it
+// exactly, or 0, 0: any head and groups.
+template <int QDT, bool PSPLIT, int DP, int NGT, int KSGT>
+__global__ void __launch_bounds__(kQaThreads)
+k_q4_split(Q4Attn a) {
+  constexpr bool ANY = NGT == 0, QSPLIT = QDT == SF_F32;
+  constexpr float kCode = PSPLIT ? 1.f : 16777216.f;  // what an operand of K's codes is to be multiplied by
+  constexpr int KS = DP / 32, DB = DP / 16, NGM = ANY ? 8 : NGT;
+  constexpr int PITCH = DP / 2 + 8;  // 16 neighbouring rows' 8 bytes fall on different banks
+  constexpr int OP = DP + 4;
+  constexpr int kTile = 64 * PITCH, kPar = 64 * NGM * 4;
+  constexpr int kWave = kTile + 4 * kPar + 256, kO = 16 * OP * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t smem[kQaWaves * (kWave > kO ? kWave : kO) + 2 * kQaWaves * 16 * 4];
+  const int D = ANY ? a.D : DP, NG = ANY ? a.D / a.g : NGT, GW = (ANY ? a.g : 32 * KSGT) / 8;
+  const int KSG = ANY ? (GW + 3) / 4 : KSGT, nks = ANY ? NG * KSG : KS;
+  const int G = a.H / a.KVH, R = a.Tq * G, nrb = (R + 15) / 16;
+  const int split = blockIdx.x, kvh = blockIdx.y / nrb, rb = blockIdx.y - kvh * nrb, b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hl = lane & 15, g = lane >> 4, nr = min(16, R - 16 * rb);
+  const int r = 16 * rb + hl, qt = min(r, R - 1) / G, qh = min(r, R - 1) - qt * G;
+  const size_t bk = (size_t)b * a.KVH + kvh, base = bk * a.T_cap;
+  const int rowb = D / 2;
+  // the word of codes that k-step ks takes of a slot (a group's words shared out over the four lanes)
+  auto word = [&](int ks) {
+    const int gi = ks / KSG, c = g * KSG + ks - gi * KSG;
+    return c < GW ? gi * GW + c : -1;
+  };
+
+  uint32_t kr[4][KS];  // the codes of slots 4 hl + h
+  u32x4 vr[DP / 32];   // 16 bytes of V codes each, slot-major
+  uint32_t pr[2][NGM];
+  auto k_codes = [](uint32_t w) { return PSPLIT ? q4_signed(w) : q4_codes(w); };
+  auto load_k = [&](int j) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const uint8_t *p = a.kc + (base + min(64 * j + 4 * hl + h, a.T_cap - 1)) * rowb;
+      if constexpr (!ANY) {
+#pragma unroll
+        for (int gi = 0; gi < NGT; ++gi) {
+          const uint8_t *w = p + 4 * (gi * 4 * KSGT + g * KSGT);
+          if constexpr (KSGT == 4) {
+            const u32x4 x = *(const u32x4 *)w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) kr[h][gi * KSGT + k] = x[k];
+          } else if constexpr (KSGT == 2) {
+            const u32x2 x = *(const u32x2 *)w;
+            kr[h][gi * KSGT] = x.x;
+            kr[h][gi * KSGT + 1] = x.y;
+          } else {
+            kr[h][gi] = *(const uint32_t *)w;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          if (ks >= nks) break;
+          const int w = word(ks);
+          kr[h][ks] = w >= 0 ? *(const uint32_t *)(p + 4 * w) : 0u;
+        }
+      }
+    }
+  };
+  auto load_v = [&](int j) {
+    const int n16 = D / 32;  // 16-byte pieces a slot, and half a one where D is an odd multiple of 16
+    if (!ANY || D % 32 == 0) {
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        if (ANY && i >= n16) break;
+        const int e = lane + 64 * i, tok = e / n16, c = e - tok * n16;
+        vr[i] = *(const u32x4 *)(a.vc + (base + min(64 * j + tok, a.T_cap - 1)) * rowb + 16 * c);
+      }
+    } else {
+      const int n8 = D / 16;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        uint32_t x[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int e = lane + 64 * (2 * i + u), tok = min(e / n8, 63), c = e - e / n8 * n8;
+          const u32x2 w = *(const u32x2 *)(a.vc + (base + min(64 * j + tok, a.T_cap - 1)) * rowb + 8 * c);
+          x[2 * u] = w.x;
+          x[2 * u + 1] = w.y;
+        }
+        vr[i] = u32x4{x[0], x[1], x[2], x[3]};
+      }
+    }
+  };
+  auto load_p = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < NGM; ++i) {
+      if (ANY && i >= NG) break;
+      const int e = lane + 64 * i, tok = e / NG;
+      const size_t at = (base + min(64 * j + tok, a.T_cap - 1)) * NG + (e - tok * NG);
+      pr[0][i] = a.kp[at];
+      pr[1][i] = a.vp[at];
+    }
+  };
+
+  const int n = q4_len(a.lengths, a.T, a.T_max, b);
+  const int ntot = max(0, n - a.Tq + (16 * rb + nr - 1) / G + 1 + 63) / 64;  // up to the last row's own slot
+  const int j0 = split + a.n_splits * wave, jstep = a.n_splits * kQaWaves;
+  if (j0 < ntot) {
+    load_k(j0);
+    load_p(j0);
+    load_v(j0);
+  }
+  const int lim = r < R ? max(0, n - a.Tq + qt + 1) : 0, lim_all = n - a.Tq + 16 * rb / G + 1;  // (of every row)
+
+  // q in the codes' order, and its sum over each group (as the codes stand, times 2^-24)
+  half8_t qh8[KS], ql8[KS];
+  float qs[NGM];
+  float qmul;
+  {
+    float f[KS][8], top = 0.f;
+    const size_t q0 = (((size_t)b * a.Tq + qt) * a.H + (size_t)kvh * G + qh) * D;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int w = ANY && ks >= nks ? -1 : word(ks);
+      if (w >= 0) sf_load8_as_f32<QDT>(a.q, q0 + 8 * w, f[ks]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[ks][i] = r < R && w >= 0 ? f[ks][i] : 0.f;
+        top = fmaxf(top, fabsf(f[ks][i]));
+      }
+    }
+    const float up = q4_fit14(max_x16_x32(top));
+    qmul = fminf(fmaxf(a.qscale / up * kCode, -3.0e38f), 3.0e38f);
+#pragma unroll
+    for (int gi = 0; gi < NGM; ++gi) {
+      float s = 0.f;
+      if (!ANY || gi < NG) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          if (ks / KSG == gi)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += f[ks][i] * up;
+      }
+      qs[gi] = sum_x16_x32(s) * (1.f / kCode);
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float v = f[ks][(i >> 1) + 4 * (i & 1)] * up, part = !PSPLIT && (i >> 1) & 1 ? 0.0625f : 1.f;
+        const f16 hi = (f16)v;
+        qh8[ks][i] = (f16)((float)hi * part);
+        ql8[ks][i] = (f16)((v - (float)hi) * part);
+      }
+  }
+
+  uint8_t *const vt = smem + wave * kWave;
+  float *const kss = (float *)(vt + kTile), *const kos = kss + 64 * NGM;  // K's s and m, or m + 8 s
+  float *const vss = kos + 64 * NGM, *const vos = vss + 64 * NGM;  // V's s and m + 8 s
+  float *const vms = vos + 64 * NGM;  // a slot's largest V scale
+  float m = -INFINITY, lsum = 0.f;               // base-2 softmax of row r
+  float pmax = 0.f, pmul = 1.f;  // largest weight times V scale so far (as the weights stand), its factor
+  float am[NGM];                 // sum of p (m + 8 s) over the lane's slots
+  float4_t O[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) O[d] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int gi = 0; gi < NGM; ++gi) am[gi] = 0.f;
+
+  for (int j = j0; j < ntot; j += jstep) {
+    const int tb = 64 * j;
+    const bool more = j + jstep < ntot;
+    // parameters and V codes into the wave's LDS; slots past the length stand for zeros
+#pragma unroll
+    for (int i = 0; i < NGM; ++i) {
+      if (ANY && i >= NG) break;
+      const int e = lane + 64 * i, tok = e / NG, gi = e - tok * NG;
+      const bool in = tb + tok < n;
+      const uint32_t k = in ? pr[0][i] : 0u;
+      kss[64 * gi + tok] = q4_lo(k);
+      kos[64 * gi + tok] = PSPLIT ? fmaf(8.f, q4_lo(k), q4_hi(k)) : q4_hi(k);
+      const uint32_t w = in ? pr[1][i] : 0u;
+      vss[64 * gi + tok] = q4_lo(w);
+      vos[64 * gi + tok] = fmaf(8.f, q4_lo(w), q4_hi(w));
+    }
+    if (!ANY || D % 32 == 0) {
+      const int n16 = D / 32;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        if (ANY && i >= n16) break;
+        const int e = lane + 64 * i, tok = e / n16, c = e - tok * n16;
+        uint2 *dst = (uint2 *)(vt + tok * PITCH + 16 * c);
+        dst[0] = uint2{vr[i].x, vr[i].y};
+        dst[1] = uint2{vr[i].z, vr[i].w};
+      }
+    } else {
+      const int n8 = D / 16;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int e = lane + 64 * (2 * i + u), tok = e / n8, c = e - tok * n8;
+          if (tok < 64) *(uint2 *)(vt + tok * PITCH + 8 * c) = uint2{vr[i][2 * u], vr[i][2 * u + 1]};
+        }
+    }
+    if (more) {
+      load_p(j + jstep);
+      load_v(j + jstep);
+    }
+    {
+      float v = 0.f;
+#pragma unroll
+      for (int gi = 0; gi < NGM; ++gi)
+        if (!ANY || gi < NG) v = fmaxf(v, vss[64 * gi + lane]);
+      vms[lane] = v;
+    }
+    float sc[16];  // value 4 h + i: slot tb + 16 g + 4 i + h
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+    for (int gi = 0; gi < NGM; ++gi) {
+      if (ANY && gi >= NG) break;
+      float4_t S[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) S[h] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (ks / KSG != gi || ks >= nks) continue;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const half8_t x = k_codes(kr[h][ks]);
+          S[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh8[ks], S[h], 0, 0, 0);
+          if constexpr (QSPLIT) S[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql8[ks], S[h], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4_t ks = *(const float4_t *)(kss + 64 * gi + 16 * g + 4 * i);
+        const float4_t ko = *(const float4_t *)(kos + 64 * gi + 16 * g + 4 * i);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) sc[4 * h + i] = fmaf(ks[h], S[h][i], fmaf(ko[h], qs[gi], sc[4 * h + i]));
+      }
+    }
+    if (more) load_k(j + jstep);
+    const bool masked = tb + 64 > lim_all;
+    const int left = lim - tb - 16 * g;  // the lane's slots 4 i + h < left
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      sc[e] *= qmul;
+      if (masked) sc[e] = 4 * (e & 3) + (e >> 2) < left ? sc[e] : -INFINITY;
+      mx = fmaxf(mx, sc[e]);
+    }
+    const float m_new = fmaxf(m, max_x16_x32(mx)), m_ref = m_new == -INFINITY ? 0.f : m_new;
+    const float c = __builtin_amdgcn_exp2f(m - m_ref);
+    m = m_new;
+    float ps = 0.f, pt = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4_t v = *(const float4_t *)(vms + 16 * g + 4 * i);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int e = 4 * h + i;
+        sc[e] = __builtin_amdgcn_exp2f(sc[e] - m_ref);
+        ps += sc[e];
+        pt = fmaxf(pt, sc[e] * v[h]);
+      }
+    }
+    lsum = fmaf(lsum, c, ps);
+    pmax = fmaxf(pmax * c, max_x16_x32(pt));
+    const float mul = q4_fit14(pmax), oc = c * mul / pmul;  // at most 2: pmax covers c times the last one
+    pmul = mul;
+    if (__any(oc != 1.f)) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) O[d] *= oc;
+    }
+#pragma unroll
+    for (int gi = 0; gi < NGM; ++gi) {
+      if (ANY && gi >= NG) break;
+      // P's operands: values (h, 0), (h, 1) of a register pair go with dword 0, (h, 2), (h, 3) with dword 1
+      u32x4 ph[2], pl[2];
+      float acc = am[gi] * c;
+      float4_t vs[4], vo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        vs[i] = *(const float4_t *)(vss + 64 * gi + 16 * g + 4 * i);
+        vo[i] = *(const float4_t *)(vos + 64 * gi + 16 * g + 4 * i);
+        if (masked) {  // what lies past a row's end weighs exactly 0, whatever its parameters hold
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            vs[i][h] = 4 * i + h < left ? vs[i][h] : 0.f;
+            vo[i][h] = 4 * i + h < left ? vo[i][h] : 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        float pv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = sc[4 * h + i];
+          acc = fmaf(vo[i][h], p, acc);
+          pv[i] = vs[i][h] * (p * mul);
+        }
+        uint32_t x, y;
+        q4_halves<PSPLIT>(pv[0], pv[1], x, y);
+        ph[0][h] = x;
+        pl[0][h] = y;
+        q4_halves<PSPLIT>(pv[2], pv[3], x, y);
+        ph[1][h] = x;
+        pl[1][h] = y;
+      }
+      am[gi] = acc;
+      typedef int v2i __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        if (ANY ? 16 * d < gi * a.g || 16 * d >= (gi + 1) * a.g : d / (2 * KSGT) != gi) continue;
+        const v2i vw = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (__attribute__((address_space(3))) v2i *)(vt + (16 * g + hl) * PITCH + 8 * d));
+        const half8_t x0 = q4_signed((uint32_t)vw.x), x1 = q4_signed((uint32_t)vw.y);
+        O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, sf_bitcast<half8_t>(ph[0]), O[d], 0, 0, 0);
+        O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, sf_bitcast<half8_t>(ph[1]), O[d], 0, 0, 0);
+        if constexpr (PSPLIT) {
+          O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, sf_bitcast<half8_t>(pl[0]), O[d], 0, 0, 0);
+          O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, sf_bitcast<half8_t>(pl[1]), O[d], 0, 0, 0);
+        }
+      }
+    }
+  }
+  lsum = sum_x16_x32(lsum);
+#pragma unroll
+  for (int gi = 0; gi < NGM; ++gi) am[gi] = sum_x16_x32(am[gi]);
+
+  // merge the wave states through LDS into the split's partial, or the output
+  __syncthreads();
+  float *os = (float *)smem;  // [wave][16][OP]
+  float *ms = (float *)(smem + kQaWaves * (kWave > kO ? kWave : kO)), *ls = ms + kQaWaves * 16;
+  if (g == 0) {
+    ms[wave * 16 + hl] = m;
+    ls[wave * 16 + hl] = lsum;
+  }
+  const float un = 1.f / pmul;
+#pragma unroll
+  for (int d = 0; d < DB; ++d) {
+    if (ANY && 16 * d >= D) break;
+    float add = am[0];
+#pragma unroll
+    for (int gi = 1; gi < NGM; ++gi)
+      if (ANY ? 16 * d / a.g == gi : d / (2 * (KSGT ? KSGT : 1)) == gi) add = am[gi];
+    *(float4_t *)(os + (wave * 16 + hl) * OP + 16 * d + 4 * g) = O[d] * un + add;
+  }
+  __syncthreads();
+  const int nq = D / 4;
+  for (int e = tid; e < nr * nq; e += kQaThreads) {
+    const int rr = e / nq, d4 = (e - rr * nq) * 4;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kQaWaves; ++w) M = fmaxf(M, ms[w * 16 + rr]);
+    const float M_ref = sf_merge_mref(M);
+    float L = 0.f;
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kQaWaves; ++w) {
+      const float wt = sf_merge_weight(ms[w * 16 + rr], M_ref);
+      L = fmaf(wt, ls[w * 16 + rr], L);
+      acc += *(const float4_t *)(os + (w * 16 + rr) * OP + d4) * wt;
+    }
+    if (a.n_splits > 1) {
+      const size_t row = (bk * R + 16 * rb + rr) * a.n_splits + split;
+      *(float4_t *)(a.part_acc + row * D + d4) = acc;
+      if (d4 == 0) *(float2_t *)(a.part_ml + row * 2) = float2_t{M, L};
+    } else {
+      const int ro = 16 * rb + rr, t = ro / G, hh = kvh * G + ro - t * G;
+      const size_t o = (((size_t)b * a.Tq + t) * a.H + hh) * D + d4;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sf_store_dt(a.out, a.odt, o + i, sf_merge_finish(L, acc[i]));
+    }
+  }
+}
+
+// The second launch: a workgroup merges one query row's partials, every thread four dims of
+// some of the splits, the parts then summed in LDS, all loads of a thread in flight at once.
+__global__ void __launch_bounds__(kQaThreads)
+k_q4_merge(const float *__restrict__ part_acc, const float *__restrict__ part_ml, void *__restrict__ out, int odt, int Tq,
+           int H, int KVH, int D, int S) {
+  constexpr int kPre = 4;
+  __shared__ __attribute__((aligned(16))) float sm[kQaMaxSplits + 4 * kQaThreads];
+  const int row = blockIdx.x, nq = D / 4, parts = kQaThreads / nq, q = threadIdx.x % nq, part = threadIdx.x / nq;
+  const int lane = threadIdx.x & 63;
+  const float2_t *ml = (const float2_t *)part_ml + (size_t)row * S;
+  const float4_t *acc = (const float4_t *)part_acc + (size_t)row * S * nq + q;
+  const float2_t e0 = ml[min(lane, S - 1)], e1 = ml[min(lane + 64, S - 1)];
+  float4_t pre[kPre];
+#pragma unroll
+  for (int k = 0; k < kPre; ++k) pre[k] = acc[(size_t)min(part + k * parts, S - 1) * nq];
+  const float m0 = lane < S ? e0.x : -INFINITY, m1 = lane + 64 < S ? e1.x : -INFINITY;
+  const float M = sf_merge_mref(sf_wave_max(fmaxf(m0, m1)));
+  const float w0 = sf_merge_weight(m0, M), w1 = sf_merge_weight(m1, M);
+  const float L = sf_wave_sum((lane < S ? w0 * e0.y : 0.f) + (lane + 64 < S ? w1 * e1.y : 0.f));
+  float *w = sm;
+  float4_t *p = (float4_t *)(sm + kQaMaxSplits);  // [parts][nq]
+  if (threadIdx.x < 64) {
+    w[lane] = w0;
+    w[lane + 64] = w1;
+  }
+  __syncthreads();
+  float4_t v = {0.f, 0.f, 0.f, 0.f};
+  if (part < parts) {
+#pragma unroll
+    for (int k = 0; k < kPre; ++k)
+      if (part + k * parts < S) v += pre[k] * w[part + k * parts];
+    for (int s = part + kPre * parts; s < S; s += parts) v += acc[(size_t)s * nq] * w[s];
+    p[part * nq + q] = v;
+  }
+  __syncthreads();
+  if (part == 0) {
+    for (int i = 1; i < parts; ++i) v += p[i * nq + q];
+    const int G = H / KVH, R = Tq * G, bk = row / R, r = row - bk * R;
+    const int b = bk / KVH, t = r / G, h = (bk - b * KVH) * G + r - t * G;
+    const size_t o = (((size_t)b * Tq + t) * H + h) * D + 4 * q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sf_store_dt(out, odt, o + i, sf_merge_finish(L, v[i]));
+  }
+}
+
+int q4_splits(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits) {
+  const long long blocks = ((long long)Tq * (H / KVH) + 15) / 16;
+  if (n_splits <= 0) {
+    const long long kb = KVH * blocks;
+    n_splits = kb * B >= 1024 ? 1 : sf_attn_default_splits_d(B, (int)kb, T_max, D);
+  }
+  const int tiles = (T_max + 63) / 64;
+  if (n_splits > tiles) n_splits = tiles;
+  return n_splits > kQaMaxSplits ? kQaMaxSplits : n_splits < 1 ? 1 : n_splits;
+}
+
+size_t q4_parts(long long rows, int D, int S, size_t *ml_off) {
+  *ml_off = sf_align256((size_t)rows * S * D * sizeof(float));
+  return S > 1 ? *ml_off + (size_t)rows * S * 2 * sizeof(float) : 0;
+}
+
+}  // namespace
+
+extern "C" size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits) {
+  if (B <= 0 || Tq <= 0 || H <= 0 || KVH <= 0 || H % KVH || T_max < 0 || T_max > kQaMaxSlots || D <= 0) return 0;
+  size_t ml;
+  return q4_parts((long long)B * Tq * H, D, q4_splits(B, Tq, H, KVH, T_max, D, n_splits), &ml);
+}
+
+extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, const void *k_params,
+                            const uint8_t *v_codes, const void *v_params, int group, void *out, int out_dtype,
+                            void *workspace, size_t workspace_bytes, int B, int Tq, int H, int KVH,
+                            const int32_t *lengths, int T, int T_max, int T_cap, int D, float scale, int n_splits,
+                            void *stream) {
+  SF_REQUIRE(B > 0 && Tq > 0 && H > 0 && KVH > 0 && D > 0 && T_cap > 0 && T_max >= 0 && T_max <= T_cap &&
+                 (lengths || (T >= 0 && T <= T_max)),
+             SF_EINVAL, "invalid attention shape B=%d Tq=%d H=%d KVH=%d T=%d T_max=%d T_cap=%d D=%d", B, Tq, H, KVH,
+             T, T_max, T_cap, D);
+  SF_REQUIRE(H % KVH == 0, SF_EINVAL, "n_heads=%d not a multiple of n_kv_heads=%d", H, KVH);
+  if (int rc = sf_q4_cache_check(D, group)) return rc;
+  SF_REQUIRE(T_max <= kQaMaxSlots, SF_EUNSUPPORTED, "T_max=%d: at most %d slots", T_max, kQaMaxSlots);
+  const long long nrb = ((long long)Tq * (H / KVH) + 15) / 16, rows = (long long)B * Tq * H;
+  SF_REQUIRE(KVH * nrb <= 65535 && B <= 65535 && rows <= 0x7fffffffLL, SF_EINVAL,
+             "B=%d KVH=%d rows=%d exceed the grid", B, KVH, Tq);
+  SF_REQUIRE(q_dtype >= SF_F32 && q_dtype <= SF_BF16 && out_dtype >= SF_F32 && out_dtype <= SF_BF16, SF_EINVAL,
+             "bad q/out dtype");
+  SF_REQUIRE(q && k_codes && k_params && v_codes && v_params && out, SF_EINVAL, "null pointer argument");
+  SF_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_params | (uintptr_t)v_params | (uintptr_t)q) & 15) == 0,
+             SF_EINVAL, "q and cache buffers must be 16-byte aligned");
+  n_splits = q4_splits(B, Tq, H, KVH, T_max, D, n_splits);
+  size_t ml_off;
+  const size_t need = q4_parts(rows, D, n_splits, &ml_off);
+  SF_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0), SF_EINVAL, "workspace must be 256-byte aligned");
+  SF_REQUIRE(workspace_bytes >= need, SF_EINVAL, "attention workspace too small: %zu < %zu", workspace_bytes, need);
+  float *acc = (float *)workspace, *ml = (float *)((char *)workspace + ml_off);
+  hipStream_t st = (hipStream_t)stream;
+  const Q4Attn a = {q, k_codes, v_codes, (const uint32_t *)k_params, (const uint32_t *)v_params, out, acc, ml, lengths,
+                    out_dtype, T, T_max, T_cap, Tq, H, KVH, D, group, n_splits,
+                    scale * 1.4426950408889634f};  // softmax in base 2
+  const dim3 grid(n_splits, (unsigned)(KVH * nrb), B);
+#define SF_QA(QD, PS, DP, NG, KSG) k_q4_split<QD, PS, DP, NG, KSG><<<grid, kQaThreads, 0, st>>>(a)
+#define SF_QA_D(QD, PS)                                  \
+  do {                                                   \
+    if (D == 64 && group == 64) SF_QA(QD, PS, 64, 1, 2); \
+    else if (D == 64 && group == 32) SF_QA(QD, PS, 64, 2, 1);    \
+    else if (D == 128 && group == 128) SF_QA(QD, PS, 128, 1, 4); \
+    else if (D == 128 && group == 64) SF_QA(QD, PS, 128, 2, 2);  \
+    else if (D == 128 && group == 32) SF_QA(QD, PS, 128, 4, 1);  \
+    else if (D <= 128) SF_QA(QD, PS, 128, 0, 0);         \
+    else SF_QA(QD, PS, 256, 0, 0);                       \
+  } while (0)
+#define SF_QA_O(QD)                             \
+  do {                                          \
+    if (out_dtype == SF_BF16) SF_QA_D(QD, false); \
+    else SF_QA_D(QD, true);                     \
+  } while (0)
+  if (q_dtype == SF_F32) SF_QA_O(SF_F32);
+  else if (q_dtype == SF_F16) SF_QA_O(SF_F16);
+  else SF_QA_O(SF_BF16);
+#undef SF_QA_O
+#undef SF_QA_D
+#undef SF_QA
+  if (n_splits > 1) k_q4_merge<<<(unsigned)rows, kQaThreads, 0, st>>>(acc, ml, out, out_dtype, Tq, H, KVH, D, n_splits);
+  return sf_check_launch("sf_attn_q4kv");
+}

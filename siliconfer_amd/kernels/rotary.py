@@ -3,9 +3,10 @@ frequencies (the reference's RoPE is rotate-half over the whole head at one
 offset, /root/reference/siliconfer/model/layers.py:58-66).
 
 `rotary(q, k, positions, inv_freq)` turns q [B, T, H, D] and k [B, T, KVH, D] (k may
-be None); any strides with contiguous dims. `rotary_kv_append` turns the q and k heads
-of fused q|k|v rows and quantizes k and v into the slots of an int8 cache, whose
-slots need not be the positions. `inv_freq` is the float64 angle a position of each
+be None); any strides with contiguous dims. `qk_norm_rotary` norms each head by its root
+mean square first, for models with a norm of queries and keys. `rotary_kv_append` turns
+the q and k heads of fused q|k|v rows and quantizes k and v into the slots of an int8
+cache, whose slots need not be the positions. `inv_freq` is the float64 angle a position of each
 pair, on the device: `siliconfer_amd.model.rope.rotary_frequencies` makes it and the
 `scale` that goes with it.
 """
@@ -19,9 +20,10 @@ import torch
 from .. import _lib
 from .._lib import SFError
 
-__all__ = ["rotary", "rotary_kv_append"]
+__all__ = ["rotary", "qk_norm_rotary", "rotary_kv_append"]
 
 _STRIDES = ctypes.c_longlong * 12
+_STRIDES_BACK = ctypes.c_longlong * 18
 _INT = (torch.int32, torch.int64)
 
 
@@ -123,6 +125,104 @@ class _Turn(torch.autograd.Function):
         positions, inv_freq = ctx.saved_tensors
         gq, gk = (g if g is None or g.stride(3) == 1 else g.contiguous() for g in (gq, gk))
         return (*rotary(gq, gk, -positions, inv_freq, **ctx.how), None, None, None, None)
+
+
+def _side(x: torch.Tensor, w: torch.Tensor, out, name: str):
+    """The output of one side's heads: `out`, checked, or a new tensor."""
+    D = x.shape[3]
+    if w.shape != (D,) or w.get_device() != x.get_device() or not w.is_contiguous():
+        raise SFError(f"{name}_weight must be a contiguous [{D}] on {name}'s device (got {list(w.shape)} on {w.device})")
+    if out is None:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise SFError(f"out_{name} must have {name}'s shape, dtype and device")
+    _rows(out, f"out_{name}")
+    if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+        raise SFError("an output's rows must not share memory")
+    return out
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+                   q_weight: torch.Tensor, k_weight: torch.Tensor | None = None, *, eps: float = 1e-6,
+                   interleaved: bool = False, scale: float = 1.0, out_q: torch.Tensor | None = None,
+                   out_k: torch.Tensor | None = None):
+    """(q, k), every head x of D dims normed, x / sqrt(mean(x^2) + eps) * weight ([D], one for
+    q's heads and one for k's), then turned as `rotary` turns it, in one pass in fp32 and one
+    rounding to q's dtype. D <= 256. `out_q` / `out_k` may be the inputs themselves; other
+    outputs must not overlap them, and inputs that need a gradient take none. Differentiable
+    in q, k and the weights (once)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        if out_q is not None or out_k is not None:
+            raise SFError("qk_norm_rotary: inputs that need a gradient take no out_q / out_k")
+        return _NormTurn.apply(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, scale)
+    _rows(q, "q")
+    B, T, H, D = q.shape
+    out_q = _side(q, q_weight, out_q, "q")
+    plain, KVH = q.is_contiguous() and out_q.is_contiguous(), 0
+    if k is not None:
+        _rows(k, "k")
+        KVH = k.shape[2]
+        if k.shape[0] != B or k.shape[1] != T or k.shape[3] != D or k.dtype != q.dtype or k.device != q.device:
+            raise SFError("k must match q in batch, rows, head_dim, dtype and device")
+        if k_weight is None or k_weight.dtype != q_weight.dtype:
+            raise SFError("k needs a k_weight of q_weight's dtype")
+        out_k = _side(k, k_weight, out_k, "k")
+        plain = plain and k.is_contiguous() and out_k.is_contiguous()
+    elif out_k is not None or k_weight is not None:
+        raise SFError("out_k / k_weight without k")
+    i64, per_seq = _positions(positions, B, T, q)
+    pairs = _pairs(inv_freq, D, q)
+    strides = None
+    if not plain:
+        strides = _STRIDES(*(t.stride(i) for t in (q, out_q, k, out_k) if t is not None for i in range(3)))
+    with _lib.on_device(q):
+        rc = _lib.load().sf_qk_norm_rotary(
+            q.data_ptr(), out_q.data_ptr(), None if k is None else k.data_ptr(), None if k is None else out_k.data_ptr(),
+            _lib.dt(q), q_weight.data_ptr(), None if k is None else k_weight.data_ptr(), _lib.dt(q_weight), eps,
+            positions.data_ptr(), i64, per_seq, inv_freq.data_ptr(), pairs, scale, interleaved, B, T, H, KVH, D, strides,
+            _lib.stream(q))
+    if rc:
+        _lib.check(rc, "sf_qk_norm_rotary")
+    return out_q, out_k
+
+
+class _NormTurn(torch.autograd.Function):
+    """`qk_norm_rotary` with its gradients, by one kernel that norms the saved rows again."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, scale):
+        ctx.save_for_backward(q, k, positions, inv_freq, q_weight, k_weight)
+        ctx.how = eps, interleaved, scale
+        return qk_norm_rotary(q, k, positions, inv_freq, q_weight, k_weight, eps=eps, interleaved=interleaved,
+                              scale=scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
+        eps, interleaved, scale = ctx.how
+        B, T, H, D = q.shape
+        KVH = 0 if k is None else k.shape[2]
+        gq, gk = (g if g is None or g.stride(3) == 1 else g.contiguous() for g in (gq, gk))
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        dk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+        dw = torch.empty((2, D), dtype=torch.float32, device=q.device)
+        if B * T == 0:
+            dw.zero_()
+        else:
+            i64, per_seq = _positions(positions, B, T, q)
+            strides = _STRIDES_BACK(*(t.stride(i) for t in (q, gq, dq, k, gk, dk) if t is not None for i in range(3)))
+            ptr = _lib.ptr
+            with _lib.on_device(q):
+                lib, st = _lib.load(), _lib.stream(q)
+                ws = _lib.scratch(q.device, st, lib.sf_qk_norm_backward_workspace_bytes(B, T, H, KVH, D))
+                _lib.check(lib.sf_qk_norm_rotary_backward(
+                    q.data_ptr(), gq.data_ptr(), dq.data_ptr(), ptr(k), ptr(gk), ptr(dk), _lib.dt(q),
+                    q_weight.data_ptr(), ptr(k_weight), _lib.dt(q_weight), dw.data_ptr(), dw[1].data_ptr(), eps,
+                    positions.data_ptr(), i64, per_seq, inv_freq.data_ptr(), inv_freq.numel(), scale, interleaved,
+                    B, T, H, KVH, D, strides, ws.data_ptr(), ws.numel(), st), "sf_qk_norm_rotary_backward")
+        return (dq, dk, None, None, dw[0].to(q_weight.dtype), None if k is None else dw[1].to(k_weight.dtype), None,
+                None, None)
 
 
 def rotary_kv_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
