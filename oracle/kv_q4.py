@@ -95,7 +95,8 @@ def values(packed, params):
     return m + s * c, s * c + abs(m)
 
 
-def attention(q, k_codes, k_params, v_codes, v_params, lengths, scale=None, weights_rounded=2.0 ** -22):
+def attention(q, k_codes, k_params, v_codes, v_params, lengths, scale=None, weights_rounded=2.0 ** -22,
+              factors_rounded=2.0 ** -22):
     """q [B, Tq, H, D]; row t sees the first lengths[b] - Tq + t + 1 slots. (out, bound): a
     score sums D products of q with s c and with m, each a fp32 sum (D + 24 half steps of
     the sizes, which do not cancel where the values do) of q's two halves (2^-22 of q); its
@@ -110,18 +111,19 @@ def attention(q, k_codes, k_params, v_codes, v_params, lengths, scale=None, weig
     out, ob = np.zeros(q.shape), np.zeros(q.shape)
     for b in range(B):
         for kv in range(KVH):
+            most = max(0, min(int(lengths[b]), k_codes.shape[2]))
+            (Ka, Ksa), (Va, Vsa) = (values(c[b, kv, :most], p[b, kv, :most]) for c, p in ((k_codes, k_params), (v_codes, v_params)))
             for t in range(Tq):
-                n = min(int(lengths[b]), k_codes.shape[2]) - Tq + t + 1
+                n = most - Tq + t + 1
                 if n <= 0:
                     continue
-                K, Ks = values(k_codes[b, kv, :n], k_params[b, kv, :n])
-                V, Vs = values(v_codes[b, kv, :n], v_params[b, kv, :n])
+                K, Ks, V, Vs = Ka[:n], Ksa[:n], Va[:n], Vsa[:n]
                 for h in range(kv * G, (kv + 1) * G):
                     s = K @ q[b, t, h] * scale
                     size = (Ks @ abs(q[b, t, h]) * abs(scale)).max()
                     w = np.exp(s - s.max())
                     w /= w.sum()
-                    rel = 2 * ((D + 24) * U + 2.0 ** -22) * size + (n + 64) * U + 2.0 ** -20 + weights_rounded
+                    rel = 2 * ((D + 24) * U + factors_rounded) * size + (n + 64) * U + 2.0 ** -20 + weights_rounded
                     out[b, t, h] = w @ V
                     ob[b, t, h] = rel * (w @ Vs)
     return out, ob

@@ -70,6 +70,17 @@ __device__ __forceinline__ half8_t q4_codes(uint32_t w) {
   return sf_bitcast<half8_t>(r);
 }
 
+// Eight codes as they are, exact: codes 0, 4, 1, 5, 2, 6, 3, 7.
+__device__ __forceinline__ half8_t q4_unsigned(uint32_t w) {
+  const uint32_t x = w >> 8;
+  const half2_t a = {(f16)-1024.f, (f16)-1024.f}, b = {(f16)-64.f, (f16)-64.f};
+  const half2_t p0 = sf_bitcast<half2_t>((w & 0x000f000fu) | 0x64006400u) + a;
+  const half2_t p1 = sf_bitcast<half2_t>((w & 0x00f000f0u) | 0x54005400u) + b;
+  const half2_t p2 = sf_bitcast<half2_t>((x & 0x000f000fu) | 0x64006400u) + a;
+  const half2_t p3 = sf_bitcast<half2_t>((x & 0x00f000f0u) | 0x54005400u) + b;
+  return half8_t{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+}
+
 // Eight codes less 8, exact: codes 0, 4, 1, 5, 2, 6, 3, 7.
 __device__ __forceinline__ half8_t q4_signed(uint32_t w) {
   const uint32_t x = w >> 8;
@@ -514,6 +525,333 @@ k_q4_merge(const float *__restrict__ part_acc, const float *__restrict__ part_ml
   }
 }
 
+// ---------------------------------------------------------------------------
+// many rows: prompts
+// ---------------------------------------------------------------------------
+// A workgroup owns 128 consecutive (row, head) columns c = t G + h of one kv head and walks
+// the 64-slot tiles up to its last row's own slot, two at a time: waves 0..3 take the even
+// ones, 32 columns each, waves 4..7 the odd ones, and their states merge at the end. A tile's
+// values m + s c are made once for its four waves, as fp16 (SPLIT: and what that leaves, a second fp16) in the order of
+// the matrix operands, 1 KB of LDS a fragment that every wave reads back whole:
+//   * K: a lane makes its slot's fragments from neighbouring words of codes, q is loaded in
+//     the same order of dims;
+//   * V: codes through LDS and ds_read_b64_tr_b4, a lane then holds one dim's codes of 16
+//     slots in the order in which S^T leaves the weights in registers.
+// Then it is S^T = K q^T, a base-2 softmax a column and O^T = V^T P^T on
+// v_mfma_f32_32x32x16_f16. For a bf16 output q, P and the values are fp16's high parts: a
+// value off by 2^-12 moves an output by less than a fifth of its own rounding (2^-9). Other
+// outputs take three products of the high and low parts.
+// What fp16 cannot hold: a tile with an s past 2^11 or an m past 2^14 is taken at 2^-6 (K's
+// scores and V's sums times 2^6 again); parameters that are not finite stand as zeros in V, and the
+// columns that see them get NaN in their group's dims.
+template <int QDT, bool SPLIT, int D>
+__global__ void __launch_bounds__(512, 2)
+k_q4_rows(Q4Attn a) {
+  constexpr int NFW = D / 32;      // K fragments a wave makes of its 32 slots, of 2 NFW
+  constexpr int NDB = D / 32;      // 32-dim blocks
+  constexpr int PARTS = SPLIT ? 2 : 1, QP = QDT == SF_F32 && SPLIT ? 2 : 1;
+  constexpr int PITCH = D / 2 + 8;
+  typedef float float16_t __attribute__((ext_vector_type(16)));
+  typedef uint32_t Words __attribute__((ext_vector_type(NFW)));  // 16 (8) bytes of codes
+  struct Tile {
+    half8_t kf[PARTS][2][2 * NFW][64], vf[PARTS][NDB][4][64];
+    uint8_t raw[64 * PITCH];
+    f16 vsm[2][NDB][64];  // s and m a group, in the order of the weights
+    uint32_t flag[2][2];  // of this tile and the next: K's, V's parameters are large (1) or not finite (2)
+  };
+  __shared__ __attribute__((aligned(16))) Tile tiles[2];
+  const int G = a.H / a.KVH, NG = D / a.g, ncol = a.Tq * G, ncb = (ncol + 127) / 128;
+  // longest columns first, the heads of all sequences side by side
+  const int bk = (int)(blockIdx.x % (unsigned)a.n_splits), c0 = (ncb - 1 - (int)(blockIdx.x / (unsigned)a.n_splits)) * 128;
+  const int b = bk / a.KVH, kvh = bk - b * a.KVH;
+  const int tid = threadIdx.x & 255, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kgrp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  Tile &T = tiles[kgrp];
+  const size_t base = ((size_t)b * a.KVH + kvh) * a.T_cap;
+  const int n = q4_len(a.lengths, a.T, a.T_max, b);
+  auto limit = [&](int c) { return max(0, n - a.Tq + c / G + 1); };  // slots column c sees
+  const int cw = c0 + 32 * wave, c = min(cw + l32, ncol - 1);
+  const int lim = limit(c), lo_lim = limit(min(cw, ncol - 1)), hi_lim = cw < ncol ? limit(min(cw + 31, ncol - 1)) : 0;  // and the wave's
+  const int ntot = (limit(min(c0 + 127, ncol - 1)) + 63) / 64;
+  const size_t qrow = ((size_t)b * a.Tq + c / G) * a.H + (size_t)kvh * G + c % G;
+
+  // what a thread makes of a tile
+  const int tb = wave >> 1, w2 = wave & 1;          // K: the slots 32 tb + l32, fragments NFW w2 ..
+  const int kword = 2 * NFW * w2 + NFW * h, kg = 8 * kword / a.g;
+  const int vtok = tid >> 2, vpiece = tid & 3;      // V: 16 (8) bytes of a slot
+  const int ptok = tid / NG, pg = tid - ptok * NG;  // V: a slot's parameters of a group
+  const bool has_p = tid < 64 * NG;
+  Words kr, vr;
+  uint32_t kpr = 0, vpr = 0;
+  auto load = [&](int j) {
+    const size_t last = a.T_cap - 1, kt = base + min((size_t)(64 * j + 32 * tb + l32), last);
+    kr = *(const Words *)(a.kc + kt * (D / 2) + 4 * kword);
+    vr = *(const Words *)(a.vc + (base + min((size_t)(64 * j + vtok), last)) * (D / 2) + 4 * NFW * vpiece);
+    kpr = a.kp[kt * NG + kg];
+    if (has_p) vpr = a.vp[(base + min((size_t)(64 * j + ptok), last)) * NG + pg];
+    if (64 * j + 32 * tb + l32 >= n) kpr = 0;  // slots past the length stand for zeros
+    if (64 * j + ptok >= n) vpr = 0;
+  };
+  auto off = [](uint32_t w) -> uint32_t {  // 1: s past 2^11 or m past 2^14, 2: not finite
+    const uint32_t x = w & 0x7fffu, y = w >> 16 & 0x7fffu;
+    return x >= 0x7c00u || y >= 0x7c00u ? 2u : x > 0x6800u || y > 0x7400u ? 1u : 0u;
+  };
+  // eight values of one slot, or of eight slots (s, m one each), as operand parts
+  auto values = [](uint32_t w, const half2_t (&s)[4], const half2_t (&m)[4], half8_t &hi, half8_t &lo) {
+    const half8_t c8 = q4_unsigned(w);
+    half2_t v[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const half2_t cp = {c8[2 * p], c8[2 * p + 1]};
+      v[p] = __builtin_elementwise_fma(cp, s[p], m[p]);
+      hi[2 * p] = v[p].x;
+      hi[2 * p + 1] = v[p].y;
+      if constexpr (SPLIT) {
+        lo[2 * p] = (f16)(fmaf((float)cp.x, (float)s[p].x, (float)m[p].x) - (float)v[p].x);
+        lo[2 * p + 1] = (f16)(fmaf((float)cp.y, (float)s[p].y, (float)m[p].y) - (float)v[p].y);
+      }
+    }
+  };
+
+  half8_t qf[QP][2 * NFW];
+  float qmul;
+  {
+    float f[2 * NFW][8], top = 0.f;
+    const float sign = a.qscale < 0.f ? -1.f : a.qscale > 0.f ? 1.f : 0.f;  // (scores are compared before they are scaled)
+#pragma unroll
+    for (int i = 0; i < 2 * NFW; ++i) {
+      const int w = 2 * NFW * (i / NFW) + NFW * h + i % NFW;
+      sf_load8_as_f32<QDT>(a.q, qrow * D + 8 * w, f[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[i][e] *= sign;
+        top = fmaxf(top, fabsf(f[i][e]));
+      }
+    }
+    const float2_t tp = sf_swap32_pair(top);
+    const float up = q4_fit14(fmaxf(tp.x, tp.y));
+    qmul = sign == 0.f ? 1.f : fminf(fmaxf(fabsf(a.qscale) / up, 1.0e-37f), 1.0e36f);
+#pragma unroll
+    for (int i = 0; i < 2 * NFW; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = f[i][(e >> 1) + 4 * (e & 1)] * up;
+        qf[0][i][e] = (f16)v;
+        if constexpr (QP == 2) qf[1][i][e] = (f16)(v - (float)qf[0][i][e]);
+      }
+  }
+
+  constexpr float kP = 13.f;  // weights times 2^13, so that their low parts are normal numbers
+  float m = -INFINITY, lsum = 0.f;
+  float16_t O[NDB];
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) O[d][e] = 0.f;
+
+  if (tid < 4) T.flag[tid >> 1][tid & 1] = 0;
+  if (kgrp < ntot) load(kgrp);
+  __syncthreads();
+  auto tell = [&](int at) {  // the loaded tile's parameters
+    const uint32_t fk = off(kpr), fv = has_p ? off(vpr) : 0u;
+    if (fk) atomicOr(&T.flag[at][0], fk);
+    if (fv) atomicOr(&T.flag[at][1], fv);
+  };
+  if (kgrp < ntot) tell(0);
+  __syncthreads();
+#pragma unroll 1
+  for (int it = 0; 2 * it < ntot; ++it) {
+    const int j = 2 * it + kgrp;
+    const bool have = j < ntot;  // (the odd tiles may end one sooner)
+    const uint32_t fk = __builtin_amdgcn_readfirstlane(T.flag[it & 1][0]), fv = __builtin_amdgcn_readfirstlane(T.flag[it & 1][1]);
+    if (tid < 2) T.flag[(it + 1) & 1][tid] = 0;  // (read two barriers ago, set again after the next one)
+    const float kdown = fk & 1 ? 0.015625f : 1.f, vdown = fv & 1 ? 0.015625f : 1.f;
+    if (have) {
+      f16 s = sf_bitcast<f16>((uint16_t)(kpr & 0xffffu)), mm = sf_bitcast<f16>((uint16_t)(kpr >> 16));
+      if (fk & 1) {
+        s = (f16)((float)s * kdown);
+        mm = (f16)((float)mm * kdown);
+      }
+      const half2_t s2 = {s, s}, m2 = {mm, mm}, sp[4] = {s2, s2, s2, s2}, mp[4] = {m2, m2, m2, m2};
+#pragma unroll
+      for (int i = 0; i < NFW; ++i) {
+        half8_t hi, lo;
+        values(kr[i], sp, mp, hi, lo);
+        T.kf[0][tb][NFW * w2 + i][lane] = hi;
+        if constexpr (SPLIT) T.kf[1][tb][NFW * w2 + i][lane] = lo;
+      }
+      // (rows on 8 bytes)
+      uint2 *dst = (uint2 *)(T.raw + vtok * PITCH + 4 * NFW * vpiece);
+#pragma unroll
+      for (int i = 0; i < NFW; i += 2) dst[i / 2] = uint2{vr[i], vr[i + 1]};
+      if (has_p) {
+        const bool fine = !(off(vpr) & 2);
+        const int u = ptok & 31, e = 4 * (u >> 3) + (u & 3);
+        const int at = 32 * (ptok >> 5) + 16 * (e >> 3) + 8 * (u >> 2 & 1) + (e & 7);
+        T.vsm[0][pg][at] = fine ? (f16)(q4_lo(vpr) * vdown) : (f16)0.f;
+        T.vsm[1][pg][at] = fine ? (f16)(q4_hi(vpr) * vdown) : (f16)0.f;
+      }
+    }
+    if (j + 2 < ntot) load(j + 2);
+    __syncthreads();  // K's fragments, V's codes and parameters are there; the last tile's V fragments are read
+    if (have) {
+      constexpr int NR = D == 128 ? 2 : 1;  // transposing reads, two fragments each
+      const int db = D == 128 ? wave : wave & 1, r0 = D == 128 ? 0 : wave >> 1, vg = 32 * db / a.g;
+      typedef int v2i __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        const int jl = lane & 15, s0 = 2 * (r0 + r), jj = jl & 7, s = s0 + (jl >> 3);
+        const int e = 8 * (s & 1) + (jj < 4 ? 2 * jj : 2 * (jj - 4) + 1);
+        const int row = 32 * (s >> 1) + 8 * (e >> 2) + 4 * h + (e & 3);
+        const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (__attribute__((address_space(3))) v2i *)(T.raw + row * PITCH + 16 * db + 8 * (lane >> 4 & 1)));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const half8_t s8 = *(const half8_t *)&T.vsm[0][vg][16 * (s0 + i) + 8 * h];
+          const half8_t m8 = *(const half8_t *)&T.vsm[1][vg][16 * (s0 + i) + 8 * h];
+          const half2_t sp[4] = {{s8[0], s8[1]}, {s8[2], s8[3]}, {s8[4], s8[5]}, {s8[6], s8[7]}};
+          const half2_t mp[4] = {{m8[0], m8[1]}, {m8[2], m8[3]}, {m8[4], m8[5]}, {m8[6], m8[7]}};
+          half8_t hi, lo;
+          values((uint32_t)(i ? w.y : w.x), sp, mp, hi, lo);
+          T.vf[0][db][s0 + i][lane] = hi;
+          if constexpr (SPLIT) T.vf[1][db][s0 + i][lane] = lo;
+        }
+      }
+    }
+    const bool any = have && 64 * j < hi_lim;  // some column of the wave sees the tile (uniform)
+    u32x4 ph[4], pl[4];
+    if (any) {
+      float16_t S[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) S[t][e] = 0.f;
+#pragma unroll
+        for (int f = 0; f < 2 * NFW; ++f) {
+          const half8_t x = T.kf[0][t][f][lane];
+          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[0][f], S[t], 0, 0, 0);
+          if constexpr (QP == 2) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[1][f], S[t], 0, 0, 0);
+          if constexpr (SPLIT) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(T.kf[1][t][f][lane], qf[0][f], S[t], 0, 0, 0);
+        }
+      }
+      const float mul = fk & 1 ? qmul * 64.f : qmul;
+      if (64 * j + 64 > lo_lim) {  // the lane's slots 32 t + 8 (e / 4) + 4 h + e % 4
+        const int left = lim - 64 * j - 4 * h;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) S[t][e] = 32 * t + 8 * (e >> 2) + (e & 3) < left ? S[t][e] : -INFINITY;
+      }
+      float mx = S[0][0];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, S[t][e]);
+      const float2_t mp = sf_swap32_pair(mx);
+      const float m_new = fmaxf(m, fmaxf(mp.x, mp.y) * mul), m_ref = m_new == -INFINITY ? 0.f : m_new;
+      if (__any(m_new != m)) {
+        const float cf = __builtin_amdgcn_exp2f(m - m_ref);  // exp2(-inf) = 0
+        lsum *= cf;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d) O[d] *= cf;
+        m = m_new;
+      }
+      const float shift = kP - m_ref;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(S[s >> 1][8 * (s & 1) + 2 * p], mul, shift));
+          const float y = __builtin_amdgcn_exp2f(fmaf(S[s >> 1][8 * (s & 1) + 2 * p + 1], mul, shift));
+          lsum += x + y;
+          uint32_t hi, lo;
+          q4_halves<SPLIT>(x, y, hi, lo);
+          ph[s][p] = hi;
+          pl[s][p] = lo;
+        }
+    }
+    if (j + 2 < ntot) tell((it + 1) & 1);
+    __syncthreads();  // V's fragments and the next tile's flags are there, K's are read
+    if (any) {
+      if (fv & 1) {
+#pragma unroll
+        for (int d = 0; d < NDB; ++d) O[d] *= 0.015625f;
+      }
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const half8_t x = T.vf[0][d][s][lane], p = sf_bitcast<half8_t>(ph[s]);
+          O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p, O[d], 0, 0, 0);
+          if constexpr (SPLIT) {
+            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, sf_bitcast<half8_t>(pl[s]), O[d], 0, 0, 0);
+            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(T.vf[1][d][s][lane], p, O[d], 0, 0, 0);
+          }
+        }
+      if (fv & 1) {
+#pragma unroll
+        for (int d = 0; d < NDB; ++d) O[d] *= 64.f;
+      }
+      if (fv & 2) {  // what is not finite, for the columns that see it
+        for (int t = 64 * j; t < min(64 * j + 64, lim); ++t)
+#pragma unroll
+          for (int d = 0; d < NDB; ++d)
+            if (off(a.vp[(base + t) * NG + 32 * d / a.g]) & 2) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) O[d][e] = NAN;
+            }
+      }
+    }
+  }
+  const float2_t lp = sf_swap32_pair(lsum);
+  lsum = lp.x + lp.y;
+  // the odd tiles' states join the even ones' (a wave without tiles holds m = -inf, l = 0, O = 0)
+  __syncthreads();  // the tiles are read
+  static_assert(sizeof(tiles) >= 4 * 64 * (16 * NDB + 2) * sizeof(float), "merge");
+  float *const x = (float *)tiles + wave * 64 * (16 * NDB + 2) + lane;
+  if (kgrp) {
+    x[0] = m;
+    x[64] = lsum;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[64 * (2 + 16 * d + e)] = O[d][e];
+  }
+  __syncthreads();
+  if (kgrp) return;
+  {
+    const float m2 = x[0], M = fmaxf(m, m2), M_ref = sf_merge_mref(M);
+    const float w1 = sf_merge_weight(m, M_ref), w2_ = sf_merge_weight(m2, M_ref);
+    lsum = fmaf(w2_, x[64], w1 * lsum);
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) O[d][e] = fmaf(x[64 * (2 + 16 * d + e)], w2_, O[d][e] * w1);
+  }
+  if (cw + l32 >= ncol) return;
+  const float inv = lsum > 0.f ? 1.f / lsum : lsum != lsum ? lsum : 0.f;
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      const size_t o = qrow * D + 32 * d + 8 * e4 + 4 * h;
+      const float4_t v = float4_t{O[d][4 * e4], O[d][4 * e4 + 1], O[d][4 * e4 + 2], O[d][4 * e4 + 3]} * inv;
+      if (a.odt == SF_F32) {
+        *(float4_t *)((float *)a.out + o) = v;
+      } else {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = a.odt == SF_BF16 ? sf_f32_to_bf16(v[i]) : sf_bitcast<uint16_t>((f16)v[i]);
+        *(u32x2 *)((uint16_t *)a.out + o) = u32x2{u[0] | u[1] << 16, u[2] | u[3] << 16};
+      }
+    }
+}
+
+// Whether the 128-column workgroups take a call: where they are enough to go round.
+bool q4_many(int B, int Tq, int H, int KVH, int D) {
+  return (D == 64 || D == 128) && (((long long)Tq * (H / KVH) + 127) / 128) * KVH * B >= 64;
+}
+
 int q4_splits(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits) {
   const long long blocks = ((long long)Tq * (H / KVH) + 15) / 16;
   if (n_splits <= 0) {
@@ -535,6 +873,7 @@ size_t q4_parts(long long rows, int D, int S, size_t *ml_off) {
 extern "C" size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits) {
   if (B <= 0 || Tq <= 0 || H <= 0 || KVH <= 0 || H % KVH || T_max < 0 || T_max > kQaMaxSlots || D <= 0) return 0;
   size_t ml;
+  if (q4_many(B, Tq, H, KVH, D)) return 0;
   return q4_parts((long long)B * Tq * H, D, q4_splits(B, Tq, H, KVH, T_max, D, n_splits), &ml);
 }
 
@@ -551,14 +890,14 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   if (int rc = sf_q4_cache_check(D, group)) return rc;
   SF_REQUIRE(T_max <= kQaMaxSlots, SF_EUNSUPPORTED, "T_max=%d: at most %d slots", T_max, kQaMaxSlots);
   const long long nrb = ((long long)Tq * (H / KVH) + 15) / 16, rows = (long long)B * Tq * H;
-  SF_REQUIRE(KVH * nrb <= 65535 && B <= 65535 && rows <= 0x7fffffffLL, SF_EINVAL,
+  SF_REQUIRE((KVH * nrb <= 65535 || q4_many(B, Tq, H, KVH, D)) && B <= 65535 && rows <= 0x7fffffffLL, SF_EINVAL,
              "B=%d KVH=%d rows=%d exceed the grid", B, KVH, Tq);
   SF_REQUIRE(q_dtype >= SF_F32 && q_dtype <= SF_BF16 && out_dtype >= SF_F32 && out_dtype <= SF_BF16, SF_EINVAL,
              "bad q/out dtype");
   SF_REQUIRE(q && k_codes && k_params && v_codes && v_params && out, SF_EINVAL, "null pointer argument");
   SF_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_params | (uintptr_t)v_params | (uintptr_t)q) & 15) == 0,
              SF_EINVAL, "q and cache buffers must be 16-byte aligned");
-  n_splits = q4_splits(B, Tq, H, KVH, T_max, D, n_splits);
+  n_splits = q4_many(B, Tq, H, KVH, D) ? 1 : q4_splits(B, Tq, H, KVH, T_max, D, n_splits);
   size_t ml_off;
   const size_t need = q4_parts(rows, D, n_splits, &ml_off);
   SF_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0), SF_EINVAL, "workspace must be 256-byte aligned");
@@ -568,6 +907,27 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   const Q4Attn a = {q, k_codes, v_codes, (const uint32_t *)k_params, (const uint32_t *)v_params, out, acc, ml, lengths,
                     out_dtype, T, T_max, T_cap, Tq, H, KVH, D, group, n_splits,
                     scale * 1.4426950408889634f};  // softmax in base 2
+  if (q4_many(B, Tq, H, KVH, D)) {
+    const unsigned blocks = (unsigned)((long long)B * KVH * (((long long)Tq * (H / KVH) + 127) / 128));
+    Q4Attn r = a;
+    r.n_splits = B * KVH;
+#define SF_QR(QD, SP)                                                          \
+  do {                                                                         \
+    if (D == 64) k_q4_rows<QD, SP, 64><<<blocks, 512, 0, st>>>(r);             \
+    else k_q4_rows<QD, SP, 128><<<blocks, 512, 0, st>>>(r);                    \
+  } while (0)
+#define SF_QR_O(QD)                             \
+  do {                                          \
+    if (out_dtype == SF_BF16) SF_QR(QD, false); \
+    else SF_QR(QD, true);                       \
+  } while (0)
+    if (q_dtype == SF_F32) SF_QR_O(SF_F32);
+    else if (q_dtype == SF_F16) SF_QR_O(SF_F16);
+    else SF_QR_O(SF_BF16);
+#undef SF_QR_O
+#undef SF_QR
+    return sf_check_launch("sf_attn_q4kv");
+  }
   const dim3 grid(n_splits, (unsigned)(KVH * nrb), B);
 #define SF_QA(QD, PS, DP, NG, KSG) k_q4_split<QD, PS, DP, NG, KSG><<<grid, kQaThreads, 0, st>>>(a)
 #define SF_QA_D(QD, PS)                                  \

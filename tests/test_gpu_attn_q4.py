@@ -22,15 +22,23 @@ def cache(B, KVH, cap, D, group, dev, seed=0, spread=1.0):
     return out
 
 
-def check(got, q, bufs, lengths, scale=None):
+def check(got, q, bufs, lengths, scale=None, many=False):
+    """many: the kernel of many rows may have taken the call, whose bf16 outputs come from q, K,
+    V and weights in fp16 (2^-11 of a step's half each, weights cut and not rounded)."""
     kc, kp, vc, vp = (t.cpu().numpy() for t in bufs)
-    rounded = 2.0 ** -11 if got.dtype == torch.bfloat16 else 2.0 ** -22  # (of the weights, before they meet the codes)
+    bf16 = got.dtype == torch.bfloat16
+    rounded = (3 if many else 1) * 2.0 ** -11 if bf16 else 2.0 ** -22  # (of the weights and V, before they are summed)
     q4 = q if q.dim() == 4 else q[:, None]
     want, bound = O.attention(q4.double().cpu().numpy(), kc, kp.astype(np.float64), vc, vp.astype(np.float64), lengths, scale,
-                              rounded)
+                              rounded, 2.0 ** -10 if many and bf16 else 2.0 ** -22)
     g = got.double().cpu().numpy().reshape(want.shape)
     tol = bound + torch.finfo(got.dtype).eps / 2 * (abs(want) + bound) + (2.0 ** -25 if got.dtype == torch.float16 else 0)
-    assert (abs(g - want) <= tol).all(), float((abs(g - want) / np.maximum(tol, 1e-300)).max())
+    top = 65520.0 if got.dtype == torch.float16 else np.inf  # fp16 rounds to infinity from there on
+    past = abs(want) - tol > top
+    assert (g[past] == np.sign(want[past]) * np.inf).all()
+    near = ~past & ((abs(want) + tol < top) | np.isfinite(g))
+    assert (near | past | (abs(want) + tol >= top)).all()
+    assert (abs(g - want)[near] <= tol[near]).all(), float((abs(g - want)[near] / np.maximum(tol[near], 1e-300)).max())
 
 
 GEOMETRIES = [(14, 2, 64, 64), (14, 2, 64, 32), (8, 2, 128, 64), (4, 1, 128, 128), (3, 3, 128, 32), (4, 2, 80, 80),
@@ -87,6 +95,54 @@ def test_prompts(dev, rows, H, KVH, D, group):
         q = (1.5 * torch.randn(2, rows, H, D, generator=g)).to(dtype).to(dev)
         for out in {torch.float32, dtype}:
             check(attention_q4kv(q, *bufs, lengths=lengths, out_dtype=out), q, bufs, lengths.tolist())
+
+
+@pytest.mark.parametrize("D,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("rows", [150, 261])
+def test_many_rows(dev, rows, D, group):
+    """Enough rows, heads and sequences for the workgroups of 128 columns: every group and type,
+    ragged, rows before a sequence's start, an empty sequence, scales of every sign."""
+    B, H, KVH, cap = 4, 16, 8, 300
+    bufs = cache(B, KVH, cap, D, group, dev, seed=rows)
+    g = torch.Generator().manual_seed(rows)
+    lengths = torch.tensor([rows, 0, 39, 300], dtype=torch.int32, device=dev)
+    for dtype in DT.values():
+        q = (1.5 * torch.randn(B, rows, H, D, generator=g)).to(dtype).to(dev)
+        for out, scale in ((torch.float32, None), (dtype, -0.07), (torch.bfloat16, 0.0)):
+            y = attention_q4kv(q, *bufs, lengths=lengths, out_dtype=out, scale=scale)
+            check(y, q, bufs, lengths.tolist(), scale, many=True)
+            assert (y[1] == 0).all() and (y[2, :max(0, rows - 39)] == 0).all()
+
+
+@pytest.mark.parametrize("out", list(DT))
+def test_many_rows_with_large_and_missing_values(dev, out):
+    """K and V past fp16's range once put together, and parameters of NaN: before, within and
+    past what a column sees."""
+    B, H, KVH, D, rows, n = 1, 64, 32, 128, 260, 330
+    bufs = cache(B, KVH, 400, D, 64, dev, seed=1)
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(B, rows, H, D, generator=g).to(dev)
+    want = attention_q4kv(q, *bufs, lengths=n, out_dtype=DT[out])
+    dirty = [t.clone() for t in bufs]
+    for t in (1, 3):
+        dirty[t][:, :, n:] = float("nan")
+    assert torch.equal(attention_q4kv(q, *dirty, lengths=n, out_dtype=DT[out]), want)
+    dirty[3][:, 3, 200, 1] = float("nan")  # of V's second group: the rows from 130 on, dims from 64 on
+    dirty[1][:, 5, 300, 0] = float("nan")  # of K: the rows from 230 on
+    y = attention_q4kv(q, *dirty, lengths=n, out_dtype=DT[out])
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[:, 130:, 6:8, 64:] = True
+    bad[:, 230:, 10:12] = True
+    assert torch.equal(y.isnan(), bad) and torch.equal(y[~bad], want[~bad])
+    large = [t.clone() for t in bufs]
+    large[3][:, :, 100:120, 0] *= 20000.0   # V up to some 80000: sums of the columns that see it
+    large[3][:, 1] *= 30000.0
+    large[1][:, 2, 40:50, 0] *= 12000.0     # K likewise: these slots take all the weight, or none
+    large[1].clamp_(-65504, 65504)
+    large[3].clamp_(-65504, 65504)
+    few = slice(0, 8)  # (of the first kv heads: enough for the oracle)
+    y = attention_q4kv(q, *large, lengths=n, out_dtype=DT[out])
+    check(y[:, :, few].contiguous(), q[:, :, few], [t[:, :4] for t in large], [n], None, many=True)
 
 
 @pytest.mark.parametrize("rows", [1, 70])
