@@ -70,26 +70,35 @@ __device__ __forceinline__ half8_t q4_codes(uint32_t w) {
   return sf_bitcast<half8_t>(r);
 }
 
-// Eight codes as they are, exact: codes 0, 4, 1, 5, 2, 6, 3, 7.
-__device__ __forceinline__ half8_t q4_unsigned(uint32_t w) {
-  const uint32_t x = w >> 8;
-  const half2_t a = {(f16)-1024.f, (f16)-1024.f}, b = {(f16)-64.f, (f16)-64.f};
-  const half2_t p0 = sf_bitcast<half2_t>((w & 0x000f000fu) | 0x64006400u) + a;
-  const half2_t p1 = sf_bitcast<half2_t>((w & 0x00f000f0u) | 0x54005400u) + b;
-  const half2_t p2 = sf_bitcast<half2_t>((x & 0x000f000fu) | 0x64006400u) + a;
-  const half2_t p3 = sf_bitcast<half2_t>((x & 0x00f000f0u) | 0x54005400u) + b;
-  return half8_t{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+// The operations that lift a word's codes into the mantissas of 1024 and 64: held in registers
+// (an instruction takes one literal), made once by a kernel.
+struct Q4Magic {
+  uint32_t a = 0x64006400u, b = 0x54005400u;
+  __device__ __forceinline__ void hold() { asm volatile("" : "+v"(a), "+v"(b)); }
+  __device__ __forceinline__ void lift(uint32_t w, half2_t (&p)[4]) const {
+    const uint32_t x = w >> 8;
+    p[0] = sf_bitcast<half2_t>((w & 0x000f000fu) | a);
+    p[1] = sf_bitcast<half2_t>((w & 0x00f000f0u) | b);
+    p[2] = sf_bitcast<half2_t>((x & 0x000f000fu) | a);
+    p[3] = sf_bitcast<half2_t>((x & 0x00f000f0u) | b);
+  }
+};
+
+// Eight codes less `less`, exact: pairs 0, 4; 1, 5; 2, 6; 3, 7.
+template <int LESS>
+__device__ __forceinline__ void q4_numbers(const Q4Magic &g, uint32_t w, half2_t (&p)[4]) {
+  constexpr f16 a = (f16)(-1024.f - LESS), b = (f16)(-64.f - LESS);
+  g.lift(w, p);
+  p[0] += half2_t{a, a};
+  p[1] += half2_t{b, b};
+  p[2] += half2_t{a, a};
+  p[3] += half2_t{b, b};
 }
 
-// Eight codes less 8, exact: codes 0, 4, 1, 5, 2, 6, 3, 7.
-__device__ __forceinline__ half8_t q4_signed(uint32_t w) {
-  const uint32_t x = w >> 8;
-  const half2_t a = {(f16)-1032.f, (f16)-1032.f}, b = {(f16)-72.f, (f16)-72.f};
-  const half2_t p0 = sf_bitcast<half2_t>((w & 0x000f000fu) | 0x64006400u) + a;
-  const half2_t p1 = sf_bitcast<half2_t>((w & 0x00f000f0u) | 0x54005400u) + b;
-  const half2_t p2 = sf_bitcast<half2_t>((x & 0x000f000fu) | 0x64006400u) + a;
-  const half2_t p3 = sf_bitcast<half2_t>((x & 0x00f000f0u) | 0x54005400u) + b;
-  return half8_t{p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+__device__ __forceinline__ half8_t q4_signed(const Q4Magic &g, uint32_t w) {
+  half2_t p[4];
+  q4_numbers<8>(g, w, p);
+  return half8_t{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
 }
 
 __device__ __forceinline__ float q4_lo(uint32_t w) { return (float)sf_bitcast<f16>((uint16_t)(w & 0xffffu)); }
@@ -137,7 +146,9 @@ k_q4_split(Q4Attn a) {
   uint32_t kr[4][KS];  // the codes of slots 4 hl + h
   u32x4 vr[DP / 32];   // 16 bytes of V codes each, slot-major
   uint32_t pr[2][NGM];
-  auto k_codes = [](uint32_t w) { return PSPLIT ? q4_signed(w) : q4_codes(w); };
+  Q4Magic magic;
+  magic.hold();
+  auto k_codes = [&](uint32_t w) { return PSPLIT ? q4_signed(magic, w) : q4_codes(w); };
   auto load_k = [&](int j) {
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
@@ -419,7 +430,7 @@ k_q4_split(Q4Attn a) {
         if (ANY ? 16 * d < gi * a.g || 16 * d >= (gi + 1) * a.g : d / (2 * KSGT) != gi) continue;
         const v2i vw = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
             (__attribute__((address_space(3))) v2i *)(vt + (16 * g + hl) * PITCH + 8 * d));
-        const half8_t x0 = q4_signed((uint32_t)vw.x), x1 = q4_signed((uint32_t)vw.y);
+        const half8_t x0 = q4_signed(magic, (uint32_t)vw.x), x1 = q4_signed(magic, (uint32_t)vw.y);
         O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, sf_bitcast<half8_t>(ph[0]), O[d], 0, 0, 0);
         O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, sf_bitcast<half8_t>(ph[1]), O[d], 0, 0, 0);
         if constexpr (PSPLIT) {
@@ -528,120 +539,219 @@ k_q4_merge(const float *__restrict__ part_acc, const float *__restrict__ part_ml
 // ---------------------------------------------------------------------------
 // many rows: prompts
 // ---------------------------------------------------------------------------
-// A workgroup owns 128 consecutive (row, head) columns c = t G + h of one kv head and walks
-// the 64-slot tiles up to its last row's own slot, two at a time: waves 0..3 take the even
-// ones, 32 columns each, waves 4..7 the odd ones, and their states merge at the end. A tile's
-// values m + s c are made once for its four waves, as fp16 (SPLIT: and what that leaves, a second fp16) in the order of
-// the matrix operands, 1 KB of LDS a fragment that every wave reads back whole:
+// Two launches. k_q4_spread takes the cache's values m + s c once for all rows, as fp16 (SPLIT:
+// and what that leaves, a second fp16), into the workspace in the order of the matrix
+// operands, 1 KB a fragment, blocks of 32 slots:
 //   * K: a lane makes its slot's fragments from neighbouring words of codes, q is loaded in
 //     the same order of dims;
 //   * V: codes through LDS and ds_read_b64_tr_b4, a lane then holds one dim's codes of 16
 //     slots in the order in which S^T leaves the weights in registers.
-// Then it is S^T = K q^T, a base-2 softmax a column and O^T = V^T P^T on
-// v_mfma_f32_32x32x16_f16. For a bf16 output q, P and the values are fp16's high parts: a
-// value off by 2^-12 moves an output by less than a fifth of its own rounding (2^-9). Other
-// outputs take three products of the high and low parts.
+// k_q4_rows: a workgroup owns 128 consecutive (row, head) columns c = t G + h of one kv head
+// and walks the tiles (64 slots; SPLIT: 32) up to its last row's own slot, two at a time:
+// waves 0..3 take the even ones, 32 columns each, waves 4..7 the odd ones, and their states
+// merge at the end. A tile goes straight to LDS, the next one while it is worked on: S^T =
+// K q^T, a base-2 softmax a column and O^T = V^T P^T on v_mfma_f32_32x32x16_f16.
+// For a bf16 output q, P and the values are fp16's high parts: a value off by 2^-12 moves an
+// output by less than a fifth of its own rounding (2^-9). Other outputs take three products
+// of the high and low parts.
 // What fp16 cannot hold: a tile with an s past 2^11 or an m past 2^14 is taken at 2^-6 (K's
-// scores and V's sums times 2^6 again); parameters that are not finite stand as zeros in V, and the
-// columns that see them get NaN in their group's dims.
-template <int QDT, bool SPLIT, int D>
-__global__ void __launch_bounds__(512, 2)
-k_q4_rows(Q4Attn a) {
+// scores and V's sums times 2^6 again); parameters that are not finite stand as zeros in V,
+// and the columns that see them get NaN in their group's dims.
+// (Made within one kernel, each workgroup its tiles' values through LDS and two barriers a
+// tile: 1500 rows behind 300, 32 / 8 heads of 128, bf16, 58 us.)
+
+// The workspace: blocks [B KVH][blocks of 32 slots][part][K fragments, V fragments], then
+// flags [B KVH][tiles of 64][2].
+__host__ __device__ constexpr size_t q4_block_bytes(int D, int parts) { return (size_t)parts * D / 8 * 1024; }
+__host__ __device__ inline size_t q4_tiles(int T_max) { return ((size_t)T_max + 63) / 64; }
+
+// What of a parameter word fp16 cannot carry: 1: s past 2^11 or m past 2^14, 2: not finite.
+__device__ __forceinline__ uint32_t q4_off(uint32_t w) {
+  const uint32_t x = w & 0x7fffu, y = w >> 16 & 0x7fffu;
+  return x >= 0x7c00u || y >= 0x7c00u ? 2u : x > 0x6800u || y > 0x7400u ? 1u : 0u;
+}
+
+// One workgroup a tile of 64 slots of one kv head.
+template <bool SPLIT, int D>
+__global__ void __launch_bounds__(256)
+k_q4_spread(Q4Attn a, uint8_t *__restrict__ ws, uint32_t *__restrict__ flags) {
   constexpr int NFW = D / 32;      // K fragments a wave makes of its 32 slots, of 2 NFW
   constexpr int NDB = D / 32;      // 32-dim blocks
-  constexpr int PARTS = SPLIT ? 2 : 1, QP = QDT == SF_F32 && SPLIT ? 2 : 1;
-  constexpr int PITCH = D / 2 + 8;
-  typedef float float16_t __attribute__((ext_vector_type(16)));
+  constexpr int PARTS = SPLIT ? 2 : 1, PITCH = D / 2 + 8;
   typedef uint32_t Words __attribute__((ext_vector_type(NFW)));  // 16 (8) bytes of codes
-  struct Tile {
-    half8_t kf[PARTS][2][2 * NFW][64], vf[PARTS][NDB][4][64];
-    uint8_t raw[64 * PITCH];
-    f16 vsm[2][NDB][64];  // s and m a group, in the order of the weights
-    uint32_t flag[2][2];  // of this tile and the next: K's, V's parameters are large (1) or not finite (2)
-  };
-  __shared__ __attribute__((aligned(16))) Tile tiles[2];
-  const int G = a.H / a.KVH, NG = D / a.g, ncol = a.Tq * G, ncb = (ncol + 127) / 128;
-  // longest columns first, the heads of all sequences side by side
-  const int bk = (int)(blockIdx.x % (unsigned)a.n_splits), c0 = (ncb - 1 - (int)(blockIdx.x / (unsigned)a.n_splits)) * 128;
-  const int b = bk / a.KVH, kvh = bk - b * a.KVH;
-  const int tid = threadIdx.x & 255, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kgrp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-  Tile &T = tiles[kgrp];
-  const size_t base = ((size_t)b * a.KVH + kvh) * a.T_cap;
+  __shared__ __attribute__((aligned(16))) uint8_t raw[64 * PITCH];
+  __shared__ __attribute__((aligned(16))) f16 vsm[2][NDB][64];  // s and m a group, in the order of the weights
+  __shared__ uint32_t flag[2];
+  const int j = blockIdx.x, bk = blockIdx.y, b = bk / a.KVH, NG = D / a.g;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = q4_len(a.lengths, a.T, a.T_max, b);
-  auto limit = [&](int c) { return max(0, n - a.Tq + c / G + 1); };  // slots column c sees
-  const int cw = c0 + 32 * wave, c = min(cw + l32, ncol - 1);
-  const int lim = limit(c), lo_lim = limit(min(cw, ncol - 1)), hi_lim = cw < ncol ? limit(min(cw + 31, ncol - 1)) : 0;  // and the wave's
-  const int ntot = (limit(min(c0 + 127, ncol - 1)) + 63) / 64;
-  const size_t qrow = ((size_t)b * a.Tq + c / G) * a.H + (size_t)kvh * G + c % G;
-
-  // what a thread makes of a tile
+  if (64 * j >= n) return;
   const int tb = wave >> 1, w2 = wave & 1;          // K: the slots 32 tb + l32, fragments NFW w2 ..
-  const int kword = 2 * NFW * w2 + NFW * h, kg = 8 * kword / a.g;
+  const int kword = 2 * NFW * w2 + NFW * h, kg = 8 * kword / a.g, krow = 32 * tb + l32;
   const int vtok = tid >> 2, vpiece = tid & 3;      // V: 16 (8) bytes of a slot
   const int ptok = tid / NG, pg = tid - ptok * NG;  // V: a slot's parameters of a group
   const bool has_p = tid < 64 * NG;
-  Words kr, vr;
-  uint32_t kpr = 0, vpr = 0;
-  auto load = [&](int j) {
-    const size_t last = a.T_cap - 1, kt = base + min((size_t)(64 * j + 32 * tb + l32), last);
-    kr = *(const Words *)(a.kc + kt * (D / 2) + 4 * kword);
-    vr = *(const Words *)(a.vc + (base + min((size_t)(64 * j + vtok), last)) * (D / 2) + 4 * NFW * vpiece);
-    kpr = a.kp[kt * NG + kg];
-    if (has_p) vpr = a.vp[(base + min((size_t)(64 * j + ptok), last)) * NG + pg];
-    if (64 * j + 32 * tb + l32 >= n) kpr = 0;  // slots past the length stand for zeros
-    if (64 * j + ptok >= n) vpr = 0;
-  };
-  auto off = [](uint32_t w) -> uint32_t {  // 1: s past 2^11 or m past 2^14, 2: not finite
-    const uint32_t x = w & 0x7fffu, y = w >> 16 & 0x7fffu;
-    return x >= 0x7c00u || y >= 0x7c00u ? 2u : x > 0x6800u || y > 0x7400u ? 1u : 0u;
-  };
+  const size_t at = (size_t)bk * a.T_cap + 64 * (size_t)j;
+  const int left = a.T_cap - 1 - 64 * j, kt = min(krow, left);  // (slots are clamped into the cache)
+  const Words kr = *(const Words *)(a.kc + at * (D / 2) + (uint32_t)(kt * (D / 2) + 4 * kword));
+  const Words vr = *(const Words *)(a.vc + at * (D / 2) + (uint32_t)(min(vtok, left) * (D / 2) + 4 * NFW * vpiece));
+  uint32_t kpr = (a.kp + at * NG)[(uint32_t)(kt * NG + kg)], vpr = 0;
+  if (has_p) vpr = (a.vp + at * NG)[(uint32_t)(min(ptok, left) * NG + pg)];
+  if (64 * j + krow >= n) kpr = 0;  // slots past the length stand for zeros
+  if (64 * j + ptok >= n) vpr = 0;
+  if (tid < 2) flag[tid] = 0;
+  __syncthreads();
+  const uint32_t ok = q4_off(kpr), ov = q4_off(vpr);
+  if (ok) atomicOr(&flag[0], ok);
+  if (ov) atomicOr(&flag[1], ov);
+  uint2 *dst = (uint2 *)(raw + vtok * PITCH + 4 * NFW * vpiece);  // (rows on 8 bytes)
+#pragma unroll
+  for (int i = 0; i < NFW; i += 2) dst[i / 2] = uint2{vr[i], vr[i + 1]};
+  __syncthreads();
+  const uint32_t fk = flag[0], fv = flag[1];
+  if (tid < 2) flags[((size_t)bk * q4_tiles(a.T_max) + j) * 2 + tid] = flag[tid];
+  const float kdown = fk & 1 ? 0.015625f : 1.f, vdown = fv & 1 ? 0.015625f : 1.f;
+  Q4Magic magic;
+  magic.hold();
   // eight values of one slot, or of eight slots (s, m one each), as operand parts
-  auto values = [](uint32_t w, const half2_t (&s)[4], const half2_t (&m)[4], half8_t &hi, half8_t &lo) {
-    const half8_t c8 = q4_unsigned(w);
-    half2_t v[4];
+  auto values = [&](uint32_t w, const half2_t (&s)[4], const half2_t (&m)[4], half8_t &hi, half8_t &lo) {
+    half2_t c8[4];
+    q4_numbers<0>(magic, w, c8);
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      const half2_t cp = {c8[2 * p], c8[2 * p + 1]};
-      v[p] = __builtin_elementwise_fma(cp, s[p], m[p]);
-      hi[2 * p] = v[p].x;
-      hi[2 * p + 1] = v[p].y;
+      const half2_t v = __builtin_elementwise_fma(c8[p], s[p], m[p]);
+      hi[2 * p] = v.x;
+      hi[2 * p + 1] = v.y;
       if constexpr (SPLIT) {
-        lo[2 * p] = (f16)(fmaf((float)cp.x, (float)s[p].x, (float)m[p].x) - (float)v[p].x);
-        lo[2 * p + 1] = (f16)(fmaf((float)cp.y, (float)s[p].y, (float)m[p].y) - (float)v[p].y);
+        lo[2 * p] = (f16)(fmaf((float)c8[p].x, (float)s[p].x, (float)m[p].x) - (float)v.x);
+        lo[2 * p + 1] = (f16)(fmaf((float)c8[p].y, (float)s[p].y, (float)m[p].y) - (float)v.y);
       }
     }
   };
+  // fragment i of K (2 NFW a block) or V (2 NDB, after them) of block t
+  uint8_t *const blocks = ws + ((size_t)bk * q4_tiles(a.T_max) + j) * 2 * q4_block_bytes(D, PARTS);
+  auto put = [&](int t, int i, const half8_t &hi, const half8_t &lo) {
+    half8_t *o = (half8_t *)(blocks + t * q4_block_bytes(D, PARTS)) + i * 64 + lane;
+    o[0] = hi;
+    if constexpr (SPLIT) o[4 * NFW * 64] = lo;
+  };
+  {
+    f16 s = (f16)(q4_lo(kpr) * kdown), m = (f16)(q4_hi(kpr) * kdown);
+    const half2_t s2 = {s, s}, m2 = {m, m}, sp[4] = {s2, s2, s2, s2}, mp[4] = {m2, m2, m2, m2};
+#pragma unroll
+    for (int i = 0; i < NFW; ++i) {
+      half8_t hi, lo;
+      values(kr[i], sp, mp, hi, lo);
+      put(tb, NFW * w2 + i, hi, lo);
+    }
+  }
+  if (has_p) {
+    const bool fine = !(ov & 2);
+    const int u = ptok & 31, e = 4 * (u >> 3) + (u & 3);
+    const int to = 32 * (ptok >> 5) + 16 * (e >> 3) + 8 * (u >> 2 & 1) + (e & 7);
+    vsm[0][pg][to] = fine ? (f16)(q4_lo(vpr) * vdown) : (f16)0.f;
+    vsm[1][pg][to] = fine ? (f16)(q4_hi(vpr) * vdown) : (f16)0.f;
+  }
+  __syncthreads();
+  constexpr int NR = D == 128 ? 2 : 1;  // transposing reads, two fragments each
+  const int db = D == 128 ? wave : wave & 1, r0 = D == 128 ? 0 : wave >> 1, vg = 32 * db / a.g;
+  typedef int v2i __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    const int jl = lane & 15, s0 = 2 * (r0 + r), jj = jl & 7, s = s0 + (jl >> 3);
+    const int e = 8 * (s & 1) + (jj < 4 ? 2 * jj : 2 * (jj - 4) + 1);
+    const int row = 32 * (s >> 1) + 8 * (e >> 2) + 4 * h + (e & 3);
+    const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+        (__attribute__((address_space(3))) v2i *)(raw + row * PITCH + 16 * db + 8 * (lane >> 4 & 1)));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const half8_t s8 = *(const half8_t *)&vsm[0][vg][16 * (s0 + i) + 8 * h];
+      const half8_t m8 = *(const half8_t *)&vsm[1][vg][16 * (s0 + i) + 8 * h];
+      const half2_t sp[4] = {{s8[0], s8[1]}, {s8[2], s8[3]}, {s8[4], s8[5]}, {s8[6], s8[7]}};
+      const half2_t mp[4] = {{m8[0], m8[1]}, {m8[2], m8[3]}, {m8[4], m8[5]}, {m8[6], m8[7]}};
+      half8_t hi, lo;
+      values((uint32_t)(i ? w.y : w.x), sp, mp, hi, lo);
+      put((s0 + i) >> 1, 2 * NFW + ((s0 + i) & 1) * NDB + db, hi, lo);
+    }
+  }
+}
+
+template <int QDT, bool SPLIT, int D>
+__global__ void __launch_bounds__(512, 2)
+k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__ flags) {
+  constexpr int NFW = D / 32, NDB = D / 32;
+  constexpr int PARTS = SPLIT ? 2 : 1, QP = QDT == SF_F32 && SPLIT ? 2 : 1;
+  constexpr int NT = SPLIT ? 1 : 2, TS = 32 * NT;  // blocks and slots a tile
+  constexpr int BLOCK = (int)q4_block_bytes(D, PARTS), KB_ = 2 * NFW;  // V's fragments come after K's
+  typedef float float16_t __attribute__((ext_vector_type(16)));
+  constexpr int kTiles = 4 * NT * BLOCK, kMerge = 4 * 64 * (16 * NDB + 2) * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kTiles > kMerge ? kTiles : kMerge];  // [half][two in turn][tile]
+  const int G = a.H / a.KVH, NG = D / a.g, ncol = a.Tq * G, ncb = (ncol + 127) / 128;
+  // longest columns first, the heads of all sequences side by side
+  const int BK = a.n_splits, bk = (int)(blockIdx.x % (unsigned)BK), c0 = (ncb - 1 - (int)(blockIdx.x / (unsigned)BK)) * 128;
+  const int b = bk / a.KVH, kvh = bk - b * a.KVH;
+  const int tid = threadIdx.x & 255, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kgrp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int n = q4_len(a.lengths, a.T, a.T_max, b);
+  auto limit = [&](int c) { return max(0, n - a.Tq + c / G + 1); };  // slots column c sees
+  const int cw = c0 + 32 * wave, c = min(cw + l32, ncol - 1);
+  const int lim = limit(c), lo_lim = limit(min(cw, ncol - 1));
+  const int hi_lim = cw < ncol ? limit(min(cw + 31, ncol - 1)) : 0;  // and the wave's
+  const int ntot = (limit(min(c0 + 127, ncol - 1)) + TS - 1) / TS;
+  const size_t qrow = ((size_t)b * a.Tq + c / G) * a.H + (size_t)kvh * G + c % G;
+
+  const uint8_t *const src = ws + (size_t)bk * q4_tiles(a.T_max) * 2 * BLOCK;
+  const uint32_t *const fl = flags + (size_t)bk * q4_tiles(a.T_max) * 2;
+  uint8_t *const mine = lds + kgrp * 2 * NT * BLOCK;
+  auto load = [&](int j, int at) {  // tile j to buffer `at`: 1 KB an instruction, the four waves in turn
+#pragma unroll
+    for (int i = 0; i < NT * BLOCK / 4096; ++i)
+      __builtin_amdgcn_global_load_lds(
+          (__attribute__((address_space(1))) void *)(src + (size_t)j * (NT * BLOCK) + 1024 * (4 * i + wave) + 16 * lane),
+          (__attribute__((address_space(3))) void *)(mine + at * NT * BLOCK + 1024 * (4 * i + wave)), 16, 0, 0);
+  };
+  if (kgrp < ntot) load(kgrp, 0);
 
   half8_t qf[QP][2 * NFW];
   float qmul;
   {
     float f[2 * NFW][8], top = 0.f;
-    const float sign = a.qscale < 0.f ? -1.f : a.qscale > 0.f ? 1.f : 0.f;  // (scores are compared before they are scaled)
 #pragma unroll
     for (int i = 0; i < 2 * NFW; ++i) {
-      const int w = 2 * NFW * (i / NFW) + NFW * h + i % NFW;
-      sf_load8_as_f32<QDT>(a.q, qrow * D + 8 * w, f[i]);
+      sf_load8_as_f32<QDT>(a.q, qrow * D + 8 * (2 * NFW * (i / NFW) + NFW * h + i % NFW), f[i]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        f[i][e] *= sign;
-        top = fmaxf(top, fabsf(f[i][e]));
-      }
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(f[i][e]));
     }
     const float2_t tp = sf_swap32_pair(top);
     const float up = q4_fit14(fmaxf(tp.x, tp.y));
-    qmul = sign == 0.f ? 1.f : fminf(fmaxf(fabsf(a.qscale) / up, 1.0e-37f), 1.0e36f);
+    qmul = a.qscale == 0.f ? 1.f : fminf(fmaxf(fabsf(a.qscale) / up, 1.0e-37f), 1.0e36f);
+    // (scores are compared before they are scaled: the scale's sign goes to q)
+    const float by = a.qscale < 0.f ? -up : a.qscale > 0.f ? up : 0.f;
 #pragma unroll
     for (int i = 0; i < 2 * NFW; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = f[i][(e >> 1) + 4 * (e & 1)] * up;
-        qf[0][i][e] = (f16)v;
-        if constexpr (QP == 2) qf[1][i][e] = (f16)(v - (float)qf[0][i][e]);
+      for (int e = 0; e < 4; ++e) {  // the codes' order: 0, 4, 1, 5, ..
+        const float x = f[i][e] * by, y = f[i][e + 4] * by;
+        if constexpr (QDT != SF_F32) {  // exact
+          const auto w = __builtin_amdgcn_cvt_pkrtz(x, y);
+          qf[0][i][2 * e] = (f16)w[0];
+          qf[0][i][2 * e + 1] = (f16)w[1];
+        } else {
+          qf[0][i][2 * e] = (f16)x;
+          qf[0][i][2 * e + 1] = (f16)y;
+          if constexpr (QP == 2) {
+            qf[1][i][2 * e] = (f16)(x - (float)qf[0][i][2 * e]);
+            qf[1][i][2 * e + 1] = (f16)(y - (float)qf[0][i][2 * e + 1]);
+          }
+        }
       }
   }
 
-  constexpr float kP = 13.f;  // weights times 2^13, so that their low parts are normal numbers
+  // Weights are 2^(score - m + 6), m a score that the row's largest passes by 8 at most: O is
+  // rescaled when it would be more (with 32 columns a wave some maximum moves in most tiles),
+  // the weights stay under fp16's end, and their low parts normal numbers down to 2^-20.
+  constexpr float kP = 6.f, kSlack = 8.f;
   float m = -INFINITY, lsum = 0.f;
   float16_t O[NDB];
 #pragma unroll
@@ -649,166 +759,137 @@ k_q4_rows(Q4Attn a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) O[d][e] = 0.f;
 
-  if (tid < 4) T.flag[tid >> 1][tid & 1] = 0;
-  if (kgrp < ntot) load(kgrp);
-  __syncthreads();
-  auto tell = [&](int at) {  // the loaded tile's parameters
-    const uint32_t fk = off(kpr), fv = has_p ? off(vpr) : 0u;
-    if (fk) atomicOr(&T.flag[at][0], fk);
-    if (fv) atomicOr(&T.flag[at][1], fv);
-  };
-  if (kgrp < ntot) tell(0);
-  __syncthreads();
 #pragma unroll 1
   for (int it = 0; 2 * it < ntot; ++it) {
     const int j = 2 * it + kgrp;
-    const bool have = j < ntot;  // (the odd tiles may end one sooner)
-    const uint32_t fk = __builtin_amdgcn_readfirstlane(T.flag[it & 1][0]), fv = __builtin_amdgcn_readfirstlane(T.flag[it & 1][1]);
-    if (tid < 2) T.flag[(it + 1) & 1][tid] = 0;  // (read two barriers ago, set again after the next one)
-    const float kdown = fk & 1 ? 0.015625f : 1.f, vdown = fv & 1 ? 0.015625f : 1.f;
-    if (have) {
-      f16 s = sf_bitcast<f16>((uint16_t)(kpr & 0xffffu)), mm = sf_bitcast<f16>((uint16_t)(kpr >> 16));
-      if (fk & 1) {
-        s = (f16)((float)s * kdown);
-        mm = (f16)((float)mm * kdown);
-      }
-      const half2_t s2 = {s, s}, m2 = {mm, mm}, sp[4] = {s2, s2, s2, s2}, mp[4] = {m2, m2, m2, m2};
+    __builtin_amdgcn_s_waitcnt((15 << 8) | (7 << 4));  // vmcnt(0): the wave's share of the tile is in LDS
+    __syncthreads();                                    // and the other waves', and the last tile is read
+    if (j + 2 < ntot) load(j + 2, (it + 1) & 1);
+    if (TS * j >= hi_lim || j >= ntot) continue;  // no column of the wave sees it (uniform)
+    const uint32_t fk = fl[2 * (NT * j / 2)], fv = fl[2 * (NT * j / 2) + 1];
+    const half8_t *const tile = (const half8_t *)(mine + (it & 1) * NT * BLOCK) + lane;
+    // fragments are read a batch ahead of the products that take them, two batches in turn;
+    // neighbouring products belong to different sums
+    auto frag = [&](int p, int t, int i) { return tile[(t * BLOCK + p * (BLOCK / PARTS) + i * 1024) / 16]; };
+    constexpr int KB = SPLIT ? 2 : 8, NKB = NT * KB_ / KB, VB = SPLIT ? 2 : 4, NVB = 2 * NT * NDB / VB;
+    float16_t S[NT];
 #pragma unroll
-      for (int i = 0; i < NFW; ++i) {
-        half8_t hi, lo;
-        values(kr[i], sp, mp, hi, lo);
-        T.kf[0][tb][NFW * w2 + i][lane] = hi;
-        if constexpr (SPLIT) T.kf[1][tb][NFW * w2 + i][lane] = lo;
-      }
-      // (rows on 8 bytes)
-      uint2 *dst = (uint2 *)(T.raw + vtok * PITCH + 4 * NFW * vpiece);
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int i = 0; i < NFW; i += 2) dst[i / 2] = uint2{vr[i], vr[i + 1]};
-      if (has_p) {
-        const bool fine = !(off(vpr) & 2);
-        const int u = ptok & 31, e = 4 * (u >> 3) + (u & 3);
-        const int at = 32 * (ptok >> 5) + 16 * (e >> 3) + 8 * (u >> 2 & 1) + (e & 7);
-        T.vsm[0][pg][at] = fine ? (f16)(q4_lo(vpr) * vdown) : (f16)0.f;
-        T.vsm[1][pg][at] = fine ? (f16)(q4_hi(vpr) * vdown) : (f16)0.f;
-      }
-    }
-    if (j + 2 < ntot) load(j + 2);
-    __syncthreads();  // K's fragments, V's codes and parameters are there; the last tile's V fragments are read
-    if (have) {
-      constexpr int NR = D == 128 ? 2 : 1;  // transposing reads, two fragments each
-      const int db = D == 128 ? wave : wave & 1, r0 = D == 128 ? 0 : wave >> 1, vg = 32 * db / a.g;
-      typedef int v2i __attribute__((ext_vector_type(2)));
+      for (int e = 0; e < 16; ++e) S[t][e] = 0.f;
+    {
+      half8_t x[2][PARTS][KB];
+      auto fetch = [&](int bi) {
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        const int jl = lane & 15, s0 = 2 * (r0 + r), jj = jl & 7, s = s0 + (jl >> 3);
-        const int e = 8 * (s & 1) + (jj < 4 ? 2 * jj : 2 * (jj - 4) + 1);
-        const int row = 32 * (s >> 1) + 8 * (e >> 2) + 4 * h + (e & 3);
-        const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-            (__attribute__((address_space(3))) v2i *)(T.raw + row * PITCH + 16 * db + 8 * (lane >> 4 & 1)));
+        for (int i = 0; i < KB; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const half8_t s8 = *(const half8_t *)&T.vsm[0][vg][16 * (s0 + i) + 8 * h];
-          const half8_t m8 = *(const half8_t *)&T.vsm[1][vg][16 * (s0 + i) + 8 * h];
-          const half2_t sp[4] = {{s8[0], s8[1]}, {s8[2], s8[3]}, {s8[4], s8[5]}, {s8[6], s8[7]}};
-          const half2_t mp[4] = {{m8[0], m8[1]}, {m8[2], m8[3]}, {m8[4], m8[5]}, {m8[6], m8[7]}};
-          half8_t hi, lo;
-          values((uint32_t)(i ? w.y : w.x), sp, mp, hi, lo);
-          T.vf[0][db][s0 + i][lane] = hi;
-          if constexpr (SPLIT) T.vf[1][db][s0 + i][lane] = lo;
+          for (int p = 0; p < PARTS; ++p) x[bi & 1][p][i] = frag(p, (bi * KB + i) % NT, (bi * KB + i) / NT);
+      };
+      fetch(0);
+#pragma unroll
+      for (int bi = 0; bi < NKB; ++bi) {
+        if (bi + 1 < NKB) fetch(bi + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < KB; ++i) {
+          const int t = (bi * KB + i) % NT, f = (bi * KB + i) / NT;
+          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[bi & 1][0][i], qf[0][f], S[t], 0, 0, 0);
+          if constexpr (QP == 2) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[bi & 1][0][i], qf[1][f], S[t], 0, 0, 0);
+          if constexpr (SPLIT) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[bi & 1][1][i], qf[0][f], S[t], 0, 0, 0);
         }
       }
     }
-    const bool any = have && 64 * j < hi_lim;  // some column of the wave sees the tile (uniform)
-    u32x4 ph[4], pl[4];
-    if (any) {
-      float16_t S[2];
+    half8_t y[2][PARTS][VB];
+    auto fetch_v = [&](int bi) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int i = 0; i < VB; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) S[t][e] = 0.f;
-#pragma unroll
-        for (int f = 0; f < 2 * NFW; ++f) {
-          const half8_t x = T.kf[0][t][f][lane];
-          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[0][f], S[t], 0, 0, 0);
-          if constexpr (QP == 2) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[1][f], S[t], 0, 0, 0);
-          if constexpr (SPLIT) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(T.kf[1][t][f][lane], qf[0][f], S[t], 0, 0, 0);
+        for (int p = 0; p < PARTS; ++p) {
+          const int s = (bi * VB + i) / NDB, d = (bi * VB + i) % NDB;
+          y[bi & 1][p][i] = frag(p, s >> 1, KB_ + (s & 1) * NDB + d);
         }
-      }
-      const float mul = fk & 1 ? qmul * 64.f : qmul;
-      if (64 * j + 64 > lo_lim) {  // the lane's slots 32 t + 8 (e / 4) + 4 h + e % 4
-        const int left = lim - 64 * j - 4 * h;
+    };
+    fetch_v(0);
+    const float mul = fk & 1 ? qmul * 64.f : qmul;
+    if (TS * j + TS > lo_lim) {  // the lane's slots 32 t + 8 (e / 4) + 4 h + e % 4
+      const int left = lim - TS * j - 4 * h;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) S[t][e] = 32 * t + 8 * (e >> 2) + (e & 3) < left ? S[t][e] : -INFINITY;
-      }
-      float mx = S[0][0];
+        for (int e = 0; e < 16; ++e) S[t][e] = 32 * t + 8 * (e >> 2) + (e & 3) < left ? S[t][e] : -INFINITY;
+    }
+    float mx = S[0][0];
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, S[t][e]);
-      const float2_t mp = sf_swap32_pair(mx);
-      const float m_new = fmaxf(m, fmaxf(mp.x, mp.y) * mul), m_ref = m_new == -INFINITY ? 0.f : m_new;
-      if (__any(m_new != m)) {
-        const float cf = __builtin_amdgcn_exp2f(m - m_ref);  // exp2(-inf) = 0
-        lsum *= cf;
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, S[t][e]);
+    const float2_t mp = sf_swap32_pair(mx);
+    const float m_new = fmaxf(m, fmaxf(mp.x, mp.y) * mul);
+    if (__any(m_new > m + kSlack)) {
+      const float cf = __builtin_amdgcn_exp2f(m - sf_merge_mref(m_new));  // exp2(-inf) = 0
+      lsum *= cf;
 #pragma unroll
-        for (int d = 0; d < NDB; ++d) O[d] *= cf;
-        m = m_new;
-      }
-      const float shift = kP - m_ref;
+      for (int d = 0; d < NDB; ++d) O[d] *= cf;
+      m = m_new;
+    }
+    const float shift = kP - sf_merge_mref(m);
+    u32x4 ph[2 * NT], pl[2 * NT];
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < 2 * NT; ++s)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(S[s >> 1][8 * (s & 1) + 2 * p], mul, shift));
-          const float y = __builtin_amdgcn_exp2f(fmaf(S[s >> 1][8 * (s & 1) + 2 * p + 1], mul, shift));
-          lsum += x + y;
+      for (int p = 0; p < 4; ++p) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(S[s >> 1][8 * (s & 1) + 2 * p], mul, shift));
+        const float z = __builtin_amdgcn_exp2f(fmaf(S[s >> 1][8 * (s & 1) + 2 * p + 1], mul, shift));
+        if constexpr (SPLIT) {
+          lsum += x + z;
           uint32_t hi, lo;
-          q4_halves<SPLIT>(x, y, hi, lo);
+          q4_halves<true>(x, z, hi, lo);
           ph[s][p] = hi;
           pl[s][p] = lo;
+        } else {  // cut to fp16; their sum is the cut weights', so that a cut takes from both alike
+          const auto w = __builtin_amdgcn_cvt_pkrtz(x, z);
+          ph[s][p] = sf_bitcast<uint32_t>(w);
+          lsum = __builtin_amdgcn_fdot2(sf_bitcast<half2_t>(w), half2_t{(f16)1.f, (f16)1.f}, lsum, false);
         }
+      }
+    if (fv & 1) {
+#pragma unroll
+      for (int d = 0; d < NDB; ++d) O[d] *= 0.015625f;
     }
-    if (j + 2 < ntot) tell((it + 1) & 1);
-    __syncthreads();  // V's fragments and the next tile's flags are there, K's are read
-    if (any) {
-      if (fv & 1) {
 #pragma unroll
-        for (int d = 0; d < NDB; ++d) O[d] *= 0.015625f;
-      }
+    for (int bi = 0; bi < NVB; ++bi) {
+      if (bi + 1 < NVB) fetch_v(bi + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int d = 0; d < NDB; ++d)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const half8_t x = T.vf[0][d][s][lane], p = sf_bitcast<half8_t>(ph[s]);
-          O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p, O[d], 0, 0, 0);
-          if constexpr (SPLIT) {
-            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, sf_bitcast<half8_t>(pl[s]), O[d], 0, 0, 0);
-            O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(T.vf[1][d][s][lane], p, O[d], 0, 0, 0);
-          }
+      for (int i = 0; i < VB; ++i) {
+        const int s = (bi * VB + i) / NDB, d = (bi * VB + i) % NDB;
+        const half8_t p = sf_bitcast<half8_t>(ph[s]);
+        O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y[bi & 1][0][i], p, O[d], 0, 0, 0);
+        if constexpr (SPLIT) {
+          O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y[bi & 1][0][i], sf_bitcast<half8_t>(pl[s]), O[d], 0, 0, 0);
+          O[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y[bi & 1][1][i], p, O[d], 0, 0, 0);
         }
-      if (fv & 1) {
-#pragma unroll
-        for (int d = 0; d < NDB; ++d) O[d] *= 64.f;
       }
-      if (fv & 2) {  // what is not finite, for the columns that see it
-        for (int t = 64 * j; t < min(64 * j + 64, lim); ++t)
+    }
+    if (fv & 1) {
 #pragma unroll
-          for (int d = 0; d < NDB; ++d)
-            if (off(a.vp[(base + t) * NG + 32 * d / a.g]) & 2) {
+      for (int d = 0; d < NDB; ++d) O[d] *= 64.f;
+    }
+    if (fv & 2) {  // what is not finite, for the columns that see it
+      for (int t = TS * j; t < min(TS * j + TS, lim); ++t)
 #pragma unroll
-              for (int e = 0; e < 16; ++e) O[d][e] = NAN;
-            }
-      }
+        for (int d = 0; d < NDB; ++d)
+          if (q4_off(a.vp[((size_t)bk * a.T_cap + t) * NG + 32 * d / a.g]) & 2) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) O[d][e] = NAN;
+          }
     }
   }
   const float2_t lp = sf_swap32_pair(lsum);
   lsum = lp.x + lp.y;
   // the odd tiles' states join the even ones' (a wave without tiles holds m = -inf, l = 0, O = 0)
   __syncthreads();  // the tiles are read
-  static_assert(sizeof(tiles) >= 4 * 64 * (16 * NDB + 2) * sizeof(float), "merge");
-  float *const x = (float *)tiles + wave * 64 * (16 * NDB + 2) + lane;
+  float *const x = (float *)lds + wave * 64 * (16 * NDB + 2) + lane;
   if (kgrp) {
     x[0] = m;
     x[64] = lsum;
@@ -821,35 +902,38 @@ k_q4_rows(Q4Attn a) {
   if (kgrp) return;
   {
     const float m2 = x[0], M = fmaxf(m, m2), M_ref = sf_merge_mref(M);
-    const float w1 = sf_merge_weight(m, M_ref), w2_ = sf_merge_weight(m2, M_ref);
-    lsum = fmaf(w2_, x[64], w1 * lsum);
+    const float w1 = sf_merge_weight(m, M_ref), w2 = sf_merge_weight(m2, M_ref);
+    lsum = fmaf(w2, x[64], w1 * lsum);
 #pragma unroll
     for (int d = 0; d < NDB; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) O[d][e] = fmaf(x[64 * (2 + 16 * d + e)], w2_, O[d][e] * w1);
+      for (int e = 0; e < 16; ++e) O[d][e] = fmaf(x[64 * (2 + 16 * d + e)], w2, O[d][e] * w1);
   }
   if (cw + l32 >= ncol) return;
   const float inv = lsum > 0.f ? 1.f / lsum : lsum != lsum ? lsum : 0.f;
+  const size_t o = qrow * D + 4 * h;
 #pragma unroll
   for (int d = 0; d < NDB; ++d)
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
-      const size_t o = qrow * D + 32 * d + 8 * e4 + 4 * h;
       const float4_t v = float4_t{O[d][4 * e4], O[d][4 * e4 + 1], O[d][4 * e4 + 2], O[d][4 * e4 + 3]} * inv;
-      if (a.odt == SF_F32) {
-        *(float4_t *)((float *)a.out + o) = v;
+      if (SPLIT && a.odt == SF_F32) {
+        *(float4_t *)((float *)a.out + o + 32 * d + 8 * e4) = v;
       } else {
         uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = a.odt == SF_BF16 ? sf_f32_to_bf16(v[i]) : sf_bitcast<uint16_t>((f16)v[i]);
-        *(u32x2 *)((uint16_t *)a.out + o) = u32x2{u[0] | u[1] << 16, u[2] | u[3] << 16};
+        for (int i = 0; i < 4; ++i) u[i] = SPLIT ? sf_bitcast<uint16_t>((f16)v[i]) : sf_f32_to_bf16(v[i]);
+        *(u32x2 *)((uint16_t *)a.out + o + 32 * d + 8 * e4) = u32x2{u[0] | u[1] << 16, u[2] | u[3] << 16};
       }
     }
 }
 
-// Whether the 128-column workgroups take a call: where they are enough to go round.
-bool q4_many(int B, int Tq, int H, int KVH, int D) {
-  return (D == 64 || D == 128) && (((long long)Tq * (H / KVH) + 127) / 128) * KVH * B >= 64;
+// The many rows' launches take a call where their workgroups are enough to go round; their
+// workspace, or 0. (Where it would pass 2 GiB the splits' launches take it.)
+size_t q4_many_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int parts) {
+  if ((D != 64 && D != 128) || (((long long)Tq * (H / KVH) + 127) / 128) * KVH * B < 64) return 0;
+  const size_t tiles = (size_t)B * KVH * q4_tiles(T_max), bytes = tiles * (2 * q4_block_bytes(D, parts) + 8);
+  return bytes > (size_t)1 << 31 ? 0 : bytes;
 }
 
 int q4_splits(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits) {
@@ -870,10 +954,10 @@ size_t q4_parts(long long rows, int D, int S, size_t *ml_off) {
 
 }  // namespace
 
-extern "C" size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits) {
+extern "C" size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int out_dtype, int n_splits) {
   if (B <= 0 || Tq <= 0 || H <= 0 || KVH <= 0 || H % KVH || T_max < 0 || T_max > kQaMaxSlots || D <= 0) return 0;
   size_t ml;
-  if (q4_many(B, Tq, H, KVH, D)) return 0;
+  if (const size_t many = q4_many_bytes(B, Tq, H, KVH, T_max, D, out_dtype == SF_BF16 ? 1 : 2)) return many;
   return q4_parts((long long)B * Tq * H, D, q4_splits(B, Tq, H, KVH, T_max, D, n_splits), &ml);
 }
 
@@ -890,16 +974,17 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   if (int rc = sf_q4_cache_check(D, group)) return rc;
   SF_REQUIRE(T_max <= kQaMaxSlots, SF_EUNSUPPORTED, "T_max=%d: at most %d slots", T_max, kQaMaxSlots);
   const long long nrb = ((long long)Tq * (H / KVH) + 15) / 16, rows = (long long)B * Tq * H;
-  SF_REQUIRE((KVH * nrb <= 65535 || q4_many(B, Tq, H, KVH, D)) && B <= 65535 && rows <= 0x7fffffffLL, SF_EINVAL,
+  const size_t many = q4_many_bytes(B, Tq, H, KVH, T_max, D, out_dtype == SF_BF16 ? 1 : 2);
+  SF_REQUIRE((many ? (long long)B * KVH <= 65535 : KVH * nrb <= 65535) && B <= 65535 && rows <= 0x7fffffffLL, SF_EINVAL,
              "B=%d KVH=%d rows=%d exceed the grid", B, KVH, Tq);
   SF_REQUIRE(q_dtype >= SF_F32 && q_dtype <= SF_BF16 && out_dtype >= SF_F32 && out_dtype <= SF_BF16, SF_EINVAL,
              "bad q/out dtype");
   SF_REQUIRE(q && k_codes && k_params && v_codes && v_params && out, SF_EINVAL, "null pointer argument");
   SF_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_params | (uintptr_t)v_params | (uintptr_t)q) & 15) == 0,
              SF_EINVAL, "q and cache buffers must be 16-byte aligned");
-  n_splits = q4_many(B, Tq, H, KVH, D) ? 1 : q4_splits(B, Tq, H, KVH, T_max, D, n_splits);
+  n_splits = many ? 1 : q4_splits(B, Tq, H, KVH, T_max, D, n_splits);
   size_t ml_off;
-  const size_t need = q4_parts(rows, D, n_splits, &ml_off);
+  const size_t parts = q4_parts(rows, D, n_splits, &ml_off), need = many ? many : parts;
   SF_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0), SF_EINVAL, "workspace must be 256-byte aligned");
   SF_REQUIRE(workspace_bytes >= need, SF_EINVAL, "attention workspace too small: %zu < %zu", workspace_bytes, need);
   float *acc = (float *)workspace, *ml = (float *)((char *)workspace + ml_off);
@@ -907,19 +992,24 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   const Q4Attn a = {q, k_codes, v_codes, (const uint32_t *)k_params, (const uint32_t *)v_params, out, acc, ml, lengths,
                     out_dtype, T, T_max, T_cap, Tq, H, KVH, D, group, n_splits,
                     scale * 1.4426950408889634f};  // softmax in base 2
-  if (q4_many(B, Tq, H, KVH, D)) {
+  if (many) {
     const unsigned blocks = (unsigned)((long long)B * KVH * (((long long)Tq * (H / KVH) + 127) / 128));
+    const dim3 tiles((unsigned)q4_tiles(T_max), (unsigned)(B * KVH));
+    uint8_t *const ws = (uint8_t *)workspace;
     Q4Attn r = a;
     r.n_splits = B * KVH;
-#define SF_QR(QD, SP)                                                          \
-  do {                                                                         \
-    if (D == 64) k_q4_rows<QD, SP, 64><<<blocks, 512, 0, st>>>(r);             \
-    else k_q4_rows<QD, SP, 128><<<blocks, 512, 0, st>>>(r);                    \
+#define SF_QR(QD, SP, DD)                                                                                        \
+  do {                                                                                                           \
+    uint32_t *const fl = (uint32_t *)(ws + tiles.x * (size_t)tiles.y * 2 * q4_block_bytes(DD, SP ? 2 : 1));      \
+    if (T_max > 0) k_q4_spread<SP, DD><<<tiles, 256, 0, st>>>(a, ws, fl);                                        \
+    k_q4_rows<QD, SP, DD><<<blocks, 512, 0, st>>>(r, ws, fl);                                                    \
   } while (0)
-#define SF_QR_O(QD)                             \
-  do {                                          \
-    if (out_dtype == SF_BF16) SF_QR(QD, false); \
-    else SF_QR(QD, true);                       \
+#define SF_QR_O(QD)                                  \
+  do {                                               \
+    if (out_dtype == SF_BF16 && D == 64) SF_QR(QD, false, 64);  \
+    else if (out_dtype == SF_BF16) SF_QR(QD, false, 128);       \
+    else if (D == 64) SF_QR(QD, true, 64);           \
+    else SF_QR(QD, true, 128);                       \
   } while (0)
     if (q_dtype == SF_F32) SF_QR_O(SF_F32);
     else if (q_dtype == SF_F16) SF_QR_O(SF_F16);
