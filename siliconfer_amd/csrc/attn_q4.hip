@@ -45,7 +45,7 @@ struct Q4Attn {
   void *out;
   float *part_acc, *part_ml;
   const int *lengths;
-  int odt, T, T_max, T_cap, Tq, H, KVH, D, g, n_splits;
+  int odt, T, T_max, T_cap, Tq, H, KVH, D, g, n_splits, first;
   float qscale;
 };
 
@@ -546,19 +546,23 @@ k_q4_merge(const float *__restrict__ part_acc, const float *__restrict__ part_ml
 //     the same order of dims;
 //   * V: codes through LDS and ds_read_b64_tr_b4, a lane then holds one dim's codes of 16
 //     slots in the order in which S^T leaves the weights in registers.
-// k_q4_rows: a workgroup owns 128 consecutive (row, head) columns c = t G + h of one kv head
-// and walks the tiles (64 slots; SPLIT: 32) up to its last row's own slot, two at a time:
-// waves 0..3 take the even ones, 32 columns each, waves 4..7 the odd ones, and their states
-// merge at the end. A tile goes straight to LDS, the next one while it is worked on: S^T =
-// K q^T, a base-2 softmax a column and O^T = V^T P^T on v_mfma_f32_32x32x16_f16.
+// k_q4_rows: a workgroup owns 128 consecutive (row, head) columns c = t G + h of one kv head,
+// 32 a wave, and walks the tiles (64 slots; SPLIT: 32) up to its last row's own slot. KG = 2:
+// two at a time, waves 0..3 the even ones, waves 4..7 the odd ones, whose states merge at the
+// end. A tile goes straight to LDS, the next one while it is worked on: S^T = K q^T, a base-2
+// softmax a column and O^T = V^T P^T on v_mfma_f32_32x32x16_f16, the next tile's scores
+// between the softmax's instructions.
 // For a bf16 output q, P and the values are fp16's high parts: a value off by 2^-12 moves an
 // output by less than a fifth of its own rounding (2^-9). Other outputs take three products
 // of the high and low parts.
 // What fp16 cannot hold: a tile with an s past 2^11 or an m past 2^14 is taken at 2^-6 (K's
 // scores and V's sums times 2^6 again); parameters that are not finite stand as zeros in V,
 // and the columns that see them get NaN in their group's dims.
-// (Made within one kernel, each workgroup its tiles' values through LDS and two barriers a
-// tile: 1500 rows behind 300, 32 / 8 heads of 128, bf16, 58 us.)
+// Measured, 32 / 8 heads of 128, bf16: 4096 rows 168 us (818 TFLOP/s of the products; a large
+// fp16 matrix product reaches 1215 on this card), 1500 rows behind 300 51.6 us, of which 6 the
+// first launch; both bound by the softmax's instructions and the products beside them, the
+// second also by the longest columns' 28 tiles one after the other. (Made within one kernel,
+// each workgroup its tiles' values through LDS and two barriers a tile: 203 and 58.)
 
 // The workspace: blocks [B KVH][blocks of 32 slots][part][K fragments, V fragments], then
 // flags [B KVH][tiles of 64][2].
@@ -677,22 +681,24 @@ k_q4_spread(Q4Attn a, uint8_t *__restrict__ ws, uint32_t *__restrict__ flags) {
   }
 }
 
-template <int QDT, bool SPLIT, int D>
-__global__ void __launch_bounds__(512, 2)
+template <int QDT, bool SPLIT, int D, int KG>
+__global__ void __launch_bounds__(256 * KG, 2)
 k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__ flags) {
   constexpr int NFW = D / 32, NDB = D / 32;
   constexpr int PARTS = SPLIT ? 2 : 1, QP = QDT == SF_F32 && SPLIT ? 2 : 1;
   constexpr int NT = SPLIT ? 1 : 2, TS = 32 * NT;  // blocks and slots a tile
   constexpr int BLOCK = (int)q4_block_bytes(D, PARTS), KB_ = 2 * NFW;  // V's fragments come after K's
   typedef float float16_t __attribute__((ext_vector_type(16)));
-  constexpr int kTiles = 4 * NT * BLOCK, kMerge = 4 * 64 * (16 * NDB + 2) * 4;
+  constexpr int kTiles = 2 * KG * NT * BLOCK, kMerge = KG == 1 ? 0 : 4 * 64 * (16 * NDB + 2) * 4;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kTiles > kMerge ? kTiles : kMerge];  // [half][two in turn][tile]
   const int G = a.H / a.KVH, NG = D / a.g, ncol = a.Tq * G, ncb = (ncol + 127) / 128;
-  // longest columns first, the heads of all sequences side by side
-  const int BK = a.n_splits, bk = (int)(blockIdx.x % (unsigned)BK), c0 = (ncb - 1 - (int)(blockIdx.x / (unsigned)BK)) * 128;
+  // The heads of all sequences side by side, the longest columns first; where all workgroups
+  // are resident at once, two on some CUs, the second of a CU comes to the shortest of the first.
+  const int BK = a.n_splits, bk = (int)(blockIdx.x % (unsigned)BK), at = (int)(blockIdx.x / (unsigned)BK);
+  const int c0 = (ncb - 1 - (at < a.first ? a.first - 1 - at : at)) * 128;
   const int b = bk / a.KVH, kvh = bk - b * a.KVH;
   const int tid = threadIdx.x & 255, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kgrp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), kgrp = KG == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   const int n = q4_len(a.lengths, a.T, a.T_max, b);
   auto limit = [&](int c) { return max(0, n - a.Tq + c / G + 1); };  // slots column c sees
   const int cw = c0 + 32 * wave, c = min(cw + l32, ncol - 1);
@@ -704,14 +710,22 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
   const uint8_t *const src = ws + (size_t)bk * q4_tiles(a.T_max) * 2 * BLOCK;
   const uint32_t *const fl = flags + (size_t)bk * q4_tiles(a.T_max) * 2;
   uint8_t *const mine = lds + kgrp * 2 * NT * BLOCK;
-  auto load = [&](int j, int at) {  // tile j to buffer `at`: 1 KB an instruction, the four waves in turn
+  // Half a tile of the wave's own run of tiles (K's or V's fragments) to a buffer: 1 KB an
+  // instruction, the four waves in turn.
+  constexpr int HALF = BLOCK / PARTS / 2;  // bytes of K's, or V's, fragments of a block's part
+  auto load = [&](int it, bool v) {
+    const int j = KG * it + kgrp;
+    if (j >= ntot) return;
 #pragma unroll
-    for (int i = 0; i < NT * BLOCK / 4096; ++i)
+    for (int i = 0; i < NT * PARTS * HALF / 4096; ++i) {
+      const int u = 4 * i + wave, blk = u / (HALF / 1024), o = blk * 2 * HALF + (v ? HALF : 0) + u % (HALF / 1024) * 1024;
       __builtin_amdgcn_global_load_lds(
-          (__attribute__((address_space(1))) void *)(src + (size_t)j * (NT * BLOCK) + 1024 * (4 * i + wave) + 16 * lane),
-          (__attribute__((address_space(3))) void *)(mine + at * NT * BLOCK + 1024 * (4 * i + wave)), 16, 0, 0);
+          (__attribute__((address_space(1))) void *)(src + (size_t)j * (NT * BLOCK) + o + 16 * lane),
+          (__attribute__((address_space(3))) void *)(mine + (it & 1) * NT * BLOCK + o), 16, 0, 0);
+    }
   };
-  if (kgrp < ntot) load(kgrp, 0);
+  load(0, false);
+  load(0, true);
 
   half8_t qf[QP][2 * NFW];
   float qmul;
@@ -759,57 +773,34 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
 #pragma unroll
     for (int e = 0; e < 16; ++e) O[d][e] = 0.f;
 
-#pragma unroll 1
-  for (int it = 0; 2 * it < ntot; ++it) {
-    const int j = 2 * it + kgrp;
-    __builtin_amdgcn_s_waitcnt((15 << 8) | (7 << 4));  // vmcnt(0): the wave's share of the tile is in LDS
-    __syncthreads();                                    // and the other waves', and the last tile is read
-    if (j + 2 < ntot) load(j + 2, (it + 1) & 1);
-    if (TS * j >= hi_lim || j >= ntot) continue;  // no column of the wave sees it (uniform)
-    const uint32_t fk = fl[2 * (NT * j / 2)], fv = fl[2 * (NT * j / 2) + 1];
-    const half8_t *const tile = (const half8_t *)(mine + (it & 1) * NT * BLOCK) + lane;
-    // fragments are read a batch ahead of the products that take them, two batches in turn;
-    // neighbouring products belong to different sums
-    auto frag = [&](int p, int t, int i) { return tile[(t * BLOCK + p * (BLOCK / PARTS) + i * 1024) / 16]; };
-    constexpr int KB = SPLIT ? 2 : 8, NKB = NT * KB_ / KB, VB = SPLIT ? 2 : 4, NVB = 2 * NT * NDB / VB;
-    float16_t S[NT];
+  // A tile's scores are made while the softmax of the one before runs: products and vector
+  // instructions of one wave side by side.
+  auto frag = [&](int it, int p, int t, int i) {
+    return ((const half8_t *)(mine + (it & 1) * NT * BLOCK) + lane)[(t * BLOCK + p * (BLOCK / PARTS) + i * 1024) / 16];
+  };
+  auto score = [&](int it, int f0, int f1, float16_t (&S)[NT]) {  // k-steps f0 .. f1 of all blocks
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int f = f0; f < f1; ++f)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) S[t][e] = 0.f;
-    {
-      half8_t x[2][PARTS][KB];
-      auto fetch = [&](int bi) {
+      for (int t = 0; t < NT; ++t) {
+        const half8_t x = frag(it, 0, t, f);
+        if (f == 0) {
 #pragma unroll
-        for (int i = 0; i < KB; ++i)
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) x[bi & 1][p][i] = frag(p, (bi * KB + i) % NT, (bi * KB + i) / NT);
-      };
-      fetch(0);
-#pragma unroll
-      for (int bi = 0; bi < NKB; ++bi) {
-        if (bi + 1 < NKB) fetch(bi + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < KB; ++i) {
-          const int t = (bi * KB + i) % NT, f = (bi * KB + i) / NT;
-          S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[bi & 1][0][i], qf[0][f], S[t], 0, 0, 0);
-          if constexpr (QP == 2) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[bi & 1][0][i], qf[1][f], S[t], 0, 0, 0);
-          if constexpr (SPLIT) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[bi & 1][1][i], qf[0][f], S[t], 0, 0, 0);
+          for (int e = 0; e < 16; ++e) S[t][e] = 0.f;
         }
+        S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[0][f], S[t], 0, 0, 0);
+        if constexpr (QP == 2) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qf[1][f], S[t], 0, 0, 0);
+        if constexpr (SPLIT) S[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(frag(it, 1, t, f), qf[0][f], S[t], 0, 0, 0);
       }
-    }
-    half8_t y[2][PARTS][VB];
-    auto fetch_v = [&](int bi) {
-#pragma unroll
-      for (int i = 0; i < VB; ++i)
-#pragma unroll
-        for (int p = 0; p < PARTS; ++p) {
-          const int s = (bi * VB + i) / NDB, d = (bi * VB + i) % NDB;
-          y[bi & 1][p][i] = frag(p, s >> 1, KB_ + (s & 1) * NDB + d);
-        }
-    };
-    fetch_v(0);
+  };
+  auto step = [&](int it, float16_t (&S)[NT], float16_t (&next)[NT]) {
+    const int j = KG * it + kgrp;
+    __builtin_amdgcn_s_waitcnt((15 << 8) | (7 << 4));  // vmcnt(0): the wave's share of this V and the next K is in LDS
+    __syncthreads();                                    // and the other waves'; the last V and this K are read
+    load(it + 2, false);
+    load(it + 1, true);
+    if (TS * j >= hi_lim || j >= ntot) return;  // no column of the wave sees it (uniform)
+    const uint32_t fk = fl[2 * (NT * j / 2)], fv = fl[2 * (NT * j / 2) + 1];
     const float mul = fk & 1 ? qmul * 64.f : qmul;
     if (TS * j + TS > lo_lim) {  // the lane's slots 32 t + 8 (e / 4) + 4 h + e % 4
       const int left = lim - TS * j - 4 * h;
@@ -818,6 +809,7 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
 #pragma unroll
         for (int e = 0; e < 16; ++e) S[t][e] = 32 * t + 8 * (e >> 2) + (e & 3) < left ? S[t][e] : -INFINITY;
     }
+    score(it + 1, 0, NFW, next);  // (past the last tile: whatever lies there, never used)
     float mx = S[0][0];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -832,7 +824,12 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
       for (int d = 0; d < NDB; ++d) O[d] *= cf;
       m = m_new;
     }
+    if (fv & 1) {
+#pragma unroll
+      for (int d = 0; d < NDB; ++d) O[d] *= 0.015625f;
+    }
     const float shift = kP - sf_merge_mref(m);
+    score(it + 1, NFW, 2 * NFW, next);
     u32x4 ph[2 * NT], pl[2 * NT];
 #pragma unroll
     for (int s = 0; s < 2 * NT; ++s)
@@ -852,10 +849,31 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
           lsum = __builtin_amdgcn_fdot2(sf_bitcast<half2_t>(w), half2_t{(f16)1.f, (f16)1.f}, lsum, false);
         }
       }
-    if (fv & 1) {
+    // (one product to some vector instructions, operands read ahead)
+    constexpr int kProducts = NFW * NT * (SPLIT ? QP + 1 : 1), kVector = (SPLIT ? 9 : 4) * 16 * NT / kProducts;
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
-      for (int d = 0; d < NDB; ++d) O[d] *= 0.015625f;
+    for (int i = 0; i < kProducts; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, kVector / 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x400, 16 * NT / kProducts, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, kVector / 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
+    // fragments are read a batch ahead of the products that take them, two batches in turn;
+    // neighbouring products belong to different sums
+    constexpr int VB = SPLIT ? 2 : 4, NVB = 2 * NT * NDB / VB;
+    half8_t y[2][PARTS][VB];
+    auto fetch_v = [&](int bi) {
+#pragma unroll
+      for (int i = 0; i < VB; ++i)
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+          const int s = (bi * VB + i) / NDB, d = (bi * VB + i) % NDB;
+          y[bi & 1][p][i] = frag(it, p, s >> 1, KB_ + (s & 1) * NDB + d);
+        }
+    };
+    fetch_v(0);
 #pragma unroll
     for (int bi = 0; bi < NVB; ++bi) {
       if (bi + 1 < NVB) fetch_v(bi + 1);
@@ -884,30 +902,46 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
             for (int e = 0; e < 16; ++e) O[d][e] = NAN;
           }
     }
+  };
+
+  float16_t S0[NT], S1[NT];
+  const int nit = (ntot + KG - 1) / KG;
+  if (nit > 0) {
+    __builtin_amdgcn_s_waitcnt((15 << 8) | (7 << 4));  // vmcnt(0)
+    __syncthreads();
+    load(1, false);
+    score(0, 0, 2 * NFW, S0);
+  }
+#pragma unroll 1
+  for (int it = 0; it < nit; it += 2) {
+    step(it, S0, S1);
+    if (it + 1 < nit) step(it + 1, S1, S0);
   }
   const float2_t lp = sf_swap32_pair(lsum);
   lsum = lp.x + lp.y;
-  // the odd tiles' states join the even ones' (a wave without tiles holds m = -inf, l = 0, O = 0)
-  __syncthreads();  // the tiles are read
-  float *const x = (float *)lds + wave * 64 * (16 * NDB + 2) + lane;
-  if (kgrp) {
-    x[0] = m;
-    x[64] = lsum;
+  if constexpr (KG == 2) {
+    // the odd tiles' states join the even ones' (a wave without tiles holds m = -inf, l = 0, O = 0)
+    __syncthreads();  // the tiles are read
+    float *const x = (float *)lds + wave * 64 * (16 * NDB + 2) + lane;
+    if (kgrp) {
+      x[0] = m;
+      x[64] = lsum;
 #pragma unroll
-    for (int d = 0; d < NDB; ++d)
+      for (int d = 0; d < NDB; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[64 * (2 + 16 * d + e)] = O[d][e];
-  }
-  __syncthreads();
-  if (kgrp) return;
-  {
-    const float m2 = x[0], M = fmaxf(m, m2), M_ref = sf_merge_mref(M);
-    const float w1 = sf_merge_weight(m, M_ref), w2 = sf_merge_weight(m2, M_ref);
-    lsum = fmaf(w2, x[64], w1 * lsum);
+        for (int e = 0; e < 16; ++e) x[64 * (2 + 16 * d + e)] = O[d][e];
+    }
+    __syncthreads();
+    if (kgrp) return;
+    {
+      const float m2 = x[0], M = fmaxf(m, m2), M_ref = sf_merge_mref(M);
+      const float w1 = sf_merge_weight(m, M_ref), w2 = sf_merge_weight(m2, M_ref);
+      lsum = fmaf(w2, x[64], w1 * lsum);
 #pragma unroll
-    for (int d = 0; d < NDB; ++d)
+      for (int d = 0; d < NDB; ++d)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) O[d][e] = fmaf(x[64 * (2 + 16 * d + e)], w2, O[d][e] * w1);
+        for (int e = 0; e < 16; ++e) O[d][e] = fmaf(x[64 * (2 + 16 * d + e)], w2, O[d][e] * w1);
+    }
   }
   if (cw + l32 >= ncol) return;
   const float inv = lsum > 0.f ? 1.f / lsum : lsum != lsum ? lsum : 0.f;
@@ -990,7 +1024,7 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   float *acc = (float *)workspace, *ml = (float *)((char *)workspace + ml_off);
   hipStream_t st = (hipStream_t)stream;
   const Q4Attn a = {q, k_codes, v_codes, (const uint32_t *)k_params, (const uint32_t *)v_params, out, acc, ml, lengths,
-                    out_dtype, T, T_max, T_cap, Tq, H, KVH, D, group, n_splits,
+                    out_dtype, T, T_max, T_cap, Tq, H, KVH, D, group, n_splits, 0,
                     scale * 1.4426950408889634f};  // softmax in base 2
   if (many) {
     const unsigned blocks = (unsigned)((long long)B * KVH * (((long long)Tq * (H / KVH) + 127) / 128));
@@ -998,11 +1032,24 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
     uint8_t *const ws = (uint8_t *)workspace;
     Q4Attn r = a;
     r.n_splits = B * KVH;
+    // The order of a head's columns where all are resident at once, one or two a CU (us, 1500 rows
+    // behind 300, 32 / 8 heads of 128, longest first / the first CUs' shortest first: bf16 55.7 /
+    // 51.6, fp32 111 / 104); longest first where there are more.
+    const int heads = B * KVH, cols = (int)(blocks / heads), per = 256 / heads;
+    if (cols > per && cols <= 2 * per) r.first = per;
+    // Four waves a workgroup where there are more workgroups than CUs, for a bf16 output: two a CU
+    // between barriers of their own; else eight, which halves the longest columns' walk. us, four /
+    // eight waves: bf16, 376 workgroups 51.6 / 54.1, 1024 (4096 rows) 168 / 181, 166 (14 / 2 heads
+    // of 64) 32.3 / 27.3; fp32 (whose tiles are half as long) at 376 110 / 104, fp16 97 / 89.
+    const bool four = out_dtype == SF_BF16 && blocks > 256;
 #define SF_QR(QD, SP, DD)                                                                                        \
   do {                                                                                                           \
     uint32_t *const fl = (uint32_t *)(ws + tiles.x * (size_t)tiles.y * 2 * q4_block_bytes(DD, SP ? 2 : 1));      \
-    if (T_max > 0) k_q4_spread<SP, DD><<<tiles, 256, 0, st>>>(a, ws, fl);                                        \
-    k_q4_rows<QD, SP, DD><<<blocks, 512, 0, st>>>(r, ws, fl);                                                    \
+    k_q4_spread<SP, DD><<<tiles, 256, 0, st>>>(a, ws, fl);                                                       \
+    if constexpr (!SP) {                                                                                         \
+      if (four) k_q4_rows<QD, SP, DD, 1><<<blocks, 256, 0, st>>>(r, ws, fl);                                     \
+    }                                                                                                            \
+    if (SP || !four) k_q4_rows<QD, SP, DD, 2><<<blocks, 512, 0, st>>>(r, ws, fl);                                \
   } while (0)
 #define SF_QR_O(QD)                                  \
   do {                                               \
