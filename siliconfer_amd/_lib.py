@@ -124,7 +124,7 @@ _SIGS = {
                                _c_f, _c_i, _c_p, _c_i, _c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_i, _c_i, _c_i,
                                _c_i, _c_i, _c_i, _c_p]),
     "sf_kv_q4_dequant": (_c_i, [_c_p, _c_p, _c_p, _c_i, _c_i, _c_p, _c_i, _c_i, _c_i, _c_i, _c_p]),
-    "sf_attn_q4_workspace_bytes": (_c_sz, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
+    "sf_attn_q4_workspace_bytes": (_c_sz, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i]),
     "sf_attn_q4kv": (_c_i, [_c_p, _c_i, _c_p, _c_p, _c_p, _c_p, _c_i, _c_p, _c_i, _c_p, _c_sz, _c_i, _c_i, _c_i, _c_i,
                             _c_p, _c_i, _c_i, _c_i, _c_i, _c_f, _c_i, _c_p]),
     "sf_kv_evict_workspace_bytes": (_c_sz, [_c_i, _c_i, _c_i, _c_i]),

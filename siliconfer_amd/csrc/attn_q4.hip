@@ -13,15 +13,15 @@
 //
 // k_q4_split: one workgroup a (split, kv head and 16 of its rows, sequence); its four waves
 // take 64-slot tiles. S^T = K q^T and O^T = V^T P^T with the query rows on the 16-wide side:
-//   * row m of S^T's block h is slot 4 m + h of the tile, so lane l holds row l % 16 and the 16
+//   * row m of S^T's block h is slot 4 m + h of the tile, so lane l holds column l % 16 and the 16
 //     neighbouring slots 16 (l / 16) .. of it, value (h, i) slot 4 i + h;
 //   * V^T comes through LDS with ds_read_b64_tr_b4, which hands a lane one dim's codes of 16
 //     slots: both B operands' order;
 //   * q (fp32) and P as fp16 high and low parts, q brought to a largest magnitude of 2^13..2^14
-//     by a power of two a row, P times the V scale likewise by the largest one that the row
-//     has met: what the low part drops is below 2^-22 of the value and 2^-38 of the row's
-//     largest. fp16 and bf16 queries are exact in the high part alone; for a bf16 output P's low
-//     part is left out (2^-12 of a weight beside the 2^-9 of the output's rounding).
+//     by a power of two a row, P times the V scale under 2^15 likewise: what the low part drops is
+//     below 2^-22 of the value and, where a row's weights span more, 2^-30 of the row's largest.
+//     fp16 and bf16 queries are exact in the high part alone; for a bf16 output the low parts are
+//     left out (2^-12 of a weight or of q beside the 2^-9 of the output's rounding).
 // Maxima, sums, m's part and the partials are fp32.
 #include <math.h>
 
@@ -45,7 +45,7 @@ struct Q4Attn {
   void *out;
   float *part_acc, *part_ml;
   const int *lengths;
-  int odt, T, T_max, T_cap, Tq, H, KVH, D, g, n_splits, first;
+  int qdt, odt, T, T_max, T_cap, Tq, H, KVH, D, g, n_splits, first;
   float qscale;
 };
 
@@ -115,26 +115,43 @@ __device__ __forceinline__ void q4_halves(float a, float b, uint32_t &hi, uint32
     lo = sf_bitcast<uint16_t>((f16)(a - (float)x)) | (uint32_t)sf_bitcast<uint16_t>((f16)(b - (float)y)) << 16;
 }
 
+// Workgroups of k_q4_split that a CU's registers hold without (much) spilling.
+__host__ __device__ constexpr int q4_resident(int DP, int groups, int PK, bool QSPLIT) {
+  return groups == 0 || DP > 128 ? 1
+         : DP == 64              ? groups == 1 ? PK > 1 ? 4 : 3 : PK == 4 && !QSPLIT ? 4 : PK == 1 ? 2 : 3
+         : groups == 1           ? QSPLIT && PK < 4 ? 2 : 3
+         : groups == 2           ? !QSPLIT && PK == 4 ? 3 : 2
+                                 : PK == 4 ? 2 : 1;
+}
+
+// Columns: where a kv head has at most 8 (4) rows, PK = 2 (4) groups of 16 / PK columns hold the
+// same rows, and a column takes only the values of a quarter's h (two, one of h = 0 .. 3): the
+// softmax's work a tile is that of the rows there are. Each column is a softmax state of its
+// own until the waves' states merge.
+// A state's reference m stays until a score passes it by 8, so that most tiles need no maximum
+// across lanes and no rescaling; the factor that takes p s to fp16's range stays likewise until
+// a product passes 2^15.
 // DP: the head's dims rounded up to 64, 128 or 256. NGT groups of 32 KSGT dims fill it
-// exactly, or 0, 0: any head and groups.
-template <int QDT, bool PSPLIT, int DP, int NGT, int KSGT>
-__global__ void __launch_bounds__(kQaThreads)
+// exactly, or 0, 0: any head and groups. QSPLIT, PSPLIT: q, P in two parts.
+template <bool QSPLIT, bool PSPLIT, int DP, int NGT, int KSGT, int PK>
+__global__ void __launch_bounds__(kQaThreads, q4_resident(DP, NGT, PK, QSPLIT))
 k_q4_split(Q4Attn a) {
-  constexpr bool ANY = NGT == 0, QSPLIT = QDT == SF_F32;
+  constexpr bool ANY = NGT == 0;
   constexpr float kCode = PSPLIT ? 1.f : 16777216.f;  // what an operand of K's codes is to be multiplied by
   constexpr int KS = DP / 32, DB = DP / 16, NGM = ANY ? 8 : NGT;
+  constexpr int RP = 16 / PK, HV = 4 / PK, NV = 4 * HV;  // rows, h's and values of a column
   constexpr int PITCH = DP / 2 + 8;  // 16 neighbouring rows' 8 bytes fall on different banks
   constexpr int OP = DP + 4;
   constexpr int kTile = 64 * PITCH, kPar = 64 * NGM * 4;
-  constexpr int kWave = kTile + 4 * kPar + 256, kO = 16 * OP * 4;
+  constexpr int kWave = kTile + 4 * kPar + (NGM > 1 ? 256 : 0), kO = 16 * OP * 4;
   __shared__ __attribute__((aligned(16))) uint8_t smem[kQaWaves * (kWave > kO ? kWave : kO) + 2 * kQaWaves * 16 * 4];
   const int D = ANY ? a.D : DP, NG = ANY ? a.D / a.g : NGT, GW = (ANY ? a.g : 32 * KSGT) / 8;
   const int KSG = ANY ? (GW + 3) / 4 : KSGT, nks = ANY ? NG * KSG : KS;
-  const int G = a.H / a.KVH, R = a.Tq * G, nrb = (R + 15) / 16;
+  const int G = a.H / a.KVH, R = a.Tq * G, nrb = PK > 1 ? 1 : (R + 15) / 16;
   const int split = blockIdx.x, kvh = blockIdx.y / nrb, rb = blockIdx.y - kvh * nrb, b = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hl = lane & 15, g = lane >> 4, nr = min(16, R - 16 * rb);
-  const int r = 16 * rb + hl, qt = min(r, R - 1) / G, qh = min(r, R - 1) - qt * G;
+  const int hl = lane & 15, g = lane >> 4, nr = min(16, R - 16 * rb), pg = hl / RP, h0 = HV * pg;
+  const int r = 16 * rb + hl % RP, qt = min(r, R - 1) / G, qh = min(r, R - 1) - qt * G;
   const size_t bk = (size_t)b * a.KVH + kvh, base = bk * a.T_cap;
   const int rowb = D / 2;
   // the word of codes that k-step ks takes of a slot (a group's words shared out over the four lanes)
@@ -149,14 +166,17 @@ k_q4_split(Q4Attn a) {
   Q4Magic magic;
   magic.hold();
   auto k_codes = [&](uint32_t w) { return PSPLIT ? q4_signed(magic, w) : q4_codes(w); };
+  // (slots are clamped into the cache; a tile's addresses are its own and a lane's 32-bit offset)
   auto load_k = [&](int j) {
+    const uint8_t *const at = a.kc + (base + 64 * (size_t)j) * rowb;
+    const int left = a.T_cap - 1 - 64 * j;
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      const uint8_t *p = a.kc + (base + min(64 * j + 4 * hl + h, a.T_cap - 1)) * rowb;
+      const uint32_t row = (uint32_t)(min(4 * hl + h, left) * rowb);
       if constexpr (!ANY) {
 #pragma unroll
         for (int gi = 0; gi < NGT; ++gi) {
-          const uint8_t *w = p + 4 * (gi * 4 * KSGT + g * KSGT);
+          const uint8_t *w = at + (row + 4 * KSGT * g + 16 * KSGT * gi);
           if constexpr (KSGT == 4) {
             const u32x4 x = *(const u32x4 *)w;
 #pragma unroll
@@ -174,19 +194,21 @@ k_q4_split(Q4Attn a) {
         for (int ks = 0; ks < KS; ++ks) {
           if (ks >= nks) break;
           const int w = word(ks);
-          kr[h][ks] = w >= 0 ? *(const uint32_t *)(p + 4 * w) : 0u;
+          kr[h][ks] = w >= 0 ? *(const uint32_t *)(at + (row + 4 * w)) : 0u;
         }
       }
     }
   };
   auto load_v = [&](int j) {
+    const uint8_t *const at = a.vc + (base + 64 * (size_t)j) * rowb;
+    const int left = a.T_cap - 1 - 64 * j;
     const int n16 = D / 32;  // 16-byte pieces a slot, and half a one where D is an odd multiple of 16
     if (!ANY || D % 32 == 0) {
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) {
         if (ANY && i >= n16) break;
         const int e = lane + 64 * i, tok = e / n16, c = e - tok * n16;
-        vr[i] = *(const u32x4 *)(a.vc + (base + min(64 * j + tok, a.T_cap - 1)) * rowb + 16 * c);
+        vr[i] = *(const u32x4 *)(at + (uint32_t)(min(tok, left) * rowb + 16 * c));
       }
     } else {
       const int n8 = D / 16;
@@ -196,7 +218,7 @@ k_q4_split(Q4Attn a) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int e = lane + 64 * (2 * i + u), tok = min(e / n8, 63), c = e - e / n8 * n8;
-          const u32x2 w = *(const u32x2 *)(a.vc + (base + min(64 * j + tok, a.T_cap - 1)) * rowb + 8 * c);
+          const u32x2 w = *(const u32x2 *)(at + (uint32_t)(min(tok, left) * rowb + 8 * c));
           x[2 * u] = w.x;
           x[2 * u + 1] = w.y;
         }
@@ -205,13 +227,14 @@ k_q4_split(Q4Attn a) {
     }
   };
   auto load_p = [&](int j) {
+    const size_t at = (base + 64 * (size_t)j) * NG;
+    const int last = (a.T_cap - 64 * j) * NG - 1;
 #pragma unroll
     for (int i = 0; i < NGM; ++i) {
       if (ANY && i >= NG) break;
-      const int e = lane + 64 * i, tok = e / NG;
-      const size_t at = (base + min(64 * j + tok, a.T_cap - 1)) * NG + (e - tok * NG);
-      pr[0][i] = a.kp[at];
-      pr[1][i] = a.vp[at];
+      const uint32_t e = (uint32_t)min(lane + 64 * i, last);
+      pr[0][i] = (a.kp + at)[e];
+      pr[1][i] = (a.vp + at)[e];
     }
   };
 
@@ -226,7 +249,7 @@ k_q4_split(Q4Attn a) {
   const int lim = r < R ? max(0, n - a.Tq + qt + 1) : 0, lim_all = n - a.Tq + 16 * rb / G + 1;  // (of every row)
 
   // q in the codes' order, and its sum over each group (as the codes stand, times 2^-24)
-  half8_t qh8[KS], ql8[KS];
+  half8_t qh8[KS], ql8[QSPLIT ? KS : 1];
   float qs[NGM];
   float qmul;
   {
@@ -235,7 +258,11 @@ k_q4_split(Q4Attn a) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int w = ANY && ks >= nks ? -1 : word(ks);
-      if (w >= 0) sf_load8_as_f32<QDT>(a.q, q0 + 8 * w, f[ks]);
+      if (w >= 0) {
+        if (a.qdt == SF_F32) sf_load8_as_f32<SF_F32>(a.q, q0 + 8 * w, f[ks]);
+        else if (a.qdt == SF_F16) sf_load8_as_f32<SF_F16>(a.q, q0 + 8 * w, f[ks]);
+        else sf_load8_as_f32<SF_BF16>(a.q, q0 + 8 * w, f[ks]);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         f[ks][i] = r < R && w >= 0 ? f[ks][i] : 0.f;
@@ -243,7 +270,9 @@ k_q4_split(Q4Attn a) {
       }
     }
     const float up = q4_fit14(max_x16_x32(top));
-    qmul = fminf(fmaxf(a.qscale / up * kCode, -3.0e38f), 3.0e38f);
+    qmul = a.qscale == 0.f ? 1.f : fminf(fmaxf(fabsf(a.qscale) / up * kCode, 1.0e-37f), 1.0e36f);
+    // (scores are compared before they are scaled: the scale's sign goes to q)
+    const float by = a.qscale < 0.f ? -up : a.qscale > 0.f ? up : 0.f;
 #pragma unroll
     for (int gi = 0; gi < NGM; ++gi) {
       float s = 0.f;
@@ -252,7 +281,7 @@ k_q4_split(Q4Attn a) {
         for (int ks = 0; ks < KS; ++ks)
           if (ks / KSG == gi)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += f[ks][i] * up;
+            for (int i = 0; i < 8; ++i) s += f[ks][i] * by;
       }
       qs[gi] = sum_x16_x32(s) * (1.f / kCode);
     }
@@ -260,20 +289,21 @@ k_q4_split(Q4Attn a) {
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float v = f[ks][(i >> 1) + 4 * (i & 1)] * up, part = !PSPLIT && (i >> 1) & 1 ? 0.0625f : 1.f;
+        const float v = f[ks][(i >> 1) + 4 * (i & 1)] * by, part = !PSPLIT && (i >> 1) & 1 ? 0.0625f : 1.f;
         const f16 hi = (f16)v;
         qh8[ks][i] = (f16)((float)hi * part);
-        ql8[ks][i] = (f16)((v - (float)hi) * part);
+        if constexpr (QSPLIT) ql8[ks][i] = (f16)((v - (float)hi) * part);
       }
   }
 
   uint8_t *const vt = smem + wave * kWave;
-  float *const kss = (float *)(vt + kTile), *const kos = kss + 64 * NGM;  // K's s and m, or m + 8 s
-  float *const vss = kos + 64 * NGM, *const vos = vss + 64 * NGM;  // V's s and m + 8 s
-  float *const vms = vos + 64 * NGM;  // a slot's largest V scale
-  float m = -INFINITY, lsum = 0.f;               // base-2 softmax of row r
-  float pmax = 0.f, pmul = 1.f;  // largest weight times V scale so far (as the weights stand), its factor
-  float am[NGM];                 // sum of p (m + 8 s) over the lane's slots
+  // parameters a group, slot 16 g + 4 i + h at 16 h + 4 g + i: K's s and m (m + 8 s), V's s and m + 8 s
+  float *const kss = (float *)(vt + kTile), *const kos = kss + 64 * NGM;
+  float *const vss = kos + 64 * NGM, *const vos = vss + 64 * NGM;
+  float *const vms = NGM > 1 ? vos + 64 * NGM : vss;  // a slot's largest V scale
+  float m = -INFINITY, lsum = 0.f;  // base-2 softmax of the column
+  float mul = 8.507059e37f;         // 2^126: the first tile sets it
+  float am[NGM];                    // sum of p (m + 8 s) over the lane's slots
   float4_t O[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) O[d] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -284,17 +314,20 @@ k_q4_split(Q4Attn a) {
     const int tb = 64 * j;
     const bool more = j + jstep < ntot;
     // parameters and V codes into the wave's LDS; slots past the length stand for zeros
+    if (tb + 64 > n) {
+#pragma unroll
+      for (int i = 0; i < NGM; ++i)
+        if ((lane + 64 * i) / NG + tb >= n) pr[0][i] = pr[1][i] = 0u;
+    }
 #pragma unroll
     for (int i = 0; i < NGM; ++i) {
       if (ANY && i >= NG) break;
       const int e = lane + 64 * i, tok = e / NG, gi = e - tok * NG;
-      const bool in = tb + tok < n;
-      const uint32_t k = in ? pr[0][i] : 0u;
-      kss[64 * gi + tok] = q4_lo(k);
-      kos[64 * gi + tok] = PSPLIT ? fmaf(8.f, q4_lo(k), q4_hi(k)) : q4_hi(k);
-      const uint32_t w = in ? pr[1][i] : 0u;
-      vss[64 * gi + tok] = q4_lo(w);
-      vos[64 * gi + tok] = fmaf(8.f, q4_lo(w), q4_hi(w));
+      const int to = 64 * gi + 16 * (tok & 3) + 4 * (tok >> 4) + (tok >> 2 & 3);
+      kss[to] = q4_lo(pr[0][i]);
+      kos[to] = PSPLIT ? fmaf(8.f, q4_lo(pr[0][i]), q4_hi(pr[0][i])) : q4_hi(pr[0][i]);
+      vss[to] = q4_lo(pr[1][i]);
+      vos[to] = fmaf(8.f, q4_lo(pr[1][i]), q4_hi(pr[1][i]));
     }
     if (!ANY || D % 32 == 0) {
       const int n16 = D / 32;
@@ -320,16 +353,16 @@ k_q4_split(Q4Attn a) {
       load_p(j + jstep);
       load_v(j + jstep);
     }
-    {
-      float v = 0.f;
+    if constexpr (NGM > 1) {
+      float v = vss[lane];
 #pragma unroll
-      for (int gi = 0; gi < NGM; ++gi)
+      for (int gi = 1; gi < NGM; ++gi)
         if (!ANY || gi < NG) v = fmaxf(v, vss[64 * gi + lane]);
       vms[lane] = v;
     }
-    float sc[16];  // value 4 h + i: slot tb + 16 g + 4 i + h
+    float sc[NV];  // value 4 hh + i: slot tb + 16 g + 4 i + h0 + hh
 #pragma unroll
-    for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+    for (int e = 0; e < NV; ++e) sc[e] = 0.f;
 #pragma unroll
     for (int gi = 0; gi < NGM; ++gi) {
       if (ANY && gi >= NG) break;
@@ -347,87 +380,101 @@ k_q4_split(Q4Attn a) {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4_t ks = *(const float4_t *)(kss + 64 * gi + 16 * g + 4 * i);
-        const float4_t ko = *(const float4_t *)(kos + 64 * gi + 16 * g + 4 * i);
+      for (int hh = 0; hh < HV; ++hh) {
+        const float4_t ks = *(const float4_t *)(kss + 64 * gi + 16 * (h0 + hh) + 4 * g);
+        const float4_t ko = *(const float4_t *)(kos + 64 * gi + 16 * (h0 + hh) + 4 * g);
 #pragma unroll
-        for (int h = 0; h < 4; ++h) sc[4 * h + i] = fmaf(ks[h], S[h][i], fmaf(ko[h], qs[gi], sc[4 * h + i]));
+        for (int i = 0; i < 4; ++i) {
+          float x = S[hh][i];
+          if constexpr (PK == 2) x = pg ? S[2 + hh][i] : x;
+          if constexpr (PK == 4) x = pg & 2 ? (pg & 1 ? S[3][i] : S[2][i]) : (pg & 1 ? S[1][i] : S[0][i]);
+          sc[4 * hh + i] = fmaf(ks[i], x, fmaf(ko[i], qs[gi], sc[4 * hh + i]));
+        }
       }
     }
     if (more) load_k(j + jstep);
     const bool masked = tb + 64 > lim_all;
-    const int left = lim - tb - 16 * g;  // the lane's slots 4 i + h < left
-    float mx = -INFINITY;
+    const int left = lim - tb - 16 * g - h0;  // the lane's slots 4 i + hh < left
+    if (masked) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      sc[e] *= qmul;
-      if (masked) sc[e] = 4 * (e & 3) + (e >> 2) < left ? sc[e] : -INFINITY;
-      mx = fmaxf(mx, sc[e]);
+      for (int e = 0; e < NV; ++e) sc[e] = 4 * (e & 3) + (e >> 2) < left ? sc[e] : -INFINITY;
     }
-    const float m_new = fmaxf(m, max_x16_x32(mx)), m_ref = m_new == -INFINITY ? 0.f : m_new;
-    const float c = __builtin_amdgcn_exp2f(m - m_ref);
-    m = m_new;
-    float ps = 0.f, pt = 0.f;
+    float mx = sc[0];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4_t v = *(const float4_t *)(vms + 16 * g + 4 * i);
+    for (int e = 1; e < NV; ++e) mx = fmaxf(mx, sc[e]);
+    mx *= qmul;
+    if (__any(mx > m + 8.f)) {
+      const float M = max_x16_x32(mx), m_new = M > m + 8.f ? M : m;
+      const float cf = __builtin_amdgcn_exp2f(m - sf_merge_mref(m_new));  // exp2(-inf) = 0
+      m = m_new;
+      lsum *= cf;
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        const int e = 4 * h + i;
-        sc[e] = __builtin_amdgcn_exp2f(sc[e] - m_ref);
-        ps += sc[e];
-        pt = fmaxf(pt, sc[e] * v[h]);
+      for (int gi = 0; gi < NGM; ++gi) am[gi] *= cf;
+#pragma unroll
+      for (int d = 0; d < DB; ++d) O[d] *= cf;
+    }
+    const float m_ref = sf_merge_mref(m);
+    float pt = 0.f;
+#pragma unroll
+    for (int hh = 0; hh < HV; ++hh) {
+      const float4_t v = *(const float4_t *)(vms + 16 * (h0 + hh) + 4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = 4 * hh + i;
+        sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], qmul, -m_ref));
+        lsum += sc[e];
+        pt = fmaxf(pt, sc[e] * v[i]);  // (0 or NaN, which counts for nothing, past a row's end)
       }
     }
-    lsum = fmaf(lsum, c, ps);
-    pmax = fmaxf(pmax * c, max_x16_x32(pt));
-    const float mul = q4_fit14(pmax), oc = c * mul / pmul;  // at most 2: pmax covers c times the last one
-    pmul = mul;
-    if (__any(oc != 1.f)) {
+    if (__any(pt * mul > 32768.f)) {
+      const float top = max_x16_x32(pt), was = mul;
+      mul = top * mul > 32768.f ? q4_fit14(top) : mul;
 #pragma unroll
-      for (int d = 0; d < DB; ++d) O[d] *= oc;
+      for (int d = 0; d < DB; ++d) O[d] *= mul / was;
     }
+    float pm[NV];
+#pragma unroll
+    for (int e = 0; e < NV; ++e) pm[e] = sc[e] * mul;
 #pragma unroll
     for (int gi = 0; gi < NGM; ++gi) {
       if (ANY && gi >= NG) break;
-      // P's operands: values (h, 0), (h, 1) of a register pair go with dword 0, (h, 2), (h, 3) with dword 1
+      // P's operands: values (h, 0), (h, 1) of a register pair go with dword 0, (h, 2), (h, 3) with
+      // dword 1; a column's registers of other h's hold zeros
       u32x4 ph[2], pl[2];
-      float acc = am[gi] * c;
-      float4_t vs[4], vo[4];
+      float acc = am[gi];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        vs[i] = *(const float4_t *)(vss + 64 * gi + 16 * g + 4 * i);
-        vo[i] = *(const float4_t *)(vos + 64 * gi + 16 * g + 4 * i);
+      for (int hh = 0; hh < HV; ++hh) {
+        float4_t vs = *(const float4_t *)(vss + 64 * gi + 16 * (h0 + hh) + 4 * g);
+        float4_t vo = *(const float4_t *)(vos + 64 * gi + 16 * (h0 + hh) + 4 * g);
         if (masked) {  // what lies past a row's end weighs exactly 0, whatever its parameters hold
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            vs[i][h] = 4 * i + h < left ? vs[i][h] : 0.f;
-            vo[i][h] = 4 * i + h < left ? vo[i][h] : 0.f;
+          for (int i = 0; i < 4; ++i) {
+            vs[i] = 4 * i + hh < left ? vs[i] : 0.f;
+            vo[i] = 4 * i + hh < left ? vo[i] : 0.f;
           }
         }
-      }
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
         float pv[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = sc[4 * h + i];
-          acc = fmaf(vo[i][h], p, acc);
-          pv[i] = vs[i][h] * (p * mul);
+          acc = fmaf(vo[i], sc[4 * hh + i], acc);
+          pv[i] = vs[i] * pm[4 * hh + i];
         }
-        uint32_t x, y;
-        q4_halves<PSPLIT>(pv[0], pv[1], x, y);
-        ph[0][h] = x;
-        pl[0][h] = y;
-        q4_halves<PSPLIT>(pv[2], pv[3], x, y);
-        ph[1][h] = x;
-        pl[1][h] = y;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint32_t x, y = 0u;
+          q4_halves<PSPLIT>(pv[2 * w], pv[2 * w + 1], x, y);
+#pragma unroll
+          for (int p = 0; p < PK; ++p) {
+            ph[w][HV * p + hh] = PK == 1 || pg == p ? x : 0u;
+            if constexpr (PSPLIT) pl[w][HV * p + hh] = PK == 1 || pg == p ? y : 0u;
+          }
+        }
       }
       am[gi] = acc;
       typedef int v2i __attribute__((ext_vector_type(2)));
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        if (ANY ? 16 * d < gi * a.g || 16 * d >= (gi + 1) * a.g : d / (2 * KSGT) != gi) continue;
+        if (ANY ? 16 * d < gi * a.g || 16 * d >= (gi + 1) * a.g : d / (2 * (KSGT ? KSGT : 1)) != gi) continue;
         const v2i vw = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
             (__attribute__((address_space(3))) v2i *)(vt + (16 * g + hl) * PITCH + 8 * d));
         const half8_t x0 = q4_signed(magic, (uint32_t)vw.x), x1 = q4_signed(magic, (uint32_t)vw.y);
@@ -444,7 +491,7 @@ k_q4_split(Q4Attn a) {
 #pragma unroll
   for (int gi = 0; gi < NGM; ++gi) am[gi] = sum_x16_x32(am[gi]);
 
-  // merge the wave states through LDS into the split's partial, or the output
+  // merge the waves' and columns' states through LDS into the split's partial, or the output
   __syncthreads();
   float *os = (float *)smem;  // [wave][16][OP]
   float *ms = (float *)(smem + kQaWaves * (kWave > kO ? kWave : kO)), *ls = ms + kQaWaves * 16;
@@ -452,7 +499,7 @@ k_q4_split(Q4Attn a) {
     ms[wave * 16 + hl] = m;
     ls[wave * 16 + hl] = lsum;
   }
-  const float un = 1.f / pmul;
+  const float un = 1.f / mul;
 #pragma unroll
   for (int d = 0; d < DB; ++d) {
     if (ANY && 16 * d >= D) break;
@@ -468,15 +515,15 @@ k_q4_split(Q4Attn a) {
     const int rr = e / nq, d4 = (e - rr * nq) * 4;
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kQaWaves; ++w) M = fmaxf(M, ms[w * 16 + rr]);
+    for (int w = 0; w < kQaWaves * PK; ++w) M = fmaxf(M, ms[w * RP + rr]);
     const float M_ref = sf_merge_mref(M);
     float L = 0.f;
     float4_t acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kQaWaves; ++w) {
-      const float wt = sf_merge_weight(ms[w * 16 + rr], M_ref);
-      L = fmaf(wt, ls[w * 16 + rr], L);
-      acc += *(const float4_t *)(os + (w * 16 + rr) * OP + d4) * wt;
+    for (int w = 0; w < kQaWaves * PK; ++w) {
+      const float wt = sf_merge_weight(ms[w * RP + rr], M_ref);
+      L = fmaf(wt, ls[w * RP + rr], L);
+      acc += *(const float4_t *)(os + (w * RP + rr) * OP + d4) * wt;
     }
     if (a.n_splits > 1) {
       const size_t row = (bk * R + 16 * rb + rr) * a.n_splits + split;
@@ -962,21 +1009,36 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
     }
 }
 
-// The many rows' launches take a call where their workgroups are enough to go round; their
-// workspace, or 0. (Where it would pass 2 GiB the splits' launches take it.)
+// The workspace of the many rows' launches where they take a call, else 0: a workgroup's walk
+// takes as long whatever the number of workgroups up to one a CU, the splits' launches as
+// much as the products. us, splits / many rows over 2000 slots, 32 / 8 heads of 128, bf16: 16
+// workgroups 31 / 43, 32 50 / 43, 64 70 / 44, fp32 32 61 / 92, 64 89 / 91, 128 132 / 100; 14 / 2
+// heads of 64, bf16: 56 20 / 30, 112 28 / 31, fp32 112 41 / 59. (Past 2 GiB the splits' take it.)
 size_t q4_many_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int parts) {
-  if ((D != 64 && D != 128) || (((long long)Tq * (H / KVH) + 127) / 128) * KVH * B < 64) return 0;
+  if (D != 64 && D != 128) return 0;
+  const long long blocks = (((long long)Tq * (H / KVH) + 127) / 128) * KVH * B;
+  if (blocks < (D == 64 ? 64 + 64 * parts : 32 * parts) || (long long)Tq * (H / KVH) < 64) return 0;
   const size_t tiles = (size_t)B * KVH * q4_tiles(T_max), bytes = tiles * (2 * q4_block_bytes(D, parts) + 8);
   return bytes > (size_t)1 << 31 ? 0 : bytes;
 }
 
-int q4_splits(int B, int Tq, int H, int KVH, int T_max, int D, int n_splits) {
-  const long long blocks = ((long long)Tq * (H / KVH) + 15) / 16;
+// The splits of a call: none up to 12 tiles; else a tile a wave, while one sequence's workgroups go
+// round the CUs once, several (ragged) sequences' as many as are resident at a time. us a call in
+// a replayed graph at the rule's count (others in parentheses), 32 / 8 heads of 128, groups of 64:
+// 500 slots 9.6 (1; 2: 10.7, 8: 9.9), 8191 11.1 (32; 16: 12.5, 64: 13.6), four ragged sequences up
+// to 32767 33.5 (24; 8: 42.8, 16: 34.6, 48: 37.7), sixteen up to 4001 with fp32 queries 23.7 (4; 6:
+// 28.3, 12: 32.0), eight up to 1000 13.1 (5; 1: 12.8, 4: 11.1, 8: 12.5); 131071 slots in groups of
+// 128 31.9 (32; 16: 52.0, 96: 36.0); 14 / 2 heads of 64, 1501 slots 8.9 (6; 1: 11.3, 24: 8.7), 16384
+// 9.1 (64; 16: 12.1, 128: 10.2); 40 / 2 heads of 128 in groups of 32, two up to 20000 21.8 (32; 16:
+// 28.9, 48: 30.1).
+int q4_splits(int B, int Tq, int H, int KVH, int T_max, int D, int group, bool split_q, int n_splits) {
+  const int R = Tq * (H / KVH), PK = R <= 4 ? 4 : R <= 8 ? 2 : 1, tiles = (T_max + 63) / 64;
+  const int groups = (D == 64 || D == 128) ? D / group : 0;
+  const long long heads = (long long)B * KVH * (PK > 1 ? 1 : (R + 15) / 16);
   if (n_splits <= 0) {
-    const long long kb = KVH * blocks;
-    n_splits = kb * B >= 1024 ? 1 : sf_attn_default_splits_d(B, (int)kb, T_max, D);
+    const long long most = (B == 1 ? 256LL : 256LL * q4_resident(D, groups, PK, split_q)) / heads;
+    n_splits = tiles <= 12 ? 1 : (int)((tiles + 3) / 4 < most ? (tiles + 3) / 4 : most);
   }
-  const int tiles = (T_max + 63) / 64;
   if (n_splits > tiles) n_splits = tiles;
   return n_splits > kQaMaxSplits ? kQaMaxSplits : n_splits < 1 ? 1 : n_splits;
 }
@@ -988,11 +1050,13 @@ size_t q4_parts(long long rows, int D, int S, size_t *ml_off) {
 
 }  // namespace
 
-extern "C" size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int out_dtype, int n_splits) {
-  if (B <= 0 || Tq <= 0 || H <= 0 || KVH <= 0 || H % KVH || T_max < 0 || T_max > kQaMaxSlots || D <= 0) return 0;
+extern "C" size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int group, int q_dtype,
+                                             int out_dtype, int n_splits) {
+  if (B <= 0 || Tq <= 0 || H <= 0 || KVH <= 0 || H % KVH || T_max < 0 || T_max > kQaMaxSlots || D <= 0 || group <= 0) return 0;
   size_t ml;
   if (const size_t many = q4_many_bytes(B, Tq, H, KVH, T_max, D, out_dtype == SF_BF16 ? 1 : 2)) return many;
-  return q4_parts((long long)B * Tq * H, D, q4_splits(B, Tq, H, KVH, T_max, D, n_splits), &ml);
+  return q4_parts((long long)B * Tq * H, D, q4_splits(B, Tq, H, KVH, T_max, D, group, out_dtype != SF_BF16 && q_dtype == SF_F32, n_splits),
+                  &ml);
 }
 
 extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, const void *k_params,
@@ -1016,7 +1080,7 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   SF_REQUIRE(q && k_codes && k_params && v_codes && v_params && out, SF_EINVAL, "null pointer argument");
   SF_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_params | (uintptr_t)v_params | (uintptr_t)q) & 15) == 0,
              SF_EINVAL, "q and cache buffers must be 16-byte aligned");
-  n_splits = many ? 1 : q4_splits(B, Tq, H, KVH, T_max, D, n_splits);
+  n_splits = many ? 1 : q4_splits(B, Tq, H, KVH, T_max, D, group, out_dtype != SF_BF16 && q_dtype == SF_F32, n_splits);
   size_t ml_off;
   const size_t parts = q4_parts(rows, D, n_splits, &ml_off), need = many ? many : parts;
   SF_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0), SF_EINVAL, "workspace must be 256-byte aligned");
@@ -1024,7 +1088,7 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   float *acc = (float *)workspace, *ml = (float *)((char *)workspace + ml_off);
   hipStream_t st = (hipStream_t)stream;
   const Q4Attn a = {q, k_codes, v_codes, (const uint32_t *)k_params, (const uint32_t *)v_params, out, acc, ml, lengths,
-                    out_dtype, T, T_max, T_cap, Tq, H, KVH, D, group, n_splits, 0,
+                    q_dtype, out_dtype, T, T_max, T_cap, Tq, H, KVH, D, group, n_splits, 0,
                     scale * 1.4426950408889634f};  // softmax in base 2
   if (many) {
     const unsigned blocks = (unsigned)((long long)B * KVH * (((long long)Tq * (H / KVH) + 127) / 128));
@@ -1066,27 +1130,29 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
     return sf_check_launch("sf_attn_q4kv");
   }
   const dim3 grid(n_splits, (unsigned)(KVH * nrb), B);
-#define SF_QA(QD, PS, DP, NG, KSG) k_q4_split<QD, PS, DP, NG, KSG><<<grid, kQaThreads, 0, st>>>(a)
-#define SF_QA_D(QD, PS)                                  \
-  do {                                                   \
-    if (D == 64 && group == 64) SF_QA(QD, PS, 64, 1, 2); \
-    else if (D == 64 && group == 32) SF_QA(QD, PS, 64, 2, 1);    \
-    else if (D == 128 && group == 128) SF_QA(QD, PS, 128, 1, 4); \
-    else if (D == 128 && group == 64) SF_QA(QD, PS, 128, 2, 2);  \
-    else if (D == 128 && group == 32) SF_QA(QD, PS, 128, 4, 1);  \
-    else if (D <= 128) SF_QA(QD, PS, 128, 0, 0);         \
-    else SF_QA(QD, PS, 256, 0, 0);                       \
+  const int R = Tq * (H / KVH);
+#define SF_QA(QS, PS, DP, NG, KSG, PK) k_q4_split<QS, PS, DP, NG, KSG, PK><<<grid, kQaThreads, 0, st>>>(a)
+#define SF_QA_R(QS, PS, DP, NG, KSG)               \
+  do {                                             \
+    if (R <= 4) SF_QA(QS, PS, DP, NG, KSG, 4);     \
+    else if (R <= 8) SF_QA(QS, PS, DP, NG, KSG, 2); \
+    else SF_QA(QS, PS, DP, NG, KSG, 1);            \
   } while (0)
-#define SF_QA_O(QD)                             \
-  do {                                          \
-    if (out_dtype == SF_BF16) SF_QA_D(QD, false); \
-    else SF_QA_D(QD, true);                     \
+#define SF_QA_D(QS, PS)                                       \
+  do {                                                        \
+    if (D == 64 && group == 64) SF_QA_R(QS, PS, 64, 1, 2);    \
+    else if (D == 64 && group == 32) SF_QA_R(QS, PS, 64, 2, 1);    \
+    else if (D == 128 && group == 128) SF_QA_R(QS, PS, 128, 1, 4); \
+    else if (D == 128 && group == 64) SF_QA_R(QS, PS, 128, 2, 2);  \
+    else if (D == 128 && group == 32) SF_QA_R(QS, PS, 128, 4, 1);  \
+    else if (D <= 128) SF_QA(QS, PS, 128, 0, 0, 1);           \
+    else SF_QA(QS, PS, 256, 0, 0, 1);                         \
   } while (0)
-  if (q_dtype == SF_F32) SF_QA_O(SF_F32);
-  else if (q_dtype == SF_F16) SF_QA_O(SF_F16);
-  else SF_QA_O(SF_BF16);
-#undef SF_QA_O
+  if (out_dtype == SF_BF16) SF_QA_D(false, false);  // (a bf16 output leaves out the low parts of fp32 queries too)
+  else if (q_dtype == SF_F32) SF_QA_D(true, true);
+  else SF_QA_D(false, true);
 #undef SF_QA_D
+#undef SF_QA_R
 #undef SF_QA
   if (n_splits > 1) k_q4_merge<<<(unsigned)rows, kQaThreads, 0, st>>>(acc, ml, out, out_dtype, Tq, H, KVH, D, n_splits);
   return sf_check_launch("sf_attn_q4kv");

@@ -142,9 +142,10 @@ def dequantize_kv_q4(codes: torch.Tensor, params: torch.Tensor, dtype: torch.dty
 
 
 @functools.lru_cache(maxsize=256)
-def _attention_bytes(B: int, Tq: int, H: int, KVH: int, T_max: int, D: int, out: int, n: int) -> int:
+def _attention_bytes(B: int, Tq: int, H: int, KVH: int, T_max: int, D: int, g: int, dt: int, out: int,
+                     n: int) -> int:
     """sf_attn_q4_workspace_bytes of a shape."""
-    return int(_lib.load().sf_attn_q4_workspace_bytes(B, Tq, H, KVH, T_max, D, out, n))
+    return int(_lib.load().sf_attn_q4_workspace_bytes(B, Tq, H, KVH, T_max, D, g, dt, out, n))
 
 
 def attention_q4kv(q: torch.Tensor, k_codes: torch.Tensor, k_params: torch.Tensor, v_codes: torch.Tensor,
@@ -185,7 +186,7 @@ def attention_q4kv(q: torch.Tensor, k_codes: torch.Tensor, k_params: torch.Tenso
     lib = _lib.load()
     with _lib.on_device(q):
         st = _lib.stream(q)
-        need = _attention_bytes(B, Tq, H, KVH, T_max, D, _lib.dt(out), n)
+        need = _attention_bytes(B, Tq, H, KVH, T_max, D, g, _lib.dt(q), _lib.dt(out), n)
         ws = _lib.scratch(q.device, st, need) if need else None
         rc = lib.sf_attn_q4kv(
             q.data_ptr(), _lib.dt(q), k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), g,

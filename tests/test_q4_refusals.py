@@ -120,10 +120,10 @@ def test_nothing_to_do_is_no_error():
 
 def test_sizes():
     lib = _lib.load()
-    assert lib.sf_attn_q4_workspace_bytes(1, 1, 14, 2, 64, 64, F32, 0) == 0  # one tile: no partials
-    assert lib.sf_attn_q4_workspace_bytes(1, 1, 14, 2, 6400, 64, F32, 3) == 14 * 3 * 64 * 4 + 14 * 3 * 8
-    assert lib.sf_attn_q4_workspace_bytes(1, 1, 14, 2, 1 << 20, 64, F32, 1000) == 14 * 128 * 64 * 4 + 14 * 128 * 8
-    assert lib.sf_attn_q4_workspace_bytes(1, 1, 14, 3, 64, 64, F32, 0) == 0
+    assert lib.sf_attn_q4_workspace_bytes(1, 1, 14, 2, 64, 64, 64, F32, F32, 0) == 0  # one tile: no partials
+    assert lib.sf_attn_q4_workspace_bytes(1, 1, 14, 2, 6400, 64, 64, F32, F32, 3) == 14 * 3 * 64 * 4 + 14 * 3 * 8
+    assert lib.sf_attn_q4_workspace_bytes(1, 1, 14, 2, 1 << 20, 64, 64, F32, F32, 1000) == 14 * 128 * 64 * 4 + 14 * 128 * 8
+    assert lib.sf_attn_q4_workspace_bytes(1, 1, 14, 3, 64, 64, 64, F32, F32, 0) == 0
     assert lib.sf_qk_norm_backward_workspace_bytes(1, 1, 14, 2, 64) > 0
 
 
