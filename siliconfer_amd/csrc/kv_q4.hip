@@ -35,8 +35,10 @@ struct Q4Append {
   uint8_t *kc, *vc;
   uint32_t *kp, *vp;      // (s, m)
   const int *lengths;     // or null: start for every sequence
-  int start, q_dtype, w_dtype, H, KVH, D, g, T, T_cap, P, interleaved, lanes_log2, n_heads;
+  int start, q_dtype, w_dtype, H, KVH, D, g, g_log2, groups, T, T_cap, P, lanes_log2, n_heads, chunks;
+  uint32_t inv_heads, inv_T, inv_P;  // for div_by
   float eps, scale;
+  double inv_D;
 };
 
 __device__ __forceinline__ double q4_load(const void *p, int dt, size_t i) {
@@ -54,9 +56,12 @@ __device__ __forceinline__ double q4_swap16(double v) {
   const uint64_t u = sf_bitcast<uint64_t>(v);
   return sf_bitcast<double>((uint64_t)(uint32_t)__shfl_xor((int)(u >> 32), 16, 64) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)u, 16, 64));
 }
+template <int CTRL>
+__device__ __forceinline__ float q4_dpp(float v) { return sf_dpp<CTRL>(v); }
+__device__ __forceinline__ float q4_swap16(float v) { return __shfl_xor(v, 16, 64); }
 // f over aligned groups of n lanes (n = 2 .. 32, uniform); every lane gets the result.
-template <class F>
-__device__ __forceinline__ double q4_over(double v, int n, F f) {
+template <class V, class F>
+__device__ __forceinline__ V q4_over(V v, int n, F f) {
   v = f(v, q4_dpp<0xB1>(v));
   if (n > 2) v = f(v, q4_dpp<0x4E>(v));
   if (n > 4) v = f(v, q4_dpp<0x141>(v));
@@ -65,140 +70,210 @@ __device__ __forceinline__ double q4_over(double v, int n, F f) {
   return v;
 }
 
-// PAIR8: a lane's partners in the rotation are 8 neighbouring dims of the head (or its own).
-template <int DT, bool PAIR8>
+// PAIR8: a lane's partners in the rotation are 8 neighbouring dims of the head (INTER: its own).
+// Bound by vector instructions: 4095 rows of 32 / 8 heads of 128, bf16, groups of 64, normed and
+// turned, 88 MB (17 us at a copy's rate) in 43 us: 60.8 with divisions for the head, the row, the
+// scale's inverse and the root and every code's remainder settled, 53 with the tables in the
+// dims' order (a head's lanes on the same banks).
+template <int DT, bool PAIR8, bool INTER>
 __global__ void __launch_bounds__(kQ4Threads)
 k_kv_q4_append(Q4Append a, RotaryPos pos, const double *__restrict__ inv_freq) {
   extern __shared__ __attribute__((aligned(16))) double q4_smem[];
   const int D = a.D, P = a.P, heads = a.H + 2 * a.KVH, hb = kQ4Threads >> a.lanes_log2, L = 1 << a.lanes_log2;
   double *const ws = q4_smem;                                  // [2][D] norm weights
   double2 *const cs = (double2 *)(q4_smem + (a.qw || a.kw ? 2 * D : 0));  // [rows][P]
-  const int first = blockIdx.x * hb, last = min(first + hb, a.n_heads) - 1;
+  // The workgroup's first head, row and token by (uniform) divisions, a lane's by what it is past
+  // them; a.chunks times hb heads, the next ones' rows loaded during the last ones' arithmetic.
+  const int first = blockIdx.x * hb * a.chunks, row0 = first / heads, off0 = first - row0 * heads;
+  const int b0 = row0 / a.T, t0 = row0 - b0 * a.T;
+  const int count = min(hb * a.chunks, a.n_heads - first);
   const int slot = threadIdx.x >> a.lanes_log2, i = threadIdx.x & (L - 1);
-  const int row0 = first / heads, rows = last / heads - row0 + 1;
-  const int e = min(first + slot, last), row = e / heads, hh = e - row * heads, b = row / a.T, t = row - b * a.T;
-  const bool live = first + slot <= last && 8 * i < D, is_q = hh < a.H, is_v = hh >= a.H + a.KVH;
-  const Q4Rows &x = is_q ? a.q : is_v ? a.v : a.k;
-  const int h = is_q ? hh : is_v ? hh - a.H - a.KVH : hh - a.H;
-  const size_t src = (size_t)(b * x.sb + t * x.st + h * x.sh);
+  const int rows = div_by(off0 + count - 1, a.inv_heads) + 1;
+  // (a row's token: rows of a workgroup are few, so that past 2^15 tokens one sequence at most ends among them)
+  auto token = [&](int r, int &b, int &t) {
+    const int x = t0 + r, n = a.T < 32768 ? div_by(x, a.inv_T) : x >= a.T;
+    b = b0 + n;
+    t = x - n * a.T;
+  };
+  const bool in = 8 * i < D, normed = a.qw || a.kw;
   const int d0 = 8 * min(i, D / 8 - 1);
-  const void *const w = is_q ? a.qw : is_v ? nullptr : a.kw;
-  const int wo = is_q ? 0 : D;
-  // dims d0 .. + 7 and the dims that turn with them
-  float own[8], oth[8];
-  const bool turns = !is_v && (PAIR8 ? d0 < 2 * P : true);
-  auto partner = [&](int d) { return d >= 2 * P ? d : a.interleaved ? d ^ 1 : d < P ? d + P : d - P; };
-  sf_load8_as_f32<DT>(x.x, src + d0, own);
-  if constexpr (PAIR8) {
-    if (!a.interleaved && turns) sf_load8_as_f32<DT>(x.x, src + partner(d0), oth);
-  } else {
+  const bool second = d0 >= P;
+  // a lane's j-th weight and pair lie beside its neighbours' j-th: 8 dims a lane in order would have
+  // every lane of a head read the same banks
+  const int oct = D / 8, pairs = INTER ? P / 4 : P / 8;
+  auto weight_at = [&](int d) { return (d & 7) * oct + (d >> 3); };
+  auto pair_at = [&](int p) { return !PAIR8 ? p : INTER ? (p & 3) * pairs + (p >> 2) : (p & 7) * pairs + (p >> 3); };
+  auto partner = [&](int d) { return d >= 2 * P ? d : INTER ? d ^ 1 : d < P ? d + P : d - P; };
+  const int p0 = second ? d0 - P : d0 + P;  // (PAIR8, half layout)
+  // a lane's head, and its dims d0 .. + 7 and those that turn with them
+  struct Head {
+    int dr, b, t, h;
+    bool is_q, is_v, live;
+    float own[8], oth[8];
+  };
+  auto take = [&](int u, Head &x) {
+    const int past = off0 + min(u * hb + slot, count - 1);
+    x.dr = div_by(past, a.inv_heads);
+    const int hh = past - x.dr * heads;
+    token(x.dr, x.b, x.t);
+    x.live = u * hb + slot < count && in;
+    x.is_q = hh < a.H;
+    x.is_v = hh >= a.H + a.KVH;
+    x.h = x.is_q ? hh : x.is_v ? hh - a.H - a.KVH : hh - a.H;
+    const Q4Rows &s = x.is_q ? a.q : x.is_v ? a.v : a.k;
+    const size_t src = (size_t)(x.b * s.sb + x.t * s.st + x.h * s.sh);
+    sf_load8_as_f32<DT>(s.x, src + d0, x.own);
+    if constexpr (!PAIR8) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) oth[j] = is_v ? 0.f : sf_load_as_f32<DT>(x.x, src + partner(d0 + j));
-  }
-  if (a.qw || a.kw)
+      for (int j = 0; j < 8; ++j) x.oth[j] = x.is_v ? 0.f : sf_load_as_f32<DT>(s.x, src + partner(d0 + j));
+    } else if constexpr (!INTER) {
+      if (!x.is_v && d0 < 2 * P) sf_load8_as_f32<DT>(s.x, src + p0, x.oth);
+    }
+  };
+  Head nxt;
+  take(0, nxt);
+  if (normed)
     for (int d = threadIdx.x; d < 2 * D; d += kQ4Threads) {
       const void *p = d < D ? a.qw : a.kw;
-      ws[d] = p ? q4_load(p, a.w_dtype, d < D ? d : d - D) : 1.0;
+      ws[d < D ? weight_at(d) : D + weight_at(d - D)] = p ? q4_load(p, a.w_dtype, d < D ? d : d - D) : 1.0;
     }
-  for (int n = threadIdx.x; n < rows * P; n += kQ4Threads) {
-    const int r = n / P, rw = row0 + r, rb = rw / a.T;
-    double c, s;
-    rotary_sincos<true>((double)pos.at(rb, rw - rb * a.T) * inv_freq[n - r * P], c, s);
-    cs[n] = double2{a.scale * c, a.scale * s};
-  }
+  if (off0 < a.H + a.KVH || rows > 1)  // (v's heads alone need none)
+    for (int n = threadIdx.x; n < rows * P; n += kQ4Threads) {
+      const int r = div_by(n, a.inv_P), pr = n - r * P;
+      int rb, rt;
+      token(r, rb, rt);
+      double c, s;
+      rotary_sincos<true>((double)pos.at(rb, rt) * inv_freq[pr], c, s);
+      cs[r * P + pair_at(pr)] = double2{a.scale * c, a.scale * s};
+    }
   __syncthreads();
 
-  double y[8];
+#pragma unroll 1
+  for (int u = 0; u * hb < count; ++u) {
+    const Head x = nxt;
+    if ((u + 1) * hb < count) take(u + 1, nxt);
+    const int b = x.b, t = x.t, h = x.h;
+    const bool turns = !x.is_v && (PAIR8 ? d0 < 2 * P : true);
+    const void *const w = x.is_q ? a.qw : x.is_v ? nullptr : a.kw;
+    const double *const wo = ws + (x.is_q ? 0 : D);
+    double y[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = own[j];
-  double r = 1.0;
-  if (a.qw || a.kw) {
-    double ss = 0.0;
+    for (int j = 0; j < 8; ++j) y[j] = x.own[j];
+    double r = 1.0;
+    if (normed) {
+      double ss = 0.0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fma(y[j], y[j], ss);
-    ss = q4_over(8 * i < D ? ss : 0.0, L, [](double p, double q) { return p + q; });
-    if (w) {
-      r = 1.0 / sqrt(ss / D + (double)a.eps);
+      for (int j = 0; j < 8; ++j) ss = fma(y[j], y[j], ss);
+      ss = q4_over(in ? ss : 0.0, L, [](double p, double q) { return p + q; });
+      if (w) {
+        // 1 / sqrt by the hardware's estimate and two steps of Newton's, to 2^-52
+        const double v = ss * a.inv_D + (double)a.eps;
+        r = __builtin_amdgcn_rsq(v);
+        r = fma(fma(-v * r, r, 1.0), 0.5 * r, r);
+        r = fma(fma(-v * r, r, 1.0), 0.5 * r, r);
+        r = v == 0.0 ? (double)INFINITY : v == (double)INFINITY ? 0.0 : r;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = y[j] * r * ws[wo + d0 + j];
-    }
-  }
-  if (turns) {
-    double z[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (PAIR8 && a.interleaved) {
-        z[j] = y[j ^ 1];
-      } else {
-        z[j] = oth[j];
-        if (w) z[j] = z[j] * r * ws[wo + partner(d0 + j)];
+        for (int j = 0; j < 8; ++j) y[j] = y[j] * r * wo[j * oct + d0 / 8];
       }
     }
-    const double2 *c = cs + (row - row0) * P;
+    if (turns) {
+      const double2 *const c = cs + x.dr * P;
+      if constexpr (PAIR8 && INTER) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const double2 cj = c[(j >> 1) * pairs + d0 / 8];
+          const double lo = fma(y[j], cj.x, -y[j + 1] * cj.y), hi = fma(y[j + 1], cj.x, y[j] * cj.y);
+          y[j] = lo;
+          y[j + 1] = hi;
+        }
+      } else if constexpr (PAIR8) {
+        const double turn = second ? r : -r;
+        const double2 *const cp = c + (second ? d0 - P : d0) / 8;
+        double z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = x.oth[j] * turn;
+        if (w) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) z[j] *= wo[j * oct + p0 / 8];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = fma(y[j], cp[j * pairs].x, z[j] * cp[j * pairs].y);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int d = d0 + j;
+          if (d >= 2 * P) continue;
+          double z = x.oth[j] * r;
+          if (w) z *= wo[weight_at(partner(d))];
+          const bool two = INTER ? d & 1 : d >= P;
+          const double2 cj = c[INTER ? d >> 1 : two ? d - P : d];
+          y[j] = fma(y[j], cj.x, two ? z * cj.y : -z * cj.y);
+        }
+      }
+    }
+    if (x.is_q) {
+      if (!x.live) continue;
+      const size_t o = (((size_t)b * a.T + t) * a.H + h) * D + d0;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = (float)y[j];
+      if (a.q_dtype == SF_F32) {
+        float4_t *p = (float4_t *)((float *)a.q_out + o);
+        p[0] = float4_t{f[0], f[1], f[2], f[3]};
+        p[1] = float4_t{f[4], f[5], f[6], f[7]};
+      } else {
+        uint32_t u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = a.q_dtype == SF_BF16 ? sf_f32_to_bf16(f[j]) : sf_bitcast<uint16_t>((f16)sf_opaque(f[j]));
+        *(u32x4 *)((uint16_t *)a.q_out + o) = u32x4{u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16};
+      }
+      continue;
+    }
+    // k or v: the group's range over its lanes (the head's lanes past its dims stand aside)
+    double lo = y[0], hi = y[0], all = 0.0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int d = d0 + j;
-      if (!PAIR8 && d >= 2 * P) continue;
-      const bool second = a.interleaved ? d & 1 : d >= P;
-      const double2 cj = c[a.interleaved ? d >> 1 : second ? d - P : d];
-      y[j] = fma(y[j], cj.x, second ? z[j] * cj.y : -z[j] * cj.y);
+      lo = fmin(lo, y[j]);
+      hi = fmax(hi, y[j]);
+      all = fma(y[j], 0.0, all);  // NaN where a value is not finite: the group reads back as NaN
     }
-  }
-  if (is_q) {
-    if (!live) return;
-    const size_t o = ((size_t)row * a.H + h) * D + d0;
-    float f[8];
+    const int GL = a.g == D ? L : a.g / 8;
+    lo = q4_over(in ? lo : (double)INFINITY, GL, [](double p, double q) { return fmin(p, q); });
+    hi = q4_over(in ? hi : -(double)INFINITY, GL, [](double p, double q) { return fmax(p, q); });
+    const bool bad = q4_over(in && all != 0.0 ? 1.f : 0.f, GL, [](float p, float q) { return fmaxf(p, q); }) != 0.f;
+    // (to fp32 first, as a conversion through fp32 would have it; held within fp16's range. A
+    // product with 1 / 15 is the quotient but for its last place in 64 bits, which fp32 drops.)
+    const float lof = sf_opaque((float)lo), stf = sf_opaque((float)((hi - lo) * (1.0 / 15.0)));
+    f16 m16 = (f16)fminf(fmaxf(lof, -65504.f), 65504.f), s16 = (f16)fminf(stf, 65504.f);
+    const double m = (double)m16, s = (double)s16, half = 0.5 * s;
+    const double inv = s > 0.0 ? __builtin_amdgcn_rcp(s) : 0.0;  // (an estimate: the remainders tell)
+    double c[8];
+    bool off = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = (float)y[j];
-    if (a.q_dtype == SF_F32) {
-      float4_t *p = (float4_t *)((float *)a.q_out + o);
-      p[0] = float4_t{f[0], f[1], f[2], f[3]};
-      p[1] = float4_t{f[4], f[5], f[6], f[7]};
-    } else {
-      uint32_t u[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = a.q_dtype == SF_BF16 ? sf_f32_to_bf16(f[j]) : sf_bitcast<uint16_t>((f16)sf_opaque(f[j]));
-      *(u32x4 *)((uint16_t *)a.q_out + o) = u32x4{u[0] | u[1] << 16, u[2] | u[3] << 16, u[4] | u[5] << 16, u[6] | u[7] << 16};
+    for (int j = 0; j < 8; ++j) {
+      const double d = y[j] - m;
+      c[j] = rint(d * inv);
+      off = off || fabs(fma(-c[j], s, d)) >= half;
     }
-    return;
-  }
-  // k or v: the group's range over its lanes (the head's lanes past its dims stand aside)
-  const bool in = 8 * i < D;
-  double lo = y[0], hi = y[0];
-  bool bad = false;  // a value that is not finite: the group reads back as NaN
+    if (__any(off)) {  // a border, or a tie, which belongs to the even code
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    lo = fmin(lo, y[j]);
-    hi = fmax(hi, y[j]);
-    bad = bad || !(fabs(y[j]) < INFINITY);
-  }
-  const int GL = a.g == D ? L : a.g / 8;
-  lo = q4_over(in ? lo : (double)INFINITY, GL, [](double p, double q) { return fmin(p, q); });
-  hi = q4_over(in ? hi : -(double)INFINITY, GL, [](double p, double q) { return fmax(p, q); });
-  bad = q4_over(in && bad ? 1.0 : 0.0, GL, [](double p, double q) { return fmax(p, q); }) != 0.0;
-  // (to fp32 first, as a conversion through fp32 would have it; held within fp16's range)
-  const float lof = sf_opaque((float)lo), stf = sf_opaque((float)((hi - lo) / 15.0));
-  f16 m16 = (f16)fminf(fmaxf(lof, -65504.f), 65504.f), s16 = (f16)fminf(stf, 65504.f);
-  const double m = (double)m16, s = (double)s16, inv = s > 0.0 ? 1.0 / s : 0.0, half = 0.5 * s;
-  uint32_t codes = 0;
+      for (int j = 0; j < 8; ++j) {
+        const double rem = fma(-c[j], s, y[j] - m), odd = c[j] - 2.0 * floor(0.5 * c[j]);
+        if (s > 0.0) c[j] += rem > half || (rem == half && odd != 0.0) ? 1.0 : rem < -half || (rem == -half && odd != 0.0) ? -1.0 : 0.0;
+      }
+    }
+    uint32_t codes = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const double d = y[j] - m;
-    double c = fmin(fmax(rint(d * inv), 0.0), 15.0);
-    // the remainder says whether a border, or a tie that belongs to the even code, was missed
-    const double rem = fma(-c, s, d);
-    const bool odd = (int)c & 1;
-    c += (rem > half || (rem == half && odd)) && s > 0.0 ? 1.0 : 0.0;
-    c -= (rem < -half || (rem == -half && odd)) && s > 0.0 ? 1.0 : 0.0;
-    codes |= (uint32_t)fmin(fmax(c, 0.0), 15.0) << (4 * j);
-  }
-  const long long len = a.lengths ? a.lengths[b] : a.start, at = len + t;
-  if (!live || len < 0 || at >= a.T_cap) return;  // no such slot: nothing is written
-  const size_t crow = ((size_t)b * a.KVH + h) * a.T_cap + (size_t)at;
-  *(uint32_t *)((is_v ? a.vc : a.kc) + crow * (D / 2) + d0 / 2) = bad ? 0u : codes;
-  if (d0 % a.g == 0) {
-    const uint32_t word = sf_bitcast<uint16_t>(s16) | (uint32_t)sf_bitcast<uint16_t>(m16) << 16;
-    (is_v ? a.vp : a.kp)[crow * (D / a.g) + d0 / a.g] = bad ? 0x7e007e00u : word;
+    for (int j = 0; j < 8; ++j) codes |= (uint32_t)fmin(fmax(c[j], 0.0), 15.0) << (4 * j);
+    const long long len = a.lengths ? a.lengths[b] : a.start, at = len + t;
+    if (!x.live || len < 0 || at >= a.T_cap) continue;  // no such slot: nothing is written
+    const size_t crow = ((size_t)b * a.KVH + h) * a.T_cap + (size_t)at;
+    *(uint32_t *)((x.is_v ? a.vc : a.kc) + crow * (D / 2) + d0 / 2) = bad ? 0u : codes;
+    const int gi = a.g == D ? 0 : d0 >> a.g_log2;
+    if (d0 == gi * a.g) {
+      const uint32_t word = sf_bitcast<uint16_t>(s16) | (uint32_t)sf_bitcast<uint16_t>(m16) << 16;
+      (x.is_v ? a.vp : a.kp)[crow * a.groups + gi] = bad ? 0x7e007e00u : word;
+    }
   }
 }
 
@@ -261,6 +336,7 @@ extern "C" int sf_kv_q4_append(const void *q, const void *k, const void *v, int 
              "KV cache overflow: %d + %d > capacity %d", start, T, T_cap);
   const long long n_heads = (long long)B * T * (H + 2LL * KVH);
   SF_REQUIRE(n_heads <= 0x7fffffffLL - 65536, SF_EINVAL, "%d x %d rows of %d heads exceed the grid", B, T, H + 2 * KVH);
+  SF_REQUIRE(H <= 16384 && KVH <= 8192, SF_EUNSUPPORTED, "%d and %d heads: at most 16384 and 8192", H, KVH);
   if (n_heads == 0) return SF_OK;
   SF_REQUIRE(k && v && strides && (H == 0 || (q && q_out)) && k_codes && k_params && v_codes && v_params &&
                  (rot_pairs == 0 || (positions && inv_freq)),
@@ -273,23 +349,34 @@ extern "C" int sf_kv_q4_append(const void *q, const void *k, const void *v, int 
              "cache buffers must be 16-byte aligned");
   Q4Append a = {{q, s[0], s[1], s[2]}, {k, s[3], s[4], s[5]}, {v, s[6], s[7], s[8]}, q_weight, k_weight, q_out, k_codes,
                 v_codes, (uint32_t *)k_params, (uint32_t *)v_params, lengths, start, q_dtype, weight_dtype, H, KVH, D,
-                group, T, T_cap, rot_pairs, interleaved, 1, (int)n_heads, eps, scale};
+                group, 5, D / group, T, T_cap, rot_pairs, 1, (int)n_heads, 1, div_inv(H + 2 * KVH), div_inv(T),
+                rot_pairs ? div_inv(rot_pairs) : 0, eps, scale, 1.0 / D};
+  while ((1 << a.g_log2) < group) ++a.g_log2;
   while ((8 << a.lanes_log2) < D) ++a.lanes_log2;
-  const int hb = kQ4Threads >> a.lanes_log2, heads = H + 2 * KVH, rows = (hb + heads - 2) / heads + 1;
+  // Four times the heads that a workgroup's threads hold, where that leaves four workgroups a CU: its
+  // weights and table serve as many (4095 rows of the above and reading them back, us: one 67.1, two
+  // 59.6, four 57.6, eight 58.1).
+  const int hb = kQ4Threads >> a.lanes_log2, heads = H + 2 * KVH;
+  a.chunks = n_heads >= 4LL * hb * 1024 ? 4 : 1;
+  const int rows = (hb * a.chunks + heads - 2) / heads + 1;
   const size_t lds = (size_t)(q_weight || k_weight ? 2 * D : 0) * 8 + (size_t)rows * rot_pairs * 16 + 16;
   const RotaryPos pos = {positions, pos_i64, pos_per_seq ? T : 0};
-  const unsigned grid = (unsigned)((n_heads + hb - 1) / hb);
+  const unsigned grid = (unsigned)((n_heads + hb * a.chunks - 1) / (hb * a.chunks));
   const bool pair8 = (interleaved ? 2 * rot_pairs : rot_pairs) % 8 == 0;
   hipStream_t st = (hipStream_t)stream;
+#define SF_Q4A_I(DT, P8, I) k_kv_q4_append<DT, P8, I><<<grid, kQ4Threads, lds, st>>>(a, pos, inv_freq)
 #define SF_Q4A(DT)                                                                            \
   do {                                                                                        \
-    if (pair8) k_kv_q4_append<DT, true><<<grid, kQ4Threads, lds, st>>>(a, pos, inv_freq);     \
-    else k_kv_q4_append<DT, false><<<grid, kQ4Threads, lds, st>>>(a, pos, inv_freq);          \
+    if (pair8 && interleaved) SF_Q4A_I(DT, true, true);                                       \
+    else if (pair8) SF_Q4A_I(DT, true, false);                                                \
+    else if (interleaved) SF_Q4A_I(DT, false, true);                                          \
+    else SF_Q4A_I(DT, false, false);                                                          \
   } while (0)
   if (in_dtype == SF_F32) SF_Q4A(SF_F32);
   else if (in_dtype == SF_F16) SF_Q4A(SF_F16);
   else SF_Q4A(SF_BF16);
 #undef SF_Q4A
+#undef SF_Q4A_I
   return sf_check_launch("sf_kv_q4_append");
 }
 

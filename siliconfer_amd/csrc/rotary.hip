@@ -32,9 +32,8 @@ constexpr int kRotTable = 1024;  // cos / sin pairs of a workgroup's rows
 // How a workgroup's work is cut: `rows` rows of `items` items, `per` a head.
 struct RotaryCut {
   int rows, items, per, n_rows;
-  uint32_t inv_items, inv_per;  // ceil(2^32 / .), exact below 2^16 items; 0 stands for a division by 1
+  uint32_t inv_items, inv_per;  // for div_by
 };
-__device__ __forceinline__ int div_by(int e, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)e, inv) : e; }
 
 // VEC: an item is 16 bytes of a head (and, half layout, the 16 bytes P dims further that
 // turn with them), loaded before the workgroup computes its cos / sin table. Else an item
@@ -253,8 +252,8 @@ extern "C" int sf_rotary(const void *q, void *q_out, const void *k, void *k_out,
   if (rows > kRotTable / rot_pairs) rows = kRotTable / rot_pairs;
   if (rows > 65535 / cut.items) rows = 65535 / cut.items;
   cut.rows = rows < 1 ? 1 : rows;
-  cut.inv_items = cut.items == 1 ? 0 : (uint32_t)(((1ull << 32) + cut.items - 1) / cut.items);
-  cut.inv_per = cut.per == 1 ? 0 : (uint32_t)(((1ull << 32) + cut.per - 1) / cut.per);
+  cut.inv_items = div_inv(cut.items);
+  cut.inv_per = div_inv(cut.per);
   const unsigned grid = (unsigned)((cut.n_rows + cut.rows - 1) / cut.rows);
 #define SF_ROT(DT, V, I) \
   k_rotary<DT, V, I><<<grid, kRotThreads, 0, st>>>(rq, rk, pos, inv_freq, rot_pairs, scale, T, D, cut)

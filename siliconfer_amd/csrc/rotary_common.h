@@ -48,6 +48,10 @@ __device__ __forceinline__ float2_t rotary_cs(long long pos, double f, float sca
   return float2_t{(float)(scale * c), (float)(scale * s)};
 }
 
+// e / n by a product with ceil(2^32 / n), exact below 2^16; 0 stands for a division by 1.
+__host__ __device__ inline uint32_t div_inv(int n) { return n == 1 ? 0 : (uint32_t)(((1ull << 32) + n - 1) / n); }
+__device__ __forceinline__ int div_by(int e, uint32_t inv) { return inv ? (int)__umulhi((uint32_t)e, inv) : e; }
+
 struct RotaryPos {
   const void *p;    // [B][T] or, stride_b = 0, [T]
   int i64;
