@@ -14,6 +14,7 @@ pair, on the device: `siliconfer_amd.model.rope.rotary_frequencies` makes it and
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -186,6 +187,12 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Ten
     return out_q, out_k
 
 
+@functools.lru_cache(maxsize=256)
+def _norm_bytes(B: int, T: int, H: int, KVH: int, D: int) -> int:
+    """sf_qk_norm_backward_workspace_bytes of a shape."""
+    return int(_lib.load().sf_qk_norm_backward_workspace_bytes(B, T, H, KVH, D))
+
+
 class _NormTurn(torch.autograd.Function):
     """`qk_norm_rotary` with its gradients, by one kernel that norms the saved rows again."""
 
@@ -203,26 +210,40 @@ class _NormTurn(torch.autograd.Function):
         eps, interleaved, scale = ctx.how
         B, T, H, D = q.shape
         KVH = 0 if k is None else k.shape[2]
-        gq, gk = (g if g is None or g.stride(3) == 1 else g.contiguous() for g in (gq, gk))
+        if gq.stride(3) != 1:
+            gq = gq.contiguous()
         dq = torch.empty_like(q, memory_format=torch.contiguous_format)
-        dk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
-        dw = torch.empty((2, D), dtype=torch.float32, device=q.device)
+        dwq = torch.empty((D,), dtype=torch.float32, device=q.device)
+        dk = dwk = None
+        plain = q.is_contiguous() and gq.is_contiguous()
+        if k is not None:
+            if gk.stride(3) != 1:
+                gk = gk.contiguous()
+            dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+            dwk = torch.empty_like(dwq)
+            plain = plain and k.is_contiguous() and gk.is_contiguous()
         if B * T == 0:
-            dw.zero_()
+            dwq.zero_()
+            if dwk is not None:
+                dwk.zero_()
         else:
-            i64, per_seq = _positions(positions, B, T, q)
-            strides = _STRIDES_BACK(*(t.stride(i) for t in (q, gq, dq, k, gk, dk) if t is not None for i in range(3)))
+            strides = None
+            if not plain:
+                strides = _STRIDES_BACK(*(t.stride(i) for t in (q, gq, dq, k, gk, dk) if t is not None for i in range(3)))
             ptr = _lib.ptr
             with _lib.on_device(q):
                 lib, st = _lib.load(), _lib.stream(q)
-                ws = _lib.scratch(q.device, st, lib.sf_qk_norm_backward_workspace_bytes(B, T, H, KVH, D))
-                _lib.check(lib.sf_qk_norm_rotary_backward(
-                    q.data_ptr(), gq.data_ptr(), dq.data_ptr(), ptr(k), ptr(gk), ptr(dk), _lib.dt(q),
-                    q_weight.data_ptr(), ptr(k_weight), _lib.dt(q_weight), dw.data_ptr(), dw[1].data_ptr(), eps,
-                    positions.data_ptr(), i64, per_seq, inv_freq.data_ptr(), inv_freq.numel(), scale, interleaved,
-                    B, T, H, KVH, D, strides, ws.data_ptr(), ws.numel(), st), "sf_qk_norm_rotary_backward")
-        return (dq, dk, None, None, dw[0].to(q_weight.dtype), None if k is None else dw[1].to(k_weight.dtype), None,
-                None, None)
+                ws = _lib.scratch(q.device, st, _norm_bytes(B, T, H, KVH, D))
+                rc = lib.sf_qk_norm_rotary_backward(
+                    q.data_ptr(), gq.data_ptr(), dq.data_ptr(), ptr(k), ptr(gk if KVH else None), ptr(dk), _lib.dt(q),
+                    q_weight.data_ptr(), ptr(k_weight), _lib.dt(q_weight), dwq.data_ptr(), ptr(dwk), eps,
+                    positions.data_ptr(), positions.dtype is torch.int64, positions.dim() == 2, inv_freq.data_ptr(),
+                    inv_freq.shape[0], scale, interleaved, B, T, H, KVH, D, strides, ws.data_ptr(), ws.numel(), st)
+            if rc:
+                _lib.check(rc, "sf_qk_norm_rotary_backward")
+        if q_weight.dtype is not torch.float32:
+            dwq, dwk = (None if t is None else t.to(q_weight.dtype) for t in (dwq, dwk))
+        return dq, dk, None, None, dwq, dwk, None, None, None
 
 
 def rotary_kv_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
