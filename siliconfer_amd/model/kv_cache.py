@@ -165,10 +165,129 @@ class QuantizedKVCache:
         return self._qk, self._sk, self._qv, self._sv
 
 
-def make_quantized_cache(n_layers: int, capacity: int = 4096,
-                         scale_dtype: torch.dtype = torch.float16) -> list[QuantizedKVCache]:
-    """One fresh QuantizedKVCache per transformer layer."""
+def make_quantized_cache(n_layers: int, capacity: int = 4096, scale_dtype: torch.dtype = torch.float16,
+                         bits: int = 8, group: int | None = None) -> list:
+    """One fresh QuantizedKVCache per transformer layer, or with bits=4 a Q4KVCache with groups
+    of `group` dims."""
+    if bits == 4:
+        return [Q4KVCache(capacity, group) for _ in range(n_layers)]
+    if bits != 8 or group is not None:
+        raise SFError(f"a cache of {bits} bits: 8, or 4 with an optional group")
     return [QuantizedKVCache(capacity, scale_dtype) for _ in range(n_layers)]
+
+
+class Q4KVCache:
+    """Per-layer KV cache in 4 bits, at any batch: groups of `group` dims of a head hold codes
+    0..15 with a scale and a minimum in fp16 (`kernels.kv_q4`), D / 2 + 4 D / group bytes a
+    head and token where the int8 cache has D + 2. `group`: 32, 64, 128 or the whole head;
+    by default 64, 32 or the head, whichever first divides it. All sequences have one
+    length. Keys are cached turned to their positions, which are the slots. Buffers are
+    allocated on the first use, and grow by doubling where `growable`."""
+
+    def __init__(self, capacity: int = 4096, group: int | None = None, growable: bool = True) -> None:
+        self.capacity = int(capacity)
+        self.group = group
+        self.growable = growable
+        self._len = 0
+        self._kc = self._kp = self._vc = self._vp = None
+
+    def length(self) -> int:
+        return self._len
+
+    def buffers(self):
+        """(k_codes, k_params, v_codes, v_params) full-capacity buffers."""
+        return self._kc, self._kp, self._vc, self._vp
+
+    def trim(self, n: int) -> None:
+        """Keep the first n positions."""
+        self._len = max(0, min(int(n), self._len))
+
+    def set_length(self, n: int) -> None:
+        """Mark the first n positions valid (a kernel wrote them in place)."""
+        if self._kc is None or not 0 <= n <= self._kc.shape[2]:
+            raise SFError(f"length {n} outside the cache's buffers")
+        self._len = int(n)
+
+    def nbytes(self) -> int:
+        """Footprint of the valid prefix: codes, scales and minima."""
+        if self._kc is None:
+            return 0
+        B, KVH, _, half = self._kc.shape
+        return 2 * B * KVH * self._len * (half + 4 * self._kp.shape[3])
+
+    def reserve(self, B: int, KVH: int, D: int, need: int, device) -> None:
+        """Make the buffers hold at least `need` positions of [B, KVH, *, D]."""
+        if self._kc is not None:
+            if self._kc.shape[0] != B or self._kc.shape[1] != KVH or 2 * self._kc.shape[3] != D:
+                raise SFError("KV cache shape changed between updates")
+            if need <= self._kc.shape[2]:
+                return
+            if not self.growable:
+                raise SFError(f"KV cache overflow: {need} > capacity {self._kc.shape[2]}")
+        g = self.group
+        if g is None:
+            g = next((n for n in (64, 32) if D % n == 0), D)
+        if D <= 0 or D % 16 or D > 256 or (g != D and (g not in (32, 64, 128) or D % g)):
+            raise SFError(f"heads of {D} dims in groups of {g}: need a multiple of 16 up to 256, in groups of 32, 64 or 128 "
+                          "that divide it or of the whole head")
+        cap = max(self.capacity, 1)
+        while cap < need:
+            cap *= 2
+        new = [t for _ in range(2) for t in (
+            torch.empty((B, KVH, cap, D // 2), dtype=torch.uint8, device=device),
+            torch.empty((B, KVH, cap, D // g, 2), dtype=torch.float16, device=device))]
+        if self._kc is not None and self._len:
+            for a, b in zip(new, self.buffers()):
+                a[:, :, :self._len].copy_(b[:, :, :self._len])
+        self._kc, self._kp, self._vc, self._vp = new
+        self.capacity = cap
+
+    def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Append keys that are turned already, and values, [B, KVH, T, D] (any strides)."""
+        from ..kernels.kv_q4 import kv_append_q4
+        if not k.is_cuda or k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+            raise SFError("k and v must be device tensors of the same shape [B, n_kv_heads, T, head_dim] and dtype")
+        _lib.dt(k)  # (all before any buffer is made for them)
+        B, KVH, T, D = k.shape
+        self.reserve(B, KVH, D, self._len + T, k.device)
+        kv_append_q4(k, v, *self.buffers(), lengths=self._len)
+        self._len += T
+
+    def update(self, k: torch.Tensor, v: torch.Tensor):
+        """Append (k, v) and return the full cache as values in k's dtype (the contract of
+        `QuantizedKVCache.update`)."""
+        from ..kernels.kv_q4 import dequantize_kv_q4
+        self.append(k, v)
+        n = self._len
+        return (dequantize_kv_q4(self._kc[:, :, :n], self._kp[:, :, :n], k.dtype),
+                dequantize_kv_q4(self._vc[:, :, :n], self._vp[:, :, :n], k.dtype))
+
+    def append_rotary(self, qkv: torch.Tensor, n_heads: int, n_kv_heads: int, rotary, q_weight=None, k_weight=None,
+                      eps: float = 1e-6, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Append the next tokens' fused q|k|v rows [B, T, (H + 2 KVH) D], q and k normed a head
+        where their weights are given and turned to their positions; returns q [B, T, H, D]."""
+        from ..kernels.kv_q4 import rotary_kv_append_q4
+        _lib.require_device(qkv, "qkv")  # (all before any buffer is made for the rows)
+        _lib.dt(qkv)
+        B, T, W = qkv.shape if qkv.dim() == 3 else (0, 0, 0)
+        heads = n_heads + 2 * n_kv_heads
+        if not (n_heads > 0 and n_kv_heads > 0 and n_heads % n_kv_heads == 0 and W > 0 and W % heads == 0):
+            raise SFError(f"qkv {list(qkv.shape)} does not hold {n_heads} and 2 x {n_kv_heads} heads")
+        self.reserve(B, n_kv_heads, W // heads, self._len + T, qkv.device)
+        positions = torch.arange(self._len, self._len + T, dtype=torch.int32, device=qkv.device)
+        q = rotary_kv_append_q4(qkv, positions, rotary.on(qkv.device), *self.buffers(), n_heads=n_heads,
+                                lengths=self._len, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                interleaved=rotary.interleaved, scale=rotary.scale, out_dtype=out_dtype)
+        self._len += T
+        return q
+
+    def attend(self, q: torch.Tensor, scale: float | None = None,
+               out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """Attention of the newest rows q [B, T, H, D] over the cache."""
+        from ..kernels.kv_q4 import attention_q4kv
+        if self._kc is None:
+            raise SFError("attention over a cache that holds nothing yet")
+        return attention_q4kv(q, *self.buffers(), lengths=self._len, scale=scale, out_dtype=out_dtype)
 
 
 class BoundedKVCache(QuantizedKVCache):

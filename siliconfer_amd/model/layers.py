@@ -19,7 +19,12 @@ device: RoPE, concatenation (or the int8 append and the dequantized cache)
 and softmax attention with the causal mask, in fp32 torch operations. With
 `rotary` (a `Rotary`) positions follow its frequencies and pair layout (by
 `kernels.rotary`, differentiable where that route is), and a
-`BoundedKVCache` keeps the tokens that attention weighs most, at any batch.
+`BoundedKVCache` keeps the tokens that attention weighs most, at any batch. A
+`Q4KVCache` holds keys and values in 4 bits, at any batch: norm, rotation and
+append in one launch, attention over the codes in place. Heads are normed
+before they turn where `q_norm` / `k_norm` are set (a checkpoint with
+`self_attn.q_norm.weight` and `self_attn.k_norm.weight`), by
+`kernels.rotary.qk_norm_rotary` or within the 4-bit cache's append.
 
 Activations: projections return fp32 (Q4Linear's contract); RMSNorm returns
 its input's dtype; the block's residual stream is kept in the input's dtype.
@@ -34,9 +39,9 @@ import torch
 
 from .. import _lib
 from .._lib import SFError
-from ..kernels.rotary import rotary, rotary_kv_append
+from ..kernels.rotary import qk_norm_rotary, rotary, rotary_kv_append
 from .config import ModelConfig, rope_freqs as _rope_freqs_np
-from .kv_cache import BoundedKVCache, QuantizedKVCache, dequantize_kv
+from .kv_cache import BoundedKVCache, Q4KVCache, QuantizedKVCache, dequantize_kv
 from .q4_linear import Q4Linear, project_group
 from .rope import Rotary
 
@@ -137,12 +142,14 @@ class Attention(torch.nn.Module):
 
     `rotary` replaces the rotate-half RoPE of `rope_freqs` (interleaved pairs, part of
     the head, scaled frequencies). A `BoundedKVCache`, at any batch, scores its slots
-    and drops the least attended ones; of a prompt, the last OBSERVED rows score."""
+    and drops the least attended ones; of a prompt, the last OBSERVED rows score. A
+    `Q4KVCache`, at any batch, is in 4 bits. `qk_norm` adds `q_norm` and `k_norm`, an
+    RMSNorm over each head of queries and keys (None otherwise)."""
 
     OBSERVED = 16
 
     def __init__(self, config: ModelConfig, rope_freqs: torch.Tensor, device=None,
-                 rotary: Rotary | None = None) -> None:
+                 rotary: Rotary | None = None, qk_norm: bool = False) -> None:
         super().__init__()
         self.rotary, self._half = rotary, None
         self.num_heads = config.num_attention_heads
@@ -155,6 +162,11 @@ class Attention(torch.nn.Module):
         self.k_proj = _dense(H, self.num_kv_heads * D, bias, device)
         self.v_proj = _dense(H, self.num_kv_heads * D, bias, device)
         self.o_proj = _dense(self.num_heads * D, H, False, device)
+        self.q_norm = self.k_norm = None
+        if qk_norm:
+            self.q_norm, self.k_norm = (RMSNorm(D, config.rms_norm_eps, device) for _ in range(2))
+            for m in (self.q_norm, self.k_norm):  # (their weights have gradients, as the projections have)
+                m.weight.requires_grad_()
         self._cos = self._sin = None
         if rotary is not None or (isinstance(rope_freqs, torch.Tensor) and not rope_freqs.is_meta):
             self._rotary_of(device)
@@ -186,18 +198,22 @@ class Attention(torch.nn.Module):
         _on_device(x)  # every route runs on the GPU; none on the host
         B, T, _ = x.shape
         H, KVH, D = self.num_heads, self.num_kv_heads, self.head_dim
-        bounded = isinstance(cache, BoundedKVCache)
+        bounded, four = isinstance(cache, BoundedKVCache), isinstance(cache, Q4KVCache)
         int8_batch1 = isinstance(cache, QuantizedKVCache) and B == 1
         qkv = None
-        if int8_batch1 or bounded:
+        if int8_batch1 or bounded or four:
             qkv = project_group(_lib.SF_GROUP_CONCAT, (self.q_proj, self.k_proj, self.v_proj), x)
         if qkv is None:
             q = _project(self.q_proj, x)
             k = _project(self.k_proj, x)
             v = _project(self.v_proj, x)
-        if int8_batch1 or bounded:
+        if int8_batch1 or bounded or four:
             if qkv is None:
                 qkv = torch.cat([t.reshape(B * T, -1) for t in (q, k, v)], dim=1).contiguous()
+        if four:
+            qw, kw, eps = self._norms()
+            q = cache.append_rotary(qkv.view(B, T, -1), H, KVH, self._rotary_of(None), qw, kw, eps)
+            return _project(self.o_proj, cache.attend(q, self.scale).reshape(B, T, H * D)), cache
         if bounded:
             out = self._bounded(qkv.view(B, T, -1), cache)
             return _project(self.o_proj, out.reshape(B, T, H * D)), cache
@@ -213,7 +229,7 @@ class Attention(torch.nn.Module):
             offset = cache[0].shape[2]
         else:
             offset = 0
-        if self.rotary is not None:
+        if self.rotary is not None or self.q_norm is not None:
             q, k = self._turn(q, k, offset)
         else:
             q = apply_rope(q, offset, self.rope_freqs)
@@ -233,20 +249,42 @@ class Attention(torch.nn.Module):
         a = _sdpa_causal(q, kc, vc, offset, self.scale)
         return _project(self.o_proj, a.transpose(1, 2).reshape(B, T, H * D)), new_cache
 
+    def _norms(self):
+        """(q's weights, k's weights, eps) of the heads' norms; None, None where there are none."""
+        if self.q_norm is None:
+            return None, None, 0.0
+        return self.q_norm.weight, self.k_norm.weight, self.q_norm.eps
+
     def _turn(self, q: torch.Tensor, k: torch.Tensor, offset: int):
-        """q, k [B, heads, T, D] turned by `rotary` at positions offset .. in their layout."""
-        r = self.rotary
+        """q, k [B, heads, T, D] (normed and) turned at positions offset .. in their layout."""
+        r = self._rotary_of(None)
         pos = torch.arange(offset, offset + q.shape[2], dtype=torch.int32, device=q.device)
-        q, k = rotary(q.transpose(1, 2), k.transpose(1, 2), pos, r.on(q.device), interleaved=r.interleaved,
-                      scale=r.scale)
+        q, k, how = q.transpose(1, 2), k.transpose(1, 2), dict(interleaved=r.interleaved, scale=r.scale)
+        qw, kw, eps = self._norms()
+        if qw is None:
+            q, k = rotary(q, k, pos, r.on(q.device), **how)
+        else:
+            q, k = qk_norm_rotary(q, k, pos, r.on(q.device), qw, kw, eps=eps, **how)
         return q.transpose(1, 2), k.transpose(1, 2)
+
+    def _normed_rows(self, qkv: torch.Tensor, cache: QuantizedKVCache, offset: int) -> torch.Tensor:
+        """q|k|v rows [B, T, (H + 2 KVH) D] with normed heads: k (turned) and v appended to an
+        int8 cache, the turned q [B, T, H, D] returned."""
+        H, KVH = self.num_heads, self.num_kv_heads
+        q, k, v = (t.transpose(1, 2) for t in qkv.unflatten(-1, (-1, self.head_dim)).split((H, KVH, KVH), dim=2))
+        q, k = self._turn(q, k, offset)
+        cache.append(k, v)
+        return q.transpose(1, 2).contiguous()
 
     def _bounded(self, qkv: torch.Tensor, cache: BoundedKVCache) -> torch.Tensor:
         """[B, T, H, D] fp32 from q|k|v rows [B, T, (H + 2 KVH) D]: the rows appended, attention
         over the whole cache, then what exceeds its bound dropped."""
         B, T, _ = qkv.shape
         H, KVH, D = self.num_heads, self.num_kv_heads, self.head_dim
-        q = cache.append_rotary(qkv, H, KVH, self._rotary_of(None))
+        if self.q_norm is not None:
+            q = self._normed_rows(qkv, cache, cache.seen)
+        else:
+            q = cache.append_rotary(qkv, H, KVH, self._rotary_of(None))
         if T <= self.OBSERVED:
             out = cache.attend(q, self.scale)
         else:
@@ -275,7 +313,10 @@ class Attention(torch.nn.Module):
         kq, ks, vq, vs = cache.buffers()
         T_cap = kq.shape[2]
         st = _lib.stream(qkv)
-        if self.rotary is not None:
+        if self.q_norm is not None:
+            q_rot = self._normed_rows(qkv.view(1, T, -1), cache, offset).view(T, H, D)
+            kq, ks, vq, vs = cache.buffers()
+        elif self.rotary is not None:
             r = self.rotary
             pos = torch.arange(offset, offset + T, dtype=torch.int32, device=device)
             q_rot = rotary_kv_append(qkv.view(1, T, -1), pos, r.on(device), kq, ks, vq, vs, n_heads=H, lengths=offset,
@@ -329,9 +370,9 @@ class TransformerBlock(torch.nn.Module):
     """x + attn(norm(x)), then + mlp(norm(x)) (layers.py:147-163)."""
 
     def __init__(self, config: ModelConfig, rope_freqs: torch.Tensor, device=None,
-                 rotary: Rotary | None = None) -> None:
+                 rotary: Rotary | None = None, qk_norm: bool = False) -> None:
         super().__init__()
-        self.self_attn = Attention(config, rope_freqs, device, rotary)
+        self.self_attn = Attention(config, rope_freqs, device, rotary, qk_norm)
         self.mlp = MLP(config, device)
         self.input_layernorm = RMSNorm(config.hidden_size, config.rms_norm_eps, device)
         self.post_attention_layernorm = RMSNorm(config.hidden_size, config.rms_norm_eps, device)
@@ -348,10 +389,15 @@ class TransformerBlock(torch.nn.Module):
         """Layer `layer` of a checkpoint dict in the HuggingFace naming: packed
         projections (`<p>.q4_packed`, `.q4_scales`, `.q4_zeros`, as
         `pack_and_replace_linears` leaves them) become Q4Linear, dense ones
-        (`<p>.weight`) torch Linear, biases and norm weights fp32."""
+        (`<p>.weight`) torch Linear, biases and norm weights fp32; norms of queries' and
+        keys' heads where the checkpoint has both."""
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-        blk = cls(config, rope_freqs, dev, rotary)
         pre = f"model.layers.{layer}"
+        norms = [f"{pre}.self_attn.{n}_norm.weight" for n in ("q", "k")]
+        normed = [n in weights for n in norms]
+        if any(normed) != all(normed):
+            raise SFError(f"{pre}: a norm of queries' or keys' heads without the other's")
+        blk = cls(config, rope_freqs, dev, rotary, qk_norm=all(normed))
         for parent, mod in (("self_attn", blk.self_attn), ("mlp", blk.mlp)):
             for name in (("q_proj", "k_proj", "v_proj", "o_proj") if parent == "self_attn"
                          else ("gate_proj", "up_proj", "down_proj")):
@@ -374,4 +420,7 @@ class TransformerBlock(torch.nn.Module):
         with torch.no_grad():
             blk.input_layernorm.weight.copy_(_f32(weights[f"{pre}.input_layernorm.weight"]))
             blk.post_attention_layernorm.weight.copy_(_f32(weights[f"{pre}.post_attention_layernorm.weight"]))
+            if blk.self_attn.q_norm is not None:
+                blk.self_attn.q_norm.weight.copy_(_f32(weights[norms[0]]))
+                blk.self_attn.k_norm.weight.copy_(_f32(weights[norms[1]]))
         return blk
