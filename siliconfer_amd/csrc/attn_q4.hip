@@ -130,7 +130,8 @@ __host__ __device__ constexpr int q4_resident(int DP, int groups, int PK, bool Q
 // own until the waves' states merge.
 // A state's reference m stays until a score passes it by 8, so that most tiles need no maximum
 // across lanes and no rescaling; the factor that takes p s to fp16's range stays likewise until
-// a product passes 2^15.
+// a product passes 2^15, and grows where a reference that moves shrinks the products behind it.
+// It is 2^110 at most: a weight, up to 2^8, stays finite times it beside a scale of 0.
 // DP: the head's dims rounded up to 64, 128 or 256. NGT groups of 32 KSGT dims fill it
 // exactly, or 0, 0: any head and groups. QSPLIT, PSPLIT: q, P in two parts.
 template <bool QSPLIT, bool PSPLIT, int DP, int NGT, int KSGT, int PK>
@@ -302,7 +303,7 @@ k_q4_split(Q4Attn a) {
   float *const vss = kos + 64 * NGM, *const vos = vss + 64 * NGM;
   float *const vms = NGM > 1 ? vos + 64 * NGM : vss;  // a slot's largest V scale
   float m = -INFINITY, lsum = 0.f;  // base-2 softmax of the column
-  float mul = 8.507059e37f;         // 2^126: the first tile sets it
+  float mul = 1.2980742e33f;        // 2^110 at most: the first tile sets it
   float am[NGM];                    // sum of p (m + 8 s) over the lane's slots
   float4_t O[DB];
 #pragma unroll
@@ -357,7 +358,7 @@ k_q4_split(Q4Attn a) {
       float v = vss[lane];
 #pragma unroll
       for (int gi = 1; gi < NGM; ++gi)
-        if (!ANY || gi < NG) v = fmaxf(v, vss[64 * gi + lane]);
+        if (!ANY || gi < NG) v = fmaxf(fabsf(v), fabsf(vss[64 * gi + lane]));
       vms[lane] = v;
     }
     float sc[NV];  // value 4 hh + i: slot tb + 16 g + 4 i + h0 + hh
@@ -403,9 +404,11 @@ k_q4_split(Q4Attn a) {
 #pragma unroll
     for (int e = 1; e < NV; ++e) mx = fmaxf(mx, sc[e]);
     mx *= qmul;
+    float behind = 0.f;  // a bound of the products so far, where references move
     if (__any(mx > m + 8.f)) {
       const float M = max_x16_x32(mx), m_new = M > m + 8.f ? M : m;
       const float cf = __builtin_amdgcn_exp2f(m - sf_merge_mref(m_new));  // exp2(-inf) = 0
+      behind = fmaxf(cf * (32768.f / mul), 6.3108872e-30f);  // (2^-97: a factor of 2^110)
       m = m_new;
       lsum *= cf;
 #pragma unroll
@@ -423,12 +426,13 @@ k_q4_split(Q4Attn a) {
         const int e = 4 * hh + i;
         sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], qmul, -m_ref));
         lsum += sc[e];
-        pt = fmaxf(pt, sc[e] * v[i]);  // (0 or NaN, which counts for nothing, past a row's end)
+        pt = fmaxf(pt, fabsf(sc[e] * v[i]));  // (0 or NaN, which counts for nothing, past a row's end)
       }
     }
-    if (__any(pt * mul > 32768.f)) {
+    if (__any(behind > 0.f || pt * mul > 32768.f)) {
       const float top = max_x16_x32(pt), was = mul;
-      mul = top * mul > 32768.f ? q4_fit14(top) : mul;
+      if (top * mul > 32768.f) mul = q4_fit14(top);
+      else if (behind > 0.f) mul = fmaxf(mul, q4_fit14(fmaxf(top, behind)));
 #pragma unroll
       for (int d = 0; d < DB; ++d) O[d] *= mul / was;
     }

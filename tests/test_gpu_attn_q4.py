@@ -186,6 +186,66 @@ def test_sharp_flat_and_far_scales(dev, rows):
         check(attention_q4kv(q, *scaled, lengths=n), q, scaled, [n])
 
 
+def held(x, group, dev):
+    c, s, m, _ = O.quantize(x, group)
+    return [torch.from_numpy(O.pack(c)).to(dev), torch.from_numpy(np.stack([s, m], -1)).to(dev)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D,group", [(64, 64), (128, 32), (80, 80)])
+@pytest.mark.parametrize("rows", [1, 3, 9])
+def test_constant_groups_under_rising_scores(dev, rows, D, group, dtype):
+    """V whose groups hold one value each (scales of 0), keys whose scores rise from slot to slot by
+    less than what moves a softmax's reference: every weight past the first tile's is over 1."""
+    B, H, KVH, n = 2, 4, 2, 700
+    g = np.random.default_rng(rows)
+    k = np.zeros((B, KVH, n, D)) + (np.arange(n) / 100)[:, None]
+    v = np.repeat(g.standard_normal((B, KVH, n, D // group)), group, -1)
+    bufs = held(k, group, dev) + held(v, group, dev)
+    assert (bufs[3][..., 0] == 0).all()
+    q = torch.full((B, rows, H, D), D ** -0.5).to(DT[dtype]).to(dev)
+    for n_splits in (1, 2, None):
+        check(attention_q4kv(q, *bufs, lengths=n, n_splits=n_splits, out_dtype=DT[dtype]), q, bufs, [n] * B)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D,group", [(64, 64), (128, 32), (80, 80)])
+@pytest.mark.parametrize("rows", [1, 3, 9])
+def test_small_values_that_outweigh_large_ones(dev, rows, D, group, dtype):
+    """Large V, then at scores that leave it no weight V of a billionth, zeros, and V of a
+    hundredth, few slots each in one wave's tiles."""
+    B, H, KVH, n = 1, 4, 2, 1030
+    g = np.random.default_rng(rows)
+    at = np.arange(n)
+    level = np.where(at < 64, 0.0, np.where((at >= 256) & (at < 261), 40.0, np.where(at < 512, -40.0, np.where(at < 1024, -20.0, 60.0))))
+    size = np.where(at < 64, 50000.0, np.where(at < 512, 3e-5, np.where(at < 1024, 0.0, 300.0)))
+    k = np.zeros((B, KVH, n, D)) + level[:, None]
+    v = g.uniform(-1, 1, (B, KVH, n, D)) * size[:, None]
+    bufs = held(k, group, dev) + held(v, group, dev)
+    q = torch.full((B, rows, H, D), D ** -0.5).to(DT[dtype]).to(dev)
+    for length in (261 + rows, 800, n):
+        for n_splits in (1, 2, None):
+            y = attention_q4kv(q, *bufs, lengths=length, n_splits=n_splits, out_dtype=DT[dtype])
+            check(y, q, bufs, [length] * B)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_resident_workgroups(dev, D):
+    """More workgroups than CUs, up to two a CU: the first ones' columns in the other order, and for
+    a bf16 output four waves each."""
+    B, H, KVH, rows, cap = 2, 64, 32, 300, 333
+    bufs = cache(B, KVH, cap, D, 64, dev, seed=D)
+    q = (1.5 * torch.randn(B, rows, H, D, generator=torch.Generator().manual_seed(D))).to(dev)
+    lengths = torch.tensor([333, 290], dtype=torch.int32, device=dev)
+    for dtype in DT.values():
+        x = q.to(dtype)
+        y = attention_q4kv(x, *bufs, lengths=lengths, out_dtype=dtype)
+        for heads in (slice(0, 2), slice(30, 32)):  # (enough for the oracle)
+            rows_of = slice(2 * heads.start, 2 * heads.stop)
+            check(y[:, :, rows_of].contiguous(), x[:, :, rows_of], [t[:, heads] for t in bufs], [333, 290], many=True)
+
+
+
 def test_long_cache(dev):
     """70000 slots through many splits; the slots far behind weigh what they should."""
     D, KVH, n = 64, 1, 70001
