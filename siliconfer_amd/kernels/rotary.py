@@ -220,7 +220,7 @@ class _NormTurn(torch.autograd.Function):
             if gk.stride(3) != 1:
                 gk = gk.contiguous()
             dk = torch.empty_like(k, memory_format=torch.contiguous_format)
-            dwk = torch.empty_like(dwq)
+            dwk = torch.empty_like(dwq) if KVH else torch.zeros_like(dwq)
             plain = plain and k.is_contiguous() and gk.is_contiguous()
         if B * T == 0:
             dwq.zero_()

@@ -235,6 +235,48 @@ def test_a_block_from_a_checkpoint(dev):
     assert not torch.equal(other, full)
 
 
+def test_two_host_threads_and_two_streams(dev):
+    """A cache's steps from two threads at once, on one stream and on one each, at sizes whose
+    workspaces differ, give what one thread gives."""
+    import threading
+
+    r = Rotary(*rotary_frequencies(64, 1e4))
+    r.on(dev)
+
+    def inputs(i):
+        g = torch.Generator().manual_seed(20 + i)
+        return [torch.randn(1 + i, T, (H + 2 * KVH) * D, generator=g).to(dev) for T in (3000 - 1700 * i, 1, 1, 40, 1)], weights(dev, i)
+
+    def work(args):
+        cache, out = Q4KVCache(512), []
+        for x in args[0]:
+            q = cache.append_rotary(x, H, KVH, r, *args[1])
+            out += [q, cache.attend(q), cache.attend(q[:, -1:].contiguous(), out_dtype=torch.bfloat16)]
+        return out + [t[:, :, :cache.length()].clone() for t in cache.buffers()]
+
+    args = [inputs(i) for i in range(2)]
+    want = [work(x) for x in args]
+    torch.cuda.synchronize()
+    for own in (False, True):
+        got, wrong = [None, None], []
+
+        def run(i):
+            try:
+                with torch.cuda.stream(torch.cuda.Stream(dev) if own else torch.cuda.default_stream(dev)):
+                    for _ in range(5):
+                        got[i] = work(args[i])
+                    torch.cuda.synchronize()
+            except BaseException as e:  # noqa: BLE001 (handed to the test)
+                wrong.append(e)
+
+        threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+        assert not wrong, wrong
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_refusals(dev):
     cache = Q4KVCache(4, growable=False)
     r = Rotary(*rotary_frequencies(64, 1e4))

@@ -186,6 +186,23 @@ def test_no_rows(dev):
     assert y.shape == q.shape and q.grad.shape == q.shape and (w.grad == 0).all()
 
 
+def test_a_side_without_heads(dev):
+    """k of no heads: its weights' gradient is zeros."""
+    g = torch.Generator().manual_seed(0)
+    q = torch.randn(2, 3, 4, 64, generator=g).to(dev).requires_grad_()
+    k = torch.empty(2, 3, 0, 64, device=dev, requires_grad=True)
+    w = [torch.ones(64, device=dev, requires_grad=True) for _ in range(2)]
+    pos, f = torch.arange(3, device=dev), torch.from_numpy(freqs(32)).to(dev)
+    for _ in range(3):  # (memory that held something else)
+        torch.full((1 << 16,), float("nan"), device=dev)
+        y, z = qk_norm_rotary(q, k, pos, f, *w)
+        assert z.shape == k.shape
+        grads = torch.autograd.grad(y.sum(), (q, k, *w), allow_unused=True)
+        alone = torch.autograd.grad(qk_norm_rotary(q, None, pos, f, w[0])[0].sum(), (q, w[0]))
+        assert torch.equal(grads[0], alone[0]) and torch.equal(grads[2], alone[1])
+        assert grads[1].shape == k.shape and (grads[3] == 0).all()
+
+
 def test_refusals(dev):
     q, w = torch.randn(1, 2, 3, 64, device=dev), torch.ones(64, device=dev)
     pos, inv = torch.arange(2, device=dev), torch.from_numpy(freqs(32)).to(dev)
