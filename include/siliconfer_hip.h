@@ -440,15 +440,15 @@ int sf_qk_norm_rotary(const void *q, void *q_out, const void *k, void *k_out, in
                       int rot_pairs, float scale, int interleaved, int B, int T, int H, int KVH, int D,
                       const long long *strides, void *stream);
 /* Its gradients: from the rows q, k as they were given and the outputs' gradients q_grad,
- * k_grad to dq_out, dk_out (all of `dtype`) and dq_weight, dk_weight (fp32 [D], summed over
- * all rows and heads in a fixed order). strides: NULL, or 18 element strides (batch, row,
+ * k_grad to dq_out, dk_out (all of `dtype`) and dq_weight, dk_weight ([D] of weight_dtype, summed
+ * over all rows and heads in fp32 in a fixed order). strides: NULL, or 18 element strides (batch, row,
  * head of q, q_grad, dq_out, k, k_grad, dk_out). B, T > 0. The workspace is 16-byte aligned;
  * nothing in it needs clearing. */
 size_t sf_qk_norm_backward_workspace_bytes(int B, int T, int H, int KVH, int D);
 int sf_qk_norm_rotary_backward(const void *q, const void *q_grad, void *dq_out, const void *k,
                                const void *k_grad, void *dk_out, int dtype, const void *q_weight,
-                               const void *k_weight, int weight_dtype, float *dq_weight,
-                               float *dk_weight, float eps, const void *positions, int pos_i64,
+                               const void *k_weight, int weight_dtype, void *dq_weight,
+                               void *dk_weight, float eps, const void *positions, int pos_i64,
                                int pos_per_seq, const double *inv_freq, int rot_pairs, float scale,
                                int interleaved, int B, int T, int H, int KVH, int D,
                                const long long *strides, void *workspace, size_t workspace_bytes,

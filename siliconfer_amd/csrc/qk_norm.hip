@@ -286,9 +286,10 @@ k_qk_norm_back(NormRows q, NormRows k, int wdt, float eps, RotaryPos pos, const 
   }
 }
 
-// The partials' sums, in a fixed order: a workgroup takes 4 dims of one side, 64 lanes each.
+// The partials' sums, in a fixed order, rounded once to the weights' type: a workgroup takes 4 dims of one side, 64 lanes each.
 __global__ void __launch_bounds__(256)
-k_qk_norm_weights(const float *__restrict__ part, int nq, int nk, int D, float *__restrict__ dwq, float *__restrict__ dwk) {
+k_qk_norm_weights(const float *__restrict__ part, int nq, int nk, int D, int wdt, void *__restrict__ dwq,
+                  void *__restrict__ dwk) {
   const int lane = threadIdx.x & 63, per = (D + 3) / 4, side = blockIdx.x / per;
   const int d = (blockIdx.x - side * per) * 4 + (threadIdx.x >> 6);
   const int n0 = side ? nq : 0, n1 = side ? nq + nk : nq;
@@ -296,7 +297,7 @@ k_qk_norm_weights(const float *__restrict__ part, int nq, int nk, int D, float *
   if (d < D)
     for (int n = n0 + lane; n < n1; n += 64) s += part[(size_t)n * D + d];
   s = sf_wave_sum(s);
-  if (d < D && lane == 0) (side ? dwk : dwq)[d] = s;
+  if (d < D && lane == 0) sf_store_dt(side ? dwk : dwq, wdt, d, s);
 }
 
 // How heads are cut into items and lanes; vec: 16 bytes at a time where every head of every
@@ -393,7 +394,7 @@ extern "C" size_t sf_qk_norm_backward_workspace_bytes(int B, int T, int H, int K
 
 extern "C" int sf_qk_norm_rotary_backward(const void *q, const void *q_grad, void *dq_out, const void *k,
                                           const void *k_grad, void *dk_out, int dtype, const void *q_weight,
-                                          const void *k_weight, int weight_dtype, float *dq_weight, float *dk_weight,
+                                          const void *k_weight, int weight_dtype, void *dq_weight, void *dk_weight,
                                           float eps, const void *positions, int pos_i64, int pos_per_seq,
                                           const double *inv_freq, int rot_pairs, float scale, int interleaved, int B,
                                           int T, int H, int KVH, int D, const long long *strides, void *workspace,
@@ -430,7 +431,7 @@ extern "C" int sf_qk_norm_rotary_backward(const void *q, const void *q_grad, voi
                                                                scale, T, D, cut, rows, nq, run, part)
   SF_NORM_DT(SF_NORM_B);
 #undef SF_NORM_B
-  k_qk_norm_weights<<<(KVH ? 2 : 1) * ((D + 3) / 4), 256, 0, st>>>(part, nq, nk, D, dq_weight, dk_weight);
+  k_qk_norm_weights<<<(KVH ? 2 : 1) * ((D + 3) / 4), 256, 0, st>>>(part, nq, nk, D, weight_dtype, dq_weight, dk_weight);
   return sf_check_launch("sf_qk_norm_rotary_backward");
 }
 #undef SF_NORM_V

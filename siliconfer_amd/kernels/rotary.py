@@ -193,6 +193,50 @@ def _norm_bytes(B: int, T: int, H: int, KVH: int, D: int) -> int:
     return int(_lib.load().sf_qk_norm_backward_workspace_bytes(B, T, H, KVH, D))
 
 
+def _norm_turn_back(ctx, gq, gk):
+    """The gradients of `_NormTurn`'s inputs."""
+    q, k, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
+    eps, interleaved, scale = ctx.how
+    B, T, H, D = q.shape
+    KVH = 0 if k is None else k.shape[2]
+    if gq.stride(3) != 1:
+        gq = gq.contiguous()
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dwq = torch.empty_like(q_weight)
+    dk = dwk = None
+    plain = q.is_contiguous() and gq.is_contiguous()
+    if k is not None:
+        if gk.stride(3) != 1:
+            gk = gk.contiguous()
+        dk = torch.empty_like(k, memory_format=torch.contiguous_format)
+        dwk = torch.empty_like(dwq) if KVH else torch.zeros_like(dwq)
+        plain = plain and k.is_contiguous() and gk.is_contiguous()
+    if B * T == 0:
+        dwq.zero_()
+        if dwk is not None:
+            dwk.zero_()
+    else:
+        strides = None
+        if not plain:
+            strides = _STRIDES_BACK(*(t.stride(i) for t in (q, gq, dq, k, gk, dk) if t is not None for i in range(3)))
+        ptr = _lib.ptr
+        with _lib.on_device(q):
+            lib, st = _lib.load(), _lib.stream(q)
+            ws = _lib.scratch(q.device, st, _norm_bytes(B, T, H, KVH, D))
+            rc = lib.sf_qk_norm_rotary_backward(
+                q.data_ptr(), gq.data_ptr(), dq.data_ptr(), ptr(k), ptr(gk if KVH else None), ptr(dk), _lib.dt(q),
+                q_weight.data_ptr(), ptr(k_weight), _lib.dt(q_weight), dwq.data_ptr(), ptr(dwk), eps,
+                positions.data_ptr(), positions.dtype is torch.int64, positions.dim() == 2, inv_freq.data_ptr(),
+                inv_freq.shape[0], scale, interleaved, B, T, H, KVH, D, strides, ws.data_ptr(), ws.numel(), st)
+        if rc:
+            _lib.check(rc, "sf_qk_norm_rotary_backward")
+    return dq, dk, None, None, dwq, dwk, None, None, None
+
+
+# (where a graph of the gradients is asked for: it refuses to be differentiated)
+_norm_turn_back_once = torch.autograd.function.once_differentiable(_norm_turn_back)
+
+
 class _NormTurn(torch.autograd.Function):
     """`qk_norm_rotary` with its gradients, by one kernel that norms the saved rows again."""
 
@@ -204,46 +248,9 @@ class _NormTurn(torch.autograd.Function):
                               scale=scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        q, k, positions, inv_freq, q_weight, k_weight = ctx.saved_tensors
-        eps, interleaved, scale = ctx.how
-        B, T, H, D = q.shape
-        KVH = 0 if k is None else k.shape[2]
-        if gq.stride(3) != 1:
-            gq = gq.contiguous()
-        dq = torch.empty_like(q, memory_format=torch.contiguous_format)
-        dwq = torch.empty((D,), dtype=torch.float32, device=q.device)
-        dk = dwk = None
-        plain = q.is_contiguous() and gq.is_contiguous()
-        if k is not None:
-            if gk.stride(3) != 1:
-                gk = gk.contiguous()
-            dk = torch.empty_like(k, memory_format=torch.contiguous_format)
-            dwk = torch.empty_like(dwq) if KVH else torch.zeros_like(dwq)
-            plain = plain and k.is_contiguous() and gk.is_contiguous()
-        if B * T == 0:
-            dwq.zero_()
-            if dwk is not None:
-                dwk.zero_()
-        else:
-            strides = None
-            if not plain:
-                strides = _STRIDES_BACK(*(t.stride(i) for t in (q, gq, dq, k, gk, dk) if t is not None for i in range(3)))
-            ptr = _lib.ptr
-            with _lib.on_device(q):
-                lib, st = _lib.load(), _lib.stream(q)
-                ws = _lib.scratch(q.device, st, _norm_bytes(B, T, H, KVH, D))
-                rc = lib.sf_qk_norm_rotary_backward(
-                    q.data_ptr(), gq.data_ptr(), dq.data_ptr(), ptr(k), ptr(gk if KVH else None), ptr(dk), _lib.dt(q),
-                    q_weight.data_ptr(), ptr(k_weight), _lib.dt(q_weight), dwq.data_ptr(), ptr(dwk), eps,
-                    positions.data_ptr(), positions.dtype is torch.int64, positions.dim() == 2, inv_freq.data_ptr(),
-                    inv_freq.shape[0], scale, interleaved, B, T, H, KVH, D, strides, ws.data_ptr(), ws.numel(), st)
-            if rc:
-                _lib.check(rc, "sf_qk_norm_rotary_backward")
-        if q_weight.dtype is not torch.float32:
-            dwq, dwk = (None if t is None else t.to(q_weight.dtype) for t in (dwq, dwk))
-        return dq, dk, None, None, dwq, dwk, None, None, None
+        # (once_differentiable's own checks cost 10 us a call)
+        return (_norm_turn_back_once if torch.is_grad_enabled() else _norm_turn_back)(ctx, gq, gk)
 
 
 def rotary_kv_append(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,

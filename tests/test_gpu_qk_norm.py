@@ -186,6 +186,19 @@ def test_no_rows(dev):
     assert y.shape == q.shape and q.grad.shape == q.shape and (w.grad == 0).all()
 
 
+def test_a_graph_of_the_gradients_is_refused(dev):
+    """With create_graph the gradients are the same, and cannot be differentiated."""
+    q = torch.randn(1, 3, 2, 64, generator=torch.Generator().manual_seed(0)).to(dev).requires_grad_()
+    w = torch.ones(64, device=dev, requires_grad=True)
+    pos, f = torch.arange(3, device=dev), torch.from_numpy(freqs(32)).to(dev)
+    y = qk_norm_rotary(q, None, pos, f, w)[0].square().sum()
+    want = torch.autograd.grad(y, (q, w), retain_graph=True)
+    got = torch.autograd.grad(y, (q, w), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        got[0].sum().backward()
+
+
 def test_a_side_without_heads(dev):
     """k of no heads: its weights' gradient is zeros."""
     g = torch.Generator().manual_seed(0)
