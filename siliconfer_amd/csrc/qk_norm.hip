@@ -29,6 +29,7 @@ struct NormRows {  // one side's tensors, strides in elements (batch, row, head)
   void *out;       // y, or dx
   long long xb, xt, xh, gb, gt, gh, ob, ot, oh;
   int heads;
+  uint32_t inv;    // for div_by: of this side's heads (forward, in q's: of both sides')
 };
 
 __device__ __forceinline__ float norm_load(const void *p, int dt, size_t i) {
@@ -66,6 +67,22 @@ struct Held {
     __device__ __forceinline__ bool turns(int j) const { return VEC ? i < turned : i + 64 * j < P; }
     __device__ __forceinline__ int pair(int j) const { return VEC ? (INTER ? i * E / 2 : i * E) + j : i + 64 * j; }
   };
+
+  // The weights of what the lane holds, and the cos and sin of its pairs, without branches: VEC,
+  // neighbouring entries of LDS; where it holds nothing (zeros), or nothing that turns, the first ones.
+  static __device__ __forceinline__ void weights(const float *w, const At &x, float (&wa)[N], float (&wb)[N]) {
+    const int d = VEC && x.live ? x.d1(0) : 0, d2 = VEC && !INTER && x.live && x.i < x.turned ? d + x.P : d;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      wa[j] = w[!VEC ? (x.one(j) ? x.d1(j) : 0) : INTER ? d + 2 * j : d + j];
+      wb[j] = w[!VEC ? (x.two(j) ? x.d2(j) : 0) : INTER ? d + 2 * j + 1 : d2 + j];
+    }
+  }
+  static __device__ __forceinline__ void angles(const float2_t *c, const At &x, float2_t (&cs)[N]) {
+    const int p = VEC && x.turns(0) ? x.pair(0) : 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) cs[j] = c[VEC ? p + j : x.turns(j) ? x.pair(j) : 0];
+  }
 
   // the bits of a head, loaded before they are needed
   struct Bits {
@@ -148,16 +165,50 @@ struct Held {
   }
 };
 
+// The turned pair.
+__device__ __forceinline__ float2_t norm_turn(float x1, float x2, float2_t cs) {
+  return float2_t{fmaf(-x2, cs.y, x1 * cs.x), fmaf(x1, cs.y, x2 * cs.x)};
+}
+
 struct NormCut {
   int per, turned, lanes_log2, n_heads;  // items a head, those that turn, log2 of its lanes, heads of a launch (or side)
+  uint32_t inv_T, inv_P;                 // for div_by
 };
 
-// The lanes' table of cos and sin, one entry a (row, pair), of the rows row0 .. row0 + rows.
-__device__ __forceinline__ void norm_table(float2_t *cs, int row0, int rows, int T, int P, RotaryPos pos,
+// The rows and heads of a workgroup's consecutive heads first ..: its first one's by (uniform)
+// divisions, the others' by what they are past it.
+struct NormAt {
+  int row0, off0, b0, t0, heads, T;
+  uint32_t inv_heads, inv_T;
+  __device__ __forceinline__ NormAt(int first, int heads, int T, uint32_t inv_heads, uint32_t inv_T)
+      : heads(heads), T(T), inv_heads(inv_heads), inv_T(inv_T) {
+    row0 = first / heads;
+    off0 = first - row0 * heads;
+    b0 = row0 / T;
+    t0 = row0 - b0 * T;
+  }
+  // the row past the first one, and the head, of the workgroup's head `past` (under 257; the
+  // quotients' operands stay below 2^16, or the quotient is 0 or 1)
+  __device__ __forceinline__ int row(int past, int &h) const {
+    const int e = off0 + past, r = heads < 32768 ? div_by(e, inv_heads) : e >= heads;
+    h = e - r * heads;
+    return r;
+  }
+  __device__ __forceinline__ void token(int r, int &b, int &t) const {
+    const int x = t0 + r, n = T < 32768 ? div_by(x, inv_T) : x >= T;
+    b = b0 + n;
+    t = x - n * T;
+  }
+};
+
+// The lanes' table of cos and sin, one entry a (row, pair), of the workgroup's first `rows` rows.
+__device__ __forceinline__ void norm_table(float2_t *cs, const NormAt &w, int rows, int P, uint32_t inv_P, RotaryPos pos,
                                            const double *inv_freq, float scale) {
   for (int i = threadIdx.x; i < rows * P; i += kNormThreads) {
-    const int r = i / P, row = row0 + r, b = row / T;
-    cs[i] = rotary_cs(pos.at(b, row - b * T), inv_freq[i - r * P], scale);
+    const int r = div_by(i, inv_P);
+    int b, t;
+    w.token(r, b, t);
+    cs[i] = rotary_cs(pos.at(b, t), inv_freq[i - r * P], scale);
   }
 }
 
@@ -167,40 +218,43 @@ __global__ void __launch_bounds__(kNormThreads)
 k_qk_norm(NormRows q, NormRows k, int wdt, float eps, RotaryPos pos, const double *__restrict__ inv_freq, int P,
           float scale, int T, int D, NormCut cut) {
   using H = Held<DT, VEC, INTER>;
+  constexpr int N = H::N;
   extern __shared__ __attribute__((aligned(16))) float smem[];
   float *const ws = smem;                              // [2][D] weights
   float2_t *const cs = (float2_t *)(smem + 2 * D);     // [rows][P]
   const int heads = q.heads + k.heads, hb = kNormThreads >> cut.lanes_log2, L = 1 << cut.lanes_log2;
-  const int first = blockIdx.x * hb, slot = threadIdx.x >> cut.lanes_log2;
-  const int last = min(first + hb, cut.n_heads) - 1, row0 = first / heads, rows = last / heads - row0 + 1;
-  const int e = min(first + slot, last), row = e / heads, hh = e - row * heads, b = row / T, t = row - b * T;
-  const bool is_q = hh < q.heads, live = first + slot <= last;
-  const NormRows &x = is_q ? q : k;
-  const int h = is_q ? hh : hh - q.heads;
-  const int i = threadIdx.x & (L - 1);
+  const int first = blockIdx.x * hb, slot = threadIdx.x >> cut.lanes_log2, count = min(hb, cut.n_heads - first);
+  const NormAt w(first, heads, T, q.inv, cut.inv_T);
+  int hh, b, t, unused;
+  const int dr = w.row(min(slot, count - 1), hh), rows = w.row(count - 1, unused) + 1;
+  w.token(dr, b, t);
+  const bool is_q = hh < q.heads, live = slot < count;
+  const int h = is_q ? hh : hh - q.heads, i = threadIdx.x & (L - 1);
   const typename H::At at = {i, P, D, cut.per, cut.turned, i < cut.per};
   H v;
-  v.set(H::fetch(x.x, (size_t)(b * x.xb + t * x.xt + h * x.xh), at));
+  v.set(H::fetch(is_q ? q.x : k.x, (size_t)(is_q ? b * q.xb + t * q.xt + h * q.xh : b * k.xb + t * k.xt + h * k.xh), at));
   for (int d = threadIdx.x; d < 2 * D; d += kNormThreads) {
     if (d < D) ws[d] = norm_load(q.w, wdt, d);
     else if (k.heads) ws[d] = norm_load(k.w, wdt, d - D);
   }
-  norm_table(cs, row0, rows, T, P, pos, inv_freq, scale);
+  norm_table(cs, w, rows, P, cut.inv_P, pos, inv_freq, scale);
   float ss = 0.f;
 #pragma unroll
-  for (int j = 0; j < H::N; ++j) ss = fmaf(v.a[j], v.a[j], fmaf(v.b[j], v.b[j], ss));
+  for (int j = 0; j < N; ++j) ss = fmaf(v.a[j], v.a[j], fmaf(v.b[j], v.b[j], ss));
   const float r = 1.f / sqrtf(sf_group_tree_sum(ss, L) / (float)D + eps);
   __syncthreads();
-  const float *w = ws + (is_q ? 0 : D);
-  const float2_t *c = cs + (row - row0) * P;
+  float wa[N], wb[N];
+  float2_t c[N];
+  H::weights(ws + (is_q ? 0 : D), at, wa, wb);
+  H::angles(cs + dr * P, at, c);
 #pragma unroll
-  for (int j = 0; j < H::N; ++j) {
-    const float y1 = at.one(j) ? v.a[j] * r * w[at.d1(j)] : 0.f, y2 = at.two(j) ? v.b[j] * r * w[at.d2(j)] : 0.f;
-    const float2_t y = at.turns(j) ? turn(y1, y2, c[at.pair(j)]) : float2_t{y1, y2};
-    v.a[j] = y.x;
-    v.b[j] = y.y;
+  for (int j = 0; j < N; ++j) {
+    const float y1 = v.a[j] * r * wa[j], y2 = v.b[j] * r * wb[j];
+    const float2_t y = norm_turn(y1, y2, c[j]);
+    v.a[j] = at.turns(j) ? y.x : y1;
+    v.b[j] = at.turns(j) ? y.y : y2;
   }
-  if (live) v.store(x.out, (size_t)(b * x.ob + t * x.ot + h * x.oh), at);
+  if (live) v.store(is_q ? q.out : k.out, (size_t)(is_q ? b * q.ob + t * q.ot + h * q.oh : b * k.ob + t * k.ot + h * k.oh), at);
 }
 
 // Backward. The first nq workgroups take q's heads, the others k's, each a run of `run`
@@ -228,14 +282,16 @@ k_qk_norm_back(NormRows q, NormRows k, int wdt, float eps, RotaryPos pos, const 
   for (int u = 0; u < run; ++u) {
     const long long first_ = ((long long)blk * run + u) * hb;
     if (first_ >= n_heads) break;
-    const int first = (int)first_, last = min(first + hb, n_heads) - 1;
-    const int row0 = first / heads, rows = last / heads - row0 + 1;
-    const int e = min(first + slot, last), row = e / heads, h = e - row * heads, b = row / T, t = row - b * T;
-    const bool live = first + slot <= last;
+    const int count = min(hb, n_heads - (int)first_);
+    const NormAt w((int)first_, heads, T, x.inv, cut.inv_T);
+    int h, b, t, unused;
+    const int dr = w.row(min(slot, count - 1), h), rows = w.row(count - 1, unused) + 1;
+    w.token(dr, b, t);
+    const bool live = slot < count;
     const auto xb = H::fetch(x.x, (size_t)(b * x.xb + t * x.xt + h * x.xh), at);
     const auto gb = H::fetch(x.g, (size_t)(b * x.gb + t * x.gt + h * x.gh), at);
     __syncthreads();  // the last chunk's table is read
-    norm_table(cs, row0, rows, T, P, pos, inv_freq, scale);
+    norm_table(cs, w, rows, P, cut.inv_P, pos, inv_freq, scale);
     __syncthreads();
     H v, g;
     v.set(xb);
@@ -244,23 +300,22 @@ k_qk_norm_back(NormRows q, NormRows k, int wdt, float eps, RotaryPos pos, const 
 #pragma unroll
     for (int j = 0; j < N; ++j) ss = fmaf(v.a[j], v.a[j], fmaf(v.b[j], v.b[j], ss));
     const float r = 1.f / sqrtf(sf_group_tree_sum(ss, L) / (float)D + eps);
-    const float2_t *c = cs + (row - row0) * P;
+    float wa[N], wb[N];
+    float2_t c[N];
+    H::weights(ws, at, wa, wb);
+    H::angles(cs + dr * P, at, c);
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      if (at.turns(j)) {  // turned back: the opposite angle
-        const float2_t cj = c[at.pair(j)], y = turn(g.a[j], g.b[j], float2_t{cj.x, -cj.y});
-        g.a[j] = y.x;
-        g.b[j] = y.y;
-      }
+      const float2_t y = norm_turn(g.a[j], g.b[j], float2_t{c[j].x, -c[j].y});  // turned back: the opposite angle
+      g.a[j] = at.turns(j) ? y.x : g.a[j];
+      g.b[j] = at.turns(j) ? y.y : g.b[j];
       v.a[j] *= r;
       v.b[j] *= r;
-      if (live) {
-        da[j] = fmaf(g.a[j], v.a[j], da[j]);
-        db[j] = fmaf(g.b[j], v.b[j], db[j]);
-      }
-      g.a[j] *= at.one(j) ? ws[at.d1(j)] : 0.f;
-      g.b[j] *= at.two(j) ? ws[at.d2(j)] : 0.f;
+      da[j] = live ? fmaf(g.a[j], v.a[j], da[j]) : da[j];
+      db[j] = live ? fmaf(g.b[j], v.b[j], db[j]) : db[j];
+      g.a[j] *= wa[j];
+      g.b[j] *= wb[j];
       dot = fmaf(g.a[j], v.a[j], fmaf(g.b[j], v.b[j], dot));
     }
     dot = sf_group_tree_sum(dot, L) / (float)D;
@@ -302,12 +357,15 @@ k_qk_norm_weights(const float *__restrict__ part, int nq, int nk, int D, int wdt
 
 // How heads are cut into items and lanes; vec: 16 bytes at a time where every head of every
 // tensor starts on 16 bytes and its parts are whole vectors.
-bool norm_cut(int dtype, int rot_pairs, int interleaved, int D, uintptr_t all, const long long *s, int n, NormCut *cut) {
+bool norm_cut(int dtype, int rot_pairs, int interleaved, int T, int D, uintptr_t all, const long long *s, int n,
+              NormCut *cut) {
   const int E = dtype == SF_F32 ? 4 : 8, rest = D - 2 * rot_pairs, turn_dims = interleaved ? 2 * rot_pairs : rot_pairs;
   bool vec = rest % E == 0 && turn_dims % E == 0 && (all & 15) == 0;
   for (int i = 0; i < n; ++i) vec = vec && s[i] % E == 0;
   cut->turned = vec ? turn_dims / E : rot_pairs;
   cut->per = vec ? (turn_dims + rest) / E : rot_pairs + rest;
+  cut->inv_T = div_inv(T);
+  cut->inv_P = div_inv(rot_pairs);
   cut->lanes_log2 = 0;
   while ((1 << cut->lanes_log2) < (vec ? cut->per : 64)) ++cut->lanes_log2;
   return vec;
@@ -356,10 +414,11 @@ extern "C" int sf_qk_norm_rotary(const void *q, void *q_out, const void *k, void
   const long long dq = (long long)H * D, dk = (long long)KVH * D;
   const long long whole[12] = {T * dq, dq, D, T * dq, dq, D, T * dk, dk, D, T * dk, dk, D};
   const long long *s = strides ? strides : whole;
-  const NormRows rq = {q, q_weight, nullptr, q_out, s[0], s[1], s[2], 0, 0, 0, s[3], s[4], s[5], H};
-  const NormRows rk = {k, k_weight, nullptr, k_out, s[6], s[7], s[8], 0, 0, 0, s[9], s[10], s[11], KVH};
+  const NormRows rq = {q, q_weight, nullptr, q_out, s[0], s[1], s[2], 0, 0, 0, s[3], s[4], s[5], H,
+                       div_inv(H + KVH)};
+  const NormRows rk = {k, k_weight, nullptr, k_out, s[6], s[7], s[8], 0, 0, 0, s[9], s[10], s[11], KVH, 0};
   NormCut cut;
-  const bool vec = norm_cut(dtype, rot_pairs, interleaved, D,
+  const bool vec = norm_cut(dtype, rot_pairs, interleaved, T, D,
                             (uintptr_t)q | (uintptr_t)q_out | (KVH ? (uintptr_t)k | (uintptr_t)k_out : 0), s, KVH ? 12 : 6, &cut);
   cut.n_heads = B * T * (H + KVH);
   const int hb = kNormThreads >> cut.lanes_log2;
@@ -410,10 +469,12 @@ extern "C" int sf_qk_norm_rotary_backward(const void *q, const void *q_grad, voi
   const long long wq = (long long)H * D, wk = (long long)KVH * D;
   const long long whole[18] = {T * wq, wq, D, T * wq, wq, D, T * wq, wq, D, T * wk, wk, D, T * wk, wk, D, T * wk, wk, D};
   const long long *s = strides ? strides : whole;
-  const NormRows rq = {q, q_weight, q_grad, dq_out, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], H};
-  const NormRows rk = {k, k_weight, k_grad, dk_out, s[9], s[10], s[11], s[12], s[13], s[14], s[15], s[16], s[17], KVH};
+  const NormRows rq = {q, q_weight, q_grad, dq_out, s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], H,
+                       div_inv(H)};
+  const NormRows rk = {k, k_weight, k_grad, dk_out, s[9], s[10], s[11], s[12], s[13], s[14], s[15], s[16], s[17], KVH,
+                       KVH ? div_inv(KVH) : 0};
   NormCut cut;
-  const bool vec = norm_cut(dtype, rot_pairs, interleaved, D,
+  const bool vec = norm_cut(dtype, rot_pairs, interleaved, T, D,
                             (uintptr_t)q | (uintptr_t)q_grad | (uintptr_t)dq_out |
                                 (KVH ? (uintptr_t)k | (uintptr_t)k_grad | (uintptr_t)dk_out : 0),
                             s, KVH ? 18 : 9, &cut);

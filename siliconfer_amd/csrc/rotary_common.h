@@ -91,7 +91,8 @@ struct Vec {
       } else if constexpr (DT == SF_F16) {
         w[j] = sf_bitcast<uint16_t>((f16)sf_opaque(v[2 * j])) | (uint32_t)sf_bitcast<uint16_t>((f16)sf_opaque(v[2 * j + 1])) << 16;
       } else {
-        w[j] = sf_f32_to_bf16(v[2 * j]) | (uint32_t)sf_f32_to_bf16(v[2 * j + 1]) << 16;
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        w[j] = sf_bitcast<uint32_t>(__builtin_convertvector(float2_t{v[2 * j], v[2 * j + 1]}, bf16x2));
       }
     }
     return w;
