@@ -497,7 +497,7 @@ int sf_kv_q4_dequant(const uint8_t *codes, const void *params, void *out, int ou
  * lengths[b] + T (device lengths, T may be negative) cut to 0 .. T_max, or T where lengths is
  * NULL; row t sees the first n_b - Tq + t + 1 slots, a row that sees none gives zeros, and what
  * a row does not see may hold anything. n_splits <= 0: the kernel's own choice; at most 128
- * are used. The workspace (sf_attn_q4_workspace_bytes, 256-byte aligned; none for 0 bytes)
+ * are used, none where many rows (prompts) go their own way. The workspace (sf_attn_q4_workspace_bytes, 256-byte aligned; none for 0 bytes)
  * needs no clearing. q and the cache's buffers 16-byte aligned. */
 size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int group,
                                   int q_dtype, int out_dtype, int n_splits);

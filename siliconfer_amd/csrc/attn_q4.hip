@@ -134,6 +134,11 @@ __host__ __device__ constexpr int q4_resident(int DP, int groups, int PK, bool Q
 // It is 2^110 at most: a weight, up to 2^8, stays finite times it beside a scale of 0.
 // DP: the head's dims rounded up to 64, 128 or 256. NGT groups of 32 KSGT dims fill it
 // exactly, or 0, 0: any head and groups. QSPLIT, PSPLIT: q, P in two parts.
+// Bound by vector instructions and the waits between them. Traced, with the merge launch, 32 / 8
+// heads of 128: four ragged sequences of up to 32767 slots, bf16, groups of 64 (111 MB) 28.7 + 5.1
+// us, the SIMDs issuing vector instructions 62% of that time (of some 680 a tile 290 turn codes
+// into operands); one sequence of 131071, fp16, groups of 128 (143 MB) 30.9 + 4.5, 4.6 TB/s in the
+// split; sixteen of up to 4001 with fp32 queries (51 MB) 20.9 + 4.0, both q and P in two parts.
 template <bool QSPLIT, bool PSPLIT, int DP, int NGT, int KSGT, int PK>
 __global__ void __launch_bounds__(kQaThreads, q4_resident(DP, NGT, PK, QSPLIT))
 k_q4_split(Q4Attn a) {
@@ -607,7 +612,8 @@ k_q4_merge(const float *__restrict__ part_acc, const float *__restrict__ part_ml
 // output by less than a fifth of its own rounding (2^-9). Other outputs take three products
 // of the high and low parts.
 // What fp16 cannot hold: a tile with an s past 2^11 or an m past 2^14 is taken at 2^-6 (K's
-// scores and V's sums times 2^6 again); parameters that are not finite stand as zeros in V,
+// scores and V's sums times 2^6 again; what such a tile holds beside them is off by 2^-19 at
+// most); parameters that are not finite stand as zeros in V,
 // and the columns that see them get NaN in their group's dims.
 // Measured, 32 / 8 heads of 128, bf16: 4096 rows 168 us (818 TFLOP/s of the products; a large
 // fp16 matrix product reaches 1215 on this card), 1500 rows behind 300 51.6 us, of which 6 the

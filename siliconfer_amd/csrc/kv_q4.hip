@@ -72,7 +72,7 @@ __device__ __forceinline__ V q4_over(V v, int n, F f) {
 
 // PAIR8: a lane's partners in the rotation are 8 neighbouring dims of the head (INTER: its own).
 // Bound by vector instructions: 4095 rows of 32 / 8 heads of 128, bf16, groups of 64, normed and
-// turned, 88 MB (17 us at a copy's rate) in 43 us: 60.8 with divisions for the head, the row, the
+// turned, 88 MB (17 us at a copy's rate) in 43 us, vector instructions in 84% of the SIMDs' time: 60.8 with divisions for the head, the row, the
 // scale's inverse and the root and every code's remainder settled, 53 with the tables in the
 // dims' order (a head's lanes on the same banks).
 template <int DT, bool PAIR8, bool INTER>
@@ -277,7 +277,8 @@ k_kv_q4_append(Q4Append a, RotaryPos pos, const double *__restrict__ inv_freq) {
   }
 }
 
-// Eight values a thread: a word of codes, 16 or 32 bytes out.
+// Eight values a thread: a word of codes, 16 or 32 bytes out. 4095 slots of 8 heads of 128 to fp32
+// (19 MB) 6.8 us traced: a few microseconds of latency around 3.7 at a copy's rate.
 template <int DT>
 __global__ void __launch_bounds__(kQ4Threads)
 k_kv_q4_dequant(const uint8_t *__restrict__ codes, const uint32_t *__restrict__ params, void *__restrict__ out, int KVH,

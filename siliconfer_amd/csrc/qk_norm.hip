@@ -13,7 +13,12 @@
 //
 // L lanes hold a head (the power of two that covers its items), an item being 16 bytes of
 // it and, half layout, the 16 bytes P dims further that turn with them: one load of the
-// row, the sum of squares over L lanes in registers, one store. Bound by the memory stream.
+// row, the sum of squares over L lanes in registers, one store. Bound by the memory stream:
+// 8191 rows of 32 / 8 heads of 128 in bf16 (168 MB) 30.6 us traced, 37.9 a call over memory that
+// is not cached, where a copy's rate gives 32; 4084 rows with half of each head turned, pairs
+// interleaved, forward 24.0 (84 MB), backward 29.2 (126 MB) and 5.5 for the weights' sums.
+// (Weights and angles read one by one behind conditions, a row found by a division a lane:
+// 34.6, 25.9 and 33.0.)
 #include <math.h>
 
 #include "rotary_common.h"

@@ -156,7 +156,9 @@ def attention_q4kv(q: torch.Tensor, k_codes: torch.Tensor, k_params: torch.Tenso
     lengths[b] + add slots of a 4-bit cache: softmax(scale q K^T) V in fp32 sums, one rounding
     to the output's dtype. Row t of Tq sees the slots up to its own, lengths[b] + add - Tq + t;
     a row that sees none gives zeros. `lengths`: int32 [B] on the device, or one int. Device
-    lengths are cut to `max_length` (the capacity where it is not given)."""
+    lengths are cut to `max_length` (the capacity where it is not given). `n_splits`: among how
+    many workgroups a sequence's slots are shared out where rows are few (its own choice by
+    default)."""
     n = n_splits or 0
     if not (_lib.INT_MIN <= add <= _lib.INT_MAX and _lib.INT_MIN <= n <= _lib.INT_MAX
             and _lib.INT_MIN <= (max_length or 0) <= _lib.INT_MAX):
