@@ -45,6 +45,14 @@ __device__ __forceinline__ double q4_load(const void *p, int dt, size_t i) {
   return dt == SF_F32 ? ((const float *)p)[i] : dt == SF_F16 ? (float)((const f16 *)p)[i] : sf_bf16_to_f32(((const uint16_t *)p)[i]);
 }
 
+// A whole number as an int, held within its range (the hardware's conversion; NaN as 0, which
+// a plain cast leaves open).
+__device__ __forceinline__ int q4_int(double v) {
+  int r;
+  asm("v_cvt_i32_f64 %0, %1" : "=v"(r) : "v"(v));
+  return r;
+}
+
 template <int CTRL>
 __device__ __forceinline__ double q4_dpp(double v) {
   const uint64_t u = sf_bitcast<uint64_t>(v);
@@ -264,7 +272,7 @@ k_kv_q4_append(Q4Append a, RotaryPos pos, const double *__restrict__ inv_freq) {
     }
     uint32_t codes = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) codes |= (uint32_t)fmin(fmax(c[j], 0.0), 15.0) << (4 * j);
+    for (int j = 0; j < 8; ++j) codes |= (uint32_t)min(max(q4_int(c[j]), 0), 15) << (4 * j);
     const long long len = a.lengths ? a.lengths[b] : a.start, at = len + t;
     if (!x.live || len < 0 || at >= a.T_cap) continue;  // no such slot: nothing is written
     const size_t crow = ((size_t)b * a.KVH + h) * a.T_cap + (size_t)at;
@@ -277,23 +285,21 @@ k_kv_q4_append(Q4Append a, RotaryPos pos, const double *__restrict__ inv_freq) {
   }
 }
 
-// Eight values a thread: a word of codes, 16 or 32 bytes out. 4095 slots of 8 heads of 128 to fp32
-// (19 MB) 6.8 us traced: a few microseconds of latency around 3.7 at a copy's rate.
+// Eight values a thread: a word of codes, 16 or 32 bytes out. `blocks` workgroups a head.
 template <int DT>
 __global__ void __launch_bounds__(kQ4Threads)
 k_kv_q4_dequant(const uint8_t *__restrict__ codes, const uint32_t *__restrict__ params, void *__restrict__ out, int KVH,
-                int T, int D, int g, long long cb, long long ch, long long ct, long long pb, long long ph, long long pt,
-                long long n) {
-  const long long e = (long long)blockIdx.x * kQ4Threads + threadIdx.x;
-  if (e >= n) return;
-  const int oct = D / 8;
-  const long long row = e / oct;
-  const int i = (int)(e - row * oct), t = (int)(row % T);
-  const long long bh = row / T;
-  const int h = (int)(bh % KVH);
-  const long long b = bh / KVH;
+                int T, int D, int g_log2, int groups, long long cb, long long ch, long long ct, long long pb, long long ph,
+                long long pt, unsigned blocks, uint32_t inv_oct) {
+  // (uniform divisions, a lane's by what it is past them)
+  const unsigned bh = blockIdx.x / blocks, s0 = (blockIdx.x - bh * blocks) * kQ4Threads, oct = D / 8;
+  const unsigned b = bh / KVH, h = bh - b * KVH, t0 = s0 / oct, past = s0 - t0 * oct + threadIdx.x;
+  const int dt = div_by(past, inv_oct), i = past - dt * oct;
+  const long long t = (long long)t0 + dt;
+  if (t >= T) return;
+  const size_t e = ((size_t)bh * T + t) * oct + i;
   const uint32_t c = *(const uint32_t *)(codes + b * cb + h * ch + t * ct + 4 * i);
-  const uint32_t w = params[b * pb + h * ph + t * pt + 8 * i / g];
+  const uint32_t w = params[b * pb + h * ph + t * pt + (groups == 1 ? 0 : 8 * i >> g_log2)];
   const float s = (float)sf_bitcast<f16>((uint16_t)(w & 0xffffu)), m = (float)sf_bitcast<f16>((uint16_t)(w >> 16));
   float f[8];
 #pragma unroll
@@ -393,13 +399,16 @@ extern "C" int sf_kv_q4_dequant(const uint8_t *codes, const void *params, void *
                  strides[0] % 4 == 0 && strides[1] % 4 == 0 && strides[2] % 4 == 0 && strides[3] % 2 == 0 &&
                  strides[4] % 2 == 0 && strides[5] % 2 == 0,
              SF_EINVAL, "codes and params must have rows on 4 bytes, out must be 16-byte aligned");
-  SF_REQUIRE(rows <= 0x7fffffffLL * 256 / T / (D / 8), SF_EINVAL, "B=%d KVH=%d T=%d exceed the grid", B, KVH, T);
-  const long long n = rows * T * (D / 8);
-  const unsigned grid = (unsigned)((n + kQ4Threads - 1) / kQ4Threads);
+  const long long blocks = ((long long)T * (D / 8) + kQ4Threads - 1) / kQ4Threads;
+  SF_REQUIRE(blocks <= 1 << 23 && rows <= 0x7fffffffLL / blocks, SF_EINVAL, "B=%d KVH=%d T=%d exceed the grid", B, KVH, T);
+  const unsigned grid = (unsigned)(rows * blocks);
+  int g_log2 = 0;
+  while ((1 << g_log2) < group) ++g_log2;
   hipStream_t st = (hipStream_t)stream;
 #define SF_Q4D(DT)                                                                                                     \
-  k_kv_q4_dequant<DT><<<grid, kQ4Threads, 0, st>>>(codes, (const uint32_t *)params, out, KVH, T, D, group, strides[0], \
-                                                   strides[1], strides[2], strides[3] / 2, strides[4] / 2, strides[5] / 2, n)
+  k_kv_q4_dequant<DT><<<grid, kQ4Threads, 0, st>>>(codes, (const uint32_t *)params, out, KVH, T, D, g_log2, D / group, \
+                                                   strides[0], strides[1], strides[2], strides[3] / 2, strides[4] / 2, \
+                                                   strides[5] / 2, (unsigned)blocks, div_inv(D / 8))
   if (out_dtype == SF_F32) SF_Q4D(SF_F32);
   else if (out_dtype == SF_F16) SF_Q4D(SF_F16);
   else SF_Q4D(SF_BF16);
