@@ -114,6 +114,30 @@ def test_turned_rows_and_reading_back(dev, dtype, KVH, D, group):
     assert ((new - odd.float()).abs() <= 0.5 * s + 2.0 ** -10 * (m.abs() + 15 * s)).all()
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("H,KVH,D,group,P", [(32, 8, 128, 64, 64), (14, 2, 64, 32, 32), (6, 3, 80, 80, 12), (3, 1, 256, 128, 128)])
+def test_many_rows_equal_their_parts(dev, H, KVH, D, group, P, interleaved):
+    """Enough heads that a workgroup takes several in turn: the bits of the same rows in parts, and
+    nothing else of the cache."""
+    hb = 256 // (1 << (D // 8 - 1).bit_length())  # heads that a workgroup's threads hold
+    B = 2
+    T = 3 * 1024 * hb // (B * (H + 2 * KVH)) + 37
+    part = T // 3 + 1
+    g = torch.Generator(device=dev).manual_seed(D)
+    qkv = torch.randn(B, T, (H + 2 * KVH) * D, generator=g, device=dev).half()
+    pos = torch.randint(0, 1 << 20, (B, T), generator=g, dtype=torch.int32, device=dev)
+    w = (1 + 0.3 * torch.randn(2, D, generator=g, device=dev)).half()
+    inv = torch.from_numpy(1e4 ** (-np.arange(P, dtype=np.float64) / P)).to(dev)
+    lengths = torch.tensor([5, 90], dtype=torch.int32, device=dev)
+    one, two = (buffers(B, KVH, T + 50, D, group, dev) for _ in range(2))  # (the second sequence runs over the end)
+    how = dict(n_heads=H, q_weight=w[0], k_weight=w[1], interleaved=interleaved, out_dtype=torch.float16)
+    q = rotary_kv_append_q4(qkv, pos, inv, *one, lengths=lengths, **how)
+    parts = [rotary_kv_append_q4(qkv[:, a:a + part].contiguous(), pos[:, a:a + part].contiguous(), inv, *two, lengths=lengths + a,
+                                 **how) for a in range(0, T, part)]
+    assert torch.equal(torch.cat(parts, 1), q)
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(one, two))
+
+
 def test_ties_constants_and_ranges(dev):
     """Exact ties go to the even code; a constant group is its minimum; a range past fp16's ends
     is held at them; what is not finite reads back as NaN, in its group alone."""
