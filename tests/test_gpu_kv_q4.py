@@ -138,6 +138,19 @@ def test_many_rows_equal_their_parts(dev, H, KVH, D, group, P, interleaved):
     assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(one, two))
 
 
+@pytest.mark.parametrize("D,group", [(48, 48), (80, 80), (112, 112), (96, 32), (240, 240), (256, 64), (64, 64)])
+def test_reading_back_many_slots(dev, D, group):
+    """Slots that several workgroups share, at words a slot that divide a workgroup's and that do not."""
+    kc, kp, _, _ = buffers(2, 3, 307, D, group, dev)
+    for a, b in ((0, 307), (6, 300)):
+        want = O.values(kc[:, :, a:b].cpu().numpy(), kp[:, :, a:b].float().cpu().numpy())[0]
+        for out in DT.values():
+            got = dequantize_kv_q4(kc[:, :, a:b], kp[:, :, a:b], out)
+            # m + s code rounded to fp32, then to the type
+            tol = (torch.finfo(out).eps / 2 + 2.0 ** -24) * (1 + 2.0 ** -8) * abs(want) + 2.0 ** -25
+            assert (abs(got.double().cpu().numpy() - want) <= tol).all()
+
+
 def test_ties_constants_and_ranges(dev):
     """Exact ties go to the even code; a constant group is its minimum; a range past fp16's ends
     is held at them; what is not finite reads back as NaN, in its group alone."""
