@@ -115,7 +115,8 @@ def test_turned_rows_and_reading_back(dev, dtype, KVH, D, group):
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
-@pytest.mark.parametrize("H,KVH,D,group,P", [(32, 8, 128, 64, 64), (14, 2, 64, 32, 32), (6, 3, 80, 80, 12), (3, 1, 256, 128, 128)])
+@pytest.mark.parametrize("H,KVH,D,group,P", [(32, 8, 128, 64, 64), (14, 2, 64, 32, 32), (6, 3, 80, 80, 12), (3, 1, 256, 128, 128),
+                                             (1, 1, 16, 16, 8)])
 def test_many_rows_equal_their_parts(dev, H, KVH, D, group, P, interleaved):
     """Enough heads that a workgroup takes several in turn: the bits of the same rows in parts, and
     nothing else of the cache."""
@@ -136,6 +137,26 @@ def test_many_rows_equal_their_parts(dev, H, KVH, D, group, P, interleaved):
                                  **how) for a in range(0, T, part)]
     assert torch.equal(torch.cat(parts, 1), q)
     assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(one, two))
+
+
+@pytest.mark.parametrize("H,KVH,D,group,P", [(32, 8, 128, 64, 64), (1, 1, 16, 16, 4), (14, 2, 64, 32, 32)])
+def test_many_sequences_equal_one_by_one(dev, H, KVH, D, group, P):
+    """One token each of more sequences than a workgroup takes heads, lengths of their own."""
+    B = 1500
+    g = torch.Generator(device=dev).manual_seed(D)
+    qkv = torch.randn(B, 1, (H + 2 * KVH) * D, generator=g, device=dev)
+    pos = torch.randint(0, 1 << 20, (B, 1), generator=g, device=dev)
+    inv = torch.from_numpy(1e4 ** (-np.arange(P, dtype=np.float64) / P)).to(dev)
+    lengths = torch.randint(-2, 9, (B,), generator=g, dtype=torch.int32, device=dev)
+    one, two = (buffers(B, KVH, 7, D, group, dev) for _ in range(2))
+    q = rotary_kv_append_q4(qkv, pos, inv, *one, n_heads=H, lengths=lengths)
+    some = [0, 1, 2, 127, 128, 511, 777, 1498, 1499]
+    for i in some:
+        at = slice(i, i + 1)
+        part = [t[at].clone() for t in two]  # (buffers of their own: a cache starts on 16 bytes)
+        y = rotary_kv_append_q4(qkv[at], pos[at], inv, *part, n_heads=H, lengths=lengths[at])
+        assert torch.equal(y, q[at])
+        assert all(torch.equal(a[at].view(torch.uint8), b.view(torch.uint8)) for a, b in zip(one, part)), i
 
 
 @pytest.mark.parametrize("D,group", [(48, 48), (80, 80), (112, 112), (96, 32), (240, 240), (256, 64), (64, 64)])

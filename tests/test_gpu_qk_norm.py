@@ -56,6 +56,25 @@ def test_forward_and_gradients(dev, dtype, interleaved, B, T, H, KVH, D, P):
     assert torch.equal(again[0], y[0]) and torch.equal(again[1], y[1]) and torch.equal(one[0], y[0]) and one[1] is None
 
 
+@pytest.mark.parametrize("B,T,H,KVH,D,P", [(2, 32768, 1, 1, 8, 4), (2, 40001, 1, 1, 6, 3), (3, 1, 40000, 33000, 8, 4),
+                                           (2, 2, 32767, 1, 16, 8), (5000, 1, 3, 1, 8, 4), (3, 32767, 1, 1, 8, 2)])
+def test_many_rows_heads_and_sequences(dev, B, T, H, KVH, D, P):
+    """Past what a lane divides by a product: rows a sequence, heads a row, sequences of a workgroup."""
+    g = torch.Generator().manual_seed(T)
+    q, k = (torch.randn(B, T, n, D, generator=g).to(dev).requires_grad_() for n in (H, KVH))
+    wq, wk = ((1 + 0.3 * torch.randn(D, generator=g)).to(dev).requires_grad_() for _ in range(2))
+    gq, gk = (torch.randn(B, T, n, D, generator=g).to(dev) for n in (H, KVH))
+    pos = torch.randint(0, 1 << 20, (B, T), generator=g, dtype=torch.int32).to(dev)
+    y = qk_norm_rotary(q, k, pos, torch.from_numpy(freqs(P)).to(dev), wq, wk)
+    got = torch.autograd.grad(y, (q, k, wq, wk), (gq, gk))
+    for i, (x, w, gy) in enumerate(((q, wq, gq), (k, wk, gk))):
+        x64, w64, g64 = (t.detach().double().cpu().numpy() for t in (x, w, gy))
+        close(y[i], *O.qk_norm_rotary(x64, w64, pos.cpu().numpy(), freqs(P)))
+        dx, dw, edx, edw = O.qk_norm_rotary_backward(x64, w64, g64, pos.cpu().numpy(), freqs(P))
+        close(got[i], dx, edx)
+        close(got[2 + i], dw, edw)
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 def test_strides_in_place_and_weight_types(dev, dtype):
     g = torch.Generator().manual_seed(3)
