@@ -21,7 +21,8 @@
 //     by a power of two a row, P times the V scale under 2^15 likewise: what the low part drops is
 //     below 2^-22 of the value and, where a row's weights span more, 2^-30 of the row's largest.
 //     fp16 and bf16 queries are exact in the high part alone; for a bf16 output the low parts are
-//     left out (2^-12 of a weight or of q beside the 2^-9 of the output's rounding).
+//     left out: a weight beside V's codes is off by 2^-11 at most, which moves an output by that
+//     much of sum(p s c), an eighth of what its rounding (2^-8) may; an fp32 q by 2^-11 of itself.
 // Maxima, sums, m's part and the partials are fp32.
 #include <math.h>
 
@@ -95,9 +96,10 @@ __device__ __forceinline__ void q4_numbers(const Q4Magic &g, uint32_t w, half2_t
   p[3] += half2_t{b, b};
 }
 
-__device__ __forceinline__ half8_t q4_signed(const Q4Magic &g, uint32_t w) {
+template <int LESS>
+__device__ __forceinline__ half8_t q4_lifted(const Q4Magic &g, uint32_t w) {
   half2_t p[4];
-  q4_numbers<8>(g, w, p);
+  q4_numbers<LESS>(g, w, p);
   return half8_t{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
 }
 
@@ -144,6 +146,9 @@ __global__ void __launch_bounds__(kQaThreads, q4_resident(DP, NGT, PK, QSPLIT))
 k_q4_split(Q4Attn a) {
   constexpr bool ANY = NGT == 0;
   constexpr float kCode = PSPLIT ? 1.f : 16777216.f;  // what an operand of K's codes is to be multiplied by
+  // V's codes less 8, the 8 s with m, where the weights' two parts leave nothing: a weight rounded to
+  // fp16 beside the codes and exact beside 8 s would leave 8 s times its rounding, whatever the value is.
+  constexpr int kLess = PSPLIT ? 8 : 0;
   constexpr int KS = DP / 32, DB = DP / 16, NGM = ANY ? 8 : NGT;
   constexpr int RP = 16 / PK, HV = 4 / PK, NV = 4 * HV;  // rows, h's and values of a column
   constexpr int PITCH = DP / 2 + 8;  // 16 neighbouring rows' 8 bytes fall on different banks
@@ -171,7 +176,7 @@ k_q4_split(Q4Attn a) {
   uint32_t pr[2][NGM];
   Q4Magic magic;
   magic.hold();
-  auto k_codes = [&](uint32_t w) { return PSPLIT ? q4_signed(magic, w) : q4_codes(w); };
+  auto k_codes = [&](uint32_t w) { return PSPLIT ? q4_lifted<8>(magic, w) : q4_codes(w); };
   // (slots are clamped into the cache; a tile's addresses are its own and a lane's 32-bit offset)
   auto load_k = [&](int j) {
     const uint8_t *const at = a.kc + (base + 64 * (size_t)j) * rowb;
@@ -303,13 +308,13 @@ k_q4_split(Q4Attn a) {
   }
 
   uint8_t *const vt = smem + wave * kWave;
-  // parameters a group, slot 16 g + 4 i + h at 16 h + 4 g + i: K's s and m (m + 8 s), V's s and m + 8 s
+  // parameters a group, slot 16 g + 4 i + h at 16 h + 4 g + i: K's s and m (m + 8 s), V's alike
   float *const kss = (float *)(vt + kTile), *const kos = kss + 64 * NGM;
   float *const vss = kos + 64 * NGM, *const vos = vss + 64 * NGM;
   float *const vms = NGM > 1 ? vos + 64 * NGM : vss;  // a slot's largest V scale
   float m = -INFINITY, lsum = 0.f;  // base-2 softmax of the column
   float mul = 1.2980742e33f;        // 2^110 at most: the first tile sets it
-  float am[NGM];                    // sum of p (m + 8 s) over the lane's slots
+  float am[NGM];                    // sum of p m (kLess: p (m + 8 s)) over the lane's slots
   float4_t O[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) O[d] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -333,7 +338,7 @@ k_q4_split(Q4Attn a) {
       kss[to] = q4_lo(pr[0][i]);
       kos[to] = PSPLIT ? fmaf(8.f, q4_lo(pr[0][i]), q4_hi(pr[0][i])) : q4_hi(pr[0][i]);
       vss[to] = q4_lo(pr[1][i]);
-      vos[to] = fmaf(8.f, q4_lo(pr[1][i]), q4_hi(pr[1][i]));
+      vos[to] = PSPLIT ? fmaf(8.f, q4_lo(pr[1][i]), q4_hi(pr[1][i])) : q4_hi(pr[1][i]);
     }
     if (!ANY || D % 32 == 0) {
       const int n16 = D / 32;
@@ -486,7 +491,7 @@ k_q4_split(Q4Attn a) {
         if (ANY ? 16 * d < gi * a.g || 16 * d >= (gi + 1) * a.g : d / (2 * (KSGT ? KSGT : 1)) != gi) continue;
         const v2i vw = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
             (__attribute__((address_space(3))) v2i *)(vt + (16 * g + hl) * PITCH + 8 * d));
-        const half8_t x0 = q4_signed(magic, (uint32_t)vw.x), x1 = q4_signed(magic, (uint32_t)vw.y);
+        const half8_t x0 = q4_lifted<kLess>(magic, (uint32_t)vw.x), x1 = q4_lifted<kLess>(magic, (uint32_t)vw.y);
         O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, sf_bitcast<half8_t>(ph[0]), O[d], 0, 0, 0);
         O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, sf_bitcast<half8_t>(ph[1]), O[d], 0, 0, 0);
         if constexpr (PSPLIT) {

@@ -1,0 +1,59 @@
+"""What attention over a 4-bit cache keeps of its operands' bits, against the 64-bit oracle: values
+of one sign, scores whose parts cancel, small values beside large ones."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_q4 as O
+from siliconfer_amd.kernels.kv_q4 import attention_q4kv
+from test_gpu_attn_q4 import DT, cache
+
+pytestmark = pytest.mark.gpu
+
+
+def of_codes(codes, s, m, group, dev):
+    """A cache's (codes, params) of codes [B, KVH, n, D] and, a group, s and m [B, KVH, n, D / group]."""
+    params = np.stack(np.broadcast_arrays(s, m), -1).astype(np.float16)
+    assert params.shape[:3] == codes.shape[:3] and params.shape[3] * group == codes.shape[3]
+    return [torch.from_numpy(O.pack(codes)).to(dev), torch.from_numpy(params).to(dev)]
+
+
+def close(got, q, bufs, lengths, rounded, factors, more=(), scale=None):
+    """|got - oracle| within its bound for weights (and V) off by `rounded` and scores' factors by
+    `factors`, half a step of got's type, and the bounds that `more` V's (codes, params) have."""
+    host = lambda bufs: [t.cpu().numpy().astype(np.float64 if t.is_floating_point() else np.uint8) for t in bufs]
+    k, x = host(bufs[:2]), q.double().cpu().numpy()
+    want, bound = O.attention(x, *k, *host(bufs[2:]), lengths, scale, rounded, factors)
+    for v in more:
+        bound = bound + O.attention(x, *k, *host(v), lengths, scale, rounded, factors)[1]
+    g = got.double().cpu().numpy()
+    tol = bound + torch.finfo(got.dtype).eps / 2 * (abs(want) + bound) + (2.0 ** -25 if got.dtype == torch.float16 else 0)
+    assert (abs(g - want) <= tol).all(), float((abs(g - want) / np.maximum(tol, 1e-300)).max())
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("H,KVH,D,group", [(4, 2, 64, 64), (4, 1, 64, 32), (8, 2, 128, 32), (4, 2, 80, 80)])
+@pytest.mark.parametrize("rows", [1, 3, 9, 20])
+def test_values_of_one_sign(dev, rows, H, KVH, D, group, dtype):
+    """Codes of 0 stand for the minimum alone. For a bf16 output weights are rounded to fp16 (2^-11)
+    beside the codes: what that leaves is in proportion to the value, so a dim of zeros is exactly 0.
+    Others hold weights to 2^-22 beside a code less 8, and 8 s in fp32 with the minimum: they are off
+    by the bound of values of 8 s besides."""
+    B, bf16 = 2, dtype == "bf16"
+    g = np.random.default_rng(rows)
+    for n in (2, 64, 700):
+        codes = g.integers(0, 16, (B, KVH, n, D))
+        codes[..., ::3] = 0
+        s = g.uniform(0.5, 1.5, (B, KVH, n, D // group)).astype(np.float16)
+        k = cache(B, KVH, n, D, group, dev, seed=n)[:2]
+        eights = of_codes(np.full_like(codes, 8), s, np.zeros_like(s), group, dev)
+        q = torch.randn(B, rows, H, D, generator=torch.Generator().manual_seed(n)).to(DT[dtype]).to(dev)
+        for part in (0.0, 1 / 32):
+            bufs = k + of_codes(codes, s, (s * part).astype(np.float16), group, dev)
+            for n_splits in (1, 2):
+                y = attention_q4kv(q, *bufs, lengths=n, n_splits=n_splits, out_dtype=DT[dtype])
+                close(y, q, bufs, [n] * B, *((2.0 ** -11, 2.0 ** -22) if bf16 else (2.0 ** -22, 2.0 ** -22)),
+                      more=() if bf16 else (eights,))
+                if part == 0 and bf16:
+                    assert (y[..., ::3] == 0).all()
