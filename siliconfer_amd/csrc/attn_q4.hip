@@ -20,9 +20,10 @@
 //   * q (fp32) and P as fp16 high and low parts, q brought to a largest magnitude of 2^13..2^14
 //     by a power of two a row, P times the V scale under 2^15 likewise: what the low part drops is
 //     below 2^-22 of the value and, where a row's weights span more, 2^-30 of the row's largest.
-//     fp16 and bf16 queries are exact in the high part alone; for a bf16 output the low parts are
-//     left out: a weight beside V's codes is off by 2^-11 at most, which moves an output by that
-//     much of sum(p s c), an eighth of what its rounding (2^-8) may; an fp32 q by 2^-11 of itself.
+//     fp16 and bf16 queries are exact in the high part alone; with them and a bf16 output P's low
+//     part is left out: a weight beside V's codes is off by 2^-11 at most, which moves an output by
+//     that much of sum(p s c), an eighth of what its rounding (2^-8) may. What an fp32 q would lose
+//     is multiplied by the score's size in the exponent: it keeps both parts whatever the output.
 // Maxima, sums, m's part and the partials are fp32.
 #include <math.h>
 
@@ -613,7 +614,7 @@ k_q4_merge(const float *__restrict__ part_acc, const float *__restrict__ part_ml
 // end. A tile goes straight to LDS, the next one while it is worked on: S^T = K q^T, a base-2
 // softmax a column and O^T = V^T P^T on v_mfma_f32_32x32x16_f16, the next tile's scores
 // between the softmax's instructions.
-// For a bf16 output q, P and the values are fp16's high parts: a value off by 2^-12 moves an
+// For a bf16 output of 16-bit queries P and the values are fp16's high parts: a value off by 2^-12 moves an
 // output by less than a fifth of its own rounding (2^-9). Other outputs take three products
 // of the high and low parts.
 // What fp16 cannot hold: a tile with an s past 2^11 or an m past 2^14 is taken at 2^-6 (K's
@@ -747,7 +748,8 @@ template <int QDT, bool SPLIT, int D, int KG>
 __global__ void __launch_bounds__(256 * KG, 2)
 k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__ flags) {
   constexpr int NFW = D / 32, NDB = D / 32;
-  constexpr int PARTS = SPLIT ? 2 : 1, QP = QDT == SF_F32 && SPLIT ? 2 : 1;
+  constexpr int PARTS = SPLIT ? 2 : 1, QP = QDT == SF_F32 ? 2 : 1;
+  static_assert(SPLIT || QDT != SF_F32, "fp32 queries keep both parts");
   constexpr int NT = SPLIT ? 1 : 2, TS = 32 * NT;  // blocks and slots a tile
   constexpr int BLOCK = (int)q4_block_bytes(D, PARTS), KB_ = 2 * NFW;  // V's fragments come after K's
   typedef float float16_t __attribute__((ext_vector_type(16)));
@@ -816,10 +818,8 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
         } else {
           qf[0][i][2 * e] = (f16)x;
           qf[0][i][2 * e + 1] = (f16)y;
-          if constexpr (QP == 2) {
-            qf[1][i][2 * e] = (f16)(x - (float)qf[0][i][2 * e]);
-            qf[1][i][2 * e + 1] = (f16)(y - (float)qf[0][i][2 * e + 1]);
-          }
+          qf[1][i][2 * e] = (f16)(x - (float)qf[0][i][2 * e]);
+          qf[1][i][2 * e + 1] = (f16)(y - (float)qf[0][i][2 * e + 1]);
         }
       }
   }
@@ -1018,7 +1018,7 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
       } else {
         uint32_t u[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = SPLIT ? sf_bitcast<uint16_t>((f16)v[i]) : sf_f32_to_bf16(v[i]);
+        for (int i = 0; i < 4; ++i) u[i] = SPLIT && a.odt == SF_F16 ? sf_bitcast<uint16_t>((f16)v[i]) : sf_f32_to_bf16(v[i]);
         *(u32x2 *)((uint16_t *)a.out + o + 32 * d + 8 * e4) = u32x2{u[0] | u[1] << 16, u[2] | u[3] << 16};
       }
     }
@@ -1058,6 +1058,10 @@ int q4_splits(int B, int Tq, int H, int KVH, int T_max, int D, int group, bool s
   return n_splits > kQaMaxSplits ? kQaMaxSplits : n_splits < 1 ? 1 : n_splits;
 }
 
+// Whether P (on prompts K and V too) go in two parts: what an fp16 part alone loses is below a bf16
+// output's rounding, but for the exponents of fp32 queries.
+bool q4_whole(int q_dtype, int out_dtype) { return out_dtype != SF_BF16 || q_dtype == SF_F32; }
+
 size_t q4_parts(long long rows, int D, int S, size_t *ml_off) {
   *ml_off = sf_align256((size_t)rows * S * D * sizeof(float));
   return S > 1 ? *ml_off + (size_t)rows * S * 2 * sizeof(float) : 0;
@@ -1069,8 +1073,8 @@ extern "C" size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int 
                                              int out_dtype, int n_splits) {
   if (B <= 0 || Tq <= 0 || H <= 0 || KVH <= 0 || H % KVH || T_max < 0 || T_max > kQaMaxSlots || D <= 0 || group <= 0) return 0;
   size_t ml;
-  if (const size_t many = q4_many_bytes(B, Tq, H, KVH, T_max, D, out_dtype == SF_BF16 ? 1 : 2)) return many;
-  return q4_parts((long long)B * Tq * H, D, q4_splits(B, Tq, H, KVH, T_max, D, group, out_dtype != SF_BF16 && q_dtype == SF_F32, n_splits),
+  if (const size_t many = q4_many_bytes(B, Tq, H, KVH, T_max, D, q4_whole(q_dtype, out_dtype) ? 2 : 1)) return many;
+  return q4_parts((long long)B * Tq * H, D, q4_splits(B, Tq, H, KVH, T_max, D, group, q_dtype == SF_F32, n_splits),
                   &ml);
 }
 
@@ -1087,7 +1091,7 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   if (int rc = sf_q4_cache_check(D, group)) return rc;
   SF_REQUIRE(T_max <= kQaMaxSlots, SF_EUNSUPPORTED, "T_max=%d: at most %d slots", T_max, kQaMaxSlots);
   const long long nrb = ((long long)Tq * (H / KVH) + 15) / 16, rows = (long long)B * Tq * H;
-  const size_t many = q4_many_bytes(B, Tq, H, KVH, T_max, D, out_dtype == SF_BF16 ? 1 : 2);
+  const size_t many = q4_many_bytes(B, Tq, H, KVH, T_max, D, q4_whole(q_dtype, out_dtype) ? 2 : 1);
   SF_REQUIRE((many ? (long long)B * KVH <= 65535 : KVH * nrb <= 65535) && B <= 65535 && rows <= 0x7fffffffLL, SF_EINVAL,
              "B=%d KVH=%d rows=%d exceed the grid", B, KVH, Tq);
   SF_REQUIRE(q_dtype >= SF_F32 && q_dtype <= SF_BF16 && out_dtype >= SF_F32 && out_dtype <= SF_BF16, SF_EINVAL,
@@ -1095,7 +1099,7 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   SF_REQUIRE(q && k_codes && k_params && v_codes && v_params && out, SF_EINVAL, "null pointer argument");
   SF_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_params | (uintptr_t)v_params | (uintptr_t)q) & 15) == 0,
              SF_EINVAL, "q and cache buffers must be 16-byte aligned");
-  n_splits = many ? 1 : q4_splits(B, Tq, H, KVH, T_max, D, group, out_dtype != SF_BF16 && q_dtype == SF_F32, n_splits);
+  n_splits = many ? 1 : q4_splits(B, Tq, H, KVH, T_max, D, group, q_dtype == SF_F32, n_splits);
   size_t ml_off;
   const size_t parts = q4_parts(rows, D, n_splits, &ml_off), need = many ? many : parts;
   SF_REQUIRE(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0), SF_EINVAL, "workspace must be 256-byte aligned");
@@ -1120,7 +1124,7 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
     // between barriers of their own; else eight, which halves the longest columns' walk. us, four /
     // eight waves: bf16, 376 workgroups 51.6 / 54.1, 1024 (4096 rows) 168 / 181, 166 (14 / 2 heads
     // of 64) 32.3 / 27.3; fp32 (whose tiles are half as long) at 376 110 / 104, fp16 97 / 89.
-    const bool four = out_dtype == SF_BF16 && blocks > 256;
+    const bool four = !q4_whole(q_dtype, out_dtype) && blocks > 256;
 #define SF_QR(QD, SP, DD)                                                                                        \
   do {                                                                                                           \
     uint32_t *const fl = (uint32_t *)(ws + tiles.x * (size_t)tiles.y * 2 * q4_block_bytes(DD, SP ? 2 : 1));      \
@@ -1130,16 +1134,16 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
     }                                                                                                            \
     if (SP || !four) k_q4_rows<QD, SP, DD, 2><<<blocks, 512, 0, st>>>(r, ws, fl);                                \
   } while (0)
-#define SF_QR_O(QD)                                  \
-  do {                                               \
-    if (out_dtype == SF_BF16 && D == 64) SF_QR(QD, false, 64);  \
-    else if (out_dtype == SF_BF16) SF_QR(QD, false, 128);       \
-    else if (D == 64) SF_QR(QD, true, 64);           \
-    else SF_QR(QD, true, 128);                       \
+#define SF_QR_O(QD, SP)                  \
+  do {                                   \
+    if (D == 64) SF_QR(QD, SP, 64);      \
+    else SF_QR(QD, SP, 128);             \
   } while (0)
-    if (q_dtype == SF_F32) SF_QR_O(SF_F32);
-    else if (q_dtype == SF_F16) SF_QR_O(SF_F16);
-    else SF_QR_O(SF_BF16);
+    if (q_dtype == SF_F32) SF_QR_O(SF_F32, true);
+    else if (q_dtype == SF_F16 && out_dtype == SF_BF16) SF_QR_O(SF_F16, false);
+    else if (q_dtype == SF_F16) SF_QR_O(SF_F16, true);
+    else if (out_dtype == SF_BF16) SF_QR_O(SF_BF16, false);
+    else SF_QR_O(SF_BF16, true);
 #undef SF_QR_O
 #undef SF_QR
     return sf_check_launch("sf_attn_q4kv");
@@ -1163,9 +1167,9 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
     else if (D <= 128) SF_QA(QS, PS, 128, 0, 0, 1);           \
     else SF_QA(QS, PS, 256, 0, 0, 1);                         \
   } while (0)
-  if (out_dtype == SF_BF16) SF_QA_D(false, false);  // (a bf16 output leaves out the low parts of fp32 queries too)
-  else if (q_dtype == SF_F32) SF_QA_D(true, true);
-  else SF_QA_D(false, true);
+  if (q_dtype == SF_F32) SF_QA_D(true, true);
+  else if (out_dtype != SF_BF16) SF_QA_D(false, true);
+  else SF_QA_D(false, false);
 #undef SF_QA_D
 #undef SF_QA_R
 #undef SF_QA

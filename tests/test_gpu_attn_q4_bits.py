@@ -57,3 +57,26 @@ def test_values_of_one_sign(dev, rows, H, KVH, D, group, dtype):
                       more=() if bf16 else (eights,))
                 if part == 0 and bf16:
                     assert (y[..., ::3] == 0).all()
+
+
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("H,KVH,D,group,rows", [(4, 2, 64, 32, 1), (8, 2, 128, 64, 3), (4, 1, 96, 32, 9), (32, 16, 64, 32, 260),
+                                                (16, 8, 128, 64, 260)])
+def test_scores_whose_parts_cancel(dev, rows, H, KVH, D, group, out):
+    """fp32 queries of two large dims, over keys of t and 2 - t there: their scores are apart by what
+    fp16 cannot hold of the queries, whatever type the output has. V is t too."""
+    B, n = 2, 300
+    g = np.random.default_rng(D)
+    codes = np.zeros((B, KVH, n, D), np.int64)
+    codes[..., 0] = g.integers(1, 16, (B, KVH, n))
+    codes[..., D // 2] = 16 - codes[..., 0]
+    s = np.full((B, KVH, n, D // group), 0.125)
+    bufs = 2 * of_codes(codes, s, np.zeros_like(s), group, dev)
+    q = torch.zeros(B, rows, H, D)
+    q[..., 0] = 1000 + torch.rand(B, rows, H, generator=torch.Generator().manual_seed(rows))
+    q[..., D // 2] = 1000 + torch.rand(B, rows, H, generator=torch.Generator().manual_seed(rows + 1))
+    q = q.to(dev)
+    y = attention_q4kv(q, *bufs, lengths=n, scale=1.0, out_dtype=DT[out])
+    # (V and weights: both in two parts; V's codes less 8, as above)
+    eights = of_codes(np.full_like(codes, 8), s, np.zeros_like(s), group, dev)
+    close(y, q, bufs, [n] * B, 2.0 ** -21, 2.0 ** -22, (eights,), 1.0)
