@@ -614,8 +614,11 @@ k_q4_merge(const float *__restrict__ part_acc, const float *__restrict__ part_ml
 // end. A tile goes straight to LDS, the next one while it is worked on: S^T = K q^T, a base-2
 // softmax a column and O^T = V^T P^T on v_mfma_f32_32x32x16_f16, the next tile's scores
 // between the softmax's instructions.
-// For a bf16 output of 16-bit queries P and the values are fp16's high parts: a value off by 2^-12 moves an
-// output by less than a fifth of its own rounding (2^-9). Other outputs take three products
+// For a bf16 output of 16-bit queries P and the values are rounded to fp16, 2^-11 of each at most: P's
+// and V's rounding move an output by that much of sum(p |v|), an eighth of what its own (2^-8) may.
+// K's is multiplied by the score's size in the exponent: a weight is off by up to 2^-11 of
+// scale sum |q k|, what a K held in fp16 would give. (K in two parts: 1500 rows below 74 us instead of
+// 52, 4096 rows 242 instead of 180.) Other outputs, and fp32 queries, take three products
 // of the high and low parts.
 // What fp16 cannot hold: a tile with an s past 2^11 or an m past 2^14 is taken at 2^-6 (K's
 // scores and V's sums times 2^6 again; what such a tile holds beside them is off by 2^-19 at
@@ -905,10 +908,10 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
           q4_halves<true>(x, z, hi, lo);
           ph[s][p] = hi;
           pl[s][p] = lo;
-        } else {  // cut to fp16; their sum is the cut weights', so that a cut takes from both alike
-          const auto w = __builtin_amdgcn_cvt_pkrtz(x, z);
+        } else {  // rounded to fp16; their sum is the rounded weights', so that both are off alike
+          const half2_t w = __builtin_convertvector(float2_t{x, z}, half2_t);
           ph[s][p] = sf_bitcast<uint32_t>(w);
-          lsum = __builtin_amdgcn_fdot2(sf_bitcast<half2_t>(w), half2_t{(f16)1.f, (f16)1.f}, lsum, false);
+          lsum = __builtin_amdgcn_fdot2(w, half2_t{(f16)1.f, (f16)1.f}, lsum, false);
         }
       }
     // (one product to some vector instructions, operands read ahead)

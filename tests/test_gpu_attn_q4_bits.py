@@ -80,3 +80,25 @@ def test_scores_whose_parts_cancel(dev, rows, H, KVH, D, group, out):
     # (V and weights: both in two parts; V's codes less 8, as above)
     eights = of_codes(np.full_like(codes, 8), s, np.zeros_like(s), group, dev)
     close(y, q, bufs, [n] * B, 2.0 ** -21, 2.0 ** -22, (eights,), 1.0)
+
+
+def test_weights_of_a_prompt_are_rounded(dev):
+    """bf16 queries and outputs, many rows: slot 0 holds 1 and weighs about what all others, which hold
+    -1, weigh together. K and V are exact in fp16, so that a row is off by its weights' rounding, 2^-11
+    at most of the others', and by its own."""
+    H, KVH, D, rows, n = 16, 8, 128, 260, 300
+    k, v = (np.zeros((1, KVH, n, D, 1)) for _ in range(2))
+    k[:, :, 1:, 0], v[:, :, :], v[:, :, 0] = 1, -1, 1  # (codes of dim 0 below: 0 for slot 0, else 1, of -1 each)
+    codes = k[..., 0].astype(np.int64)
+    s, zero = np.full((1, KVH, n, 2), -1.0), np.zeros((1, KVH, n, 2))
+    bufs = of_codes(codes, s, zero, 64, dev) + of_codes(np.zeros_like(codes), zero, v[..., :2, 0], 64, dev)
+    others = torch.arange(n - rows, n, dtype=torch.float64)
+    q = torch.zeros(1, rows, H, D, dtype=torch.float64)
+    q[..., 0] = (others.log()[None, :, None] + torch.randn(1, rows, H, generator=torch.Generator().manual_seed(0)) / 32)
+    q = q.to(dev, torch.bfloat16)
+    y = attention_q4kv(q, *bufs, lengths=n, scale=1.0, out_dtype=torch.bfloat16).double().cpu()
+    w = others[:, None] * torch.exp(-q[0, :, :, 0].double().cpu())  # of the others together, slot 0 weighing 1
+    want = (1 - w) / (1 + w)
+    # fp32: a score's products with 1.44 and 2^f, the sums of 300 weights
+    tol = w / (1 + w) * 2.0 ** -11 * (want + 1 + 2.0 ** -10) + want.abs() * 2.0 ** -8 + 400 * 2.0 ** -24
+    assert ((y[0] - want[..., None]).abs() <= tol[..., None]).all(), ((y[0] - want[..., None]).abs() / tol[..., None]).max().item()
