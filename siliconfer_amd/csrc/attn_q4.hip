@@ -240,7 +240,7 @@ k_q4_split(Q4Attn a) {
   };
   auto load_p = [&](int j) {
     const size_t at = (base + 64 * (size_t)j) * NG;
-    const int last = (a.T_cap - 64 * j) * NG - 1;
+    const int last = min(a.T_cap - 64 * j, 64) * NG - 1;  // (slots first: a capacity times its groups may pass 2^31)
 #pragma unroll
     for (int i = 0; i < NGM; ++i) {
       if (ANY && i >= NG) break;
