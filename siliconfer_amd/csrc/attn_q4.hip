@@ -620,10 +620,10 @@ k_q4_merge(const float *__restrict__ part_acc, const float *__restrict__ part_ml
 // scale sum |q k|, what a K held in fp16 would give. (K in two parts: 1500 rows below 74 us instead of
 // 52, 4096 rows 242 instead of 180.) Other outputs, and fp32 queries, take three products
 // of the high and low parts.
-// What fp16 cannot hold: a tile with an s past 2^11 or an m past 2^14 is taken at 2^-6 (K's
-// scores and V's sums times 2^6 again; what such a tile holds beside them is off by 2^-19 at
-// most); parameters that are not finite stand as zeros in V,
-// and the columns that see them get NaN in their group's dims.
+// What fp16 cannot hold: a tile of K, and a group of a tile of V, that has values past 65504 is taken
+// at 2^-6 (K's scores and V's sums times 2^6 again; what it holds beside them is off by 2^-15 at
+// most: s and m by 2^-19 each); parameters that are not finite stand as zeros in V, and the columns
+// that see them get NaN in their group's dims.
 // Measured, 32 / 8 heads of 128, bf16: 4096 rows 168 us (818 TFLOP/s of the products; a large
 // fp16 matrix product reaches 1215 on this card), 1500 rows behind 300 51.6 us, of which 6 the
 // first launch; both bound by the softmax's instructions and the products beside them, the
@@ -635,11 +635,12 @@ k_q4_merge(const float *__restrict__ part_acc, const float *__restrict__ part_ml
 __host__ __device__ constexpr size_t q4_block_bytes(int D, int parts) { return (size_t)parts * D / 8 * 1024; }
 __host__ __device__ inline size_t q4_tiles(int T_max) { return ((size_t)T_max + 63) / 64; }
 
-// What of a parameter word fp16 cannot carry: 1: s past 2^11 or m past 2^14, 2: not finite.
-__device__ __forceinline__ uint32_t q4_off(uint32_t w) {
-  const uint32_t x = w & 0x7fffu, y = w >> 16 & 0x7fffu;
-  return x >= 0x7c00u || y >= 0x7c00u ? 2u : x > 0x6800u || y > 0x7400u ? 1u : 0u;
-}
+// Whether a parameter word is not finite, or stands for values past fp16's range (the last
+// code's; m itself is fp16).
+__device__ __forceinline__ bool q4_none(uint32_t w) { return (w & 0x7fffu) >= 0x7c00u || (w >> 16 & 0x7fffu) >= 0x7c00u; }
+__device__ __forceinline__ bool q4_past(uint32_t w) { return !q4_none(w) && fabsf(fmaf(15.f, q4_lo(w), q4_hi(w))) >= 65520.f; }
+// A tile's flags of V: a bit a group that is taken at 2^-6, and
+constexpr uint32_t kV6 = 15, kVNone = 256;  // something not finite
 
 // One workgroup a tile of 64 slots of one kv head.
 template <bool SPLIT, int D>
@@ -672,16 +673,17 @@ k_q4_spread(Q4Attn a, uint8_t *__restrict__ ws, uint32_t *__restrict__ flags) {
   if (64 * j + ptok >= n) vpr = 0;
   if (tid < 2) flag[tid] = 0;
   __syncthreads();
-  const uint32_t ok = q4_off(kpr), ov = q4_off(vpr);
-  if (ok) atomicOr(&flag[0], ok);
-  if (ov) atomicOr(&flag[1], ov);
+  const bool none = q4_none(vpr);
+  if (q4_past(kpr)) atomicOr(&flag[0], 1u);
+  if (q4_past(vpr)) atomicOr(&flag[1], 1u << pg);
+  if (none) atomicOr(&flag[1], kVNone);
   uint2 *dst = (uint2 *)(raw + vtok * PITCH + 4 * NFW * vpiece);  // (rows on 8 bytes)
 #pragma unroll
   for (int i = 0; i < NFW; i += 2) dst[i / 2] = uint2{vr[i], vr[i + 1]};
   __syncthreads();
   const uint32_t fk = flag[0], fv = flag[1];
   if (tid < 2) flags[((size_t)bk * q4_tiles(a.T_max) + j) * 2 + tid] = flag[tid];
-  const float kdown = fk & 1 ? 0.015625f : 1.f, vdown = fv & 1 ? 0.015625f : 1.f;
+  const float kdown = fk ? 0.015625f : 1.f, vdown = fv >> pg & 1 & kV6 ? 0.015625f : 1.f;
   Q4Magic magic;
   magic.hold();
   // eight values of one slot, or of eight slots (s, m one each), as operand parts
@@ -717,11 +719,10 @@ k_q4_spread(Q4Attn a, uint8_t *__restrict__ ws, uint32_t *__restrict__ flags) {
     }
   }
   if (has_p) {
-    const bool fine = !(ov & 2);
     const int u = ptok & 31, e = 4 * (u >> 3) + (u & 3);
     const int to = 32 * (ptok >> 5) + 16 * (e >> 3) + 8 * (u >> 2 & 1) + (e & 7);
-    vsm[0][pg][to] = fine ? (f16)(q4_lo(vpr) * vdown) : (f16)0.f;
-    vsm[1][pg][to] = fine ? (f16)(q4_hi(vpr) * vdown) : (f16)0.f;
+    vsm[0][pg][to] = none ? (f16)0.f : (f16)(q4_lo(vpr) * vdown);
+    vsm[1][pg][to] = none ? (f16)0.f : (f16)(q4_hi(vpr) * vdown);
   }
   __syncthreads();
   constexpr int NR = D == 128 ? 2 : 1;  // transposing reads, two fragments each
@@ -866,7 +867,7 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
     load(it + 1, true);
     if (TS * j >= hi_lim || j >= ntot) return;  // no column of the wave sees it (uniform)
     const uint32_t fk = fl[2 * (NT * j / 2)], fv = fl[2 * (NT * j / 2) + 1];
-    const float mul = fk & 1 ? qmul * 64.f : qmul;
+    const float mul = fk ? qmul * 64.f : qmul;
     if (TS * j + TS > lo_lim) {  // the lane's slots 32 t + 8 (e / 4) + 4 h + e % 4
       const int left = lim - TS * j - 4 * h;
 #pragma unroll
@@ -889,9 +890,9 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
       for (int d = 0; d < NDB; ++d) O[d] *= cf;
       m = m_new;
     }
-    if (fv & 1) {
+    if (fv & kV6) {
 #pragma unroll
-      for (int d = 0; d < NDB; ++d) O[d] *= 0.015625f;
+      for (int d = 0; d < NDB; ++d) O[d] *= fv >> 32 * d / a.g & 1 ? 0.015625f : 1.f;
     }
     const float shift = kP - sf_merge_mref(m);
     score(it + 1, NFW, 2 * NFW, next);
@@ -954,15 +955,15 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
         }
       }
     }
-    if (fv & 1) {
+    if (fv & kV6) {
 #pragma unroll
-      for (int d = 0; d < NDB; ++d) O[d] *= 64.f;
+      for (int d = 0; d < NDB; ++d) O[d] *= fv >> 32 * d / a.g & 1 ? 64.f : 1.f;
     }
-    if (fv & 2) {  // what is not finite, for the columns that see it
+    if (fv & kVNone) {  // what is not finite, for the columns that see it
       for (int t = TS * j; t < min(TS * j + TS, lim); ++t)
 #pragma unroll
         for (int d = 0; d < NDB; ++d)
-          if (q4_off(a.vp[((size_t)bk * a.T_cap + t) * NG + 32 * d / a.g]) & 2) {
+          if (q4_none(a.vp[((size_t)bk * a.T_cap + t) * NG + 32 * d / a.g])) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) O[d][e] = NAN;
           }

@@ -102,3 +102,31 @@ def test_weights_of_a_prompt_are_rounded(dev):
     # fp32: a score's products with 1.44 and 2^f, the sums of 300 weights
     tol = w / (1 + w) * 2.0 ** -11 * (want + 1 + 2.0 ** -10) + want.abs() * 2.0 ** -8 + 400 * 2.0 ** -24
     assert ((y[0] - want[..., None]).abs() <= tol[..., None]).all(), ((y[0] - want[..., None]).abs() / tol[..., None]).max().item()
+
+
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("H,KVH,D,group", [(32, 16, 64, 32), (16, 8, 128, 64)])
+def test_small_values_beside_large_ones_of_a_prompt(dev, H, KVH, D, group, out):
+    """Many rows over tiles whose first group holds values up to 20000 and whose others a thousandth: in K
+    (the queries are 0 beside the large ones, and large beside the small) and in V. Then some of V's
+    large ones past fp16's range: the other groups keep theirs all the same."""
+    B, n, rows = 2, 300, 260
+    g = np.random.default_rng(D)
+    codes = [g.integers(0, 16, (B, KVH, n, D)) for _ in range(2)]
+    s = g.uniform(0.5, 1.5, (B, KVH, n, D // group)) * 1e-4
+    m = -7.5 * s
+    s[..., 0], m[..., 0] = 2700, -20000
+    bufs = of_codes(codes[0], s, m, group, dev) + of_codes(codes[1], s, m, group, dev)
+    gen = torch.Generator().manual_seed(D)
+    q = 3000 * torch.randn(B, rows, H, D, generator=gen)
+    q[..., :group] = 0
+    q = q.to(DT[out]).to(dev)
+    whole = out != "bf16"  # (a bf16 output: weights and V in fp16, and K where rows are many)
+    how = (2.0 ** -21, 2.0 ** -22) if whole else (2.0 ** -10, 2.0 ** -11)
+    eights = of_codes(np.full_like(codes[1], 8), s, np.zeros_like(s), group, dev)  # (where codes are taken less 8)
+    y = attention_q4kv(q, *bufs, lengths=n, out_dtype=DT[out])
+    close(y, q, bufs, [n] * B, *how, more=(eights,) if whole else ())
+    far = [t.clone() for t in bufs]
+    far[3][:, :, ::7, 0, 0] = 60000  # up to 880000 in the first group
+    z = attention_q4kv(q, *far, lengths=n, out_dtype=DT[out])
+    assert torch.equal(z[..., group:], y[..., group:])
