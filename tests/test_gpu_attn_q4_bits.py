@@ -129,4 +129,9 @@ def test_small_values_beside_large_ones_of_a_prompt(dev, H, KVH, D, group, out):
     far = [t.clone() for t in bufs]
     far[3][:, :, ::7, 0, 0] = 60000  # up to 880000 in the first group
     z = attention_q4kv(q, *far, lengths=n, out_dtype=DT[out])
-    assert torch.equal(z[..., group:], y[..., group:])
+    # (160 workgroups of 64 dims in two parts are too few for the kernel of many rows; few rows' weights share one
+    # factor: 2^-38 of the largest weight times scale is their last place, here 60000 2^-38 beside scales of 1e-4)
+    if D == 128 or not whole:
+        assert torch.equal(z[..., group:], y[..., group:])
+    else:
+        assert ((z - y)[..., group:].abs() <= n * 8 * 60000 * 2.0 ** -38).all()
