@@ -498,7 +498,7 @@ int sf_kv_q4_dequant(const uint8_t *codes, const void *params, void *out, int ou
  * NULL; row t sees the first n_b - Tq + t + 1 slots, a row that sees none gives zeros, and what
  * a row does not see may hold anything. n_splits <= 0: the kernel's own choice; at most 128
  * are used, none where many rows (prompts) go their own way. The workspace (sf_attn_q4_workspace_bytes, 256-byte aligned; none for 0 bytes)
- * needs no clearing. q and the cache's buffers 16-byte aligned. */
+ * needs no clearing. q, out and the cache's buffers 16-byte aligned. */
 size_t sf_attn_q4_workspace_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int group,
                                   int q_dtype, int out_dtype, int n_splits);
 int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, const void *k_params,

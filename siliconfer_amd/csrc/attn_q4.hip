@@ -1101,8 +1101,9 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   SF_REQUIRE(q_dtype >= SF_F32 && q_dtype <= SF_BF16 && out_dtype >= SF_F32 && out_dtype <= SF_BF16, SF_EINVAL,
              "bad q/out dtype");
   SF_REQUIRE(q && k_codes && k_params && v_codes && v_params && out, SF_EINVAL, "null pointer argument");
-  SF_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_params | (uintptr_t)v_params | (uintptr_t)q) & 15) == 0,
-             SF_EINVAL, "q and cache buffers must be 16-byte aligned");
+  SF_REQUIRE((((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)k_params | (uintptr_t)v_params | (uintptr_t)q |
+               (uintptr_t)out) & 15) == 0,
+             SF_EINVAL, "q, out and cache buffers must be 16-byte aligned");
   n_splits = many ? 1 : q4_splits(B, Tq, H, KVH, T_max, D, group, q_dtype == SF_F32, n_splits);
   size_t ml_off;
   const size_t parts = q4_parts(rows, D, n_splits, &ml_off), need = many ? many : parts;

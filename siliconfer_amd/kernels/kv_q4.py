@@ -187,6 +187,9 @@ def attention_q4kv(q: torch.Tensor, k_codes: torch.Tensor, k_params: torch.Tenso
         out = torch.empty_like(q, dtype=out_dtype)
     elif out.shape != q.shape or out.device != q.device or not out.is_contiguous():
         raise SFError("out must be contiguous, of q's shape and on its device")
+    elif out.data_ptr() % 16:
+        return out.copy_(attention_q4kv(q, k_codes, k_params, v_codes, v_params, lengths=lengths, add=add,
+                                        max_length=max_length, n_splits=n_splits, scale=scale, out_dtype=out.dtype))
     lib = _lib.load()
     with _lib.on_device(q):
         st = _lib.stream(q)

@@ -135,3 +135,18 @@ def test_small_values_beside_large_ones_of_a_prompt(dev, H, KVH, D, group, out):
         assert torch.equal(z[..., group:], y[..., group:])
     else:
         assert ((z - y)[..., group:].abs() <= n * 8 * 60000 * 2.0 ** -38).all()
+
+
+@pytest.mark.parametrize("out", list(DT))
+@pytest.mark.parametrize("rows", [1, 5, 260])
+def test_an_output_at_any_address(dev, rows, out):
+    """A contiguous `out` that starts off 16 bytes holds what an aligned one holds, and nothing around
+    it is written."""
+    bufs = cache(1, 16, 300, 128, 64, dev)
+    q = torch.randn(1, rows, 32, 128, generator=torch.Generator().manual_seed(0)).to(dev, DT[out])
+    want = attention_q4kv(q, *bufs, lengths=300, out_dtype=DT[out])
+    for off in (1, 2, 4, 7, 8):
+        flat = torch.full((want.numel() + 16,), 7.0, dtype=DT[out], device=dev)
+        y = flat[off:off + want.numel()].view(want.shape)
+        assert attention_q4kv(q, *bufs, lengths=300, out=y) is y
+        assert torch.equal(y, want) and (flat[:off] == 7).all() and (flat[off + want.numel():] == 7).all()
