@@ -42,7 +42,7 @@ from .._lib import SFError
 from ..kernels.rotary import qk_norm_rotary, rotary, rotary_kv_append
 from .config import ModelConfig, rope_freqs as _rope_freqs_np
 from .kv_cache import BoundedKVCache, Q4KVCache, QuantizedKVCache, dequantize_kv
-from .q4_linear import Q4Linear, project_group
+from .q4_linear import Q4Linear, _plain, project_group
 from .rope import Rotary
 
 
@@ -144,7 +144,8 @@ class Attention(torch.nn.Module):
     the head, scaled frequencies). A `BoundedKVCache`, at any batch, scores its slots
     and drops the least attended ones; of a prompt, the last OBSERVED rows score. A
     `Q4KVCache`, at any batch, is in 4 bits. `qk_norm` adds `q_norm` and `k_norm`, an
-    RMSNorm over each head of queries and keys (None otherwise)."""
+    RMSNorm over each head of queries and keys (None otherwise). They go with the turn in one launch;
+    a hooked or replaced one is called on the heads [B, T, heads, D] instead."""
 
     OBSERVED = 16
 
@@ -211,8 +212,11 @@ class Attention(torch.nn.Module):
             if qkv is None:
                 qkv = torch.cat([t.reshape(B * T, -1) for t in (q, k, v)], dim=1).contiguous()
         if four:
-            qw, kw, eps = self._norms()
-            q = cache.append_rotary(qkv.view(B, T, -1), H, KVH, self._rotary_of(None), qw, kw, eps)
+            norms = self._norms()
+            if norms is None:
+                q = self._normed_rows(qkv.view(B, T, -1), cache, cache.length())
+            else:
+                q = cache.append_rotary(qkv.view(B, T, -1), H, KVH, self._rotary_of(None), *norms)
             return _project(self.o_proj, cache.attend(q, self.scale).reshape(B, T, H * D)), cache
         if bounded:
             out = self._bounded(qkv.view(B, T, -1), cache)
@@ -250,26 +254,35 @@ class Attention(torch.nn.Module):
         return _project(self.o_proj, a.transpose(1, 2).reshape(B, T, H * D)), new_cache
 
     def _norms(self):
-        """(q's weights, k's weights, eps) of the heads' norms; None, None where there are none."""
-        if self.q_norm is None:
+        """(q's weights, k's weights, eps) of the heads' norms, as one launch takes them; None, None where
+        there are none. None: two eps, or a norm whose own call does something else."""
+        a, b = self.q_norm, self.k_norm
+        if a is None:
             return None, None, 0.0
-        return self.q_norm.weight, self.k_norm.weight, self.q_norm.eps
+        return (a.weight, b.weight, a.eps) if _plain(a, RMSNorm) and _plain(b, RMSNorm) and a.eps == b.eps else None
 
     def _turn(self, q: torch.Tensor, k: torch.Tensor, offset: int):
         """q, k [B, heads, T, D] (normed and) turned at positions offset .. in their layout."""
         r = self._rotary_of(None)
         pos = torch.arange(offset, offset + q.shape[2], dtype=torch.int32, device=q.device)
         q, k, how = q.transpose(1, 2), k.transpose(1, 2), dict(interleaved=r.interleaved, scale=r.scale)
-        qw, kw, eps = self._norms()
-        if qw is None:
-            q, k = rotary(q, k, pos, r.on(q.device), **how)
+        norms, f = self._norms(), r.on(q.device)
+        if norms is None:
+            a, b = self.q_norm, self.k_norm
+            if _plain(a, RMSNorm) and _plain(b, RMSNorm):  # (each with its own eps)
+                q, k = (qk_norm_rotary(x, None, pos, f, m.weight, eps=m.eps, **how)[0] for x, m in ((q, a), (k, b)))
+            else:
+                q, k = rotary(a(q), b(k), pos, f, **how)
+        elif norms[0] is None:
+            q, k = rotary(q, k, pos, f, **how)
         else:
-            q, k = qk_norm_rotary(q, k, pos, r.on(q.device), qw, kw, eps=eps, **how)
+            qw, kw, eps = norms
+            q, k = qk_norm_rotary(q, k, pos, f, qw, kw, eps=eps, **how)
         return q.transpose(1, 2), k.transpose(1, 2)
 
-    def _normed_rows(self, qkv: torch.Tensor, cache: QuantizedKVCache, offset: int) -> torch.Tensor:
-        """q|k|v rows [B, T, (H + 2 KVH) D] with normed heads: k (turned) and v appended to an
-        int8 cache, the turned q [B, T, H, D] returned."""
+    def _normed_rows(self, qkv: torch.Tensor, cache, offset: int) -> torch.Tensor:
+        """q|k|v rows [B, T, (H + 2 KVH) D] with normed heads: k (turned) and v appended to a
+        cache in codes, the turned q [B, T, H, D] returned."""
         H, KVH = self.num_heads, self.num_kv_heads
         q, k, v = (t.transpose(1, 2) for t in qkv.unflatten(-1, (-1, self.head_dim)).split((H, KVH, KVH), dim=2))
         q, k = self._turn(q, k, offset)

@@ -71,10 +71,10 @@ def _rows(x2: torch.Tensor) -> torch.Tensor:
     return x2 if x2.dtype in _ACT_DTYPES else x2.float()
 
 
-def _plain(lin) -> bool:
-    """lin(x) is Q4Linear.forward and nothing else: no hook, override or subclass sees the call."""
-    return (type(lin) is Q4Linear and "forward" not in lin.__dict__ and not lin._forward_hooks
-            and not lin._forward_pre_hooks and not lin._backward_hooks and not lin._backward_pre_hooks
+def _plain(module, cls=Q4Linear) -> bool:
+    """module(x) is cls.forward and nothing else: no hook, override or subclass sees the call."""
+    return (type(module) is cls and "forward" not in module.__dict__ and not module._forward_hooks
+            and not module._forward_pre_hooks and not module._backward_hooks and not module._backward_pre_hooks
             and not torch.nn.modules.module._has_any_global_hook())
 
 
