@@ -433,7 +433,10 @@ class TransformerBlock(torch.nn.Module):
         with torch.no_grad():
             blk.input_layernorm.weight.copy_(_f32(weights[f"{pre}.input_layernorm.weight"]))
             blk.post_attention_layernorm.weight.copy_(_f32(weights[f"{pre}.post_attention_layernorm.weight"]))
-            if blk.self_attn.q_norm is not None:
-                blk.self_attn.q_norm.weight.copy_(_f32(weights[norms[0]]))
-                blk.self_attn.k_norm.weight.copy_(_f32(weights[norms[1]]))
+            at = blk.self_attn
+            for norm, proj, name in ((at.q_norm, at.q_proj, norms[0]), (at.k_norm, at.k_proj, norms[1])):
+                if norm is not None:
+                    norm.weight.copy_(_f32(weights[name]))
+                    # (beside int4 codes nothing else of the layer has a gradient)
+                    norm.weight.requires_grad_(not isinstance(proj, Q4Linear))
         return blk

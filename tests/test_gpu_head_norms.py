@@ -79,3 +79,33 @@ def test_hooks_of_the_norms_are_called(dev, cache, B):
         handle.remove()
         plain.k_norm.weight.div_(2)
         assert torch.equal(run(attn, x, CACHES[cache]()), run(plain, x, CACHES[cache]()))
+
+
+def test_int4_layers_keep_no_graph(dev, tmp_path):
+    """Beside int4 projections a checkpoint's head norms take no gradients: steps over a cache of tensors
+    without `no_grad` keep no graph. Asked for, they have them; dense layers' norms do as the projections."""
+    import numpy as np
+
+    from siliconfer_amd.engine.loader import load_model
+    from siliconfer_amd.engine.q4_loader import pack_and_replace_linears
+    from siliconfer_amd.model import TransformerBlock, compute_rope_freqs
+    from test_loader import TINY, tiny_checkpoint
+
+    tiny_checkpoint(tmp_path, cfg=TINY, seed=1)
+    cfg, w = load_model(tmp_path)
+    for n in "qk":
+        w[f"model.layers.0.self_attn.{n}_norm.weight"] = np.ones(cfg.head_dim, np.float32)
+    freqs = compute_rope_freqs(cfg, dev)
+    dense = TransformerBlock.from_weights(cfg, w, 0, freqs, device=dev).self_attn
+    pack_and_replace_linears(w, cfg, 64, pack_sym=True)
+    attn = TransformerBlock.from_weights(cfg, w, 0, freqs, 64, dev).self_attn
+    for m, on in ((dense, True), (attn, False)):
+        assert m.q_norm.weight.requires_grad is on and m.k_norm.weight.requires_grad is on
+    x = torch.randn(1, 4, cfg.hidden_size, generator=torch.Generator().manual_seed(0)).to(dev)
+    cache = None
+    for t in range(4):
+        y, cache = attn(x[:, t:t + 1], cache)
+        assert not y.requires_grad and not cache[0].requires_grad
+    attn.k_norm.weight.requires_grad_()
+    attn(x)[1][0].sum().backward()
+    assert attn.k_norm.weight.grad.shape == (cfg.head_dim,)
