@@ -17,6 +17,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .._lib import SFError
@@ -57,12 +58,25 @@ def _rows(x: torch.Tensor, name: str) -> None:
         raise SFError(f"{name}: a head's dims must be contiguous")
 
 
+def _no_tangents(*tensors) -> None:
+    """Raise for a tensor with a forward-mode tangent, which a kernel would drop."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise SFError("no forward-mode derivatives here: a tensor has a tangent")
+
+
+def _forward_mode() -> bool:
+    # (_current_level: asking each tensor costs a microsecond a call)
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, *,
            interleaved: bool = False, scale: float = 1.0, out_q: torch.Tensor | None = None,
            out_k: torch.Tensor | None = None):
     """(q turned, k turned) at positions [B, T] or [T], in q's dtype. `out_q` /
     `out_k` may be the inputs themselves; other outputs must not overlap them, and
-    inputs that need a gradient take none. Differentiable in q and k."""
+    inputs that need a gradient take none. Differentiable in q and k (in reverse mode)."""
+    if _forward_mode():
+        _no_tangents(q, k)
     if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
         if out_q is not None or out_k is not None:
             raise SFError("rotary: inputs that need a gradient take no out_q / out_k")
@@ -151,7 +165,9 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Ten
     q's heads and one for k's), then turned as `rotary` turns it, in one pass in fp32 and one
     rounding to q's dtype. D <= 256. `out_q` / `out_k` may be the inputs themselves; other
     outputs must not overlap them, and inputs that need a gradient take none. Differentiable
-    in q, k and the weights (once)."""
+    in q, k and the weights (once, in reverse mode)."""
+    if _forward_mode():
+        _no_tangents(q, k, q_weight, k_weight)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         if out_q is not None or out_k is not None:
             raise SFError("qk_norm_rotary: inputs that need a gradient take no out_q / out_k")
