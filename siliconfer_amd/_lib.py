@@ -234,14 +234,15 @@ class _Scratch(threading.local):
 
 
 _scratch = _Scratch()
+SCRATCH_HELD = 64 << 20  # bytes that a thread keeps a stream; more goes back to torch's allocator after its call
 
 
 def scratch(device: torch.device, stream_handle: int, nbytes: int) -> torch.Tensor:
     """Workspace of one call: kept a (host thread, device, stream) and grown on demand. A
     thread's calls on a stream run one after the other; two threads' launches on it may
     interleave, since a call gives up the interpreter's lock. While a graph is recorded a
-    tensor of the graph's own, so that no two graphs share one."""
-    if torch._C._cuda_isCurrentStreamCapturing():
+    tensor of the graph's own, so that no two graphs share one; past SCRATCH_HELD one of the call's own."""
+    if nbytes > SCRATCH_HELD or torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
     held, key = _scratch.held, (device, stream_handle)
     ws = held.get(key)
