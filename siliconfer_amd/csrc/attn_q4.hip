@@ -1094,6 +1094,7 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   SF_REQUIRE(H % KVH == 0, SF_EINVAL, "n_heads=%d not a multiple of n_kv_heads=%d", H, KVH);
   if (int rc = sf_q4_cache_check(D, group)) return rc;
   SF_REQUIRE(T_max <= kQaMaxSlots, SF_EUNSUPPORTED, "T_max=%d: at most %d slots", T_max, kQaMaxSlots);
+  SF_REQUIRE(isfinite(scale * 1.4426950408889634f), SF_EINVAL, "scale %g is not finite in base 2", scale);
   const long long nrb = ((long long)Tq * (H / KVH) + 15) / 16, rows = (long long)B * Tq * H;
   const size_t many = q4_many_bytes(B, Tq, H, KVH, T_max, D, q4_whole(q_dtype, out_dtype) ? 2 : 1);
   SF_REQUIRE((many ? (long long)B * KVH <= 65535 : KVH * nrb <= 65535) && B <= 65535 && rows <= 0x7fffffffLL, SF_EINVAL,
