@@ -410,6 +410,10 @@ class TransformerBlock(torch.nn.Module):
         normed = [n in weights for n in norms]
         if any(normed) != all(normed):
             raise SFError(f"{pre}: a norm of queries' or keys' heads without the other's")
+        for n in norms if all(normed) else ():
+            shape = tuple(weights[n].shape)
+            if shape != (config.head_dim,) or n[:-len("weight")] + "bias" in weights:
+                raise SFError(f"{n} {list(shape)}: need one weight a dim of a head, [{config.head_dim}], and no bias")
         blk = cls(config, rope_freqs, dev, rotary, qk_norm=all(normed))
         for parent, mod in (("self_attn", blk.self_attn), ("mlp", blk.mlp)):
             for name in (("q_proj", "k_proj", "v_proj", "o_proj") if parent == "self_attn"
