@@ -169,6 +169,8 @@ def make_quantized_cache(n_layers: int, capacity: int = 4096, scale_dtype: torch
                          bits: int = 8, group: int | None = None) -> list:
     """One fresh QuantizedKVCache per transformer layer, or with bits=4 a Q4KVCache with groups
     of `group` dims."""
+    if bits == 4 and scale_dtype is not torch.float16:
+        raise SFError(f"a 4-bit cache holds scales and minima in float16, not {scale_dtype}")
     if bits == 4:
         return [Q4KVCache(capacity, group) for _ in range(n_layers)]
     if bits != 8 or group is not None:
