@@ -16,6 +16,8 @@ reference's fp32 scales).
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from .. import _lib
@@ -244,6 +246,16 @@ class Q4KVCache:
         self._kc, self._kp, self._vc, self._vp = new
         self.capacity = cap
 
+    @contextlib.contextmanager
+    def _or_as_before(self):
+        """An append that is refused leaves the buffers as they were."""
+        held = self._kc, self._kp, self._vc, self._vp, self.capacity
+        try:
+            yield
+        except BaseException:
+            self._kc, self._kp, self._vc, self._vp, self.capacity = held
+            raise
+
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """Append keys that are turned already, and values, [B, KVH, T, D] (any strides)."""
         from ..kernels.kv_q4 import kv_append_q4
@@ -251,8 +263,9 @@ class Q4KVCache:
             raise SFError("k and v must be device tensors of the same shape [B, n_kv_heads, T, head_dim] and dtype")
         _lib.dt(k)  # (all before any buffer is made for them)
         B, KVH, T, D = k.shape
-        self.reserve(B, KVH, D, self._len + T, k.device)
-        kv_append_q4(k, v, *self.buffers(), lengths=self._len)
+        with self._or_as_before():
+            self.reserve(B, KVH, D, self._len + T, k.device)
+            kv_append_q4(k, v, *self.buffers(), lengths=self._len)
         self._len += T
 
     def update(self, k: torch.Tensor, v: torch.Tensor):
@@ -275,11 +288,12 @@ class Q4KVCache:
         heads = n_heads + 2 * n_kv_heads
         if not (n_heads > 0 and n_kv_heads > 0 and n_heads % n_kv_heads == 0 and W > 0 and W % heads == 0):
             raise SFError(f"qkv {list(qkv.shape)} does not hold {n_heads} and 2 x {n_kv_heads} heads")
-        self.reserve(B, n_kv_heads, W // heads, self._len + T, qkv.device)
-        positions = torch.arange(self._len, self._len + T, dtype=torch.int32, device=qkv.device)
-        q = rotary_kv_append_q4(qkv, positions, rotary.on(qkv.device), *self.buffers(), n_heads=n_heads,
-                                lengths=self._len, q_weight=q_weight, k_weight=k_weight, eps=eps,
-                                interleaved=rotary.interleaved, scale=rotary.scale, out_dtype=out_dtype)
+        with self._or_as_before():
+            self.reserve(B, n_kv_heads, W // heads, self._len + T, qkv.device)
+            positions = torch.arange(self._len, self._len + T, dtype=torch.int32, device=qkv.device)
+            q = rotary_kv_append_q4(qkv, positions, rotary.on(qkv.device), *self.buffers(), n_heads=n_heads,
+                                    lengths=self._len, q_weight=q_weight, k_weight=k_weight, eps=eps,
+                                    interleaved=rotary.interleaved, scale=rotary.scale, out_dtype=out_dtype)
         self._len += T
         return q
 
