@@ -233,7 +233,7 @@ class Attention(torch.nn.Module):
             offset = cache[0].shape[2]
         else:
             offset = 0
-        if self.rotary is not None or self.q_norm is not None:
+        if self.rotary is not None or self._normed():
             q, k = self._turn(q, k, offset)
         else:
             q = apply_rope(q, offset, self.rope_freqs)
@@ -253,11 +253,14 @@ class Attention(torch.nn.Module):
         a = _sdpa_causal(q, kc, vc, offset, self.scale)
         return _project(self.o_proj, a.transpose(1, 2).reshape(B, T, H * D)), new_cache
 
+    def _normed(self) -> bool:
+        return self.q_norm is not None or self.k_norm is not None
+
     def _norms(self):
         """(q's weights, k's weights, eps) of the heads' norms, as one launch takes them; None, None where
-        there are none. None: two eps, or a norm whose own call does something else."""
+        there are none. None: one alone, two eps, or a norm whose own call does something else."""
         a, b = self.q_norm, self.k_norm
-        if a is None:
+        if not self._normed():
             return None, None, 0.0
         return (a.weight, b.weight, a.eps) if _plain(a, RMSNorm) and _plain(b, RMSNorm) and a.eps == b.eps else None
 
@@ -272,7 +275,7 @@ class Attention(torch.nn.Module):
             if _plain(a, RMSNorm) and _plain(b, RMSNorm):  # (each with its own eps)
                 q, k = (qk_norm_rotary(x, None, pos, f, m.weight, eps=m.eps, **how)[0] for x, m in ((q, a), (k, b)))
             else:
-                q, k = rotary(a(q), b(k), pos, f, **how)
+                q, k = rotary(q if a is None else a(q), k if b is None else b(k), pos, f, **how)
         elif norms[0] is None:
             q, k = rotary(q, k, pos, f, **how)
         else:
@@ -294,7 +297,7 @@ class Attention(torch.nn.Module):
         over the whole cache, then what exceeds its bound dropped."""
         B, T, _ = qkv.shape
         H, KVH, D = self.num_heads, self.num_kv_heads, self.head_dim
-        if self.q_norm is not None:
+        if self._normed():
             q = self._normed_rows(qkv, cache, cache.seen)
         else:
             q = cache.append_rotary(qkv, H, KVH, self._rotary_of(None))
@@ -326,7 +329,7 @@ class Attention(torch.nn.Module):
         kq, ks, vq, vs = cache.buffers()
         T_cap = kq.shape[2]
         st = _lib.stream(qkv)
-        if self.q_norm is not None:
+        if self._normed():
             q_rot = self._normed_rows(qkv.view(1, T, -1), cache, offset).view(T, H, D)
             kq, ks, vq, vs = cache.buffers()
         elif self.rotary is not None:

@@ -81,6 +81,19 @@ def test_hooks_of_the_norms_are_called(dev, cache, B):
         assert torch.equal(run(attn, x, CACHES[cache]()), run(plain, x, CACHES[cache]()))
 
 
+@pytest.mark.parametrize("cache", list(CACHES))
+@pytest.mark.parametrize("name", ["q_norm", "k_norm"])
+def test_one_norm_alone(dev, cache, name):
+    """With the other taken out: as with one that leaves its heads as they are."""
+    attn, plain = layer(dev, None), layer(dev, None)
+    setattr(attn, name, None)
+    setattr(plain, name, torch.nn.Identity())
+    x = torch.randn(1, 24, 128, generator=torch.Generator().manual_seed(2)).to(dev)
+    with torch.no_grad():
+        assert torch.equal(run(attn, x, CACHES[cache]()), run(plain, x, CACHES[cache]()))
+        assert err(run(layer(dev, None), x, CACHES[cache]()), run(plain, x, CACHES[cache]())) > 0.05
+
+
 def test_int4_layers_keep_no_graph(dev, tmp_path):
     """Beside int4 projections a checkpoint's head norms take no gradients: steps over a cache of tensors
     without `no_grad` keep no graph. Asked for, they have them; dense layers' norms do as the projections."""
