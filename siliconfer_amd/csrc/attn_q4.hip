@@ -20,10 +20,11 @@
 //   * q (fp32) and P as fp16 high and low parts, q brought to a largest magnitude of 2^13..2^14
 //     by a power of two a row, P times the V scale under 2^15 likewise: what the low part drops is
 //     below 2^-22 of the value and, where a row's weights span more, 2^-30 of the row's largest.
-//     fp16 and bf16 queries are exact in the high part alone; with them and a bf16 output P's low
-//     part is left out: a weight beside V's codes is off by 2^-11 at most, which moves an output by
-//     that much of sum(p s c), an eighth of what its rounding (2^-8) may. What an fp32 q would lose
-//     is multiplied by the score's size in the exponent: it keeps both parts whatever the output.
+//     fp16 and bf16 queries are exact in the high part alone. (Without P's low part, a bf16 output of
+//     four ragged sequences of up to 32767 slots takes 32.5 us, not 36.7: every weight off by up to
+//     2^-11, some percent of the outputs rounded the other way.)
+//   * codes less 8, with 8 s joined to m, keep the products' sums small: the matrix units cut what
+//     they add to a sum, 2^-24 of it each time. For a bf16 output the codes stand as they are.
 // Maxima, sums, m's part and the partials are fp32.
 #include <math.h>
 
@@ -107,15 +108,13 @@ __device__ __forceinline__ half8_t q4_lifted(const Q4Magic &g, uint32_t w) {
 __device__ __forceinline__ float q4_lo(uint32_t w) { return (float)sf_bitcast<f16>((uint16_t)(w & 0xffffu)); }
 __device__ __forceinline__ float q4_hi(uint32_t w) { return (float)sf_bitcast<f16>((uint16_t)(w >> 16)); }
 
-// Two fp32 values as a pair of fp16 high parts and, SPLIT, of what they leave.
-template <bool SPLIT>
+// Two fp32 values as a pair of fp16 high parts and one of what they leave.
 __device__ __forceinline__ void q4_halves(float a, float b, uint32_t &hi, uint32_t &lo) {
   a = sf_opaque(a);
   b = sf_opaque(b);
   const f16 x = (f16)a, y = (f16)b;
   hi = sf_bitcast<uint16_t>(x) | (uint32_t)sf_bitcast<uint16_t>(y) << 16;
-  if constexpr (SPLIT)
-    lo = sf_bitcast<uint16_t>((f16)(a - (float)x)) | (uint32_t)sf_bitcast<uint16_t>((f16)(b - (float)y)) << 16;
+  lo = sf_bitcast<uint16_t>((f16)(a - (float)x)) | (uint32_t)sf_bitcast<uint16_t>((f16)(b - (float)y)) << 16;
 }
 
 // Workgroups of k_q4_split that a CU's registers hold without (much) spilling.
@@ -136,20 +135,17 @@ __host__ __device__ constexpr int q4_resident(int DP, int groups, int PK, bool Q
 // a product passes 2^15, and grows where a reference that moves shrinks the products behind it.
 // It is 2^110 at most: a weight, up to 2^8, stays finite times it beside a scale of 0.
 // DP: the head's dims rounded up to 64, 128 or 256. NGT groups of 32 KSGT dims fill it
-// exactly, or 0, 0: any head and groups. QSPLIT, PSPLIT: q, P in two parts.
+// exactly, or 0, 0: any head and groups. QSPLIT: q in two parts. SIGNED: codes less 8.
 // Bound by vector instructions and the waits between them. Traced, with the merge launch, 32 / 8
 // heads of 128: four ragged sequences of up to 32767 slots, bf16, groups of 64 (111 MB) 28.7 + 5.1
 // us, the SIMDs issuing vector instructions 62% of that time (of some 680 a tile 290 turn codes
 // into operands); one sequence of 131071, fp16, groups of 128 (143 MB) 30.9 + 4.5, 4.6 TB/s in the
 // split; sixteen of up to 4001 with fp32 queries (51 MB) 20.9 + 4.0, both q and P in two parts.
-template <bool QSPLIT, bool PSPLIT, int DP, int NGT, int KSGT, int PK>
+template <bool QSPLIT, bool SIGNED, int DP, int NGT, int KSGT, int PK>
 __global__ void __launch_bounds__(kQaThreads, q4_resident(DP, NGT, PK, QSPLIT))
 k_q4_split(Q4Attn a) {
   constexpr bool ANY = NGT == 0;
-  constexpr float kCode = PSPLIT ? 1.f : 16777216.f;  // what an operand of K's codes is to be multiplied by
-  // V's codes less 8, the 8 s with m, where the weights' two parts leave nothing: a weight rounded to
-  // fp16 beside the codes and exact beside 8 s would leave 8 s times its rounding, whatever the value is.
-  constexpr int kLess = PSPLIT ? 8 : 0;
+  constexpr float kCode = SIGNED ? 1.f : 16777216.f;  // what an operand of K's codes is to be multiplied by
   constexpr int KS = DP / 32, DB = DP / 16, NGM = ANY ? 8 : NGT;
   constexpr int RP = 16 / PK, HV = 4 / PK, NV = 4 * HV;  // rows, h's and values of a column
   constexpr int PITCH = DP / 2 + 8;  // 16 neighbouring rows' 8 bytes fall on different banks
@@ -177,7 +173,7 @@ k_q4_split(Q4Attn a) {
   uint32_t pr[2][NGM];
   Q4Magic magic;
   magic.hold();
-  auto k_codes = [&](uint32_t w) { return PSPLIT ? q4_lifted<8>(magic, w) : q4_codes(w); };
+  auto k_codes = [&](uint32_t w) { return SIGNED ? q4_lifted<8>(magic, w) : q4_codes(w); };
   // (slots are clamped into the cache; a tile's addresses are its own and a lane's 32-bit offset)
   auto load_k = [&](int j) {
     const uint8_t *const at = a.kc + (base + 64 * (size_t)j) * rowb;
@@ -301,7 +297,7 @@ k_q4_split(Q4Attn a) {
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float v = f[ks][(i >> 1) + 4 * (i & 1)] * by, part = !PSPLIT && (i >> 1) & 1 ? 0.0625f : 1.f;
+        const float v = f[ks][(i >> 1) + 4 * (i & 1)] * by, part = !SIGNED && (i >> 1) & 1 ? 0.0625f : 1.f;
         const f16 hi = (f16)v;
         qh8[ks][i] = (f16)((float)hi * part);
         if constexpr (QSPLIT) ql8[ks][i] = (f16)((v - (float)hi) * part);
@@ -309,13 +305,13 @@ k_q4_split(Q4Attn a) {
   }
 
   uint8_t *const vt = smem + wave * kWave;
-  // parameters a group, slot 16 g + 4 i + h at 16 h + 4 g + i: K's s and m (m + 8 s), V's alike
+  // parameters a group, slot 16 g + 4 i + h at 16 h + 4 g + i: K's s and m (SIGNED: m + 8 s), V's alike
   float *const kss = (float *)(vt + kTile), *const kos = kss + 64 * NGM;
   float *const vss = kos + 64 * NGM, *const vos = vss + 64 * NGM;
   float *const vms = NGM > 1 ? vos + 64 * NGM : vss;  // a slot's largest V scale
   float m = -INFINITY, lsum = 0.f;  // base-2 softmax of the column
   float mul = 1.2980742e33f;        // 2^110 at most: the first tile sets it
-  float am[NGM];                    // sum of p m (kLess: p (m + 8 s)) over the lane's slots
+  float am[NGM];                    // sum of p m (SIGNED: p (m + 8 s)) over the lane's slots
   float4_t O[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) O[d] = float4_t{0.f, 0.f, 0.f, 0.f};
@@ -337,9 +333,9 @@ k_q4_split(Q4Attn a) {
       const int e = lane + 64 * i, tok = e / NG, gi = e - tok * NG;
       const int to = 64 * gi + 16 * (tok & 3) + 4 * (tok >> 4) + (tok >> 2 & 3);
       kss[to] = q4_lo(pr[0][i]);
-      kos[to] = PSPLIT ? fmaf(8.f, q4_lo(pr[0][i]), q4_hi(pr[0][i])) : q4_hi(pr[0][i]);
+      kos[to] = SIGNED ? fmaf(8.f, q4_lo(pr[0][i]), q4_hi(pr[0][i])) : q4_hi(pr[0][i]);
       vss[to] = q4_lo(pr[1][i]);
-      vos[to] = PSPLIT ? fmaf(8.f, q4_lo(pr[1][i]), q4_hi(pr[1][i])) : q4_hi(pr[1][i]);
+      vos[to] = SIGNED ? fmaf(8.f, q4_lo(pr[1][i]), q4_hi(pr[1][i])) : q4_hi(pr[1][i]);
     }
     if (!ANY || D % 32 == 0) {
       const int n16 = D / 32;
@@ -476,12 +472,12 @@ k_q4_split(Q4Attn a) {
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          uint32_t x, y = 0u;
-          q4_halves<PSPLIT>(pv[2 * w], pv[2 * w + 1], x, y);
+          uint32_t x, y;
+          q4_halves(pv[2 * w], pv[2 * w + 1], x, y);
 #pragma unroll
           for (int p = 0; p < PK; ++p) {
             ph[w][HV * p + hh] = PK == 1 || pg == p ? x : 0u;
-            if constexpr (PSPLIT) pl[w][HV * p + hh] = PK == 1 || pg == p ? y : 0u;
+            pl[w][HV * p + hh] = PK == 1 || pg == p ? y : 0u;
           }
         }
       }
@@ -492,13 +488,11 @@ k_q4_split(Q4Attn a) {
         if (ANY ? 16 * d < gi * a.g || 16 * d >= (gi + 1) * a.g : d / (2 * (KSGT ? KSGT : 1)) != gi) continue;
         const v2i vw = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
             (__attribute__((address_space(3))) v2i *)(vt + (16 * g + hl) * PITCH + 8 * d));
-        const half8_t x0 = q4_lifted<kLess>(magic, (uint32_t)vw.x), x1 = q4_lifted<kLess>(magic, (uint32_t)vw.y);
+        const half8_t x0 = q4_lifted<SIGNED ? 8 : 0>(magic, (uint32_t)vw.x), x1 = q4_lifted<SIGNED ? 8 : 0>(magic, (uint32_t)vw.y);
         O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, sf_bitcast<half8_t>(ph[0]), O[d], 0, 0, 0);
         O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, sf_bitcast<half8_t>(ph[1]), O[d], 0, 0, 0);
-        if constexpr (PSPLIT) {
-          O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, sf_bitcast<half8_t>(pl[0]), O[d], 0, 0, 0);
-          O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, sf_bitcast<half8_t>(pl[1]), O[d], 0, 0, 0);
-        }
+        O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x0, sf_bitcast<half8_t>(pl[0]), O[d], 0, 0, 0);
+        O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x1, sf_bitcast<half8_t>(pl[1]), O[d], 0, 0, 0);
       }
     }
   }
@@ -906,7 +900,7 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
         if constexpr (SPLIT) {
           lsum += x + z;
           uint32_t hi, lo;
-          q4_halves<true>(x, z, hi, lo);
+          q4_halves(x, z, hi, lo);
           ph[s][p] = hi;
           pl[s][p] = lo;
         } else {  // rounded to fp16; their sum is the rounded weights', so that both are off alike
@@ -1062,7 +1056,7 @@ int q4_splits(int B, int Tq, int H, int KVH, int T_max, int D, int group, bool s
   return n_splits > kQaMaxSplits ? kQaMaxSplits : n_splits < 1 ? 1 : n_splits;
 }
 
-// Whether P (on prompts K and V too) go in two parts: what an fp16 part alone loses is below a bf16
+// Whether P, K and V of many rows go in two parts: what an fp16 part alone loses is below a bf16
 // output's rounding, but for the exponents of fp32 queries.
 bool q4_whole(int q_dtype, int out_dtype) { return out_dtype != SF_BF16 || q_dtype == SF_F32; }
 
@@ -1156,22 +1150,22 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
   }
   const dim3 grid(n_splits, (unsigned)(KVH * nrb), B);
   const int R = Tq * (H / KVH);
-#define SF_QA(QS, PS, DP, NG, KSG, PK) k_q4_split<QS, PS, DP, NG, KSG, PK><<<grid, kQaThreads, 0, st>>>(a)
-#define SF_QA_R(QS, PS, DP, NG, KSG)               \
+#define SF_QA(QS, SG, DP, NG, KSG, PK) k_q4_split<QS, SG, DP, NG, KSG, PK><<<grid, kQaThreads, 0, st>>>(a)
+#define SF_QA_R(QS, SG, DP, NG, KSG)               \
   do {                                             \
-    if (R <= 4) SF_QA(QS, PS, DP, NG, KSG, 4);     \
-    else if (R <= 8) SF_QA(QS, PS, DP, NG, KSG, 2); \
-    else SF_QA(QS, PS, DP, NG, KSG, 1);            \
+    if (R <= 4) SF_QA(QS, SG, DP, NG, KSG, 4);     \
+    else if (R <= 8) SF_QA(QS, SG, DP, NG, KSG, 2); \
+    else SF_QA(QS, SG, DP, NG, KSG, 1);            \
   } while (0)
-#define SF_QA_D(QS, PS)                                       \
+#define SF_QA_D(QS, SG)                                       \
   do {                                                        \
-    if (D == 64 && group == 64) SF_QA_R(QS, PS, 64, 1, 2);    \
-    else if (D == 64 && group == 32) SF_QA_R(QS, PS, 64, 2, 1);    \
-    else if (D == 128 && group == 128) SF_QA_R(QS, PS, 128, 1, 4); \
-    else if (D == 128 && group == 64) SF_QA_R(QS, PS, 128, 2, 2);  \
-    else if (D == 128 && group == 32) SF_QA_R(QS, PS, 128, 4, 1);  \
-    else if (D <= 128) SF_QA(QS, PS, 128, 0, 0, 1);           \
-    else SF_QA(QS, PS, 256, 0, 0, 1);                         \
+    if (D == 64 && group == 64) SF_QA_R(QS, SG, 64, 1, 2);    \
+    else if (D == 64 && group == 32) SF_QA_R(QS, SG, 64, 2, 1);    \
+    else if (D == 128 && group == 128) SF_QA_R(QS, SG, 128, 1, 4); \
+    else if (D == 128 && group == 64) SF_QA_R(QS, SG, 128, 2, 2);  \
+    else if (D == 128 && group == 32) SF_QA_R(QS, SG, 128, 4, 1);  \
+    else if (D <= 128) SF_QA(QS, SG, 128, 0, 0, 1);           \
+    else SF_QA(QS, SG, 256, 0, 0, 1);                         \
   } while (0)
   if (q_dtype == SF_F32) SF_QA_D(true, true);
   else if (out_dtype != SF_BF16) SF_QA_D(false, true);

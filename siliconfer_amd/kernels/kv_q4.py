@@ -154,9 +154,9 @@ def attention_q4kv(q: torch.Tensor, k_codes: torch.Tensor, k_params: torch.Tenso
                    out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """Attention of q [B, H, D], or of the Tq newest rows q [B, Tq, H, D], over the first
     lengths[b] + add slots of a 4-bit cache: softmax(scale q K^T) V in fp32 sums, one rounding
-    to the output's dtype. With 16-bit q and a bf16 output the softmax's weights meet V in fp16
-    (2^-11 of each), and where rows are many K and V are rounded to fp16 too, which moves a weight
-    by up to 2^-11 of scale sum |q K|; fp16 and fp32 outputs, and fp32 q, keep 2^-22. Row t of Tq sees the slots up to its own, lengths[b] + add - Tq + t;
+    to the output's dtype, factors held to 2^-22. (Where rows are many, and q has 16 bits, a bf16
+    output is made of weights, K and V rounded to fp16: 2^-11 of each, and of a weight by K's
+    rounding up to 2^-11 of scale sum |q K|.) Row t of Tq sees the slots up to its own, lengths[b] + add - Tq + t;
     a row that sees none gives zeros. `lengths`: int32 [B] on the device, or one int. Device
     lengths are cut to `max_length` (the capacity where it is not given). `n_splits`: among how
     many workgroups a sequence's slots are shared out where rows are few (its own choice by

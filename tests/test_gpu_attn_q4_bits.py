@@ -36,10 +36,9 @@ def close(got, q, bufs, lengths, rounded, factors, more=(), scale=None):
 @pytest.mark.parametrize("H,KVH,D,group", [(4, 2, 64, 64), (4, 1, 64, 32), (8, 2, 128, 32), (4, 2, 80, 80)])
 @pytest.mark.parametrize("rows", [1, 3, 9, 20])
 def test_values_of_one_sign(dev, rows, H, KVH, D, group, dtype):
-    """Codes of 0 stand for the minimum alone. For a bf16 output weights are rounded to fp16 (2^-11)
-    beside the codes: what that leaves is in proportion to the value, so a dim of zeros is exactly 0.
-    Others hold weights to 2^-22 beside a code less 8, and 8 s in fp32 with the minimum: they are off
-    by the bound of values of 8 s besides."""
+    """Codes of 0 stand for the minimum alone. For a bf16 output the codes stand beside the weights as
+    they are, so that a dim of zeros is exactly 0. Others hold weights to 2^-22 beside a code less 8,
+    and 8 s in fp32 with the minimum: they are off by the bound of values of 8 s besides."""
     B, bf16 = 2, dtype == "bf16"
     g = np.random.default_rng(rows)
     for n in (2, 64, 700):
@@ -53,8 +52,7 @@ def test_values_of_one_sign(dev, rows, H, KVH, D, group, dtype):
             bufs = k + of_codes(codes, s, (s * part).astype(np.float16), group, dev)
             for n_splits in (1, 2):
                 y = attention_q4kv(q, *bufs, lengths=n, n_splits=n_splits, out_dtype=DT[dtype])
-                close(y, q, bufs, [n] * B, *((2.0 ** -11, 2.0 ** -22) if bf16 else (2.0 ** -22, 2.0 ** -22)),
-                      more=() if bf16 else (eights,))
+                close(y, q, bufs, [n] * B, 2.0 ** -22, 2.0 ** -22, () if bf16 else (eights,))
                 if part == 0 and bf16:
                     assert (y[..., ::3] == 0).all()
 
