@@ -117,13 +117,16 @@ __device__ __forceinline__ void q4_halves(float a, float b, uint32_t &hi, uint32
   lo = sf_bitcast<uint16_t>((f16)(a - (float)x)) | (uint32_t)sf_bitcast<uint16_t>((f16)(b - (float)y)) << 16;
 }
 
-// Workgroups of k_q4_split that a CU's registers hold without (much) spilling.
+// Workgroups of k_q4_split that a CU's registers hold without spilling (three at 128 dims in two groups
+// with PK = 4 spill six registers: four ragged sequences of up to 32767 slots, bf16, 36.5 us, not 33.3; one
+// 19.0, not 16.1). Only the form for any head (groups = 0) spills at one, where DP is 128: 95 with fp32
+// queries, 56 with others (69 for bf16 outputs), 29 at DP = 256 with fp32 queries.
 __host__ __device__ constexpr int q4_resident(int DP, int groups, int PK, bool QSPLIT) {
   return groups == 0 || DP > 128 ? 1
          : DP == 64              ? groups == 1 ? PK > 1 ? 4 : 3 : PK == 4 && !QSPLIT ? 4 : PK == 1 ? 2 : 3
          : groups == 1           ? QSPLIT && PK < 4 ? 2 : 3
-         : groups == 2           ? !QSPLIT && PK == 4 ? 3 : 2
-                                 : PK == 4 ? 2 : 1;
+         : groups == 2 || PK == 4 ? 2
+                                  : 1;
 }
 
 // Columns: where a kv head has at most 8 (4) rows, PK = 2 (4) groups of 16 / PK columns hold the
@@ -1039,7 +1042,7 @@ size_t q4_many_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int parts)
 // round the CUs once, several (ragged) sequences' as many as are resident at a time. us a call in
 // a replayed graph at the rule's count (others in parentheses), 32 / 8 heads of 128, groups of 64:
 // 500 slots 9.6 (1; 2: 10.7, 8: 9.9), 8191 11.1 (32; 16: 12.5, 64: 13.6), four ragged sequences up
-// to 32767 33.5 (24; 8: 42.8, 16: 34.6, 48: 37.7), sixteen up to 4001 with fp32 queries 23.7 (4; 6:
+// to 32767 32.4 (16; 8: 35.3, 12: 36.4, 24: 39.0), sixteen up to 4001 with fp32 queries 23.7 (4; 6:
 // 28.3, 12: 32.0), eight up to 1000 13.1 (5; 1: 12.8, 4: 11.1, 8: 12.5); 131071 slots in groups of
 // 128 31.9 (32; 16: 52.0, 96: 36.0); 14 / 2 heads of 64, 1501 slots 8.9 (6; 1: 11.3, 24: 8.7), 16384
 // 9.1 (64; 16: 12.1, 128: 10.2); 40 / 2 heads of 128 in groups of 32, two up to 20000 21.8 (32; 16:
