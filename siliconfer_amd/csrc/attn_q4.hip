@@ -140,10 +140,12 @@ __host__ __device__ constexpr int q4_resident(int DP, int groups, int PK, bool Q
 // DP: the head's dims rounded up to 64, 128 or 256. NGT groups of 32 KSGT dims fill it
 // exactly, or 0, 0: any head and groups. QSPLIT: q in two parts. SIGNED: codes less 8.
 // Bound by vector instructions and the waits between them. Traced, with the merge launch, 32 / 8
-// heads of 128: four ragged sequences of up to 32767 slots, bf16, groups of 64 (111 MB) 28.7 + 5.1
-// us, the SIMDs issuing vector instructions 62% of that time (of some 680 a tile 290 turn codes
-// into operands); one sequence of 131071, fp16, groups of 128 (143 MB) 30.9 + 4.5, 4.6 TB/s in the
-// split; sixteen of up to 4001 with fp32 queries (51 MB) 20.9 + 4.0, both q and P in two parts.
+// heads of 128: four ragged sequences of up to 32767 slots, bf16, groups of 64 (111 MB) 29.4 + 4.7
+// us, the SIMDs issuing vector instructions 59% of the time of busy CUs (of some 690 a tile 290 turn
+// codes into operands); one sequence of 131071, fp16, groups of 128 (143 MB) 30.9 + 4.5, 4.6 TB/s in
+// the split; sixteen of up to 4001 with fp32 queries (51 MB) 20.8 + 3.9, q in two parts. The form for
+// any head is far from that: 32767 slots of 9 / 3 heads of 80 (8.7 MB) 28 us a call in fp32, 16 / 4
+// heads of 256 in groups of 64 (38 MB) 50.
 template <bool QSPLIT, bool SIGNED, int DP, int NGT, int KSGT, int PK>
 __global__ void __launch_bounds__(kQaThreads, q4_resident(DP, NGT, PK, QSPLIT))
 k_q4_split(Q4Attn a) {

@@ -3,6 +3,7 @@
 // A head's D dims of a token are cut into groups of g; a group holds
 //   m = f16(min x),  s = f16((max x - min x) / 15),
 //   code = clip(rint((x - m) / s), 0, 15)  (0 where s is 0),  x ~ m + s code,
+// s and m held at the ends of fp16's range;
 // codes two a byte (the even dim in the low half), (s, m) one 32-bit word a group. Beside
 // the int8 cache's D + 2 bytes a head and token this is D / 2 + 4 D / g.
 //
@@ -80,7 +81,7 @@ __device__ __forceinline__ V q4_over(V v, int n, F f) {
 
 // PAIR8: a lane's partners in the rotation are 8 neighbouring dims of the head (INTER: its own).
 // Bound by vector instructions: 4095 rows of 32 / 8 heads of 128, bf16, groups of 64, normed and
-// turned, 88 MB (17 us at a copy's rate) in 43 us, vector instructions in 84% of the SIMDs' time: 60.8 with divisions for the head, the row, the
+// turned, 88 MB (17 us at a copy's rate) in 42 us, vector instructions in 85% of the SIMDs' time: 60.8 with divisions for the head, the row, the
 // scale's inverse and the root and every code's remainder settled, 53 with the tables in the
 // dims' order (a head's lanes on the same banks).
 template <int DT, bool PAIR8, bool INTER>

@@ -8,8 +8,8 @@ s = (max x - min x) / 15, the code rint((x - m) / s). A buffer pair is
   codes   uint8 [B, KVH, T_cap, D / 2], the even dim of two in the low half of a byte
   params  fp16 [B, KVH, T_cap, D / group, 2], (s, m) a group
 
-with D a multiple of 16 up to 256 and group 32, 64, 128 (dividing D) or D itself. Values past
-fp16's range are held at its end; a group with a value that is not finite reads back as NaN.
+with D a multiple of 16 up to 256 and group 32, 64, 128 (dividing D) or D itself. A minimum or a
+scale past fp16's range is held at its end; a group with a value that is not finite reads back as NaN.
 Keys are cached turned to their positions. Nothing here is differentiable.
 """
 
