@@ -1029,13 +1029,17 @@ k_q4_rows(Q4Attn a, const uint8_t *__restrict__ ws, const uint32_t *__restrict__
 
 // The workspace of the many rows' launches where they take a call, else 0: a workgroup's walk
 // takes as long whatever the number of workgroups up to one a CU, the splits' launches as
-// much as the products. us, splits / many rows over 2000 slots, 32 / 8 heads of 128, bf16: 16
-// workgroups 31 / 43, 32 50 / 43, 64 70 / 44, fp32 32 61 / 92, 64 89 / 91, 128 132 / 100; 14 / 2
-// heads of 64, bf16: 56 20 / 30, 112 28 / 31, fp32 112 41 / 59. (Past 2 GiB the splits' take it.)
+// much as the products, at any length. us, splits / many rows, of so many workgroups (of many rows):
+// 32 / 8 heads of 128, one part: 2000 slots 64 38 / 44, 80 54 / 44, 128 69 / 45; 16384 slots 64 219 / 249,
+// 80 312 / 250; 65536 slots 64 796 / 989, 128 1522 / 1002; no slots but the rows' own 64 13 / 17, 80 22 / 19.
+// Two parts: 2000 slots 128 73 / 92, 176 95 / 96, 256 122 / 103; 16384 slots 160 559 / 618, 176 656 / 619;
+// 65536 slots 128 1760 / 2490. 14 / 2 heads of 64, 16384 slots: one part 90 166 / 171, 100 208 / 171; two
+// 176 341 / 385, 220 390 / 393; eight sequences in groups of 32 over 2000, two parts: 144 53 / 61, 176 65 /
+// 63. Four sequences in groups of 32 over 2000, one part: 64 73 / 50. (Past 2 GiB the splits' take it.)
 size_t q4_many_bytes(int B, int Tq, int H, int KVH, int T_max, int D, int parts) {
   if (D != 64 && D != 128) return 0;
   const long long blocks = (((long long)Tq * (H / KVH) + 127) / 128) * KVH * B;
-  if (blocks < (D == 64 ? 64 + 64 * parts : 32 * parts) || (long long)Tq * (H / KVH) < 64) return 0;
+  if (blocks < (parts == 1 ? 80 : 176) || (long long)Tq * (H / KVH) < 64) return 0;
   const size_t tiles = (size_t)B * KVH * q4_tiles(T_max), bytes = tiles * (2 * q4_block_bytes(D, parts) + 8);
   return bytes > (size_t)1 << 31 ? 0 : bytes;
 }

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from oracle import kv_q4 as O
+from siliconfer_amd import _lib
 from siliconfer_amd.kernels.kv_q4 import attention_q4kv
 from test_gpu_attn_q4 import DT, cache
 
@@ -17,6 +18,14 @@ def of_codes(codes, s, m, group, dev):
     params = np.stack(np.broadcast_arrays(s, m), -1).astype(np.float16)
     assert params.shape[:3] == codes.shape[:3] and params.shape[3] * group == codes.shape[3]
     return [torch.from_numpy(O.pack(codes)).to(dev), torch.from_numpy(params).to(dev)]
+
+
+def by_many_rows(q, bufs, length, out):
+    """Whether the kernel of many rows takes a call (few rows in one split need no workspace)."""
+    B, rows, H, D = q.shape
+    code = [_lib.dt(torch.empty(0, dtype=t)) for t in (q.dtype, DT[out])]
+    KVH, group = bufs[0].shape[1], D // bufs[1].shape[3]
+    return _lib.load().sf_attn_q4_workspace_bytes(B, rows, H, KVH, length, D, group, *code, 1) > 0
 
 
 def close(got, q, bufs, lengths, rounded, factors, more=(), scale=None):
@@ -58,8 +67,8 @@ def test_values_of_one_sign(dev, rows, H, KVH, D, group, dtype):
 
 
 @pytest.mark.parametrize("out", list(DT))
-@pytest.mark.parametrize("H,KVH,D,group,rows", [(4, 2, 64, 32, 1), (8, 2, 128, 64, 3), (4, 1, 96, 32, 9), (32, 16, 64, 32, 260),
-                                                (16, 8, 128, 64, 260)])
+@pytest.mark.parametrize("H,KVH,D,group,rows", [(4, 2, 64, 32, 1), (8, 2, 128, 64, 3), (4, 1, 96, 32, 9), (36, 18, 64, 32, 260),
+                                                (36, 18, 128, 64, 260)])
 def test_scores_whose_parts_cancel(dev, rows, H, KVH, D, group, out):
     """fp32 queries of two large dims, over keys of t and 2 - t there: their scores are apart by what
     fp16 cannot hold of the queries, whatever type the output has. V is t too."""
@@ -74,6 +83,7 @@ def test_scores_whose_parts_cancel(dev, rows, H, KVH, D, group, out):
     q[..., 0] = 1000 + torch.rand(B, rows, H, generator=torch.Generator().manual_seed(rows))
     q[..., D // 2] = 1000 + torch.rand(B, rows, H, generator=torch.Generator().manual_seed(rows + 1))
     q = q.to(dev)
+    assert by_many_rows(q, bufs, n, out) is (rows == 260)
     y = attention_q4kv(q, *bufs, lengths=n, scale=1.0, out_dtype=DT[out])
     # (V and weights: both in two parts; V's codes less 8, as above)
     eights = of_codes(np.full_like(codes, 8), s, np.zeros_like(s), group, dev)
@@ -84,7 +94,7 @@ def test_weights_of_a_prompt_are_rounded(dev):
     """bf16 queries and outputs, many rows: slot 0 holds 1 and weighs about what all others, which hold
     -1, weigh together. K and V are exact in fp16, so that a row is off by its weights' rounding, 2^-11
     at most of the others', and by its own."""
-    H, KVH, D, rows, n = 16, 8, 128, 260, 300
+    H, KVH, D, rows, n = 32, 16, 128, 260, 300
     k, v = (np.zeros((1, KVH, n, D, 1)) for _ in range(2))
     k[:, :, 1:, 0], v[:, :, :], v[:, :, 0] = 1, -1, 1  # (codes of dim 0 below: 0 for slot 0, else 1, of -1 each)
     codes = k[..., 0].astype(np.int64)
@@ -94,6 +104,7 @@ def test_weights_of_a_prompt_are_rounded(dev):
     q = torch.zeros(1, rows, H, D, dtype=torch.float64)
     q[..., 0] = (others.log()[None, :, None] + torch.randn(1, rows, H, generator=torch.Generator().manual_seed(0)) / 32)
     q = q.to(dev, torch.bfloat16)
+    assert by_many_rows(q, bufs, n, "bf16")
     y = attention_q4kv(q, *bufs, lengths=n, scale=1.0, out_dtype=torch.bfloat16).double().cpu()
     w = others[:, None] * torch.exp(-q[0, :, :, 0].double().cpu())  # of the others together, slot 0 weighing 1
     want = (1 - w) / (1 + w)
@@ -103,7 +114,7 @@ def test_weights_of_a_prompt_are_rounded(dev):
 
 
 @pytest.mark.parametrize("out", list(DT))
-@pytest.mark.parametrize("H,KVH,D,group", [(32, 16, 64, 32), (16, 8, 128, 64)])
+@pytest.mark.parametrize("H,KVH,D,group", [(32, 16, 64, 32), (16, 8, 128, 64), (36, 18, 64, 32), (36, 18, 128, 64)])
 def test_small_values_beside_large_ones_of_a_prompt(dev, H, KVH, D, group, out):
     """Many rows over tiles whose first group holds values up to 20000 and whose others a thousandth: in K
     (the queries are 0 beside the large ones, and large beside the small) and in V. Then some of V's
@@ -127,9 +138,11 @@ def test_small_values_beside_large_ones_of_a_prompt(dev, H, KVH, D, group, out):
     far = [t.clone() for t in bufs]
     far[3][:, :, ::7, 0, 0] = 60000  # up to 880000 in the first group
     z = attention_q4kv(q, *far, lengths=n, out_dtype=DT[out])
-    # (160 workgroups of 64 dims in two parts are too few for the kernel of many rows; few rows' weights share one
-    # factor: 2^-38 of the largest weight times scale is their last place, here 60000 2^-38 beside scales of 1e-4)
-    if D == 128 or not whole:
+    # (few rows' weights share one factor: 2^-38 of the largest weight times scale is their last place, here
+    # 60000 2^-38 beside scales of 1e-4)
+    many = by_many_rows(q, bufs, n, out)
+    assert many is (not whole or KVH == 18)
+    if many:
         assert torch.equal(z[..., group:], y[..., group:])
     else:
         assert ((z - y)[..., group:].abs() <= n * 8 * 60000 * 2.0 ** -38).all()
@@ -140,8 +153,9 @@ def test_small_values_beside_large_ones_of_a_prompt(dev, H, KVH, D, group, out):
 def test_an_output_at_any_address(dev, rows, out):
     """A contiguous `out` that starts off 16 bytes holds what an aligned one holds, and nothing around
     it is written."""
-    bufs = cache(1, 16, 300, 128, 64, dev)
-    q = torch.randn(1, rows, 32, 128, generator=torch.Generator().manual_seed(0)).to(dev, DT[out])
+    bufs = cache(1, 36, 300, 128, 64, dev)
+    q = torch.randn(1, rows, 72, 128, generator=torch.Generator().manual_seed(0)).to(dev, DT[out])
+    assert by_many_rows(q, bufs, 300, out) is (rows == 260)
     want = attention_q4kv(q, *bufs, lengths=300, out_dtype=DT[out])
     for off in (1, 2, 4, 7, 8):
         flat = torch.full((want.numel() + 16,), 7.0, dtype=DT[out], device=dev)
