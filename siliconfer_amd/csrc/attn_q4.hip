@@ -1124,24 +1124,27 @@ extern "C" int sf_attn_q4kv(const void *q, int q_dtype, const uint8_t *k_codes, 
     uint8_t *const ws = (uint8_t *)workspace;
     Q4Attn r = a;
     r.n_splits = B * KVH;
-    // The order of a head's columns where all are resident at once, one or two a CU (us, 1500 rows
-    // behind 300, 32 / 8 heads of 128, longest first / the first CUs' shortest first: bf16 55.7 /
-    // 51.6, fp32 111 / 104); longest first where there are more.
+    // The order of a head's columns where all are resident at once, one or two a CU (us, longest first /
+    // the first CUs' shortest first: bf16, 32 / 8 heads of 128, 1200 rows 38.0 / 36.9, 1500 behind 300
+    // 52.3 / 49.9, 2000 behind 8000 321 / 314, 40 / 2 heads 1400 behind 1000 69.5 / 64.7; fp32 1500
+    // behind 300 97.6 / 95.1; 14 / 2 heads of 64, bf16, 3000 rows 49.3 / 48.8); longest first where
+    // there are more.
     const int heads = B * KVH, cols = (int)(blocks / heads), per = 256 / heads;
     if (cols > per && cols <= 2 * per) r.first = per;
-    // Four waves a workgroup where there are more workgroups than CUs, for a bf16 output: two a CU
+    // Four waves a workgroup for one part of 128 dims, where there are more workgroups than CUs: two a CU
     // between barriers of their own; else eight, which halves the longest columns' walk. us, four /
-    // eight waves: bf16, 376 workgroups 51.6 / 54.1, 1024 (4096 rows) 168 / 181, 166 (14 / 2 heads
-    // of 64) 32.3 / 27.3; fp32 (whose tiles are half as long) at 376 110 / 104, fp16 97 / 89.
-    const bool four = !q4_whole(q_dtype, out_dtype) && blocks > 256;
+    // eight waves, bf16: 128 dims, 304 workgroups 36.9 / 35.2, 376 49.9 / 49.9, 438 64.8 / 71.5, 504 behind
+    // 8000 slots 314 / 324, 1024 166 / 173, 160 65.9 / 58.3; 64 dims, 252 39.0 / 31.6, 330 49.0 / 39.4,
+    // 504 72.2 / 62.0, 876 166 / 166. (Two parts at 376 110 / 104 with fp32 queries, 97 / 89 with fp16.)
+    const bool four = !q4_whole(q_dtype, out_dtype) && D == 128 && blocks > 256;
 #define SF_QR(QD, SP, DD)                                                                                        \
   do {                                                                                                           \
     uint32_t *const fl = (uint32_t *)(ws + tiles.x * (size_t)tiles.y * 2 * q4_block_bytes(DD, SP ? 2 : 1));      \
     k_q4_spread<SP, DD><<<tiles, 256, 0, st>>>(a, ws, fl);                                                       \
-    if constexpr (!SP) {                                                                                         \
+    if constexpr (!SP && DD == 128) {                                                                            \
       if (four) k_q4_rows<QD, SP, DD, 1><<<blocks, 256, 0, st>>>(r, ws, fl);                                     \
     }                                                                                                            \
-    if (SP || !four) k_q4_rows<QD, SP, DD, 2><<<blocks, 512, 0, st>>>(r, ws, fl);                                \
+    if (!four) k_q4_rows<QD, SP, DD, 2><<<blocks, 512, 0, st>>>(r, ws, fl);                                \
   } while (0)
 #define SF_QR_O(QD, SP)                  \
   do {                                   \
