@@ -364,7 +364,10 @@ extern "C" int sf_kv_q4_append(const void *q, const void *k, const void *v, int 
   while ((8 << a.lanes_log2) < D) ++a.lanes_log2;
   // Three times the heads that a workgroup's threads hold, where that leaves four workgroups a CU: its
   // weights and table serve as many (us a call, 4095 / 2048 / 1024 rows of the above: one 51.4 / 27.5 /
-  // 16.6, two 44.8 / 24.7 / 15.8, three 42.0 / 23.2 / 14.6, four 42.2 / 25.1 / 15.4, six 42.3 / 24.0 / 17.7).
+  // 16.6, two 44.8 / 24.7 / 15.8, three 42.0 / 23.2 / 14.6, four 42.2 / 25.1 / 15.4, six 42.3 / 24.0 / 17.7;
+  // in a replayed graph at the border and at four times as many, one / three: 14 / 2 heads of 64 18.1 / 16.8 and 58.2 /
+  // 48.1, 9 / 3 of 80 17.7 / 17.6 and 58.5 / 51.3, 16 / 4 of 256 16.7 / 14.1 and 53.4 / 40.9, 32 / 32 of 128 15.7 / 14.7
+  // and 49.1 / 43.2; k and v alone, 4095 rows of 8 heads of 128, 16.3 / 16.7, 16000 rows 50.9 / 45.1).
   const int hb = kQ4Threads >> a.lanes_log2, heads = H + 2 * KVH;
   a.chunks = n_heads >= 3LL * hb * 1024 ? 3 : 1;
   const int rows = (hb * a.chunks + heads - 2) / heads + 1;
