@@ -493,7 +493,8 @@ int sf_kv_q4_append(const void *q, const void *k, const void *v, int in_dtype, c
 int sf_kv_q4_dequant(const uint8_t *codes, const void *params, void *out, int out_dtype, int group,
                      const long long *strides, int B, int KVH, int T, int D, void *stream);
 /* Attention of the Tq newest rows a sequence, q [B][Tq][H][D], over the first n_b slots of
- * such a cache: softmax(scale q K^T) V to out [B][Tq][H][D], rounded once to out_dtype. n_b =
+ * such a cache: softmax(scale q K^T) V to out [B][Tq][H][D], rounded once to out_dtype (prompts of 16-bit q
+ * with a bf16 out: weights, K and V rounded to fp16 before). scale must be finite. n_b =
  * lengths[b] + T (device lengths, T may be negative) cut to 0 .. T_max, or T where lengths is
  * NULL; row t sees the first n_b - Tq + t + 1 slots, a row that sees none gives zeros, and what
  * a row does not see may hold anything. n_splits <= 0: the kernel's own choice; at most 128
